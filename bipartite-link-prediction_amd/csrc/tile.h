@@ -1,0 +1,295 @@
+// The tile engine of the latent-factor products (latent.hip, scores8.hip): C[q][p] = sum_k P(p, k) Q(q, k)
+// on the matrix cores, with the caller's epilogue over the accumulators. gfx950 only.
+//
+// A workgroup owns a tile of BP x BQ outputs and walks k in stages of 128 bytes (64 halves, 32 floats,
+// 128 8-bit integers). A stage of each operand is copied from memory straight into LDS (16 bytes a lane,
+// no register in between); the next stage is in flight while this one is multiplied, in the other of two
+// buffers, so a stage costs one barrier. A fragment is 16 bytes of a row: 8 halves, 4 floats or 16 8-bit
+// integers, one 16-row matrix instruction (four of them for floats).
+//
+// Layouts of an operand: ROW -- k contiguous, element (p, k) at base + p ld + k size; COL -- p contiguous,
+// element (p, k) at base + k ld + p size, whose halves are transposed on their way out of LDS
+// (ds_read_b64_tr_b16: 16 lanes read 4 rows of 16 halves and get columns).
+// LDS banks: ROW tiles hold 128 bytes a row, its 16-byte granule c stored at c ^ (row & 7), so the rows a
+// fragment read touches together fall on different banks; COL tiles XOR the granule with bits of k.
+//
+// Bounds: an operand's granules outside its rows or its k are not read (the lane's buffer offset is set
+// out of the buffer's range, which loads zeros). Bases and row strides are multiples of 16 bytes and rows
+// are padded to whole granules (the callers pack what is not).
+//
+// The matrix instruction leaves lane l with q = l % 16 and the four p = 4 (l / 16) + 0..3 of a 16 x 16
+// block: p is the contiguous dimension of what is written, and a row's reduction over p is in-lane first.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace blp {
+namespace tile {
+
+enum Type { F32 = 0, BF16 = 1, F16 = 2, I8 = 3 };
+enum Layout { ROW = 0, COL = 1 };
+
+typedef int frag_t __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int STAGE = 128;  // bytes of k a stage holds
+
+__host__ __device__ constexpr int size_of(int t) { return t == F32 ? 4 : t == I8 ? 1 : 2; }
+
+template <int T>
+struct Acc {
+  typedef f32x4 type;
+};
+template <>
+struct Acc<I8> {
+  typedef i32x4 type;
+};
+
+template <int T>
+__device__ inline typename Acc<T>::type mma(frag_t p, frag_t q, typename Acc<T>::type c) {
+  if constexpr (T == BF16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
+  } else if constexpr (T == F16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, p), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
+  } else if constexpr (T == I8) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(p, q, c, 0, 0, 0);
+  } else {
+    const f32x4 a = __builtin_bit_cast(f32x4, p), b = __builtin_bit_cast(f32x4, q);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+}
+
+// One operand of a product, in bytes (`rows`: valid p; `k`: valid k, both in elements).
+struct Operand {
+  const char* base;
+  int64_t ld;
+  int64_t rows;
+};
+
+// Workgroup shape: WP x WQ waves, each FP x FQ blocks of 16 x 16.
+template <int WP_, int WQ_, int FP_, int FQ_>
+struct Shape {
+  static constexpr int WP = WP_, WQ = WQ_, FP = FP_, FQ = FQ_;
+  static constexpr int WAVES = WP * WQ, THREADS = WAVES * 64;
+  static constexpr int BP = WP * FP * 16, BQ = WQ * FQ * 16;
+};
+
+typedef __attribute__((address_space(3))) char lds_char;
+
+__device__ inline __amdgpu_buffer_rsrc_t rsrc_at(const char* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, 0x7fffffff, 0x00020000);
+}
+constexpr uint32_t OUT_OF_RANGE = 0x80000000u;
+
+// COL tiles: which granules of a row trade places, by k. Halves: the 16 lanes of a transposing read take
+// 4 rows (k & 3) of 32 bytes, the next 16 the rows 8 further; floats: 16 lanes take 64 bytes of one row,
+// the next 16 the row 4 further.
+template <int T>
+__device__ inline int col_swz(int k) {
+  return T == F32 ? ((k >> 2) & 3) << 2 : ((k & 3) | ((k >> 3) & 1) << 2) << 1;
+}
+
+// Copy stage [k0, k0 + STAGE/size) of a tile of R rows starting at row r0 into LDS (asynchronous: counted
+// by vmcnt). Every wave copies R / WAVES rows' worth of granules.
+template <int T, int LAYOUT, int R, int WAVES>
+__device__ inline void load_stage(lds_char* lds, const Operand& o, int64_t r0, int64_t k0, int64_t kend) {
+  constexpr int ES = size_of(T), KE = STAGE / ES, GE = 16 / ES;
+  constexpr int PASS = WAVES * 64;                    // granules a pass of the workgroup copies
+  constexpr int GRANULES = R * STAGE / 16;
+  static_assert(GRANULES % PASS == 0, "tile too small for the workgroup");
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if constexpr (LAYOUT == ROW) {
+    const __amdgpu_buffer_rsrc_t rs = rsrc_at(o.base + r0 * o.ld + k0 * ES);
+    const int row0 = wave * 8 + (lane >> 3);
+    const int c = (lane & 7) ^ (row0 & 7);
+    const bool k_ok = k0 + c * GE < kend;
+    const uint32_t ld = (uint32_t)o.ld;
+    const int64_t left = o.rows - r0;
+    uint32_t off = (uint32_t)row0 * ld + c * 16;
+#pragma unroll
+    for (int i = 0; i < GRANULES / PASS; ++i) {
+      const bool ok = k_ok && row0 + i * (PASS / 8) < left;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rs, (__attribute__((address_space(3))) void*)(lds + (i * PASS + wave * 64) * 16), 16,
+          ok ? off : OUT_OF_RANGE, 0, 0, 0);
+      off += (PASS / 8) * ld;
+    }
+  } else {
+    constexpr int GR = R / GE;  // granules a k row
+    const __amdgpu_buffer_rsrc_t rs = rsrc_at(o.base + k0 * o.ld + r0 * ES);
+    const uint32_t ld = (uint32_t)o.ld;
+    const int64_t left = o.rows - r0;
+#pragma unroll
+    for (int i = 0; i < GRANULES / PASS; ++i) {
+      const int g = (i * WAVES + wave) * 64 + lane;
+      const int k = g / GR, c = (g % GR) ^ (col_swz<T>(k) & (GR - 1));
+      const bool ok = k0 + k < kend && c * GE < left;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rs, (__attribute__((address_space(3))) void*)(lds + (i * PASS + wave * 64) * 16), 16,
+          ok ? (uint32_t)k * ld + c * 16 : OUT_OF_RANGE, 0, 0, 0);
+    }
+    (void)KE;
+  }
+}
+
+// The fragment of rows [row, row + 16) and k granule `g` = 4 kk + lane / 16 of a stage in LDS.
+template <int T, int LAYOUT, int R>
+__device__ inline frag_t read_frag(const lds_char* lds, int row, int kk) {
+  const int lane = threadIdx.x & 63, i = lane & 15, h = lane >> 4;
+  if constexpr (LAYOUT == ROW) {
+    const int r = row + i, c = (kk * 4 + h) ^ (i & 7);  // row is a multiple of 16
+    return *(const __attribute__((address_space(3))) frag_t*)(lds + r * STAGE + c * 16);
+  } else if constexpr (T == F32) {
+    constexpr int GR = R / 4;
+    f32x4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = (kk * 4 + h) * 4 + j;
+      const int c = ((row + i) >> 2) ^ (col_swz<T>(k) & (GR - 1));
+      v[j] = *(const __attribute__((address_space(3))) float*)(lds + k * R * 4 + c * 16 + (i & 3) * 4);
+    }
+    return __builtin_bit_cast(frag_t, v);
+  } else {
+    static_assert(T == BF16 || T == F16, "column layout: halves and floats");
+    constexpr int GR = R / 8;
+    i32x4 v;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int k = (kk * 4 + h) * 8 + s * 4 + (i >> 2);
+      const int c = ((row >> 3) + ((i & 3) >> 1)) ^ (col_swz<T>(k) & (GR - 1));
+      const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(lds + k * R * 2 + c * 16 + (i & 1) * 8));
+      const i32x2 w = __builtin_bit_cast(i32x2, t);
+      v[2 * s] = w[0];
+      v[2 * s + 1] = w[1];
+    }
+    return v;
+  }
+}
+
+template <int T, int LP, int LQ, class S>
+__device__ inline void mul_stage(const lds_char* lp, const lds_char* lq, int wp, int wq,
+                                 typename Acc<T>::type (&acc)[S::FP][S::FQ]) {
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk) {
+    frag_t p[S::FP], q[S::FQ];
+#pragma unroll
+    for (int i = 0; i < S::FP; ++i) p[i] = read_frag<T, LP, S::BP>(lp, (wp * S::FP + i) * 16, kk);
+#pragma unroll
+    for (int j = 0; j < S::FQ; ++j) q[j] = read_frag<T, LQ, S::BQ>(lq, (wq * S::FQ + j) * 16, kk);
+#pragma unroll
+    for (int i = 0; i < S::FP; ++i)
+#pragma unroll
+      for (int j = 0; j < S::FQ; ++j) acc[i][j] = mma<T>(p[i], q[j], acc[i][j]);
+  }
+}
+
+__device__ inline void stage_barrier() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies have landed (lgkmcnt, expcnt: any)
+  __syncthreads();
+}
+
+struct Problem {
+  Operand p, q;
+  int64_t k;        // valid k, in elements
+  int64_t k_slice;  // k of one slice (blockIdx.y), a multiple of the stage
+  int tiles_p, tiles_q;
+};
+
+// The workgroup's tile: consecutive workgroups go to the 8 dies in turn, so each die gets one contiguous
+// range of tiles, and walks it in bands of 8 q tiles: the p tile stays in the die's L2 while they pass.
+__device__ inline void tile_of(const Problem& a, int* tp, int* tq) {
+  const int n = a.tiles_p * a.tiles_q, b = blockIdx.x;
+  const int per = n >> 3, extra = n & 7, xcd = b & 7, at = b >> 3;
+  const int t = xcd * per + min(xcd, extra) + at;
+  constexpr int BAND = 8;
+  const int band = t / (BAND * a.tiles_p), in = t - band * BAND * a.tiles_p;
+  const int width = min(BAND, a.tiles_q - band * BAND);
+  *tp = in / width;
+  *tq = band * BAND + in - *tp * width;
+}
+
+template <int T, int LP, int LQ, class S, class Epi>
+__global__ __launch_bounds__(S::THREADS) void k_product(Problem a, Epi epi) {
+  constexpr int KE = STAGE / size_of(T);
+  __shared__ __attribute__((aligned(1024))) char s_p0[S::BP * STAGE], s_q0[S::BQ * STAGE];
+  __shared__ __attribute__((aligned(1024))) char s_p1[S::BP * STAGE], s_q1[S::BQ * STAGE];
+  int tp, tq;
+  tile_of(a, &tp, &tq);
+  const int64_t p0 = (int64_t)tp * S::BP, q0 = (int64_t)tq * S::BQ;
+  const int64_t kb = (int64_t)blockIdx.y * a.k_slice, ke = min(a.k, kb + a.k_slice);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wp = wave % S::WP, wq = wave / S::WP;
+  typename Acc<T>::type acc[S::FP][S::FQ];
+#pragma unroll
+  for (int i = 0; i < S::FP; ++i)
+#pragma unroll
+    for (int j = 0; j < S::FQ; ++j) acc[i][j] = 0;
+  const int stages = ke > kb ? (int)((ke - kb + KE - 1) / KE) : 0;
+  lds_char *lp0 = (lds_char*)s_p0, *lq0 = (lds_char*)s_q0, *lp1 = (lds_char*)s_p1, *lq1 = (lds_char*)s_q1;
+  if (stages > 0) {
+    load_stage<T, LP, S::BP, S::WAVES>(lp0, a.p, p0, kb, ke);
+    load_stage<T, LQ, S::BQ, S::WAVES>(lq0, a.q, q0, kb, ke);
+  }
+  for (int t = 0; t < stages; t += 2) {
+    stage_barrier();
+    if (t + 1 < stages) {
+      load_stage<T, LP, S::BP, S::WAVES>(lp1, a.p, p0, kb + (int64_t)(t + 1) * KE, ke);
+      load_stage<T, LQ, S::BQ, S::WAVES>(lq1, a.q, q0, kb + (int64_t)(t + 1) * KE, ke);
+    }
+    mul_stage<T, LP, LQ, S>(lp0, lq0, wp, wq, acc);
+    if (t + 1 >= stages) break;
+    stage_barrier();
+    if (t + 2 < stages) {
+      load_stage<T, LP, S::BP, S::WAVES>(lp0, a.p, p0, kb + (int64_t)(t + 2) * KE, ke);
+      load_stage<T, LQ, S::BQ, S::WAVES>(lq0, a.q, q0, kb + (int64_t)(t + 2) * KE, ke);
+    }
+    mul_stage<T, LP, LQ, S>(lp1, lq1, wp, wq, acc);
+  }
+  epi.template run<S>(acc, p0 + wp * S::FP * 16, q0 + wq * S::FQ * 16, tp * S::WP + wp);
+}
+
+// round to the type once; four consecutive values
+template <int T>
+__device__ inline void store4(char* at, f32x4 v) {
+  if constexpr (T == F32) {
+    *reinterpret_cast<f32x4*>(at) = v;
+  } else if constexpr (T == BF16) {
+    *reinterpret_cast<bf16x4*>(at) = __builtin_convertvector(v, bf16x4);
+  } else {
+    *reinterpret_cast<f16x4*>(at) = __builtin_convertvector(v, f16x4);
+  }
+}
+template <int T>
+__device__ inline void store1(char* at, float v) {
+  if constexpr (T == F32) {
+    *reinterpret_cast<float*>(at) = v;
+  } else if constexpr (T == BF16) {
+    *reinterpret_cast<__bf16*>(at) = (__bf16)v;
+  } else {
+    *reinterpret_cast<_Float16*>(at) = (_Float16)v;
+  }
+}
+template <int T>
+__device__ inline float load1(const char* at) {
+  if constexpr (T == F32) {
+    return *reinterpret_cast<const float*>(at);
+  } else if constexpr (T == BF16) {
+    return (float)*reinterpret_cast<const __bf16*>(at);
+  } else {
+    return (float)*reinterpret_cast<const _Float16*>(at);
+  }
+}
+
+}  // namespace tile
+}  // namespace blp

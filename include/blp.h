@@ -428,6 +428,38 @@ int blp_walk_run(blp_walk* w, const int32_t* starts, int64_t n_starts, int itera
 int blp_walk_run_dense(blp_walk* w, int32_t start, int iterations, double scale, double* p_out);
 int blp_walk_stats(blp_walk* w, double* total_ms, int64_t* launches);
 
+/* ---------------------------------------------------------------- latent factors: the softmax loss
+ * Operators for training and serving latent factors (the rows DeviceSVD scores): x (rows x k) against
+ * every row of a catalogue `table` (cols x k). All pointers are device pointers of `device`; the work is
+ * queued on `stream` (a hipStream_t passed as void*; NULL = the null stream) and nothing is waited for.
+ * Row strides (ld*) count elements. `type` is the type of x, table and their gradients. Any number of
+ * threads may call at once; a workspace belongs to one call until its work is done. The calling thread's
+ * current device is left as it was. Every result is the same each time (no float atomics).
+ *   z_ij = scale x_i . table_j     lse_i = log sum_j exp z_ij     loss_i = lse_i - z_{i, target_i}
+ * target: int32, or int64 with target64; outside [0, cols) the row is ignored (loss 0, gradient 0,
+ * whatever x holds). The scores are not kept: the workspace holds one piece of the catalogue's.
+ *   blp_softmax_loss_workspace: bytes of workspace (256-byte aligned) for the same arguments;
+ *     `forward` / `grads`: whether the call runs the forward / the backward pass.
+ *   blp_softmax_loss: loss[rows], lse[rows] (float); total (or NULL): total[0] = the sum of the losses
+ *     or, with mean, that over the rows not ignored (0 if none), total[1] = their number (at least 1).
+ *     With grads also dx (rows x k) and dtable (cols x k), either may be NULL: the gradients of the sum
+ *     of the losses (of the mean when total and mean are given), each rounded to `type` once.
+ *   blp_softmax_loss_backward: the gradients from lse: row i's gradient is grad[i * grad_stride] (NULL:
+ *     1; grad_stride 0 or 1) divided by *count (NULL: 1).                                     */
+#define BLP_F32 0
+#define BLP_BF16 1
+#define BLP_F16 2
+int blp_softmax_loss_workspace(int type, const void* x, int64_t ldx, const void* table, int64_t ldt, int64_t rows,
+                               int64_t cols, int k, int forward, int grads, int64_t* bytes);
+int blp_softmax_loss(int device, void* stream, int type, const void* x, int64_t ldx, const void* table, int64_t ldt,
+                     const void* target, int target64, int64_t rows, int64_t cols, int k, float scale, float* loss,
+                     float* lse, float* total, int mean, int grads, void* dx, int64_t lddx, void* dtable, int64_t lddt,
+                     void* ws, int64_t ws_bytes);
+int blp_softmax_loss_backward(int device, void* stream, int type, const void* x, int64_t ldx, const void* table,
+                              int64_t ldt, const void* target, int target64, int64_t rows, int64_t cols, int k, float scale,
+                              const float* lse, const float* grad, int grad_stride, const float* count, void* dx,
+                              int64_t lddx, void* dtable, int64_t lddt, void* ws, int64_t ws_bytes);
+
 /* ---------------------------------------------------------------- stats
  * Per-kernel device time (ms, HIP events on the handle's stream) accumulated since the
  * last reset, for bench.py's roofline figure. kernel: 0 = pair scorer, 1 = grouping

@@ -1,0 +1,307 @@
+"""The softmax loss over the catalogue (blp.latent.softmax_loss*) against its definition in 64 bits.
+
+Bounds, from the operator's own roundings (u = 2^-23, a 32-bit step: products are added inside the matrix
+instruction, whose inner rounding may truncate):
+  a score         dz_i  = (k + 4) u S_i, S_i = max_j scale sum |x w|
+  log-sum-exp     dz_i + (depth + 8) u + 4 u |lse|     depth: additions in a chain of partial sums
+  a probability   relative r_i = 2 dz_i + (depth + 16) u + 4 u (S_i + |lse_i|)
+  dS              h |dS| more for its rounding to the type (h half a step; halves hold 2^-14 less than
+                  2^-25 of the largest row gradient)
+  a gradient      scale sum (error of dS) |w| + (n + 8) u sum |dS w|, then h of the result
+"""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -23
+
+
+def _torch():
+    return pytest.importorskip("torch")
+
+
+def _half_step(t):
+    import torch
+
+    return torch.finfo(t).eps / 2
+
+
+def make(m, n, k, dtype, seed=0, ignored=0.0, spread=3.0, scale=1.0, device="cuda"):
+    import torch
+
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, k, generator=g).to(dtype)
+    w = (torch.randn(n, k, generator=g) * (spread / scale / k ** 0.5)).to(dtype)
+    t = torch.randint(0, n, (m,), generator=g)
+    t[torch.rand(m, generator=g) < ignored] = -1
+    return x.to(device), w.to(device), t.to(device)
+
+
+def reference(x, w, t, scale, g=None, reduction="mean"):
+    """-> dict of the definition's values and error bounds, on the inputs' device in 64 bits."""
+    import torch
+
+    X, W = x.double(), w.double()
+    n, k = W.shape
+    ok = (t >= 0) & (t < n)
+    X = torch.where(ok[:, None], X, 0.0)
+    at = t.clamp(0, n - 1).long()[:, None]
+    z = scale * (X @ W.t().contiguous())
+    S = abs(scale) * (X.abs() @ W.abs().t().contiguous()).amax(1)
+    lse = torch.logsumexp(z, 1)
+    loss = torch.where(ok, lse - z.gather(1, at)[:, 0], 0.0)
+    depth = 64 + n / 64  # within a tile, then along the tiles' pairs
+    dz = (k + 4) * U * S
+    bl = 2 * dz + (depth + 8) * U + 8 * U * (lse.abs() + S)
+    count = max(int(ok.sum()), 1)
+    gi = torch.ones_like(lse) if g is None else g.double().expand(len(lse))
+    if reduction == "mean":
+        gi = gi / count
+    gi = torch.where(ok, gi, 0.0)
+    p = torch.exp(z - lse[:, None])
+    hit = torch.zeros_like(p).scatter_(1, at, 1.0)
+    d = gi[:, None] * (p - hit)
+    h = _half_step(x.dtype)
+    r = 2 * dz + (depth + 16) * U + 4 * U * (S + lse.abs())
+    # bound on dS: the probability's, a 32-bit step of the difference, the rounding to the type
+    e = gi.abs()[:, None] * (p * r[:, None] + 2 * U) + h * d.abs()
+    if x.dtype == torch.float16:
+        e = e + gi.abs().max() * 2.0 ** -39
+    out = {"loss": loss, "b_loss": bl, "ok": ok, "count": count, "lse": lse}
+    tiny = 2.0 ** -25 if x.dtype == torch.float16 else 0.0
+    mm = lambda a, b: a @ b.contiguous()
+    out["dx"] = scale * mm(d, W)
+    out["b_dx"] = abs(scale) * (mm(e, W.abs()) + (n + 8) * U * mm(d.abs(), W.abs()))
+    out["dw"] = scale * mm(d.t(), X)
+    out["b_dw"] = abs(scale) * (mm(e.t(), X.abs()) + (len(lse) + 8) * U * mm(d.t().abs(), X.abs()))
+    for q in ("dx", "dw"):
+        out["b_" + q] = out["b_" + q] * (1 + 2 * h) + h * out[q].abs() + tiny
+    return out
+
+
+def near(got, want, bound):
+    import torch
+
+    assert tuple(got.shape) == tuple(want.shape)
+    off = (got.double() - want).abs() - bound
+    assert bool((off <= 0).all()), "off by %.3g more than %.3g" % (float(off.max()), float(bound.flatten()[off.argmax()]))
+    assert bool(torch.isfinite(got).all())
+
+
+SIZES = [(1, 1, 1), (1, 7, 3), (2, 100, 50), (31, 33, 8), (32, 257, 64), (33, 64, 65), (130, 1000, 64), (257, 513, 72),
+         (64, 5003, 128), (300, 300, 200), (700, 129, 24)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_loss_and_gradients(gpu, m, n, k, dtype):
+    torch = _torch()
+    from blp import latent
+
+    x, w, t = make(m, n, k, getattr(torch, dtype), seed=m + n, ignored=0.2 if m > 5 else 0.0, scale=1.5)
+    ref = reference(x, w, t, 1.5)
+    loss = latent.softmax_loss(x, w, t, scale=1.5, reduction="none")
+    near(loss, ref["loss"], ref["b_loss"])
+    total, dx, dw = latent.softmax_loss_grad(x, w, t, scale=1.5)
+    near(total, ref["loss"].sum() / ref["count"], ref["b_loss"].mean() * m / ref["count"] + U * abs(float(total)))
+    near(dx, ref["dx"], ref["b_dx"])
+    near(dw, ref["dw"], ref["b_dw"])
+    assert dx.dtype == x.dtype and dw.dtype == w.dtype and total.dtype == torch.float32
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("m,n,k", [(2100, 3000, 64), (600, 9001, 328), (1500, 2500, 1000)])
+def test_large_tiles(gpu, m, n, k, dtype):
+    torch = _torch()
+    from blp import latent
+
+    x, w, t = make(m, n, k, getattr(torch, dtype), seed=k, ignored=0.1)
+    ref = reference(x, w, t, 1.0)
+    total, dx, dw = latent.softmax_loss_grad(x, w, t)
+    near(total, ref["loss"].sum() / ref["count"], ref["b_loss"].mean() * m / ref["count"] + U * abs(float(total)))
+    near(dx, ref["dx"], ref["b_dx"])
+    near(dw, ref["dw"], ref["b_dw"])
+
+
+def test_pieces_of_the_catalogue(gpu):
+    """More scores than one workspace piece holds (512 MiB of float32: 134M of them)."""
+    torch = _torch()
+    from blp import latent
+
+    x, w, t = make(12000, 24011, 20, torch.float32, seed=3, ignored=0.02)
+    ref = reference(x, w, t, 1.0)
+    total, dx, dw = latent.softmax_loss_grad(x, w, t, reduction="sum")
+    near(dx / ref["count"], ref["dx"], ref["b_dx"] * (1 + 2 * U) + U * ref["dx"].abs())
+    near(dw / ref["count"], ref["dw"], ref["b_dw"] * (1 + 2 * U) + U * ref["dw"].abs())
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_autograd_gradients_per_row(gpu, dtype):
+    """reduction none: every row's own gradient, of both signs and very different sizes, zero among them."""
+    torch = _torch()
+    from blp import latent
+
+    x, w, t = make(140, 700, 56, getattr(torch, dtype), seed=9, ignored=0.1)
+    g = torch.logspace(-4, 3, 140, device="cuda") * torch.where(torch.arange(140, device="cuda") % 2 == 0, 1.0, -1.0)
+    g[7] = 0.0
+    ref = reference(x, w, t, 0.75, g, "none")
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    loss = latent.softmax_loss(x, w, t, scale=0.75, reduction="none")
+    dx, dw = torch.autograd.grad(loss, (x, w), g)
+    near(dx, ref["dx"], ref["b_dx"])
+    near(dw, ref["dw"], ref["b_dw"])
+    # one of the two only
+    (dx2,) = torch.autograd.grad(latent.softmax_loss(x, w.detach(), t, scale=0.75, reduction="none"), (x,), g)
+    assert torch.equal(dx, dx2)
+
+
+def test_against_differences(gpu):
+    """The gradient against the loss's own differences, taken in 64 bits."""
+    torch = _torch()
+    from blp import latent
+
+    x, w, t = make(9, 40, 6, torch.float32, seed=4)
+    _, dx, dw = latent.softmax_loss_grad(x, w, t)
+
+    def f(X, W):
+        z = X @ W.t()
+        return float((torch.logsumexp(z, 1) - z.gather(1, t[:, None])[:, 0]).mean())
+
+    X, W, step = x.double().cpu(), w.double().cpu(), 1e-5
+    t = t.cpu()
+    for A, got in ((X, dx), (W, dw)):
+        for i, j in ((0, 0), (3, 5), (8, 2)):
+            keep = float(A[i, j])
+            A[i, j] = keep + step
+            hi = f(X, W)
+            A[i, j] = keep - step
+            lo = f(X, W)
+            A[i, j] = keep
+            # differences: third derivatives below 10 times step^2, and 1e-16 / step; 32-bit gradient
+            assert abs((hi - lo) / (2 * step) - float(got[i, j])) < 10 * step ** 2 + 1e-10 + 1e-5 * float(got.abs().max())
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_ignored_rows_hold_anything(gpu, dtype):
+    torch = _torch()
+    from blp import latent
+
+    x, w, t = make(70, 300, 40, getattr(torch, dtype), seed=5)
+    t[3], t[20], t[69] = -1, 300, -100
+    for wide in (True, False):
+        tt = t if wide else t.to(torch.int32)
+        clean = latent.softmax_loss_grad(x, w, tt)
+        bad = x.clone()
+        bad[3], bad[20], bad[69] = float("nan"), float("inf"), float("-inf")
+        got = latent.softmax_loss_grad(bad, w, tt)
+        for a, b in zip(clean, got):
+            assert torch.equal(a, b)
+        loss = latent.softmax_loss(bad, w, tt, reduction="none")
+        assert loss[3] == 0 and loss[20] == 0 and loss[69] == 0
+        assert not got[1][3].any() and not got[1][20].any() and not got[1][69].any()
+
+
+def test_no_row_left_and_no_rows(gpu):
+    torch = _torch()
+    from blp import latent
+
+    x, w, t = make(40, 90, 16, torch.bfloat16, seed=6)
+    loss, dx, dw = latent.softmax_loss_grad(x, w, torch.full_like(t, -1))
+    assert float(loss) == 0 and not dx.any() and not dw.any()
+    loss, dx, dw = latent.softmax_loss_grad(x[:0], w, t[:0])
+    assert float(loss) == 0 and dx.shape == (0, 16) and not dw.any()
+    assert latent.softmax_loss(x[:0], w, t[:0], reduction="none").shape == (0,)
+
+
+def test_infinite_and_nan_scores_stay_in_their_rows(gpu):
+    torch = _torch()
+    from blp import latent
+
+    x, w, t = make(20, 50, 8, torch.float32, seed=7)
+    want = latent.softmax_loss(x, w, t, reduction="none")
+    x[4, 0] = float("nan")
+    x[5] = 1e30  # scores beyond 32 bits' exponents: infinite
+    x[5, 0] = -1e38
+    got = latent.softmax_loss(x, w, t, reduction="none")
+    keep = [i for i in range(20) if i not in (4, 5)]
+    assert torch.equal(got[keep], want[keep]) and torch.isnan(got[4])
+    # large equal scores: the running maximum keeps exp in range
+    big = torch.full((3, 4), 100.0, device="cuda")
+    loss = latent.softmax_loss(big, torch.full((1000, 4), 50.0, device="cuda"), t[:3], reduction="none")
+    np.testing.assert_allclose(loss.cpu().numpy(), np.log(1000.0), rtol=0, atol=20000 * 4 * U)
+
+
+def test_strided_and_unaligned_rows(gpu):
+    """Slices of wider tensors: row strides, and starts that no 16-byte load can take."""
+    torch = _torch()
+    from blp import latent
+
+    for dtype in (torch.bfloat16, torch.float32):
+        X, W, t = make(50, 400, 96, dtype, seed=8)
+        for lo, hi in ((0, 64), (8, 72), (1, 65), (3, 90)):
+            x, w = X[:, lo:hi], W[:, lo:hi]
+            a = latent.softmax_loss_grad(x, w, t)
+            b = latent.softmax_loss_grad(x.contiguous(), w.contiguous(), t)
+            for p, q in zip(a, b):
+                assert torch.equal(p, q)
+
+
+def test_same_result_twice_and_on_another_stream(gpu):
+    torch = _torch()
+    from blp import latent
+
+    x, w, t = make(500, 3000, 64, torch.bfloat16, seed=10)
+    a = latent.softmax_loss_grad(x, w, t)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        b = latent.softmax_loss_grad(x, w, t)
+    torch.cuda.current_stream().wait_stream(side)
+    for p, q in zip(a, b):
+        assert torch.equal(p, q)
+
+
+def test_captured_and_replayed(gpu):
+    """Two captured graphs and eager calls between their replays, on changing inputs."""
+    torch = _torch()
+    from blp import latent
+
+    x, w, t = make(90, 500, 50, torch.bfloat16, seed=11)
+    x2, w2, t2 = make(90, 500, 50, torch.bfloat16, seed=12)
+    latent.softmax_loss_grad(x, w, t)
+    torch.cuda.synchronize()
+    graphs = []
+    for args in ((x, w, t), (x2, w2, t2)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = latent.softmax_loss_grad(*args)
+        graphs.append((g, out, args))
+    for i in range(4):
+        for g, out, args in graphs:
+            fresh = make(90, 500, 50, torch.bfloat16, seed=20 + i)
+            for dst, src in zip(args, fresh):
+                dst.copy_(src)
+            g.replay()
+            want = latent.softmax_loss_grad(*fresh)
+            for p, q in zip(out, want):
+                assert torch.equal(p, q)
+
+
+def test_refusals(gpu):
+    torch = _torch()
+    from blp import latent
+
+    x, w, t = make(10, 20, 8, torch.float32)
+    for bad in (lambda: latent.softmax_loss(x.double(), w, t), lambda: latent.softmax_loss(x, w.half(), t),
+                lambda: latent.softmax_loss(x[:, :4], w, t), lambda: latent.softmax_loss(x, w, t[:5]),
+                lambda: latent.softmax_loss(x, w, t.float()), lambda: latent.softmax_loss(x, w, t.cpu()),
+                lambda: latent.softmax_loss(x.cpu(), w, t), lambda: latent.softmax_loss(x, w[:0], t),
+                lambda: latent.softmax_loss(x.t(), w, t), lambda: latent.softmax_loss(x[0], w, t),
+                lambda: latent.softmax_loss(x[:1].expand(10, 8), w, t), lambda: latent.softmax_loss(x, w, t, reduction="max"),
+                lambda: latent.softmax_loss(x, w, t, scale=float("nan")),
+                lambda: latent.softmax_loss_grad(x, w, t, reduction="none"),
+                lambda: latent.softmax_loss_backward(torch.ones(3, device="cuda"), torch.ones(10, device="cuda"), None, x, w, t)):
+        with pytest.raises(ValueError):
+            bad()
