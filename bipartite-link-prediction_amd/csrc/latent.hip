@@ -13,7 +13,7 @@
 #include <algorithm>
 
 #include "blp_internal.h"
-#include "tile.h"
+#include "latent.h"
 
 namespace {
 
@@ -22,30 +22,8 @@ using namespace blp::tile;
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LN2 = 0.69314718055994530942f;
 
-struct DeviceGuard {
-  int before = -1, rc = 0;
-  explicit DeviceGuard(int device) {
-    hipError_t e = hipGetDevice(&before);
-    if (e == hipSuccess && before != device) e = hipSetDevice(device);
-    if (e != hipSuccess) rc = blp::hip_fail(e, "hipSetDevice", __FILE__, __LINE__);
-    device_ = device;
-  }
-  ~DeviceGuard() {
-    if (before >= 0 && before != device_) (void)hipSetDevice(before);
-  }
-  int device_;
-};
-
-// the target of row i, or -1 (ignored)
-struct Targets {
-  const void* at;
-  int wide;  // int64, else int32
-  int64_t n_cols;
-  __device__ int64_t operator()(int64_t i) const {
-    const int64_t t = wide ? reinterpret_cast<const int64_t*>(at)[i] : reinterpret_cast<const int32_t*>(at)[i];
-    return t >= 0 && t < n_cols ? t : -1;
-  }
-};
+using blp::DeviceGuard;
+using Targets = blp::Ids;  // the target of row i, or -1 (ignored)
 
 // ---------------------------------------------------------------- packing
 // Rows as the tile engine takes them: `kp` elements a row (whole granules, zeros past k), 16-byte aligned;

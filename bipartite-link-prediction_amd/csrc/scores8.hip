@@ -1,0 +1,237 @@
+// Scores of the catalogue from 8-bit factors (blp_quantize_rows, blp_scores8).
+//
+//   s_i = max_k |x_ik| / 127      q_ik = x_ik / s_i rounded to the nearest whole number, halves to the even one
+//   C_ij = s_i t_j sum_k q_ik p_jk
+//
+// The sum of products is a whole number in 32 bits, exact for k < 2^17; it is scaled in 32-bit floats and
+// rounded to the output's type once.
+#include <algorithm>
+
+#include "blp_internal.h"
+#include "latent.h"
+
+namespace {
+
+using namespace blp::tile;
+using blp::DeviceGuard;
+
+struct __attribute__((packed, aligned(2))) Raw16 {
+  i32x4 v;
+};
+template <class V>
+struct __attribute__((packed, aligned(2))) Raw {
+  V v;
+};
+
+// ---------------------------------------------------------------- quantising
+// x / s rounded to nearest, halves to even -- of the true quotient, not of its 32-bit rounding: the first
+// guess is off by one at most (a division: 1 / s may not be a number of 32 bits), and x - q s is exact in an fma (both are multiples of the smaller last
+// place of x and s, and the difference is at most s), so comparing it with s / 2 settles the guess.
+__device__ inline int to8(float x, float s) {
+  float q = rintf(x / s);
+  const float r = fmaf(-q, s, x), half = 0.5f * s;
+  const bool odd = ((int)q & 1) != 0;
+  if (r > half || (r == half && odd)) q += 1.f;
+  if (r < -half || (r == -half && odd)) q -= 1.f;
+  return (int)fminf(fmaxf(q, -127.f), 127.f);
+}
+
+// `lanes` (a power of two up to 64) lanes a row, 16 elements a step; two passes over the row, the second
+// out of the cache. Bytes [k, kp) of a row are set to zero. A row with a NaN or an infinity gets the scale
+// NaN and zeros, so its scores are NaN; a row of zeros the scale 0.
+template <int T>
+__global__ __launch_bounds__(256) void k_quantize(const char* __restrict__ x, int64_t ld, int64_t rows, int k, int kp, int lanes,
+                                                  int8_t* __restrict__ q, int64_t ldq, float* __restrict__ s) {
+  constexpr int ES = size_of(T);
+  const int64_t row = (blockIdx.x * 256ll + threadIdx.x) / lanes;
+  const int l = threadIdx.x & (lanes - 1);
+  if (row >= rows) return;
+  const char* src = x + row * ld;
+  uint32_t top = 0;
+  for (int e0 = l * 4; e0 < k; e0 += lanes * 4)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e0 + e < k) top = max(top, __builtin_bit_cast(uint32_t, load1<T>(src + (int64_t)(e0 + e) * ES)) & 0x7fffffffu);
+  for (int o = lanes >> 1; o; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+  const bool bad = top >= 0x7f800000u;
+  const float scale = bad ? NAN : __builtin_bit_cast(float, top) / 127.f;
+  const bool none = bad || scale == 0.f;
+  if (l == 0) s[row] = scale;
+  int8_t* dst = q + row * ldq;
+  for (int e0 = l * 4; e0 < kp; e0 += lanes * 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int at = e0 + e;
+      if (at < kp) dst[at] = at < k && !none ? (int8_t)to8(load1<T>(src + (int64_t)at * ES), scale) : 0;
+    }
+  }
+}
+
+// 8-bit rows as the tile engine takes them: whole granules, zeros past k.
+__global__ __launch_bounds__(256) void k_pack8(const int8_t* __restrict__ src, int64_t ld, int64_t rows, int k, int kp,
+                                               int8_t* __restrict__ dst) {
+  const int per = kp / 16;
+  const int64_t n = rows * per, step = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += step) {
+    const int64_t r = i / per;
+    const int e0 = (int)(i - r * per) * 16;
+    const int8_t* s = src + r * ld + e0;
+    uint32_t w[4] = {0, 0, 0, 0};
+    for (int j = 0; j < 16; ++j)
+      if (e0 + j < k) w[j >> 2] |= (uint32_t)(uint8_t)s[j] << (8 * (j & 3));
+    reinterpret_cast<i32x4*>(dst)[i] = i32x4{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+  }
+}
+
+// ---------------------------------------------------------------- scores
+template <int TO>
+struct EpiScores {
+  char* out;
+  int64_t ld;  // bytes
+  const float *s, *t;
+  int64_t np, nq;
+  template <class S>
+  __device__ void run(i32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int) const {
+    const int lane = threadIdx.x & 63, h = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < S::FQ; ++j) {
+      const int64_t q = q0 + j * 16 + (lane & 15);
+      if (q >= nq) continue;
+      const float sq = s[q];
+#pragma unroll
+      for (int i = 0; i < S::FP; ++i) {
+        const int64_t p = p0 + i * 16 + h * 4;
+        char* at = out + q * ld + p * size_of(TO);
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = p + e < np ? (float)acc[i][j][e] * sq * t[p + e] : 0.f;
+        if (p + 4 <= np) {
+          if constexpr (TO == F32)
+            reinterpret_cast<Raw<f32x4>*>(at)->v = v;
+          else if constexpr (TO == BF16)
+            reinterpret_cast<Raw<bf16x4>*>(at)->v = __builtin_convertvector(v, bf16x4);
+          else
+            reinterpret_cast<Raw<f16x4>*>(at)->v = __builtin_convertvector(v, f16x4);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (p + e < np) store1<TO>(at + e * size_of(TO), v[e]);
+        }
+      }
+    }
+  }
+};
+
+int64_t div_up(int64_t v, int64_t by) { return (v + by - 1) / by; }
+int64_t up(int64_t v, int64_t to) { return div_up(v, to) * to; }
+
+using Big = Shape<2, 4, 8, 4>;      // 256 x 256
+using Mid = Shape<2, 2, 4, 4>;      // 128 x 128
+using NarrowQ = Shape<4, 1, 4, 2>;  // 256 x 32
+
+template <int TO, class S>
+int launch(Problem a, EpiScores<TO> epi, hipStream_t st) {
+  const int64_t tp = div_up(a.p.rows, S::BP), tq = div_up(a.q.rows, S::BQ);
+  BLP_CHECK(tp * tq <= 0x7fffffff, BLP_E_ARG, "scores8: too many tiles for one launch");
+  a.tiles_p = (int)tp;
+  a.tiles_q = (int)tq;
+  k_product<I8, ROW, ROW, S, EpiScores<TO>><<<(unsigned)(tp * tq), S::THREADS, 0, st>>>(a, epi);
+  BLP_HIP(hipGetLastError());
+  return 0;
+}
+
+template <int TO>
+int scores(const Operand& w, const Operand& x, int k, const float* s, const float* t, void* out, int64_t ldo, hipStream_t st) {
+  const Problem a = {w, x, k, up(k, STAGE), 0, 0};
+  const EpiScores<TO> epi = {(char*)out, ldo * size_of(TO), s, t, w.rows, x.rows};
+  if (x.rows <= 32) return launch<TO, NarrowQ>(a, epi, st);
+  if (div_up(w.rows, 256) * div_up(x.rows, 256) >= 192) return launch<TO, Big>(a, epi, st);
+  return launch<TO, Mid>(a, epi, st);
+}
+
+bool whole(const void* p, int64_t ld, int k) { return (((uintptr_t)p | (uintptr_t)ld | (uintptr_t)k) & 15) == 0; }
+
+int check_args(int64_t rows, int64_t cols, int k) {
+  BLP_CHECK(rows >= 0 && rows < (1ll << 31) && cols >= 1 && cols < (1ll << 31), BLP_E_ARG,
+            "scores8: rows must be in [0, 2^31), columns in [1, 2^31)");
+  BLP_CHECK(k >= 1 && k < (1 << 17), BLP_E_ARG, "scores8: k must be in [1, 2^17)");
+  return 0;
+}
+
+int64_t workspace(const void* q, int64_t ldq, const void* p, int64_t ldp, int64_t rows, int64_t cols, int k) {
+  const int64_t kp = up(k, 16);
+  return std::max<int64_t>((whole(q, ldq, k) ? 0 : up(rows * kp, 256)) + (whole(p, ldp, k) ? 0 : up(cols * kp, 256)), 256);
+}
+
+int pack(Operand& o, int k, char*& ws, hipStream_t st) {
+  const int64_t kp = up(k, 16), n = o.rows * kp / 16;
+  k_pack8<<<(unsigned)std::max<int64_t>(std::min<int64_t>(div_up(n, 256), 8192), 1), 256, 0, st>>>(
+      (const int8_t*)o.base, o.ld, o.rows, k, (int)kp, (int8_t*)ws);
+  BLP_HIP(hipGetLastError());
+  o = {ws, kp, o.rows};
+  ws += up(o.rows * kp, 256);
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int blp_quantize_rows(int device, void* stream, int type, const void* x, int64_t ldx, int64_t rows, int k, int8_t* q,
+                                 int64_t ldq, float* s) {
+  BLP_CHECK(type >= 0 && type <= 2, BLP_E_ARG, "quantize_rows: type must be BLP_F32, BLP_BF16 or BLP_F16");
+  BLP_CHECK(rows >= 0 && rows < (1ll << 31) && k >= 1 && k <= (1 << 20), BLP_E_ARG,
+            "quantize_rows: rows must be in [0, 2^31), k in [1, 2^20]");
+  if (rows == 0) return 0;
+  BLP_CHECK(x && q && s, BLP_E_ARG, "quantize_rows: null pointer");
+  BLP_CHECK(ldx >= k && ldq >= k, BLP_E_ARG, "quantize_rows: a row stride is smaller than k");
+  DeviceGuard guard(device);
+  if (guard.rc) return guard.rc;
+  hipStream_t st = (hipStream_t)stream;
+  int lanes = 1;
+  while (lanes < 64 && lanes * 4 < k) lanes <<= 1;
+  const unsigned grid = (unsigned)div_up(rows * lanes, 256);
+  const int kp = (int)std::min<int64_t>(ldq, up(k, 16));
+  if (type == F32)
+    k_quantize<F32><<<grid, 256, 0, st>>>((const char*)x, ldx * 4, rows, k, kp, lanes, q, ldq, s);
+  else if (type == BF16)
+    k_quantize<BF16><<<grid, 256, 0, st>>>((const char*)x, ldx * 2, rows, k, kp, lanes, q, ldq, s);
+  else
+    k_quantize<F16><<<grid, 256, 0, st>>>((const char*)x, ldx * 2, rows, k, kp, lanes, q, ldq, s);
+  BLP_HIP(hipGetLastError());
+  return 0;
+}
+
+extern "C" int blp_scores8_workspace(const int8_t* q, int64_t ldq, const int8_t* table, int64_t ldt, int64_t rows, int64_t cols,
+                                     int k, int64_t* bytes) {
+  int rc = check_args(rows, cols, k);
+  if (rc) return rc;
+  BLP_CHECK(bytes, BLP_E_ARG, "scores8: null pointer");
+  *bytes = workspace(q, ldq, table, ldt, rows, cols, k);
+  return 0;
+}
+
+extern "C" int blp_scores8(int device, void* stream, const int8_t* q, int64_t ldq, const float* s, const int8_t* table, int64_t ldt,
+                           const float* ts, int64_t rows, int64_t cols, int k, int out_type, void* out, int64_t ldo, void* ws,
+                           int64_t ws_bytes) {
+  int rc = check_args(rows, cols, k);
+  if (rc) return rc;
+  if (rows == 0) return 0;
+  BLP_CHECK(out_type >= 0 && out_type <= 2, BLP_E_ARG, "scores8: type must be BLP_F32, BLP_BF16 or BLP_F16");
+  BLP_CHECK(q && s && table && ts && out && ws, BLP_E_ARG, "scores8: null pointer");
+  BLP_CHECK(ldq >= k && ldt >= k && ldo >= cols, BLP_E_ARG, "scores8: a row stride is smaller than the row");
+  BLP_CHECK(std::max(ldq, ldt) <= (1 << 22), BLP_E_ARG, "scores8: row strides must be at most 2^22");
+  BLP_CHECK(ws_bytes >= workspace(q, ldq, table, ldt, rows, cols, k), BLP_E_ARG,
+            "scores8: the workspace is too small (blp_scores8_workspace)");
+  BLP_CHECK(((uintptr_t)ws & 255) == 0, BLP_E_ARG, "scores8: the workspace must be 256-byte aligned");
+  DeviceGuard guard(device);
+  if (guard.rc) return guard.rc;
+  hipStream_t st = (hipStream_t)stream;
+  char* at = (char*)ws;
+  Operand x = {(const char*)q, ldq, rows}, w = {(const char*)table, ldt, cols};
+  if (!whole(q, ldq, k)) rc = pack(x, k, at, st);
+  if (!rc && !whole(table, ldt, k)) rc = pack(w, k, at, st);
+  if (rc) return rc;
+  const int kp = (int)up(k, 16);
+  if (out_type == F32) return scores<F32>(w, x, kp, s, ts, out, ldo, st);
+  if (out_type == BF16) return scores<BF16>(w, x, kp, s, ts, out, ldo, st);
+  return scores<F16>(w, x, kp, s, ts, out, ldo, st);
+}

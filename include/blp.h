@@ -460,6 +460,34 @@ int blp_softmax_loss_backward(int device, void* stream, int type, const void* x,
                               const float* lse, const float* grad, int grad_stride, const float* count, void* dx,
                               int64_t lddx, void* dtable, int64_t lddt, void* ws, int64_t ws_bytes);
 
+/* ---------------------------------------------------------------- latent factors: rows by id
+ * (conventions as for the softmax loss; ids int32, or int64 with ids64)
+ *   blp_lookup: out[i] = scale table[ids[i]] (k elements a row, rounded once); ids outside [0, rows)
+ *     give zeros.
+ *   blp_lookup_grad: out[r] (rows x k) = scale * the sum of grad[i] over ids[i] == r, ascending i, in 32
+ *     bits; rows without ids are zero. With add, the sums are added to what out holds (rows without
+ *     ids are left alone).                                                                  */
+int blp_lookup(int device, void* stream, int type, const void* table, int64_t ldt, int64_t rows, int k, const void* ids,
+               int ids64, int64_t n, float scale, void* out, int64_t ldo);
+int blp_lookup_grad_workspace(int type, int64_t n, int64_t rows, int k, int64_t* bytes);
+int blp_lookup_grad(int device, void* stream, int type, const void* grad, int64_t ldg, const void* ids, int ids64,
+                    int64_t n, int64_t rows, int k, float scale, void* out, int64_t ldo, int add, void* ws,
+                    int64_t ws_bytes);
+
+/* ---------------------------------------------------------------- latent factors: 8-bit scores
+ *   blp_quantize_rows: s[i] = max|x_i| / 127, q[i] = x_i / s[i] rounded to the nearest whole number (halves
+ *     to even). A row of zeros: s = 0; one with a NaN or an infinity: s = NaN, q = 0. Bytes k to
+ *     min(ldq, k rounded up to 16) of a row of q are set to 0.
+ *   blp_scores8: out[i][j] = s[i] ts[j] sum_k q[i][k] table[j][k], k < 2^17: the sum exact in 32-bit
+ *     integers, the rest in float, rounded to out_type once.                                */
+int blp_quantize_rows(int device, void* stream, int type, const void* x, int64_t ldx, int64_t rows, int k, int8_t* q,
+                      int64_t ldq, float* s);
+int blp_scores8_workspace(const int8_t* q, int64_t ldq, const int8_t* table, int64_t ldt, int64_t rows, int64_t cols, int k,
+                          int64_t* bytes);
+int blp_scores8(int device, void* stream, const int8_t* q, int64_t ldq, const float* s, const int8_t* table, int64_t ldt,
+                const float* ts, int64_t rows, int64_t cols, int k, int out_type, void* out, int64_t ldo, void* ws,
+                int64_t ws_bytes);
+
 /* ---------------------------------------------------------------- stats
  * Per-kernel device time (ms, HIP events on the handle's stream) accumulated since the
  * last reset, for bench.py's roofline figure. kernel: 0 = pair scorer, 1 = grouping

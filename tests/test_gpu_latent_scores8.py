@@ -1,0 +1,193 @@
+"""8-bit factor rows and their scores of the catalogue (blp.latent.quantize_rows, int8_scores), and the latent
+operators together.
+
+The sum of a score is a whole number and exact; its conversion and the two scales round three times in 32
+bits (2^-24 each), then to the output's type (half a step). Quantised values equal their definition.
+"""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def _torch():
+    return pytest.importorskip("torch")
+
+
+def quantize(x):
+    """The definition in 64 bits: (whole numbers, float32 scales)."""
+    import torch
+
+    x = x.double()
+    s = (x.abs().amax(1) / 127).float()
+    q = torch.where(s[:, None] > 0, torch.round(x / s.double()[:, None]), 0.0).clamp(-127, 127)
+    return q.to(torch.int8), s
+
+
+def check_scores(got, q, s, p, t):
+    import torch
+
+    want = (q.double() @ p.double().t().contiguous()) * s.double()[:, None] * t.double()[None, :]
+    h = torch.finfo(got.dtype).eps / 2
+    tiny = 2.0 ** -25 if got.dtype == torch.float16 else 0.0
+    off = (got.double() - want).abs() - (want.abs() * (3 * 2.0 ** -24 + h) * 1.001 + tiny)
+    assert got.shape == want.shape and bool((off <= 0).all()), float(off.max())
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("n,k", [(1, 1), (3, 5), (100, 64), (257, 50), (33, 1000), (7, 8200)])
+def test_quantized_rows(gpu, n, k, dtype):
+    torch = _torch()
+    from blp import latent
+
+    g = torch.Generator(device="cuda").manual_seed(n * k)
+    x = (torch.randn(n, k, device="cuda", generator=g) * 10.0 ** torch.randint(-3, 3, (n, 1), device="cuda", generator=g)).to(
+        getattr(torch, dtype))
+    x[n // 2] = 0
+    q, s = latent.quantize_rows(x)
+    wq, ws = quantize(x)
+    assert torch.equal(s, ws) and torch.equal(q, wq)
+    assert q.stride(0) % 16 == 0
+
+
+def test_quotients_on_a_border(gpu):
+    """Values that lie on or next to halves of the scale, tiny rows and rows that are not finite."""
+    torch = _torch()
+    from blp import latent
+
+    s0 = torch.tensor([1.0, 0.3, 1e-30, 3e38 / 127, 7.77], device="cuda")
+    half = (torch.arange(-126, 127, device="cuda") + 0.5)[None, :] * s0[:, None]
+    x = torch.cat([half, torch.nextafter(half, half * 2), torch.nextafter(half, half * 0), 127 * s0[:, None]], 1)
+    q, s = latent.quantize_rows(x)
+    wq, ws = quantize(x)
+    assert torch.equal(s, ws) and torch.equal(q, wq)
+    x = torch.zeros(5, 20, device="cuda")
+    x[0, 3] = 1e-44
+    x[1, 19] = float("inf")
+    x[2, 0] = float("nan")
+    x[3, 1] = -1e-39
+    q, s = latent.quantize_rows(x)
+    assert not q[1].any() and not q[2].any() and torch.isnan(s[1:3]).all() and s[4] == 0 and not q[4].any()
+    assert int(q[3, 1]) == -127 and s[3] > 0
+
+
+@pytest.mark.parametrize("out", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 5003, 64), (7, 300, 50), (32, 1000, 200), (33, 129, 128), (130, 4099, 64),
+                                   (300, 301, 1000), (3500, 4600, 272)])
+def test_scores(gpu, m, n, k, out):
+    torch = _torch()
+    from blp import latent
+
+    g = torch.Generator(device="cuda").manual_seed(m + n + k)
+    q = torch.randint(-128, 128, (m, k), device="cuda", generator=g).to(torch.int8)
+    p = torch.randint(-128, 128, (n, k), device="cuda", generator=g).to(torch.int8)
+    s = torch.rand(m, device="cuda", generator=g) * 1e-3
+    t = torch.rand(n, device="cuda", generator=g) * 1e-2
+    got = latent.int8_scores(q, s, p, t, dtype=getattr(torch, out))
+    check_scores(got, q, s, p, t)
+
+
+def test_longest_sums(gpu):
+    """The largest k: sums next to 2^31."""
+    torch = _torch()
+    from blp import latent
+
+    k = (1 << 17) - 1
+    q = torch.full((3, k), -128, dtype=torch.int8, device="cuda")
+    p = torch.full((5, k), -128, dtype=torch.int8, device="cuda")
+    p[1] = 127
+    one = torch.ones(5, device="cuda")
+    got = latent.int8_scores(q, one[:3], p, one)
+    assert float(got[0, 0]) == 2 ** 31 - 2 ** 14 and got[2, 1] == torch.tensor(-128.0 * 127 * k)
+    with pytest.raises(ValueError):
+        latent.int8_scores(torch.zeros(1, k + 1, dtype=torch.int8, device="cuda"), one[:1],
+                           torch.zeros(1, k + 1, dtype=torch.int8, device="cuda"), one[:1])
+
+
+def test_strides_padding_and_no_rows(gpu):
+    torch = _torch()
+    from blp import latent
+
+    x, w = torch.randn(40, 70, device="cuda"), torch.randn(90, 70, device="cuda")
+    q, s = latent.quantize_rows(x)
+    p, t = latent.quantize_rows(w)
+    a = latent.int8_scores(q, s, p, t)
+    check_scores(a, q, s, p, t)
+    # the padding's bytes are no part of a row
+    wide = torch.full((90, 96), 77, dtype=torch.int8, device="cuda")
+    wide[:, 5:75] = p
+    assert torch.equal(a, latent.int8_scores(q.contiguous(), s, wide[:, 5:75], t))
+    assert latent.int8_scores(q[:0], s[:0], p, t).shape == (0, 90)
+    assert latent.quantize_rows(x[:0])[0].shape == (0, 70)
+    s2 = s.clone()
+    s2[3] = float("nan")
+    b = latent.int8_scores(q, s2, p, t)
+    assert torch.isnan(b[3]).all() and torch.equal(b[4:], a[4:])
+
+
+def test_replayed(gpu):
+    torch = _torch()
+    from blp import latent
+
+    x = torch.randn(33, 100, device="cuda")
+    p, t = latent.quantize_rows(torch.randn(700, 100, device="cuda"))
+    latent.int8_scores(*latent.quantize_rows(x), p, t)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = latent.int8_scores(*latent.quantize_rows(x), p, t)
+    for _ in range(4):
+        x.copy_(torch.randn(33, 100, device="cuda"))
+        graph.replay()
+        assert torch.equal(out, latent.int8_scores(*latent.quantize_rows(x), p, t))
+
+
+def test_refusals(gpu):
+    torch = _torch()
+    from blp import latent
+
+    q, s = latent.quantize_rows(torch.randn(4, 32, device="cuda"))
+    for bad in (lambda: latent.quantize_rows(q), lambda: latent.quantize_rows(torch.randn(4, 8)),
+                lambda: latent.quantize_rows(torch.randn(8, 4, device="cuda").t()),
+                lambda: latent.int8_scores(q.float(), s, q, s), lambda: latent.int8_scores(q, s[:2], q, s),
+                lambda: latent.int8_scores(q, s, q[:, :16], s), lambda: latent.int8_scores(q, s.double(), q, s),
+                lambda: latent.int8_scores(q, s, q, s, dtype=torch.float64), lambda: latent.int8_scores(q, s, q[:0], s[:0])):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_training_step_then_scores(gpu):
+    """As they are used together: the users' rows looked up, the softmax loss over the businesses, both tables'
+    gradients, a step down them, then the 8-bit scores of the trained tables."""
+    torch = _torch()
+    from blp import latent
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    users = (torch.randn(500, 64, device="cuda", generator=g) * 0.1).requires_grad_(True)
+    businesses = (torch.randn(900, 64, device="cuda", generator=g) * 0.1).requires_grad_(True)
+    ids = torch.randint(0, 500, (300,), device="cuda", generator=g)
+    ids[::10] = -1
+    target = torch.randint(0, 900, (300,), device="cuda", generator=g)
+    target[::10] = -1
+    loss = latent.softmax_loss(latent.lookup(users, ids, 8.0), businesses, target)
+    du, db = torch.autograd.grad(loss, (users, businesses))
+    U, B = users.detach().double().requires_grad_(True), businesses.detach().double().requires_grad_(True)
+    keep = ids >= 0
+    z = (8.0 * U[ids[keep]]) @ B.t()
+    want = torch.nn.functional.cross_entropy(z, target[keep])
+    dU, dB = torch.autograd.grad(want, (U, B))
+    loss, want = loss.detach(), want.detach()
+    # 32-bit sums of 64 and 900 products of values below 1, relative to the gradients' size
+    assert abs(float(loss) - float(want)) < 2e-6 * float(want)
+    for got, ref in ((du, dU), (db, dB)):
+        assert float((got.double() - ref).abs().max()) < 1e-5 * float(ref.abs().max())
+    with torch.no_grad():
+        users -= 50.0 * du
+        businesses -= 50.0 * db
+        q, s = latent.quantize_rows(latent.lookup(users, ids.clamp(min=0)))
+        p, t = latent.quantize_rows(businesses)
+        got = latent.int8_scores(q, s, p, t)
+        full = users[ids.clamp(min=0)].double() @ businesses.double().t()
+        # each factor is off by half a scale: sum (|x| t / 2 + |w| s / 2 + s t / 4)
+        x, w = users[ids.clamp(min=0)].double().abs().sum(1), businesses.double().abs().sum(1)
+        bound = 0.5 * x[:, None] * t.double() + 0.5 * s.double()[:, None] * w + 16.0 * s.double()[:, None] * t.double()
+        assert bool(((got.double() - full).abs() <= bound * 1.0001).all())
