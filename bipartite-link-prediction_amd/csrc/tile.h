@@ -143,33 +143,40 @@ __device__ inline void load_stage(lds_char* lds, const Operand& o, int64_t r0, i
   }
 }
 
-// The fragment of rows [row, row + 16) and k granule `g` = 4 kk + lane / 16 of a stage in LDS.
+// Where this lane's part of fragment 0 of a stage lies (bytes). The others differ by constants and by an
+// exclusive or with the fragment's number, so one register a stage addresses them all.
 template <int T, int LAYOUT, int R>
-__device__ inline frag_t read_frag(const lds_char* lds, int row, int kk) {
+__device__ inline uint32_t lane_base() {
   const int lane = threadIdx.x & 63, i = lane & 15, h = lane >> 4;
   if constexpr (LAYOUT == ROW) {
-    const int r = row + i, c = (kk * 4 + h) ^ (i & 7);  // row is a multiple of 16
-    return *(const __attribute__((address_space(3))) frag_t*)(lds + r * STAGE + c * 16);
+    return i * STAGE + (h ^ (i & 7)) * 16;
   } else if constexpr (T == F32) {
-    constexpr int GR = R / 4;
+    const int k = h * 4;
+    return k * R * 4 + ((i >> 2) ^ (col_swz<T>(k) & (R / 4 - 1))) * 16 + (i & 3) * 4;
+  } else {
+    const int k = h * 8 + (i >> 2);
+    return k * R * 2 + (((i & 3) >> 1) ^ (col_swz<T>(k) & (R / 8 - 1))) * 16 + (i & 1) * 8;
+  }
+}
+
+// Fragment f (rows 16 f ..) of the half stage kk: granules 4 kk + lane / 16 of k.
+template <int T, int LAYOUT, int R>
+__device__ inline frag_t read_frag(const lds_char* lds, uint32_t base, int f, int kk) {
+  if constexpr (LAYOUT == ROW) {
+    return *(const __attribute__((address_space(3))) frag_t*)(lds + (base ^ (kk * 64)) + f * 16 * STAGE);
+  } else if constexpr (T == F32) {
+    const lds_char* at = lds + (base ^ (f << 6)) + kk * 16 * R * 4;
     f32x4 v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int k = (kk * 4 + h) * 4 + j;
-      const int c = ((row + i) >> 2) ^ (col_swz<T>(k) & (GR - 1));
-      v[j] = *(const __attribute__((address_space(3))) float*)(lds + k * R * 4 + c * 16 + (i & 3) * 4);
-    }
+    for (int j = 0; j < 4; ++j) v[j] = *(const __attribute__((address_space(3))) float*)(at + j * R * 4);
     return __builtin_bit_cast(frag_t, v);
   } else {
     static_assert(T == BF16 || T == F16, "column layout: halves and floats");
-    constexpr int GR = R / 8;
+    const lds_char* at = lds + (base ^ (f << 5)) + kk * 32 * R * 2;
     i32x4 v;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int k = (kk * 4 + h) * 8 + s * 4 + (i >> 2);
-      const int c = ((row >> 3) + ((i & 3) >> 1)) ^ (col_swz<T>(k) & (GR - 1));
-      const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4*)(lds + k * R * 2 + c * 16 + (i & 1) * 8));
+      const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + s * 4 * R * 2));
       const i32x2 w = __builtin_bit_cast(i32x2, t);
       v[2 * s] = w[0];
       v[2 * s + 1] = w[1];
@@ -179,15 +186,17 @@ __device__ inline frag_t read_frag(const lds_char* lds, int row, int kk) {
 }
 
 template <int T, int LP, int LQ, class S>
-__device__ inline void mul_stage(const lds_char* lp, const lds_char* lq, int wp, int wq,
+__device__ inline void mul_stage(const lds_char* lp, const lds_char* lq, uint32_t bp, uint32_t bq, int wp, int wq,
                                  typename Acc<T>::type (&acc)[S::FP][S::FQ]) {
+  // the addresses are made anew each stage: kept across the loop they would cost the accumulators their registers
+  asm volatile("" : "+v"(bp), "+v"(bq));
 #pragma unroll
   for (int kk = 0; kk < 2; ++kk) {
     frag_t p[S::FP], q[S::FQ];
 #pragma unroll
-    for (int i = 0; i < S::FP; ++i) p[i] = read_frag<T, LP, S::BP>(lp, (wp * S::FP + i) * 16, kk);
+    for (int j = 0; j < S::FQ; ++j) q[j] = read_frag<T, LQ, S::BQ>(lq, bq, wq * S::FQ + j, kk);
 #pragma unroll
-    for (int j = 0; j < S::FQ; ++j) q[j] = read_frag<T, LQ, S::BQ>(lq, (wq * S::FQ + j) * 16, kk);
+    for (int i = 0; i < S::FP; ++i) p[i] = read_frag<T, LP, S::BP>(lp, bp, wp * S::FP + i, kk);
 #pragma unroll
     for (int i = 0; i < S::FP; ++i)
 #pragma unroll
@@ -235,26 +244,29 @@ __global__ __launch_bounds__(S::THREADS) void k_product(Problem a, Epi epi) {
   for (int i = 0; i < S::FP; ++i)
 #pragma unroll
     for (int j = 0; j < S::FQ; ++j) acc[i][j] = 0;
+  const uint32_t bp = lane_base<T, LP, S::BP>(), bq = lane_base<T, LQ, S::BQ>();
   const int stages = ke > kb ? (int)((ke - kb + KE - 1) / KE) : 0;
   lds_char *lp0 = (lds_char*)s_p0, *lq0 = (lds_char*)s_q0, *lp1 = (lds_char*)s_p1, *lq1 = (lds_char*)s_q1;
   if (stages > 0) {
     load_stage<T, LP, S::BP, S::WAVES>(lp0, a.p, p0, kb, ke);
     load_stage<T, LQ, S::BQ, S::WAVES>(lq0, a.q, q0, kb, ke);
   }
-  for (int t = 0; t < stages; t += 2) {
+  int t = 0;
+  for (; t + 2 <= stages; t += 2) {
     stage_barrier();
-    if (t + 1 < stages) {
-      load_stage<T, LP, S::BP, S::WAVES>(lp1, a.p, p0, kb + (int64_t)(t + 1) * KE, ke);
-      load_stage<T, LQ, S::BQ, S::WAVES>(lq1, a.q, q0, kb + (int64_t)(t + 1) * KE, ke);
-    }
-    mul_stage<T, LP, LQ, S>(lp0, lq0, wp, wq, acc);
-    if (t + 1 >= stages) break;
+    load_stage<T, LP, S::BP, S::WAVES>(lp1, a.p, p0, kb + (int64_t)(t + 1) * KE, ke);
+    load_stage<T, LQ, S::BQ, S::WAVES>(lq1, a.q, q0, kb + (int64_t)(t + 1) * KE, ke);
+    mul_stage<T, LP, LQ, S>(lp0, lq0, bp, bq, wp, wq, acc);
     stage_barrier();
     if (t + 2 < stages) {
       load_stage<T, LP, S::BP, S::WAVES>(lp0, a.p, p0, kb + (int64_t)(t + 2) * KE, ke);
       load_stage<T, LQ, S::BQ, S::WAVES>(lq0, a.q, q0, kb + (int64_t)(t + 2) * KE, ke);
     }
-    mul_stage<T, LP, LQ, S>(lp1, lq1, wp, wq, acc);
+    mul_stage<T, LP, LQ, S>(lp1, lq1, bp, bq, wp, wq, acc);
+  }
+  if (t < stages) {
+    stage_barrier();
+    mul_stage<T, LP, LQ, S>(lp0, lq0, bp, bq, wp, wq, acc);
   }
   epi.template run<S>(acc, p0 + wp * S::FP * 16, q0 + wq * S::FQ * 16, tp * S::WP + wp);
 }
