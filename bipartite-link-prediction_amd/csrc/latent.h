@@ -33,4 +33,15 @@ struct Ids {
   }
 };
 
+// n / d for n < 2^31 by a multiplication (d >= 1): with s = ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1,
+// the quotient is (n + floor(m n / 2^32)) >> s. A vector unit has no integer division.
+struct FastDiv {
+  uint32_t d, m, s;
+  __host__ explicit FastDiv(uint32_t by) : d(by), s(0) {
+    while ((1ull << s) < by) ++s;
+    m = (uint32_t)((((1ull << s) - by) << 32) / by + 1);
+  }
+  __device__ uint32_t operator()(uint32_t n) const { return (n + __umulhi(m, n)) >> s; }
+};
+
 }  // namespace blp

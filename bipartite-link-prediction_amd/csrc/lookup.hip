@@ -3,10 +3,10 @@
 //   y_i = scale table[id_i] (an id outside the table: zeros)      dT_r = scale sum_{i : id_i = r} dy_i
 //
 // The gradient is a sum over each row's positions in ascending order, with no float atomics: the ids are
-// sorted (stable, with their positions), chunks of CHUNK sorted entries are summed by one group of lanes
-// each, a row's sum that lies inside a chunk is written at once and one that crosses chunks is left as
-// partial sums, which a second kernel adds up in the chunks' order. Everything is read once and the result
-// does not depend on timing. Bound by the reads of dy (one row per id) and the writes of dT.
+// sorted (stable, with their positions), chunks of sorted entries are summed by one group of lanes each, a
+// row's sum that lies inside a chunk is written at once and one that crosses chunks is left as partial
+// sums, which a second kernel adds up in the chunks' order. Every row of dy is read once, every row of dT
+// written once, and the result does not depend on timing.
 #include <algorithm>
 
 #include "blp_internal.h"
@@ -16,6 +16,7 @@ namespace {
 
 using namespace blp::tile;
 using blp::DeviceGuard;
+using blp::FastDiv;
 using blp::Ids;
 
 // ---------------------------------------------------------------- vectors of a row
@@ -81,64 +82,44 @@ __device__ inline void store_vec(char* at, int left, const Vec<T>& r) {
 }
 
 // ---------------------------------------------------------------- lookup
-// One vector a thread, four rows in flight.
+// One vector a thread, four in flight. `n` rows with n * per < 2^31 (the host takes longer lists in parts).
 template <int T>
-__global__ __launch_bounds__(256) void k_lookup(const char* __restrict__ table, int64_t ld, Ids ids, int64_t n, int k,
-                                                float scale, char* __restrict__ out, int64_t ldo) {
+__global__ __launch_bounds__(256) void k_lookup(const char* __restrict__ table, int64_t ld, Ids ids, int64_t i0, uint32_t n,
+                                                int k, FastDiv per, float scale, char* __restrict__ out, int64_t ldo) {
   constexpr int NE = Vec<T>::NE, U = 4;
-  const int per = (k + NE - 1) / NE;
-  const int64_t total = n * per, step = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t i0 = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i0 < total; i0 += step * U) {
+  const uint32_t total = n * per.d, step = gridDim.x * blockDim.x;
+  for (uint32_t at = blockIdx.x * blockDim.x + threadIdx.x; at < total; at += step * U) {
     Vec<T> v[U];
-    int64_t row[U];
-    int e0[U];
+    int64_t id[U];
+    uint32_t row[U], e0[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t i = i0 + u * step;
-      row[u] = i < total ? i / per : -1;
-      e0[u] = i < total ? (int)(i - row[u] * per) * NE : 0;
-      const int64_t id = row[u] >= 0 ? ids(row[u]) : -1;
+      const uint32_t i = at + u * step;
+      row[u] = per(min(i, total - 1));
+      e0[u] = (min(i, total - 1) - row[u] * per.d) * NE;
+      id[u] = ids(i0 + row[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
       v[u] = Vec<T>{};
-      if (id >= 0) v[u] = load_vec<T>(table + id * ld + (int64_t)e0[u] * size_of(T), k - e0[u]);
+      if (id[u] >= 0) v[u] = load_vec<T>(table + id[u] * ld + (int64_t)e0[u] * size_of(T), k - (int)e0[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (row[u] >= 0) {
+      if (at + u * step < total) {
 #pragma unroll
         for (int j = 0; j < NE / 4; ++j) v[u].v[j] *= scale;
-        store_vec<T>(out + row[u] * ldo + (int64_t)e0[u] * size_of(T), k - e0[u], v[u]);
+        store_vec<T>(out + (i0 + row[u]) * ldo + (int64_t)e0[u] * size_of(T), k - (int)e0[u], v[u]);
       }
   }
 }
 
 // ---------------------------------------------------------------- sort
 // Stable radix sort of (id, position), least significant digit first, BITS bits a pass. A block takes
-// SORT_N consecutive entries; wave w of it the w-th quarter, 64 at a time in order. The entries of one
+// 256 ROUNDS consecutive entries; wave w of it the w-th quarter, 64 at a time in order. The entries of one
 // digit are found with ballots (a lane's rank among them by counting the lanes below), so ranks follow
 // positions; ids outside the table get the largest key and end up last.
-constexpr int BITS = 10, BINS = 1 << BITS, SORT_WAVES = 4, SORT_ROUNDS = 8;
-constexpr int SORT_N = SORT_WAVES * SORT_ROUNDS * 64;
-
-// counts[digit * blocks + block]; with `zero`, also clears the gradient (16 bytes a thread).
-struct Clear {
-  char* out;
-  int64_t ld, rows;  // bytes
-  int row_bytes;
-  __device__ void run(int64_t at, int64_t step) const {
-    if (!out) return;
-    const int per = (row_bytes + 15) / 16;
-    for (int64_t i = at; i < rows * per; i += step) {
-      const int64_t r = i / per;
-      const int b = (int)(i - r * per) * 16;
-      char* p = out + r * ld + b;
-      if (b + 16 <= row_bytes) {
-        reinterpret_cast<Raw16*>(p)->v = i32x4{0, 0, 0, 0};
-      } else {
-        for (int j = 0; j < row_bytes - b; j += 2) *reinterpret_cast<uint16_t*>(p + j) = 0;
-      }
-    }
-  }
-};
+constexpr int BITS = 10, BINS = 1 << BITS, SORT_WAVES = 4;
 
 __device__ inline uint32_t key_at(const Ids& ids, const uint32_t* keys, int64_t i) {
   if (keys) return keys[i];
@@ -146,38 +127,45 @@ __device__ inline uint32_t key_at(const Ids& ids, const uint32_t* keys, int64_t 
   return id >= 0 ? (uint32_t)id : (uint32_t)ids.rows;
 }
 
+// counts[block][digit]
+template <int ROUNDS>
 __global__ __launch_bounds__(256) void k_digit_counts(Ids ids, const uint32_t* __restrict__ keys, int64_t n, int shift,
-                                                      uint32_t* __restrict__ counts, Clear clear) {
+                                                      uint32_t* __restrict__ counts) {
   __shared__ uint32_t s_count[BINS];
   for (int i = threadIdx.x; i < BINS; i += 256) s_count[i] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * SORT_N;
-  for (int r = 0; r < SORT_N / 256; ++r) {
+  const int64_t base = (int64_t)blockIdx.x * (256 * ROUNDS);
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
     const int64_t i = base + r * 256 + threadIdx.x;
     if (i < n) atomicAdd(&s_count[(key_at(ids, keys, i) >> shift) & (BINS - 1)], 1u);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < BINS; i += 256) counts[(int64_t)i * gridDim.x + blockIdx.x] = s_count[i];
-  clear.run(blockIdx.x * 256ll + threadIdx.x, gridDim.x * 256ll);
+  for (int i = threadIdx.x; i < BINS; i += 256) counts[(int64_t)blockIdx.x * BINS + i] = s_count[i];
 }
 
-// One wave a digit: its counts become the exclusive sums over the blocks; total[digit].
-__global__ __launch_bounds__(64) void k_digit_sums(uint32_t* __restrict__ counts, int blocks, uint32_t* __restrict__ total) {
+// 64 digits a block, 16 waves over the blocks' rows: counts become exclusive sums over the blocks; total[digit].
+__global__ __launch_bounds__(1024) void k_digit_sums(uint32_t* __restrict__ counts, int blocks, uint32_t* __restrict__ total) {
+  __shared__ uint32_t s_sum[16][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, d = blockIdx.x * 64 + lane;
+  const int per = (blocks + 15) / 16, b0 = min(blocks, w * per), b1 = min(blocks, b0 + per);
+  uint32_t sum = 0;
+#pragma unroll 8
+  for (int b = b0; b < b1; ++b) sum += counts[(int64_t)b * BINS + d];
+  s_sum[w][lane] = sum;
+  __syncthreads();
   uint32_t run = 0;
-  for (int b0 = 0; b0 < blocks; b0 += 64) {
-    const int b = b0 + threadIdx.x;
-    const uint32_t c = b < blocks ? counts[(int64_t)blockIdx.x * blocks + b] : 0;
-    uint32_t s = c;
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t t = __shfl_up(s, o, 64);
-      if ((int)threadIdx.x >= o) s += t;
-    }
-    if (b < blocks) counts[(int64_t)blockIdx.x * blocks + b] = run + s - c;
-    run += __shfl(s, 63, 64);
+  for (int i = 0; i < w; ++i) run += s_sum[i][lane];
+  if (w == 15) total[d] = run + sum;
+#pragma unroll 8
+  for (int b = b0; b < b1; ++b) {
+    const uint32_t c = counts[(int64_t)b * BINS + d];
+    counts[(int64_t)b * BINS + d] = run;
+    run += c;
   }
-  if (threadIdx.x == 0) total[blockIdx.x] = run;
 }
 
+template <int ROUNDS>
 __global__ __launch_bounds__(256) void k_scatter(Ids ids, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
                                                  int64_t n, int shift, const uint32_t* __restrict__ counts,
                                                  const uint32_t* __restrict__ total, uint32_t* __restrict__ keys_out,
@@ -186,7 +174,15 @@ __global__ __launch_bounds__(256) void k_scatter(Ids ids, const uint32_t* __rest
   __shared__ uint16_t s_wave[SORT_WAVES][BINS];
   __shared__ uint32_t s_sum[SORT_WAVES];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  for (int i = threadIdx.x; i < SORT_WAVES * BINS; i += 256) (&s_wave[0][0])[i] = 0;
+  const int64_t base = (int64_t)blockIdx.x * (256 * ROUNDS) + w * (64 * ROUNDS);
+  uint32_t key[ROUNDS], at[ROUNDS];
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const int64_t i = min(base + r * 64 + lane, n - 1);
+    key[r] = key_at(ids, keys, i);
+    at[r] = pos ? pos[i] : (uint32_t)i;
+  }
+  for (int i = threadIdx.x; i < SORT_WAVES * BINS / 2; i += 256) reinterpret_cast<uint32_t*>(&s_wave[0][0])[i] = 0;
   // where each digit starts: exclusive sums of the totals, four digits a thread
   uint32_t c[BINS / 256], sum = 0;
 #pragma unroll
@@ -206,17 +202,13 @@ __global__ __launch_bounds__(256) void k_scatter(Ids ids, const uint32_t* __rest
 #pragma unroll
   for (int j = 0; j < BINS / 256; ++j) {
     const int d = threadIdx.x * (BINS / 256) + j;
-    s_base[d] = before + c[j] + counts[(int64_t)d * gridDim.x + blockIdx.x];
+    s_base[d] = before + c[j] + counts[(int64_t)blockIdx.x * BINS + d];
   }
   // ranks within the wave
-  const int64_t base = (int64_t)blockIdx.x * SORT_N + w * (SORT_ROUNDS * 64);
-  uint32_t key[SORT_ROUNDS];
-  uint16_t rank[SORT_ROUNDS];
+  uint16_t rank[ROUNDS];
 #pragma unroll
-  for (int r = 0; r < SORT_ROUNDS; ++r) {
-    const int64_t i = base + r * 64 + lane;
-    const bool in = i < n;
-    key[r] = in ? key_at(ids, keys, i) : 0;
+  for (int r = 0; r < ROUNDS; ++r) {
+    const bool in = base + r * 64 + lane < n;
     const uint32_t d = (key[r] >> shift) & (BINS - 1);
     unsigned long long same = __ballot(in);
 #pragma unroll
@@ -245,25 +237,20 @@ __global__ __launch_bounds__(256) void k_scatter(Ids ids, const uint32_t* __rest
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < SORT_ROUNDS; ++r) {
-    const int64_t i = base + r * 64 + lane;
-    if (i < n) {
+  for (int r = 0; r < ROUNDS; ++r) {
+    if (base + r * 64 + lane < n) {
       const uint32_t d = (key[r] >> shift) & (BINS - 1);
-      const uint32_t at = s_base[d] + s_wave[w][d] + rank[r];
-      keys_out[at] = key[r];
-      pos_out[at] = pos ? pos[i] : (uint32_t)i;
+      const uint32_t to = s_base[d] + s_wave[w][d] + rank[r];
+      keys_out[to] = key[r];
+      pos_out[to] = at[r];
     }
   }
 }
 
-// Up to SMALL entries: one block, a bitonic sort of (id, position) pairs in LDS. The other blocks clear.
+// Up to SMALL entries: one block, a bitonic sort of (id, position) pairs in LDS.
 constexpr int SMALL = 2048;
 __global__ __launch_bounds__(1024) void k_sort_small(Ids ids, int n, uint32_t* __restrict__ keys_out,
-                                                     uint32_t* __restrict__ pos_out, Clear clear) {
-  if (blockIdx.x > 0) {
-    clear.run((blockIdx.x - 1) * 1024ll + threadIdx.x, (gridDim.x - 1) * 1024ll);
-    return;
-  }
+                                                     uint32_t* __restrict__ pos_out) {
   __shared__ unsigned long long s_v[SMALL];
   int size = 64;
   while (size < n) size <<= 1;
@@ -289,7 +276,7 @@ __global__ __launch_bounds__(1024) void k_sort_small(Ids ids, int n, uint32_t* _
 }
 
 // ---------------------------------------------------------------- sums
-constexpr int CHUNK = 64;  // sorted entries a group of lanes adds up
+constexpr int HEAVY = 32;  // chunks: a row that crosses more of them is added up by a whole block
 
 template <int T>
 __device__ inline void put(char* out, int64_t ldo, uint32_t key, int e0, int k, const Vec<T>& sum, float scale, int add) {
@@ -314,103 +301,189 @@ __device__ inline void put_part(float* part, int64_t slot, int64_t kv, int vec, 
   for (int j = 0; j < Vec<T>::NE / 4; ++j) at[j] = sum.v[j];
 }
 
-// `lanes` (a power of two up to 64) lanes a chunk, blockIdx.y the column tile of lanes * NE elements.
+struct Sums {
+  const uint32_t *keys, *pos;
+  int64_t n, chunk, chunks;  // entries, entries a chunk
+  uint32_t rows;
+  int k, lanes;              // lanes of a chunk: a power of two up to 64; blockIdx.y: their column tile
+  float scale;
+  char* out;
+  int64_t ldo;
+  int add;
+  float* part;
+  int64_t kv;  // floats of a partial sum
+};
+
+// The blocks past `sum_blocks` clear the rows without ids: 64 rows a wave, each lane looks its row up in the
+// sorted ids.
 template <int T>
-__global__ __launch_bounds__(256) void k_chunk_sums(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos, int64_t n,
-                                                    uint32_t rows, const char* __restrict__ dy, int64_t ld, int k, int lanes,
-                                                    float scale, char* __restrict__ out, int64_t ldo, int add,
-                                                    float* __restrict__ part, int64_t kv) {
-  constexpr int NE = Vec<T>::NE, U = 4;
-  const int64_t chunk = (blockIdx.x * 256ll + threadIdx.x) / lanes;
-  const int vec = blockIdx.y * lanes + (threadIdx.x & (lanes - 1)), e0 = vec * NE;
-  const int64_t b = chunk * CHUNK, e = min(n, b + CHUNK);
-  if (b >= n || e0 >= k) return;
+__device__ void clear_rows(const Sums& a, int64_t wave) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = wave * 64 + lane;
+  bool absent = false;
+  if (r < a.rows) {
+    int64_t lo = 0, hi = a.n;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (a.keys[mid] < (uint32_t)r)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    absent = lo == a.n || a.keys[lo] != (uint32_t)r;
+  }
+  unsigned long long left = __ballot(absent);
+  const int vecs = (a.k + Vec<T>::NE - 1) / Vec<T>::NE;
+  // short rows: several at a time
+  const int each = a.lanes, groups = 64 / each, g = lane / each, l = lane & (each - 1);
+  while (left) {
+    unsigned long long mine = left;
+    for (int i = 0; i < g && mine; ++i) mine &= mine - 1;
+    if (mine) {
+      char* at = a.out + (wave * 64 + __builtin_ctzll(mine)) * a.ldo;
+      for (int v = l; v < vecs; v += each)
+        store_vec<T>(at + (int64_t)v * 16, a.k - v * Vec<T>::NE, Vec<T>{});
+    }
+    for (int i = 0; i < groups && left; ++i) left &= left - 1;
+  }
+}
+
+template <int T>
+__global__ __launch_bounds__(256) void k_chunk_sums(Sums a, const char* __restrict__ dy, int64_t ld, unsigned sum_blocks) {
+  constexpr int NE = Vec<T>::NE, U = 8;
+  if (blockIdx.x >= sum_blocks) {
+    if (blockIdx.y == 0) clear_rows<T>(a, (blockIdx.x - sum_blocks) * 4ll + (threadIdx.x >> 6));
+    return;
+  }
+  const int64_t chunk = (blockIdx.x * 256ll + threadIdx.x) / a.lanes;
+  const int vec = blockIdx.y * a.lanes + (threadIdx.x & (a.lanes - 1)), e0 = vec * NE, k = a.k;
+  const int64_t b = chunk * a.chunk, e = min(a.n, b + a.chunk);
+  const uint32_t rows = a.rows;
+  if (b >= a.n || e0 >= k) return;
   const char* src = dy + (int64_t)e0 * size_of(T);
-  uint32_t cur = keys[b];
-  bool head = b > 0 && keys[b - 1] == cur;  // the running row began in an earlier chunk
+  uint32_t cur = a.keys[b];
+  bool head = b > 0 && a.keys[b - 1] == cur;  // the running row began in an earlier chunk
   Vec<T> sum{};
   for (int64_t i = b; i < e; i += U) {
-    uint32_t key[U];
+    uint32_t key[U], pos[U];
     Vec<T> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      key[u] = i + u < e ? keys[i + u] : rows;
+      key[u] = i + u < e ? a.keys[i + u] : rows;
+      pos[u] = i + u < e ? a.pos[i + u] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
       v[u] = Vec<T>{};
-      if (key[u] < rows) v[u] = load_vec<T>(src + (int64_t)pos[i + u] * ld, k - e0);
+      if (key[u] < rows) v[u] = load_vec<T>(src + (int64_t)pos[u] * ld, k - e0);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (i + u < e && key[u] != cur) {  // `cur` ended before this entry
         if (cur < rows) {
           if (head)
-            put_part<T>(part, 2 * chunk, kv, vec, sum);
+            put_part<T>(a.part, 2 * chunk, a.kv, vec, sum);
           else
-            put<T>(out, ldo, cur, e0, k, sum, scale, add);
+            put<T>(a.out, a.ldo, cur, e0, k, sum, a.scale, a.add);
         }
         head = false;
         cur = key[u];
         sum = Vec<T>{};
       }
-      if (i + u < e)
 #pragma unroll
-        for (int j = 0; j < NE / 4; ++j) sum.v[j] += v[u].v[j];
+      for (int j = 0; j < NE / 4; ++j) sum.v[j] += v[u].v[j];
     }
   }
   if (cur >= rows) return;
-  const bool goes_on = e < n && keys[e] == cur;
+  const bool goes_on = e < a.n && a.keys[e] == cur;
   if (head)
-    put_part<T>(part, 2 * chunk, kv, vec, sum);
+    put_part<T>(a.part, 2 * chunk, a.kv, vec, sum);
   else if (goes_on)
-    put_part<T>(part, 2 * chunk + 1, kv, vec, sum);
+    put_part<T>(a.part, 2 * chunk + 1, a.kv, vec, sum);
   else
-    put<T>(out, ldo, cur, e0, k, sum, scale, add);
+    put<T>(a.out, a.ldo, cur, e0, k, sum, a.scale, a.add);
 }
 
-// The rows that cross chunks: the block of the chunk in which such a row begins adds its partial sums, one
-// group of lanes every (256 / lanes)-th of them in 64 bits, then the groups' in order.
+// Whether a row begins in `chunk` and goes on in the next; its key. (A chunk's last row, so at most one.)
+__device__ inline bool crosses(const Sums& a, int64_t chunk, uint32_t* key) {
+  const int64_t b = chunk * a.chunk, e = b + a.chunk;
+  if (e >= a.n) return false;
+  *key = a.keys[e - 1];
+  if (*key >= a.rows || a.keys[e] != *key) return false;
+  return !(b > 0 && a.keys[b] == *key && a.keys[b - 1] == *key);
+}
+__device__ inline bool heavy(const Sums& a, int64_t chunk, uint32_t key) {
+  const int64_t far = (chunk + HEAVY + 1) * a.chunk;
+  return far < a.n && a.keys[far] == key;
+}
+
+// The rows that cross chunks. The first blocks: a group of lanes a chunk, the partial sums of the row that
+// begins there in the chunks' order. The others: HEAVY chunks each, in which one heavy row can begin; its
+// partial sums go to the groups in turn, then the groups' sums are added in order. In 64 bits.
 template <int T>
-__global__ __launch_bounds__(256) void k_join_chunks(const uint32_t* __restrict__ keys, int64_t n, uint32_t rows, int k, int lanes,
-                                                     float scale, char* __restrict__ out, int64_t ldo, int add,
-                                                     const float* __restrict__ part, int64_t kv) {
+__global__ __launch_bounds__(256) void k_join_chunks(Sums a, unsigned light_blocks) {
   constexpr int NE = Vec<T>::NE;
   __shared__ double s_sum[256 * NE];
-  const int64_t chunk = blockIdx.x, e = (chunk + 1) * CHUNK;
-  if (e >= n) return;
-  const uint32_t key = keys[e - 1];
-  if (key >= rows || keys[e] != key) return;
-  if (chunk * CHUNK > 0 && keys[chunk * CHUNK] == key && keys[chunk * CHUNK - 1] == key) return;  // began earlier
-  // the last chunk with this row: a search for the first entry behind it
-  int64_t lo = e, hi = n;
+  __shared__ int s_at;
+  const int groups = 256 / a.lanes, g = threadIdx.x / a.lanes, l = threadIdx.x & (a.lanes - 1);
+  const int vec = blockIdx.y * a.lanes + l, e0 = vec * NE;
+  double sum[NE];
+#pragma unroll
+  for (int j = 0; j < NE; ++j) sum[j] = 0.0;
+  uint32_t key;
+  if (blockIdx.x < light_blocks) {
+    const int64_t chunk = (int64_t)blockIdx.x * groups + g;
+    if (chunk >= a.chunks || e0 >= a.k || !crosses(a, chunk, &key) || heavy(a, chunk, key)) return;
+    int64_t c = chunk;
+    do {
+      const f32x4* at = reinterpret_cast<const f32x4*>(a.part + (2 * c + (c == chunk ? 1 : 0)) * a.kv + (int64_t)e0);
+#pragma unroll
+      for (int j = 0; j < NE; ++j) sum[j] += (double)at[j >> 2][j & 3];
+      ++c;
+    } while (c * a.chunk < a.n && a.keys[c * a.chunk] == key);
+    Vec<T> r;
+#pragma unroll
+    for (int j = 0; j < NE; ++j) r.v[j >> 2][j & 3] = (float)sum[j];
+    put<T>(a.out, a.ldo, key, e0, a.k, r, a.scale, a.add);
+    return;
+  }
+  if (threadIdx.x == 0) s_at = -1;
+  __syncthreads();
+  const int64_t first = (blockIdx.x - light_blocks) * (int64_t)HEAVY;
+  if (threadIdx.x < HEAVY && first + threadIdx.x < a.chunks && crosses(a, first + threadIdx.x, &key) &&
+      heavy(a, first + threadIdx.x, key))
+    s_at = threadIdx.x;
+  __syncthreads();
+  if (s_at < 0) return;
+  const int64_t chunk = first + s_at;
+  key = a.keys[(chunk + 1) * a.chunk - 1];
+  int64_t lo = chunk + 1, hi = a.chunks;  // the first chunk that does not begin with the row
   while (lo < hi) {
     const int64_t mid = (lo + hi) >> 1;
-    if (keys[mid] == key)
+    if (a.keys[mid * a.chunk] == key)
       lo = mid + 1;
     else
       hi = mid;
   }
-  const int64_t last = (lo - 1) / CHUNK;
-  const int groups = 256 / lanes, g = threadIdx.x / lanes, l = threadIdx.x & (lanes - 1);
-  const int vec = blockIdx.y * lanes + l, e0 = vec * NE;
-  double sum[NE];
-#pragma unroll
-  for (int j = 0; j < NE; ++j) sum[j] = 0.0;
-  if (e0 < k)
-    for (int64_t c = chunk + g; c <= last; c += groups) {
-      const f32x4* at = reinterpret_cast<const f32x4*>(part + (2 * c + (c == chunk ? 1 : 0)) * kv + (int64_t)e0);
+  if (e0 < a.k) {
+#pragma unroll 4
+    for (int64_t c = chunk + g; c < lo; c += groups) {
+      const f32x4* at = reinterpret_cast<const f32x4*>(a.part + (2 * c + (c == chunk ? 1 : 0)) * a.kv + (int64_t)e0);
 #pragma unroll
       for (int j = 0; j < NE; ++j) sum[j] += (double)at[j >> 2][j & 3];
     }
+  }
 #pragma unroll
   for (int j = 0; j < NE; ++j) s_sum[j * 256 + threadIdx.x] = sum[j];
   __syncthreads();
-  if (g == 0 && e0 < k) {
+  if (g == 0 && e0 < a.k) {
     Vec<T> r;
 #pragma unroll
     for (int j = 0; j < NE; ++j) {
-      for (int i = 1; i < groups; ++i) sum[j] += s_sum[j * 256 + i * lanes + l];
+      for (int i = 1; i < groups; ++i) sum[j] += s_sum[j * 256 + i * a.lanes + l];
       r.v[j >> 2][j & 3] = (float)sum[j];
     }
-    put<T>(out, ldo, key, e0, k, r, scale, add);
+    put<T>(a.out, a.ldo, key, e0, a.k, r, a.scale, a.add);
   }
 }
 
@@ -419,8 +492,8 @@ int64_t div_up(int64_t v, int64_t by) { return (v + by - 1) / by; }
 int64_t up(int64_t v, int64_t to) { return div_up(v, to) * to; }
 
 struct Plan {
-  int passes;
-  int64_t blocks, chunks, kv;
+  int passes, rounds, lanes, tiles;
+  int64_t blocks, chunk, chunks, kv;
   int64_t o_keys[2], o_pos[2], o_counts, o_total, o_part, bytes;
 };
 
@@ -435,8 +508,16 @@ Plan plan_of(int type, int64_t n, int64_t rows, int k) {
   int bits = 1;
   while (bits < 32 && (rows >> bits)) ++bits;
   p.passes = n <= SMALL ? 0 : (int)div_up(bits, BITS);
-  p.blocks = div_up(n, SORT_N);
-  p.chunks = div_up(n, CHUNK);
+  p.rounds = n <= 128 * 1024 ? 2 : 8;  // short lists: more blocks, each done sooner
+  p.blocks = div_up(n, 256 * p.rounds);
+  const int64_t vecs = div_up(k, 16 / size_of(type));
+  p.lanes = 1;
+  while (p.lanes < 64 && p.lanes < vecs) p.lanes <<= 1;
+  p.tiles = (int)div_up(vecs, p.lanes);
+  // chunks: long enough that partial sums stay few, short enough for 16 waves a compute unit
+  p.chunk = 64;
+  while (p.chunk > 8 && div_up(n, p.chunk) * p.lanes * p.tiles / 64 < 4096) p.chunk >>= 1;
+  p.chunks = div_up(n, p.chunk);
   p.kv = up(k, 16 / size_of(type));
   for (int i = 0; i < 2; ++i) {
     p.o_keys[i] = take(4 * n);
@@ -451,11 +532,35 @@ Plan plan_of(int type, int64_t n, int64_t rows, int k) {
 
 template <int T>
 int lookup(hipStream_t st, const void* table, int64_t ld, Ids ids, int64_t n, int k, float scale, void* out, int64_t ldo) {
-  const int64_t total = n * div_up(k, 16 / size_of(T));
-  const unsigned grid = (unsigned)std::min<int64_t>(div_up(total, 1024), 1 << 20);
-  k_lookup<T><<<std::max(grid, 1u), 256, 0, st>>>((const char*)table, ld * size_of(T), ids, n, k, scale, (char*)out,
-                                                  ldo * size_of(T));
-  BLP_HIP(hipGetLastError());
+  const FastDiv per((uint32_t)div_up(k, 16 / size_of(T)));
+  const int64_t most = 0x40000000 / per.d;
+  for (int64_t i0 = 0; i0 < n; i0 += most) {
+    const uint32_t m = (uint32_t)std::min(most, n - i0);
+    const unsigned grid = (unsigned)std::min<int64_t>(div_up((int64_t)m * per.d, 1024), 1 << 18);
+    k_lookup<T><<<grid, 256, 0, st>>>((const char*)table, ld * size_of(T), ids, i0, m, k, per, scale, (char*)out,
+                                      ldo * size_of(T));
+    BLP_HIP(hipGetLastError());
+  }
+  return 0;
+}
+
+template <int ROUNDS>
+int sort(hipStream_t st, const Plan& p, Ids ids, int64_t n, uint32_t* const* keys, uint32_t* const* pos, uint32_t* counts,
+         uint32_t* total, int* last) {
+  int cur = 0;
+  for (int s = 0; s < p.passes; ++s) {
+    const uint32_t* kin = s ? keys[cur] : nullptr;
+    const int to = s ? cur ^ 1 : 0;
+    k_digit_counts<ROUNDS><<<(unsigned)p.blocks, 256, 0, st>>>(ids, kin, n, s * BITS, counts);
+    BLP_HIP(hipGetLastError());
+    k_digit_sums<<<BINS / 64, 1024, 0, st>>>(counts, (int)p.blocks, total);
+    BLP_HIP(hipGetLastError());
+    k_scatter<ROUNDS><<<(unsigned)p.blocks, 256, 0, st>>>(ids, kin, s ? pos[cur] : nullptr, n, s * BITS, counts, total, keys[to],
+                                                          pos[to]);
+    BLP_HIP(hipGetLastError());
+    cur = to;
+  }
+  *last = cur;
   return 0;
 }
 
@@ -466,38 +571,24 @@ int lookup_grad(hipStream_t st, const Plan& p, const void* dy, int64_t ld, Ids i
   uint32_t* keys[2] = {(uint32_t*)(ws + p.o_keys[0]), (uint32_t*)(ws + p.o_keys[1])};
   uint32_t* pos[2] = {(uint32_t*)(ws + p.o_pos[0]), (uint32_t*)(ws + p.o_pos[1])};
   uint32_t *counts = (uint32_t*)(ws + p.o_counts), *total = (uint32_t*)(ws + p.o_total);
-  const Clear none = {nullptr, 0, 0, 0}, clear = {add ? nullptr : (char*)out, ldo * ES, ids.rows, k * ES};
-  int cur = 0;
+  int cur = 0, rc = 0;
   if (p.passes == 0) {
-    const int64_t words = ids.rows * div_up((int64_t)k * ES, 16);
-    const unsigned grid = 1 + (unsigned)std::min<int64_t>(add ? 1 : div_up(words, 4096), 1024);
-    k_sort_small<<<grid, 1024, 0, st>>>(ids, (int)n, keys[0], pos[0], clear);
+    if (n > 0) k_sort_small<<<1, 1024, 0, st>>>(ids, (int)n, keys[0], pos[0]);
     BLP_HIP(hipGetLastError());
+  } else {
+    rc = p.rounds == 2 ? sort<2>(st, p, ids, n, keys, pos, counts, total, &cur)
+                       : sort<8>(st, p, ids, n, keys, pos, counts, total, &cur);
+    if (rc) return rc;
   }
-  for (int s = 0; s < p.passes; ++s) {
-    const uint32_t* kin = s ? keys[cur] : nullptr;
-    const int to = s ? cur ^ 1 : 0;
-    k_digit_counts<<<(unsigned)p.blocks, 256, 0, st>>>(ids, kin, n, s * BITS, counts, s ? none : clear);
-    BLP_HIP(hipGetLastError());
-    k_digit_sums<<<BINS, 64, 0, st>>>(counts, (int)p.blocks, total);
-    BLP_HIP(hipGetLastError());
-    k_scatter<<<(unsigned)p.blocks, 256, 0, st>>>(ids, kin, s ? pos[cur] : nullptr, n, s * BITS, counts, total, keys[to], pos[to]);
-    BLP_HIP(hipGetLastError());
-    cur = to;
-  }
-  if (n == 0) return 0;
-  constexpr int NE = Vec<T>::NE;
-  const int64_t vecs = div_up(k, NE);
-  int lanes = 1;
-  while (lanes < 64 && lanes < vecs) lanes <<= 1;
-  const unsigned tiles = (unsigned)div_up(vecs, lanes);
-  float* part = (float*)(ws + p.o_part);
-  k_chunk_sums<T><<<dim3((unsigned)div_up(p.chunks * lanes, 256), tiles), 256, 0, st>>>(
-      keys[cur], pos[cur], n, (uint32_t)ids.rows, (const char*)dy, ld * ES, k, lanes, scale, (char*)out, ldo * ES, add, part, p.kv);
+  const Sums a = {keys[cur], pos[cur], n, p.chunk, p.chunks, (uint32_t)ids.rows, k, p.lanes, scale, (char*)out, ldo * ES, add,
+                  (float*)(ws + p.o_part), p.kv};
+  const unsigned sum_blocks = (unsigned)div_up(p.chunks * p.lanes, 256), clear_blocks = add ? 0 : (unsigned)div_up(ids.rows, 256);
+  if (sum_blocks + clear_blocks == 0) return 0;
+  k_chunk_sums<T><<<dim3(sum_blocks + clear_blocks, p.tiles), 256, 0, st>>>(a, (const char*)dy, ld * ES, sum_blocks);
   BLP_HIP(hipGetLastError());
   if (p.chunks > 1) {
-    k_join_chunks<T><<<dim3((unsigned)(p.chunks - 1), tiles), 256, 0, st>>>(keys[cur], n, (uint32_t)ids.rows, k, lanes, scale,
-                                                                            (char*)out, ldo * ES, add, part, p.kv);
+    const unsigned light = (unsigned)div_up(p.chunks, 256 / p.lanes), rest = (unsigned)div_up(p.chunks, HEAVY);
+    k_join_chunks<T><<<dim3(light + rest, p.tiles), 256, 0, st>>>(a, light);
     BLP_HIP(hipGetLastError());
   }
   return 0;
