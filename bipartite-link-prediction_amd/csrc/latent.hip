@@ -65,7 +65,7 @@ struct EpiLse {
   int64_t n, m;
   float scale;
   template <class S>
-  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int tile) const {
+  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int tile, int) const {
     const int lane = threadIdx.x & 63, h = lane >> 4;
     const float c = scale * LOG2E;
 #pragma unroll
@@ -215,7 +215,7 @@ struct EpiGrad {
   int64_t n, m;
   float scale;
   template <class S>
-  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int) const {
+  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int) const {
     const int lane = threadIdx.x & 63, h = lane >> 4;
     const float c = scale * LOG2E;
 #pragma unroll
@@ -251,7 +251,7 @@ struct EpiOut {
   RowGrad g;
   float scale;
   template <class S>
-  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int) const {
+  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int) const {
     const int lane = threadIdx.x & 63, h = lane >> 4;
     const float alpha = scale * g.all();
     const bool whole = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)ld) & (4 * size_of(T) - 1)) == 0;
@@ -281,9 +281,9 @@ struct EpiPart {
   int64_t ld, np, nq;  // elements; ld a multiple of 4
   int add;
   template <class S>
-  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int) const {
+  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int slice) const {
     const int lane = threadIdx.x & 63, h = lane >> 4;
-    float* base = part + (int64_t)blockIdx.y * nq * ld;
+    float* base = part + (int64_t)slice * nq * ld;
 #pragma unroll
     for (int j = 0; j < S::FQ; ++j) {
       const int64_t q = q0 + j * 16 + (lane & 15);
@@ -311,6 +311,330 @@ __global__ __launch_bounds__(256) void k_sum_parts(const float* __restrict__ par
     for (int s = 0; s < slices; ++s) v += *reinterpret_cast<const f32x4*>(part + (s * nq + q) * ld + p);
     for (int e = 0; e < 4; ++e)
       if (p + e < np) store1<T>(out + q * ldo + (p + e) * size_of(T), v[e] * alpha);
+  }
+}
+
+// ---------------------------------------------------------------- narrow factors
+// Halves with k up to 128: the scores never leave the registers, in the backward pass either. A wave holds
+// 16 FO rows of one side ("own") as fragments for the whole kernel and the other side ("stream") passes through
+// LDS, 64 rows a stage, two stages in turn:
+//   LSE  own x, stream w: a running (max, sum of exp2) a lane, joined over the lanes at the end
+//   DX   own x, stream w: dS of 32 stream rows at a time, rounded to halves in place, is the second product's
+//        operand as it lies (the matrix instruction's k order is free, so its rows of w are read from LDS,
+//        transposed, in the order in which the lanes hold dS); dx accumulates in registers
+//   DW   own w, stream x: the same with the sides changed
+// Per 64 scores a wave spends about 26 (LSE) and 22 (DX, DW) cycles in the vector unit, 16 of them in exp2, and
+// k / 8 (k / 4) in the matrix unit: exp2 is what bounds these kernels, and computing it again in DX and DW costs less
+// than writing dS once and reading it twice.
+struct Rows {  // per 64 rows of x: log2(e) lse - log2(extra) (infinite: ignored), g / max|g|, target, in blocks of 3 x 64
+  float* at;
+  __device__ float* of(int64_t block) const { return at + block * 256; }
+};
+
+__global__ __launch_bounds__(64) void k_rows(const float* __restrict__ lse, RowGrad g, Targets targets, int64_t m, Rows rows) {
+  const int64_t i = blockIdx.x * 64ll + threadIdx.x;
+  const int64_t t = i < m ? targets(i) : -1;
+  float* at = rows.of(blockIdx.x) + threadIdx.x;
+  at[0] = t >= 0 ? fmaf(lse[i], LOG2E, -__builtin_amdgcn_logf(g.extra)) : INFINITY;
+  at[64] = t >= 0 ? g.row(i) / g.extra : 0.f;
+  reinterpret_cast<int*>(at)[128] = (int)t;
+  at[192] = 0.f;
+}
+
+enum NarrowMode { LSE, DX, DW };
+
+struct NarrowArgs {
+  Operand own, stream;
+  int kp;
+  int64_t range;  // stream rows of a split, a multiple of 64
+  int own_tiles, splits;
+  float scale, extra;
+  Targets targets;  // LSE
+  float2* part;     // LSE
+  float* hit;       // LSE
+  Rows rows;        // DX, DW
+};
+
+template <int KS_, int FO_>
+struct NarrowShape {  // the second product's accumulators, for the epilogues
+  static constexpr int FP = 2 * KS_, FQ = FO_;
+};
+
+template <int T>
+__device__ inline int pack2(float a, float b) {
+  if constexpr (T == BF16) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(int, b2{(__bf16)a, (__bf16)b});
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(int, h2{(_Float16)a, (_Float16)b});
+  }
+}
+
+template <int T, int KS, int MODE, bool PER_ROW, class Epi>
+__global__ __launch_bounds__(256, 2) void k_narrow(NarrowArgs a, Epi epi) {
+  constexpr int FO = KS > 2 && MODE != LSE ? 2 : 4;  // own fragments of 16 rows a wave
+  constexpr int HALVES = KS > 2 ? 2 : 1;             // 128-byte parts of a row
+  constexpr int PART = 64 * STAGE;                   // bytes of one part of a stage
+  constexpr int BUF = HALVES * PART;
+  __shared__ __attribute__((aligned(1024))) char s_a[BUF], s_b[BUF];
+  __shared__ __attribute__((aligned(1024))) char s_ra[MODE == DW ? 1024 : 16], s_rb[MODE == DW ? 1024 : 16];
+  // a die's workgroups take neighbouring own tiles of one split: the split's rows stay in its L2
+  const int n_blocks = a.own_tiles * a.splits, per = n_blocks >> 3, more = n_blocks & 7, xcd = blockIdx.x & 7;
+  const int id = xcd * per + min(xcd, more) + (blockIdx.x >> 3);
+  const int split = id / a.own_tiles, own_tile = id - split * a.own_tiles;
+  const int lane = threadIdx.x & 63, l = lane & 15, h = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t own0 = (int64_t)own_tile * (64 * FO) + wave * (16 * FO);
+  const int64_t s0 = split * a.range, s1 = min(a.stream.rows, s0 + a.range);
+  const int stages = s1 > s0 ? (int)((s1 - s0 + 63) >> 6) : 0;
+  const float c = fmaxf(fabsf(a.scale) * LOG2E, 1.2e-38f);  // positive: -inf c is -inf for a scale of 0, too
+  const Operand stream = {a.stream.base, a.stream.ld, s1};
+
+  frag_t own[FO][KS];
+#pragma unroll
+  for (int j = 0; j < FO; ++j) {
+    const int64_t r = own0 + j * 16 + l;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      own[j][s] = frag_t{0, 0, 0, 0};
+      if (r < a.own.rows && s * 32 + h * 8 < a.kp)
+        own[j][s] = *reinterpret_cast<const frag_t*>(a.own.base + r * a.own.ld + (s * 32 + h * 8) * 2);
+      if (a.scale < 0.f) own[j][s] ^= (int)0x80008000;  // the scores' sign, so that c is positive
+    }
+  }
+  // a lane's own rows: LSE: targets; DX: lse and targets; DW: w rows (nothing)
+  int target[FO];
+  float lane_l2[FO], lane_g[FO];
+#pragma unroll
+  for (int j = 0; j < FO; ++j) {
+    const int64_t r = own0 + j * 16 + l;
+    target[j] = -1;
+    lane_l2[j] = INFINITY;
+    lane_g[j] = 0.f;
+    if constexpr (MODE == LSE) {
+      if (r < a.own.rows) target[j] = (int)a.targets(r);
+    } else if constexpr (MODE == DX) {
+      if (r < a.own.rows) {
+        const float* at = a.rows.of(r >> 6) + (r & 63);
+        lane_l2[j] = at[0];
+        lane_g[j] = at[64];
+        target[j] = reinterpret_cast<const int*>(at)[128];
+      }
+    }
+  }
+  float top[FO], sum[FO];           // LSE: the running maximum of the products (not yet times c) and sum
+  f32x4 out[2 * KS][FO];            // DX, DW
+#pragma unroll
+  for (int j = 0; j < FO; ++j) {
+    top[j] = -INFINITY;
+    sum[j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2 * KS; ++i) out[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const uint32_t base_row = lane_base<T, ROW, 64>();
+  const uint32_t base_tr = (4 * h + (l >> 2)) * STAGE + (((l & 3) >> 1) ^ (4 * (h & 1) + (l >> 2))) * 16 + (l & 1) * 8;
+
+  auto load = [&](char* buf, char* rbuf, int t) {
+    const int64_t r0 = s0 + (int64_t)t * 64;
+#pragma unroll
+    for (int p = 0; p < HALVES; ++p)
+      load_stage<T, ROW, 64, 4>((lds_char*)buf + p * PART, stream, r0, p * 64, a.kp);
+    if constexpr (MODE == DW) {
+      if (wave == 0)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_at((const char*)a.rows.of(r0 >> 6)),
+                                                 (__attribute__((address_space(3))) void*)(lds_char*)rbuf, 16, lane * 16, 0, 0, 0);
+    }
+  };
+  auto compute = [&](const char* buf, const char* rbuf, int t) {
+    const lds_char* lds = (const lds_char*)buf;
+    const int r0 = (int)(s0 + (int64_t)t * 64);  // stream rows fit 31 bits
+    if constexpr (MODE == LSE) {
+      bool mine = false;
+#pragma unroll
+      for (int j = 0; j < FO; ++j) mine |= (unsigned)(target[j] - r0) < 64u;
+      const bool any = __any(mine);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        f32x4 acc[2][FO];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < FO; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          frag_t p[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) p[i] = read_frag<T, ROW, 64>(lds + (s >> 1) * PART, base_row, half * 2 + i, s & 1);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < FO; ++j) acc[i][j] = mma<T>(p[i], own[j][s], acc[i][j]);
+        }
+        const int first = r0 + half * 32 + h * 4;  // the lane's stream rows: first + 16 i + e
+        if (s1 - r0 < 64) {                        // the range's last stage: rows past its end hold zeros
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (first + i * 16 + e >= (int)s1)
+#pragma unroll
+                for (int j = 0; j < FO; ++j) acc[i][j][e] = -INFINITY;
+        }
+        if (any) {  // the targets' scores: rare
+#pragma unroll
+          for (int j = 0; j < FO; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (target[j] == first + i * 16 + e) a.hit[own0 + j * 16 + l] = acc[i][j][e] * fabsf(a.scale);
+        }
+        bool rise = false;
+        float high[FO];
+#pragma unroll
+        for (int j = 0; j < FO; ++j) {
+          high[j] = fmaxf(fmaxf(acc[0][j][0], acc[0][j][1]), acc[0][j][2]);
+          high[j] = fmaxf(fmaxf(high[j], acc[0][j][3]), acc[1][j][0]);
+          high[j] = fmaxf(fmaxf(high[j], acc[1][j][1]), acc[1][j][2]);
+          high[j] = fmaxf(high[j], acc[1][j][3]);
+          rise |= high[j] > top[j];
+        }
+        if (__any(rise)) {  // rare once the largest rows have passed
+#pragma unroll
+          for (int j = 0; j < FO; ++j) {
+            const float now = fmaxf(top[j], high[j]);
+            if (top[j] != -INFINITY) sum[j] *= __builtin_amdgcn_exp2f((top[j] - now) * c);
+            top[j] = now;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < FO; ++j) {
+          const float m = top[j] == -INFINITY ? 0.f : -top[j] * c;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[j] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, m));
+        }
+      }
+    } else {
+      const __attribute__((address_space(3))) float* rp = (const __attribute__((address_space(3))) float*)(const lds_char*)rbuf;
+      bool mine = false;  // a target of these rows lies in this wave's block
+      if constexpr (MODE == DX) {
+#pragma unroll
+        for (int j = 0; j < FO; ++j) mine |= (unsigned)(target[j] - r0) < 64u;
+      } else {
+        const int t64 = ((const __attribute__((address_space(3))) int*)rp)[128 + lane];
+        mine = (unsigned)(t64 - (int)own0) < 16u * FO;
+      }
+      const bool any = __any(mine);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        f32x4 acc[2][FO];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < FO; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          frag_t p[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) p[i] = read_frag<T, ROW, 64>(lds + (s >> 1) * PART, base_row, half * 2 + i, s & 1);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < FO; ++j) acc[i][j] = mma<T>(p[i], own[j][s], acc[i][j]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          f32x4 l2, g;
+          if constexpr (MODE == DW) {
+            l2 = *(const __attribute__((address_space(3))) f32x4*)(rp + half * 32 + i * 16 + h * 4);
+            if constexpr (PER_ROW) g = *(const __attribute__((address_space(3))) f32x4*)(rp + 64 + half * 32 + i * 16 + h * 4);
+          }
+#pragma unroll
+          for (int j = 0; j < FO; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (MODE == DX)
+                acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, -lane_l2[j]));
+              else
+                acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, -l2[e]));
+            }
+          if (any) {  // rare
+            if constexpr (MODE == DX) {
+#pragma unroll
+              for (int j = 0; j < FO; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (target[j] == r0 + half * 32 + i * 16 + h * 4 + e) acc[i][j][e] -= a.extra;
+            } else {
+              const i32x4 t = *(const __attribute__((address_space(3))) i32x4*)(rp + 128 + half * 32 + i * 16 + h * 4);
+#pragma unroll
+              for (int j = 0; j < FO; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (t[e] == (int)own0 + j * 16 + l) acc[i][j][e] -= a.extra;
+            }
+          }
+          if constexpr (MODE == DW && PER_ROW)
+#pragma unroll
+            for (int j = 0; j < FO; ++j) acc[i][j] *= g;
+        }
+        frag_t q[FO];
+#pragma unroll
+        for (int j = 0; j < FO; ++j)
+          q[j] = frag_t{pack2<T>(acc[0][j][0], acc[0][j][1]), pack2<T>(acc[0][j][2], acc[0][j][3]),
+                        pack2<T>(acc[1][j][0], acc[1][j][1]), pack2<T>(acc[1][j][2], acc[1][j][3])};
+#pragma unroll
+        for (int d = 0; d < 2 * KS; ++d) {
+          const lds_char* at = lds + (base_tr ^ ((d & 3) << 5)) + (d >> 2) * PART + half * 32 * STAGE;
+          i32x4 v;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const s16x4 tr = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + s * 16 * STAGE));
+            const i32x2 w = __builtin_bit_cast(i32x2, tr);
+            v[2 * s] = w[0];
+            v[2 * s + 1] = w[1];
+          }
+#pragma unroll
+          for (int j = 0; j < FO; ++j) out[d][j] = mma<T>(v, q[j], out[d][j]);
+        }
+      }
+    }
+  };
+
+  if (stages > 0) load(s_a, s_ra, 0);
+  int t = 0;
+  for (; t + 2 <= stages; t += 2) {
+    stage_barrier();
+    load(s_b, s_rb, t + 1);
+    compute(s_a, s_ra, t);
+    stage_barrier();
+    if (t + 2 < stages) load(s_a, s_ra, t + 2);
+    compute(s_b, s_rb, t + 1);
+  }
+  if (t < stages) {
+    stage_barrier();
+    compute(s_a, s_ra, t);
+  }
+
+  if constexpr (MODE == LSE) {
+#pragma unroll
+    for (int j = 0; j < FO; ++j) {
+      float m = top[j] == -INFINITY ? top[j] : top[j] * c;
+#pragma unroll
+      for (int o = 16; o <= 32; o <<= 1) merge(m, sum[j], __shfl_xor(m, o, 64), __shfl_xor(sum[j], o, 64));
+      const int64_t r = own0 + j * 16 + l;
+      if (h == 0 && r < a.own.rows) a.part[(int64_t)split * a.own.rows + r] = make_float2(m, sum[j]);
+    }
+  } else {
+    if constexpr (MODE == DX && PER_ROW)
+#pragma unroll
+      for (int j = 0; j < FO; ++j)
+#pragma unroll
+        for (int d = 0; d < 2 * KS; ++d) out[d][j] *= lane_g[j];
+    epi.template run<NarrowShape<KS, FO>>(out, 0, own0, 0, split);
   }
 }
 
@@ -365,7 +689,27 @@ Slices slices_of(int64_t np, int64_t nq, int64_t k, int ke) {
   return s;
 }
 
+// The splits of the stream rows of a narrow kernel: two workgroups a compute unit, two stages each at least.
+struct Splits {
+  int own_tiles, n;
+  int64_t range;
+};
+Splits splits_of(int64_t own, int own_rows, int64_t stream) {
+  Splits s;
+  s.own_tiles = (int)div_up(own, own_rows);
+  const int64_t stages = div_up(stream, 64);
+  const int64_t n = std::max<int64_t>(std::min(GOAL / std::max(s.own_tiles, 1), stages / 2), 1);
+  const int64_t per = std::max<int64_t>(div_up(stages, n), 1);
+  s.n = (int)div_up(stages, per);
+  s.range = per * 64;
+  return s;
+}
+
 struct Plan {
+  bool narrow;  // halves, k <= 128: k_narrow
+  int ks;
+  Splits nl, nx, nw;
+  int64_t o_rows;
   int type, es, ge, ke, kp;
   int64_t m, n;
   int k;
@@ -398,6 +742,22 @@ Plan plan_of(int type, int64_t m, int64_t n, int k, bool forward, bool grads, bo
   Layout l;
   p.o_x = l.take(p.pack_x ? m * p.kp * p.es : 0);
   p.o_w = l.take(pack_w ? n * p.kp * p.es : 0);
+  p.narrow = type != F32 && p.kp <= 128;
+  if (p.narrow) {
+    p.ks = (p.kp + 31) / 32;
+    const int rows = p.ks > 2 ? 128 : 256;
+    p.nl = splits_of(m, 256, n);
+    p.nx = splits_of(m, rows, n);
+    p.nw = splits_of(n, rows, m);
+    p.o_part = l.take(forward ? p.nl.n * m * 8 : 0);
+    p.o_hit = l.take(forward ? m * 4 : 0);
+    p.o_top = l.take(16);
+    p.o_rows = l.take(grads ? div_up(m, 64) * 1024 : 0);
+    p.o_px = l.take(grads && p.nx.n > 1 ? p.nx.n * m * up(k, 4) * 4 : 0);
+    p.o_pw = l.take(grads && p.nw.n > 1 ? p.nw.n * n * up(k, 4) * 4 : 0);
+    p.bytes = std::max<int64_t>(l.bytes, 256);
+    return p;
+  }
   p.fwd = shape_of(n, m);
   p.fwd_tiles = div_up(n, bp_of(p.fwd)) * wp_of(p.fwd);
   p.o_part = l.take(forward ? p.fwd_tiles * m * 8 : 0);
@@ -476,16 +836,68 @@ int bind(Call& c, const void* x, int64_t ldx, const void* w, int64_t ldw) {
   return rc;
 }
 
+struct NoEpilogue {
+  template <class S>
+  __device__ void run(f32x4 (&)[S::FP][S::FQ], int64_t, int64_t, int, int) const {}
+};
+
+template <int T, int MODE, bool PER_ROW, class Epi>
+int narrow(const Plan& p, const NarrowArgs& a, Epi epi, hipStream_t st) {
+  const int64_t blocks = (int64_t)a.own_tiles * a.splits;
+  BLP_CHECK(blocks <= 0x7fffffff, BLP_E_ARG, "softmax loss: too many tiles for one launch");
+  if (blocks == 0) return 0;
+  const unsigned grid = (unsigned)blocks;
+  if (p.ks == 1)
+    k_narrow<T, 1, MODE, PER_ROW, Epi><<<grid, 256, 0, st>>>(a, epi);
+  else if (p.ks == 2)
+    k_narrow<T, 2, MODE, PER_ROW, Epi><<<grid, 256, 0, st>>>(a, epi);
+  else if (p.ks == 3)
+    k_narrow<T, 3, MODE, PER_ROW, Epi><<<grid, 256, 0, st>>>(a, epi);
+  else
+    k_narrow<T, 4, MODE, PER_ROW, Epi><<<grid, 256, 0, st>>>(a, epi);
+  BLP_HIP(hipGetLastError());
+  return 0;
+}
+
+// One gradient of the narrow path: straight into `out`, or by way of the splits' partial sums.
+template <int T, int MODE>
+int narrow_grad(const Call& c, NarrowArgs a, const Splits& s, RowGrad g, float* part, void* out, int64_t ldo, int64_t rows) {
+  const Plan& p = c.p;
+  const int64_t ldp = up(p.k, 4);
+  a.own_tiles = s.own_tiles;
+  a.splits = s.n;
+  a.range = s.range;
+  const bool per_row = g.g && g.stride;
+  if (s.n == 1) {
+    const EpiOut<T> e = {(char*)out, ldo * p.es, p.k, rows, g, c.scale};
+    return per_row ? narrow<T, MODE, true>(p, a, e, c.st) : narrow<T, MODE, false>(p, a, e, c.st);
+  }
+  const EpiPart e = {part, ldp, p.k, rows, 0};
+  const int rc = per_row ? narrow<T, MODE, true>(p, a, e, c.st) : narrow<T, MODE, false>(p, a, e, c.st);
+  if (rc) return rc;
+  k_sum_parts<T><<<grid_for(rows * (ldp / 4)), 256, 0, c.st>>>(part, s.n, ldp, p.k, rows, g, c.scale, (char*)out, ldo * p.es);
+  BLP_HIP(hipGetLastError());
+  return 0;
+}
+
 template <int T>
 int forward(const Call& c, float* loss, float* lse, float* total, int mean) {
   const Plan& p = c.p;
   if (p.m > 0) {
     float2* part = (float2*)(c.ws + p.o_part);
     float* hit = (float*)(c.ws + p.o_hit);
-    const Problem a = {c.w, c.x, p.kp, up(p.kp, p.ke), 0, 0};
-    int rc = product<T, ROW, ROW>(p.fwd, a, 1, EpiLse<T>{part, hit, c.targets, p.n, p.m, c.scale}, c.st);
+    int rc = 0;
+    if constexpr (T != F32) {
+      if (p.narrow)
+        rc = narrow<T, LSE, false>(p, NarrowArgs{c.x, c.w, p.kp, p.nl.range, p.nl.own_tiles, p.nl.n, c.scale, 1.f, c.targets, part, hit},
+                                   NoEpilogue{}, c.st);
+    }
+    if (!p.narrow) {
+      const Problem a = {c.w, c.x, p.kp, up(p.kp, p.ke), 0, 0};
+      rc = product<T, ROW, ROW>(p.fwd, a, 1, EpiLse<T>{part, hit, c.targets, p.n, p.m, c.scale}, c.st);
+    }
     if (rc) return rc;
-    k_join<<<(unsigned)div_up(p.m, 32), 256, 0, c.st>>>(part, p.fwd_tiles, p.m, hit, c.targets, loss, lse);
+    k_join<<<(unsigned)div_up(p.m, 32), 256, 0, c.st>>>(part, p.narrow ? p.nl.n : p.fwd_tiles, p.m, hit, c.targets, loss, lse);
     BLP_HIP(hipGetLastError());
   }
   if (total) {
@@ -513,6 +925,17 @@ int backward(const Call& c, const float* lse, RowGrad g, void* dx, int64_t lddx,
     k_top_grad<<<1, 1024, 0, c.st>>>(g.g, c.targets, p.m, top);
     BLP_HIP(hipGetLastError());
     g.top = top;
+  }
+  if constexpr (T != F32) {
+    if (p.narrow) {
+      NarrowArgs a = {c.x, c.w, p.kp, 0, 0, 0, c.scale, g.extra, c.targets, nullptr, nullptr, Rows{(float*)(c.ws + p.o_rows)}};
+      k_rows<<<(unsigned)div_up(p.m, 64), 64, 0, c.st>>>(lse, g, c.targets, p.m, a.rows);
+      BLP_HIP(hipGetLastError());
+      int rc = dx ? narrow_grad<T, DX>(c, a, p.nx, g, (float*)(c.ws + p.o_px), dx, lddx, p.m) : 0;
+      std::swap(a.own, a.stream);
+      if (!rc && dw) rc = narrow_grad<T, DW>(c, a, p.nw, g, (float*)(c.ws + p.o_pw), dw, lddw, p.n);
+      return rc;
+    }
   }
   char* ds = c.ws + p.o_ds;
   float *px = (float*)(c.ws + p.o_px), *pw = (float*)(c.ws + p.o_pw);

@@ -91,7 +91,7 @@ struct EpiScores {
   const float *s, *t;
   int64_t np, nq;
   template <class S>
-  __device__ void run(i32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int) const {
+  __device__ void run(i32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int) const {
     const int lane = threadIdx.x & 63, h = lane >> 4;
 #pragma unroll
     for (int j = 0; j < S::FQ; ++j) {

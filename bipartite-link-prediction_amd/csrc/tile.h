@@ -268,7 +268,7 @@ __global__ __launch_bounds__(S::THREADS) void k_product(Problem a, Epi epi) {
     stage_barrier();
     mul_stage<T, LP, LQ, S>(lp0, lq0, bp, bq, wp, wq, acc);
   }
-  epi.template run<S>(acc, p0 + wp * S::FP * 16, q0 + wq * S::FQ * 16, tp * S::WP + wp);
+  epi.template run<S>(acc, p0 + wp * S::FP * 16, q0 + wq * S::FQ * 16, tp * S::WP + wp, blockIdx.y);
 }
 
 // round to the type once; four consecutive values
