@@ -372,13 +372,15 @@ __device__ inline int pack2(float a, float b) {
 }
 
 template <int T, int KS, int MODE, bool PER_ROW, class Epi>
-__global__ __launch_bounds__(256, 2) void k_narrow(NarrowArgs a, Epi epi) {
-  constexpr int FO = KS > 2 && MODE != LSE ? 2 : 4;  // own fragments of 16 rows a wave
+__global__ __launch_bounds__(256, KS > 2 ? 3 : 4) void k_narrow(NarrowArgs a, Epi epi) {
+  constexpr int FO = 2;                              // own fragments of 16 rows a wave
   constexpr int HALVES = KS > 2 ? 2 : 1;             // 128-byte parts of a row
   constexpr int PART = 64 * STAGE;                   // bytes of one part of a stage
   constexpr int BUF = HALVES * PART;
-  __shared__ __attribute__((aligned(1024))) char s_a[BUF], s_b[BUF];
-  __shared__ __attribute__((aligned(1024))) char s_ra[MODE == DW ? 1024 : 16], s_rb[MODE == DW ? 1024 : 16];
+  constexpr int COPIES = 2 * HALVES + (MODE == DW);  // a wave issues for a stage
+  __shared__ __attribute__((aligned(1024))) char s_a[BUF], s_b[BUF], s_c[BUF];
+  __shared__ __attribute__((aligned(1024))) char s_ra[MODE == DW ? 1024 : 16], s_rb[MODE == DW ? 1024 : 16],
+      s_rc[MODE == DW ? 1024 : 16];
   // a die's workgroups take neighbouring own tiles of one split: the split's rows stay in its L2
   const int n_blocks = a.own_tiles * a.splits, per = n_blocks >> 3, more = n_blocks & 7, xcd = blockIdx.x & 7;
   const int id = xcd * per + min(xcd, more) + (blockIdx.x >> 3);
@@ -387,7 +389,7 @@ __global__ __launch_bounds__(256, 2) void k_narrow(NarrowArgs a, Epi epi) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t own0 = (int64_t)own_tile * (64 * FO) + wave * (16 * FO);
   const int64_t s0 = split * a.range, s1 = min(a.stream.rows, s0 + a.range);
-  const int stages = s1 > s0 ? (int)((s1 - s0 + 63) >> 6) : 0;
+  const int stages = (int)((s1 - s0 + 63) >> 6);
   const float c = fmaxf(fabsf(a.scale) * LOG2E, 1.2e-38f);  // positive: -inf c is -inf for a scale of 0, too
   const Operand stream = {a.stream.base, a.stream.ld, s1};
 
@@ -423,11 +425,13 @@ __global__ __launch_bounds__(256, 2) void k_narrow(NarrowArgs a, Epi epi) {
       }
     }
   }
-  float top[FO], sum[FO];           // LSE: the running maximum of the products (not yet times c) and sum
+  // LSE: the running maximum of the products (not yet times c), its -top c (0 while it is infinite), the sum
+  float top[FO], shift[FO], sum[FO];
   f32x4 out[2 * KS][FO];            // DX, DW
 #pragma unroll
   for (int j = 0; j < FO; ++j) {
     top[j] = -INFINITY;
+    shift[j] = 0.f;
     sum[j] = 0.f;
 #pragma unroll
     for (int i = 0; i < 2 * KS; ++i) out[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -440,27 +444,15 @@ __global__ __launch_bounds__(256, 2) void k_narrow(NarrowArgs a, Epi epi) {
 #pragma unroll
     for (int p = 0; p < HALVES; ++p)
       load_stage<T, ROW, 64, 4>((lds_char*)buf + p * PART, stream, r0, p * 64, a.kp);
-    if constexpr (MODE == DW) {
-      if (wave == 0)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_at((const char*)a.rows.of(r0 >> 6)),
-                                                 (__attribute__((address_space(3))) void*)(lds_char*)rbuf, 16, lane * 16, 0, 0, 0);
-    }
+    if constexpr (MODE == DW)  // by every wave alike, so that their counts agree
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_at((const char*)a.rows.of(min(r0, a.stream.rows - 1) >> 6)),
+                                               (__attribute__((address_space(3))) void*)(lds_char*)rbuf, 16, lane * 16, 0, 0, 0);
   };
   auto compute = [&](const char* buf, const char* rbuf, int t) {
     const lds_char* lds = (const lds_char*)buf;
     const int r0 = (int)(s0 + (int64_t)t * 64);  // stream rows fit 31 bits
     if constexpr (MODE == LSE) {
-      bool mine = false;
-#pragma unroll
-      for (int j = 0; j < FO; ++j) mine |= (unsigned)(target[j] - r0) < 64u;
-      const bool any = __any(mine);
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        f32x4 acc[2][FO];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < FO; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      auto products = [&](int half, f32x4(&acc)[2][FO]) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           frag_t p[2];
@@ -469,52 +461,63 @@ __global__ __launch_bounds__(256, 2) void k_narrow(NarrowArgs a, Epi epi) {
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < FO; ++j) acc[i][j] = mma<T>(p[i], own[j][s], acc[i][j]);
+            for (int j = 0; j < FO; ++j) acc[i][j] = mma<T>(p[i], own[j][s], s ? acc[i][j] : f32x4{0.f, 0.f, 0.f, 0.f});
         }
-        const int first = r0 + half * 32 + h * 4;  // the lane's stream rows: first + 16 i + e
-        if (s1 - r0 < 64) {                        // the range's last stage: rows past its end hold zeros
+      };
+      bool slow = t == 0 || s1 - r0 < 64;
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+      for (int j = 0; j < FO; ++j) slow |= (unsigned)(target[j] - r0) < 64u;
+      if (!__any(slow)) {
+        // The stale maximum does as long as no sum grows past 2^60 (or is NaN): no maximum to take.
+        float add[FO];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (first + i * 16 + e >= (int)s1)
+        for (int j = 0; j < FO; ++j) add[j] = 0.f;
 #pragma unroll
-                for (int j = 0; j < FO; ++j) acc[i][j][e] = -INFINITY;
-        }
-        if (any) {  // the targets' scores: rare
+        for (int half = 0; half < 2; ++half) {
+          f32x4 acc[2][FO];
+          products(half, acc);
 #pragma unroll
           for (int j = 0; j < FO; ++j)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (target[j] == first + i * 16 + e) a.hit[own0 + j * 16 + l] = acc[i][j][e] * fabsf(a.scale);
+              for (int e = 0; e < 4; ++e) add[j] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, shift[j]));
         }
-        bool rise = false;
-        float high[FO];
+#pragma unroll
+        for (int j = 0; j < FO; ++j) slow |= !(add[j] < 0x1p60f);
+        if (!__any(slow)) {
+#pragma unroll
+          for (int j = 0; j < FO; ++j) sum[j] += add[j];
+          return;
+        }
+      }
+      // The first and the last stage, targets' scores, and rows that rise far: rare.
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        f32x4 acc[2][FO];
+        products(half, acc);
+        const int first = r0 + half * 32 + h * 4;  // the lane's stream rows: first + 16 i + e
 #pragma unroll
         for (int j = 0; j < FO; ++j) {
-          high[j] = fmaxf(fmaxf(acc[0][j][0], acc[0][j][1]), acc[0][j][2]);
-          high[j] = fmaxf(fmaxf(high[j], acc[0][j][3]), acc[1][j][0]);
-          high[j] = fmaxf(fmaxf(high[j], acc[1][j][1]), acc[1][j][2]);
-          high[j] = fmaxf(high[j], acc[1][j][3]);
-          rise |= high[j] > top[j];
-        }
-        if (__any(rise)) {  // rare once the largest rows have passed
-#pragma unroll
-          for (int j = 0; j < FO; ++j) {
-            const float now = fmaxf(top[j], high[j]);
-            if (top[j] != -INFINITY) sum[j] *= __builtin_amdgcn_exp2f((top[j] - now) * c);
-            top[j] = now;
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < FO; ++j) {
-          const float m = top[j] == -INFINITY ? 0.f : -top[j] * c;
+          float high = top[j];
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum[j] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, m));
+            for (int e = 0; e < 4; ++e) {
+              const int r = first + i * 16 + e;
+              if (r == target[j]) a.hit[own0 + j * 16 + l] = acc[i][j][e] * fabsf(a.scale);
+              if (r >= (int)s1) acc[i][j][e] = -INFINITY;  // past the range's end: zeros in LDS
+              high = fmaxf(high, acc[i][j][e]);
+            }
+          if (high > top[j]) {
+            if (top[j] != -INFINITY) sum[j] *= __builtin_amdgcn_exp2f((top[j] - high) * c);
+            top[j] = high;
+            shift[j] = -high * c;
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[j] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, shift[j]));
         }
       }
     } else {
@@ -532,10 +535,6 @@ __global__ __launch_bounds__(256, 2) void k_narrow(NarrowArgs a, Epi epi) {
       for (int half = 0; half < 2; ++half) {
         f32x4 acc[2][FO];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < FO; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
         for (int s = 0; s < KS; ++s) {
           frag_t p[2];
 #pragma unroll
@@ -543,7 +542,7 @@ __global__ __launch_bounds__(256, 2) void k_narrow(NarrowArgs a, Epi epi) {
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < FO; ++j) acc[i][j] = mma<T>(p[i], own[j][s], acc[i][j]);
+            for (int j = 0; j < FO; ++j) acc[i][j] = mma<T>(p[i], own[j][s], s ? acc[i][j] : f32x4{0.f, 0.f, 0.f, 0.f});
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -604,20 +603,23 @@ __global__ __launch_bounds__(256, 2) void k_narrow(NarrowArgs a, Epi epi) {
     }
   };
 
-  if (stages > 0) load(s_a, s_ra, 0);
-  int t = 0;
-  for (; t + 2 <= stages; t += 2) {
-    stage_barrier();
-    load(s_b, s_rb, t + 1);
+  // Three buffers, two stages ahead. Stages past the range copy nothing and count for nothing: their rows are zeros
+  // (LSE masks them), so every trip takes three and the counts of outstanding copies stay the same.
+  load(s_a, s_ra, 0);
+  load(s_b, s_rb, 1);
+#pragma unroll 1
+  for (int t = 0; t < stages; t += 3) {
+    ring_barrier<COPIES>();
+    load(s_c, s_rc, t + 2);
     compute(s_a, s_ra, t);
-    stage_barrier();
-    if (t + 2 < stages) load(s_a, s_ra, t + 2);
+    ring_barrier<COPIES>();
+    load(s_a, s_ra, t + 3);
     compute(s_b, s_rb, t + 1);
+    ring_barrier<COPIES>();
+    load(s_b, s_rb, t + 4);
+    compute(s_c, s_rc, t + 2);
   }
-  if (t < stages) {
-    stage_barrier();
-    compute(s_a, s_ra, t);
-  }
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // nothing in flight towards LDS when the workgroup ends
 
   if constexpr (MODE == LSE) {
 #pragma unroll
@@ -694,13 +696,13 @@ struct Splits {
   int own_tiles, n;
   int64_t range;
 };
-Splits splits_of(int64_t own, int own_rows, int64_t stream) {
+Splits splits_of(int64_t own, int own_rows, int64_t stream, int64_t goal) {
   Splits s;
   s.own_tiles = (int)div_up(own, own_rows);
   const int64_t stages = div_up(stream, 64);
-  const int64_t n = std::max<int64_t>(std::min(GOAL / std::max(s.own_tiles, 1), stages / 2), 1);
-  const int64_t per = std::max<int64_t>(div_up(stages, n), 1);
-  s.n = (int)div_up(stages, per);
+  const int64_t n = std::max<int64_t>(std::min(goal / std::max(s.own_tiles, 1), stages / 2), 1);
+  const int64_t per = up(std::max<int64_t>(div_up(stages, n), 1), 3);  // three stages a trip
+  s.n = (int)std::max<int64_t>(div_up(stages, per), 1);
   s.range = per * 64;
   return s;
 }
@@ -745,10 +747,9 @@ Plan plan_of(int type, int64_t m, int64_t n, int k, bool forward, bool grads, bo
   p.narrow = type != F32 && p.kp <= 128;
   if (p.narrow) {
     p.ks = (p.kp + 31) / 32;
-    const int rows = p.ks > 2 ? 128 : 256;
-    p.nl = splits_of(m, 256, n);
-    p.nx = splits_of(m, rows, n);
-    p.nw = splits_of(n, rows, m);
+    p.nl = splits_of(m, 128, n, 4 * GOAL);
+    p.nx = splits_of(m, 128, n, 2 * GOAL);
+    p.nw = splits_of(n, 128, m, 2 * GOAL);
     p.o_part = l.take(forward ? p.nl.n * m * 8 : 0);
     p.o_hit = l.take(forward ? m * 4 : 0);
     p.o_top = l.take(16);

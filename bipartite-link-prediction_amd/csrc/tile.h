@@ -209,6 +209,17 @@ __device__ inline void stage_barrier() {
   __syncthreads();
 }
 
+// The same with this wave's last `LEFT` copies still in flight: a stage's copies have landed when only those of
+// the LEFT issued after it are outstanding (they land in order). Every read of LDS issued before has returned.
+template <int LEFT>
+__device__ inline void ring_barrier() {
+  static_assert(LEFT < 16, "the count's low bits");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | LEFT);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 struct Problem {
   Operand p, q;
   int64_t k;        // valid k, in elements
