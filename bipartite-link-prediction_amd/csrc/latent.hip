@@ -59,13 +59,14 @@ __global__ __launch_bounds__(256) void k_pack(const char* __restrict__ src, int6
 // One (max, sum of exp2) pair a row and wave tile, in base 2: part[tile * rows + row].
 template <int T>
 struct EpiLse {
+  static constexpr bool SCRATCH = false;
   float2* part;
   float* hit;  // z of the target
   Targets targets;
   int64_t n, m;
   float scale;
   template <class S>
-  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int tile, int) const {
+  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int tile, int, lds_char*) const {
     const int lane = threadIdx.x & 63, h = lane >> 4;
     const float c = scale * LOG2E;
 #pragma unroll
@@ -206,6 +207,7 @@ __global__ __launch_bounds__(1024) void k_top_grad(const float* __restrict__ g, 
 // dS of one piece: ds[row * ld + p - 0], zeros past the catalogue's end.
 template <int T>
 struct EpiGrad {
+  static constexpr bool SCRATCH = true;
   char* ds;
   int64_t ld;  // elements
   const float* lse;
@@ -215,73 +217,61 @@ struct EpiGrad {
   int64_t n, m;
   float scale;
   template <class S>
-  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int) const {
-    const int lane = threadIdx.x & 63, h = lane >> 4;
+  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int, lds_char* scratch) const {
+    if (p0 >= ld || q0 >= m) return;
+    const int lane = threadIdx.x & 63, l = lane & 15, h = lane >> 4;
     const float c = scale * LOG2E;
+    const int left = (int)min(n - p0, (int64_t)(S::FP * 16)), rows = (int)min(m - q0, (int64_t)(S::FQ * 16));
+    int hit[S::FQ];  // the target's place in the lane's block; far off: none
+    float gr[S::FQ], l2[S::FQ];
 #pragma unroll
     for (int j = 0; j < S::FQ; ++j) {
-      const int64_t row = q0 + j * 16 + (lane & 15);
-      if (row >= m) continue;
-      const int64_t t = targets(row) - j0;  // negative: not here or ignored
-      const bool valid = targets(row) >= 0;
-      const float gr = valid ? g.row(row) : 0.f, l2 = lse[row] * LOG2E;
-      char* at = ds + row * ld * size_of(T);
-#pragma unroll
-      for (int i = 0; i < S::FP; ++i) {
-        const int64_t p = p0 + i * 16 + h * 4;
-        if (p >= ld) continue;
-        f32x4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float d = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, -l2)) - (p + e == t ? 1.f : 0.f);
-          v[e] = valid && p + e < n ? d * gr : 0.f;
-        }
-        store4<T>(at + p * size_of(T), v);
-      }
+      const int64_t row = q0 + min(j * 16 + l, rows - 1), t = targets(row);
+      hit[j] = t >= 0 && t - j0 - p0 >= 0 && t - j0 - p0 < S::FP * 16 ? (int)(t - j0 - p0) - h * 4 : -1000;
+      gr[j] = t >= 0 ? g.row(row) : 0.f;
+      l2[j] = t >= 0 ? -lse[row] * LOG2E : -INFINITY;
     }
+    store_block<T, S>(scratch, ds + (q0 * ld + p0) * size_of(T), ld * size_of(T), (int)min(ld - p0, (int64_t)(S::FP * 16)), rows,
+                      [&](int i, int j) {
+                        f32x4 v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                          float d = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, l2[j]));
+                          if (hit[j] == i * 16 + e) d -= 1.f;
+                          d *= gr[j];
+                          v[e] = left == S::FP * 16 || i * 16 + h * 4 + e < left ? d : 0.f;
+                        }
+                        return v;
+                      });
   }
 };
 
 // out[q][p] = alpha acc, rounded once.
 template <int T>
 struct EpiOut {
+  static constexpr bool SCRATCH = true;
   char* out;
   int64_t ld;  // bytes
   int64_t np, nq;
   RowGrad g;
   float scale;
   template <class S>
-  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int) const {
-    const int lane = threadIdx.x & 63, h = lane >> 4;
+  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int, lds_char* scratch) const {
+    if (p0 >= np || q0 >= nq) return;
     const float alpha = scale * g.all();
-    const bool whole = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)ld) & (4 * size_of(T) - 1)) == 0;
-#pragma unroll
-    for (int j = 0; j < S::FQ; ++j) {
-      const int64_t q = q0 + j * 16 + (lane & 15);
-      if (q >= nq) continue;
-#pragma unroll
-      for (int i = 0; i < S::FP; ++i) {
-        const int64_t p = p0 + i * 16 + h * 4;
-        char* at = out + q * ld + p * size_of(T);
-        if (whole && p + 4 <= np) {
-          store4<T>(at, acc[i][j] * alpha);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (p + e < np) store1<T>(at + e * size_of(T), acc[i][j][e] * alpha);
-        }
-      }
-    }
+    const int left = (int)min(np - p0, (int64_t)(S::FP * 16)), rows = (int)min(nq - q0, (int64_t)(S::FQ * 16));
+    store_block<T, S>(scratch, out + q0 * ld + p0 * size_of(T), ld, left, rows, [&](int i, int j) { return acc[i][j] * alpha; });
   }
 };
 
 // part[slice][q][p] (+)= acc: the sums over slices of k and pieces of the catalogue, in 32 bits.
 struct EpiPart {
+  static constexpr bool SCRATCH = false;
   float* part;
   int64_t ld, np, nq;  // elements; ld a multiple of 4
   int add;
   template <class S>
-  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int slice) const {
+  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int slice, lds_char*) const {
     const int lane = threadIdx.x & 63, h = lane >> 4;
     float* base = part + (int64_t)slice * nq * ld;
 #pragma unroll
@@ -636,7 +626,17 @@ __global__ __launch_bounds__(256, KS > 2 ? 3 : 4) void k_narrow(NarrowArgs a, Ep
       for (int j = 0; j < FO; ++j)
 #pragma unroll
         for (int d = 0; d < 2 * KS; ++d) out[d][j] *= lane_g[j];
-    epi.template run<NarrowShape<KS, FO>>(out, 0, own0, 0, split);
+    lds_char* scratch = nullptr;
+    if constexpr (Epi::SCRATCH) {  // a wave's 32 rows of up to 128 halves: the ring's buffers in parts
+      __syncthreads();
+      constexpr int WAVE = 16 * FO * pow2_up(64 * KS);
+      if constexpr (WAVE * 4 <= BUF)
+        scratch = (lds_char*)s_a + wave * WAVE;
+      else
+        scratch = wave < 2 ? (lds_char*)s_a + wave * WAVE : (lds_char*)s_b + (wave - 2) * WAVE;
+      static_assert(WAVE * 2 <= BUF, "two waves a buffer");
+    }
+    epi.template run<NarrowShape<KS, FO>>(out, 0, own0, 0, split, scratch);
   }
 }
 
@@ -838,8 +838,9 @@ int bind(Call& c, const void* x, int64_t ldx, const void* w, int64_t ldw) {
 }
 
 struct NoEpilogue {
+  static constexpr bool SCRATCH = false;
   template <class S>
-  __device__ void run(f32x4 (&)[S::FP][S::FQ], int64_t, int64_t, int, int) const {}
+  __device__ void run(f32x4 (&)[S::FP][S::FQ], int64_t, int64_t, int, int, lds_char*) const {}
 };
 
 template <int T, int MODE, bool PER_ROW, class Epi>

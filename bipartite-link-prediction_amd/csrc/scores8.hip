@@ -15,13 +15,6 @@ namespace {
 using namespace blp::tile;
 using blp::DeviceGuard;
 
-struct __attribute__((packed, aligned(2))) Raw16 {
-  i32x4 v;
-};
-template <class V>
-struct __attribute__((packed, aligned(2))) Raw {
-  V v;
-};
 
 // ---------------------------------------------------------------- quantising
 // x / s rounded to nearest, halves to even -- of the true quotient, not of its 32-bit rounding: the first
@@ -86,39 +79,30 @@ __global__ __launch_bounds__(256) void k_pack8(const int8_t* __restrict__ src, i
 // ---------------------------------------------------------------- scores
 template <int TO>
 struct EpiScores {
+  static constexpr bool SCRATCH = true;
   char* out;
   int64_t ld;  // bytes
   const float *s, *t;
   int64_t np, nq;
   template <class S>
-  __device__ void run(i32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int) const {
-    const int lane = threadIdx.x & 63, h = lane >> 4;
+  __device__ void run(i32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int, lds_char* scratch) const {
+    if (p0 >= np || q0 >= nq) return;
+    const int lane = threadIdx.x & 63, l = lane & 15, h = lane >> 4;
+    const int left = (int)min(np - p0, (int64_t)(S::FP * 16)), rows = (int)min(nq - q0, (int64_t)(S::FQ * 16));
+    f32x4 tp[S::FP];
+    float sq[S::FQ];
 #pragma unroll
-    for (int j = 0; j < S::FQ; ++j) {
-      const int64_t q = q0 + j * 16 + (lane & 15);
-      if (q >= nq) continue;
-      const float sq = s[q];
+    for (int i = 0; i < S::FP; ++i)
 #pragma unroll
-      for (int i = 0; i < S::FP; ++i) {
-        const int64_t p = p0 + i * 16 + h * 4;
-        char* at = out + q * ld + p * size_of(TO);
-        f32x4 v;
+      for (int e = 0; e < 4; ++e) tp[i][e] = t[p0 + min(i * 16 + h * 4 + e, left - 1)];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = p + e < np ? (float)acc[i][j][e] * sq * t[p + e] : 0.f;
-        if (p + 4 <= np) {
-          if constexpr (TO == F32)
-            reinterpret_cast<Raw<f32x4>*>(at)->v = v;
-          else if constexpr (TO == BF16)
-            reinterpret_cast<Raw<bf16x4>*>(at)->v = __builtin_convertvector(v, bf16x4);
-          else
-            reinterpret_cast<Raw<f16x4>*>(at)->v = __builtin_convertvector(v, f16x4);
-        } else {
+    for (int j = 0; j < S::FQ; ++j) sq[j] = s[q0 + min(j * 16 + l, rows - 1)];
+    store_block<TO, S>(scratch, out + q0 * ld + p0 * size_of(TO), ld, left, rows, [&](int i, int j) {
+      f32x4 v;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (p + e < np) store1<TO>(at + e * size_of(TO), v[e]);
-        }
-      }
-    }
+      for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j][e] * sq[j] * tp[i][e];
+      return v;
+    });
   }
 };
 
@@ -145,7 +129,8 @@ int scores(const Operand& w, const Operand& x, int k, const float* s, const floa
   const Problem a = {w, x, k, up(k, STAGE), 0, 0};
   const EpiScores<TO> epi = {(char*)out, ldo * size_of(TO), s, t, w.rows, x.rows};
   if (x.rows <= 32) return launch<TO, NarrowQ>(a, epi, st);
-  if (div_up(w.rows, 256) * div_up(x.rows, 256) >= 192) return launch<TO, Big>(a, epi, st);
+  // one or two stages of k: two small workgroups a compute unit, so that one's stores run beside the other's loads
+  if (k > 2 * STAGE && div_up(w.rows, 256) * div_up(x.rows, 256) >= 192) return launch<TO, Big>(a, epi, st);
   return launch<TO, Mid>(a, epi, st);
 }
 

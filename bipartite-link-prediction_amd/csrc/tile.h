@@ -279,7 +279,19 @@ __global__ __launch_bounds__(S::THREADS) void k_product(Problem a, Epi epi) {
     stage_barrier();
     mul_stage<T, LP, LQ, S>(lp0, lq0, bp, bq, wp, wq, acc);
   }
-  epi.template run<S>(acc, p0 + wp * S::FP * 16, q0 + wq * S::FQ * 16, tp * S::WP + wp, blockIdx.y);
+  lds_char* scratch = nullptr;  // 16 KiB of the stages' LDS for each wave's outputs
+  if constexpr (Epi::SCRATCH) {
+    __syncthreads();
+    if constexpr (S::BP == 256 && S::BQ == 256)
+      scratch = (wave < 4 ? (wave < 2 ? lp0 : lq0) : (wave < 6 ? lp1 : lq1)) + (wave & 1) * 16384;
+    else if constexpr (S::BP == 128 && S::BQ == 128)
+      scratch = wave < 2 ? (wave == 0 ? lp0 : lq0) : (wave == 2 ? lp1 : lq1);
+    else if constexpr (S::BQ == 256)
+      scratch = (wave < 2 ? lq0 : lq1) + (wave & 1) * 16384;
+    else
+      scratch = (wave < 2 ? lp0 : lp1) + (wave & 1) * 16384;
+  }
+  epi.template run<S>(acc, p0 + wp * S::FP * 16, q0 + wq * S::FQ * 16, tp * S::WP + wp, blockIdx.y, scratch);
 }
 
 // round to the type once; four consecutive values
@@ -311,6 +323,74 @@ __device__ inline float load1(const char* at) {
     return (float)*reinterpret_cast<const __bf16*>(at);
   } else {
     return (float)*reinterpret_cast<const _Float16*>(at);
+  }
+}
+
+struct __attribute__((packed, aligned(2))) Unaligned16 {  // global memory takes any alignment
+  i32x4 v;
+};
+
+// A wave's 16 FP x 16 FQ outputs, already values of the type (`value(i, j)`: the four of a lane in block (i, j)),
+// into rows of `out` (row q of the block at out + q ld bytes; element p at p * size): by way of LDS, so that a row's
+// elements leave as whole lines, 16 bytes a lane, instead of 8 bytes from 16 rows each. Rows from nq and elements
+// from np on are not written. LDS rows are a power of two of bytes; their granules are swapped by the row's number,
+// which spreads both the writes and the reads over the banks.
+__host__ __device__ constexpr int pow2_up(int v) {
+  int p = 1;
+  while (p < v) p <<= 1;
+  return p;
+}
+template <int TO, class S, class F>
+__device__ inline void store_block(lds_char* scratch, char* out, int64_t ld, int64_t np, int64_t nq, F value) {
+  constexpr int ES = size_of(TO), ROWB = pow2_up(S::FP * 16 * ES), GR = ROWB / 16;  // bytes, granules of an LDS row
+  constexpr int J = S::FQ * 16 * ROWB > 16384 ? S::FQ / 2 : S::FQ;         // blocks of 16 rows a pass
+  constexpr int LANES = GR < 64 ? GR : 64, RPI = 64 / LANES;               // lanes a row, rows an instruction
+  const int lane = threadIdx.x & 63, l = lane & 15, h = lane >> 4;
+#pragma unroll
+  for (int j0 = 0; j0 < S::FQ; j0 += J) {
+    if (j0) __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < S::FP; ++i) {
+        const f32x4 v = value(i, j0 + j);
+        const int row = j * 16 + l;
+        if constexpr (TO == F32) {
+          const int g = (i * 4 + h) ^ (row & (GR - 1) & 15);
+          *(__attribute__((address_space(3))) f32x4*)(scratch + row * ROWB + g * 16) = v;
+        } else {
+          const int g = (i * 2 + (h >> 1)) ^ (row & (GR - 1) & 15);
+          __attribute__((address_space(3))) i32x2* at =
+              (__attribute__((address_space(3))) i32x2*)(scratch + row * ROWB + g * 16 + (h & 1) * 8);
+          if constexpr (TO == BF16)
+            *at = __builtin_bit_cast(i32x2, __builtin_convertvector(v, bf16x4));
+          else
+            *at = __builtin_bit_cast(i32x2, __builtin_convertvector(v, f16x4));
+        }
+      }
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int g = lane & (LANES - 1), p = g * (16 / ES);
+#pragma unroll
+    for (int r0 = 0; r0 < J * 16; r0 += RPI) {
+      const int row = r0 + lane / LANES;
+      const i32x4 v = *(const __attribute__((address_space(3))) i32x4*)(scratch + row * ROWB + (g ^ (row & (GR - 1) & 15)) * 16);
+      const int64_t q = j0 * 16 + row;
+      if (q >= nq) continue;
+      char* at = out + q * ld + p * ES;
+      if (p + 16 / ES <= np) {
+        reinterpret_cast<Unaligned16*>(at)->v = v;
+      } else if (p < np) {
+#pragma unroll
+        for (int e = 0; e < 16 / ES; ++e)
+          if (p + e < np) {
+            if constexpr (ES == 4)
+              reinterpret_cast<int*>(at)[e] = v[e];
+            else
+              reinterpret_cast<uint16_t*>(at)[e] = (uint16_t)((uint32_t)v[e >> 1] >> (16 * (e & 1)));
+          }
+      }
+    }
   }
 }
 
