@@ -16,70 +16,9 @@ namespace {
 
 using namespace blp::tile;
 using blp::DeviceGuard;
+using namespace blp::rows;
 using blp::FastDiv;
 using blp::Ids;
-
-// ---------------------------------------------------------------- vectors of a row
-// NE elements of 16 bytes, wherever they start (global memory takes any alignment); the row's last
-// vector may be short.
-template <int T>
-struct Vec {
-  static constexpr int NE = 16 / size_of(T);
-  f32x4 v[NE / 4];
-};
-struct __attribute__((packed, aligned(2))) Raw16 {
-  i32x4 v;
-};
-
-template <int T>
-__device__ inline Vec<T> load_vec(const char* at, int left) {
-  constexpr int NE = Vec<T>::NE;
-  Vec<T> r;
-  if (left >= NE) {
-    const i32x4 raw = reinterpret_cast<const Raw16*>(at)->v;
-    if constexpr (T == F32) {
-      r.v[0] = __builtin_bit_cast(f32x4, raw);
-    } else if constexpr (T == BF16) {
-      const bf16x8 b = __builtin_bit_cast(bf16x8, raw);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) r.v[e >> 2][e & 3] = (float)b[e];
-    } else {
-      const f16x8 b = __builtin_bit_cast(f16x8, raw);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) r.v[e >> 2][e & 3] = (float)b[e];
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < NE; ++e) r.v[e >> 2][e & 3] = e < left ? load1<T>(at + e * size_of(T)) : 0.f;
-  }
-  return r;
-}
-
-template <int T>
-__device__ inline void store_vec(char* at, int left, const Vec<T>& r) {
-  constexpr int NE = Vec<T>::NE;
-  if (left >= NE) {
-    Raw16 raw;
-    if constexpr (T == F32) {
-      raw.v = __builtin_bit_cast(i32x4, r.v[0]);
-    } else if constexpr (T == BF16) {
-      bf16x8 b;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) b[e] = (__bf16)r.v[e >> 2][e & 3];
-      raw.v = __builtin_bit_cast(i32x4, b);
-    } else {
-      f16x8 b;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) b[e] = (_Float16)r.v[e >> 2][e & 3];
-      raw.v = __builtin_bit_cast(i32x4, b);
-    }
-    *reinterpret_cast<Raw16*>(at) = raw;
-  } else {
-#pragma unroll
-    for (int e = 0; e < NE; ++e)
-      if (e < left) store1<T>(at + e * size_of(T), r.v[e >> 2][e & 3]);
-  }
-}
 
 // ---------------------------------------------------------------- lookup
 // One vector a thread, four in flight. `n` rows with n * per < 2^31 (the host takes longer lists in parts).

@@ -13,7 +13,12 @@
 namespace {
 
 using namespace blp::tile;
+using namespace blp::rows;
 using blp::DeviceGuard;
+
+struct __attribute__((packed, aligned(1))) Unaligned4 {
+  uint32_t v;
+};
 
 
 // ---------------------------------------------------------------- quantising
@@ -29,33 +34,47 @@ __device__ inline int to8(float x, float s) {
   return (int)fminf(fmaxf(q, -127.f), 127.f);
 }
 
-// `lanes` (a power of two up to 64) lanes a row, 16 elements a step; two passes over the row, the second
-// out of the cache. Bytes [k, kp) of a row are set to zero. A row with a NaN or an infinity gets the scale
-// NaN and zeros, so its scores are NaN; a row of zeros the scale 0.
+// `lanes` (a power of two up to 64) lanes a row, one 16-byte vector each a step; two passes over the row, the
+// second out of the cache. Bytes [k, kp) of a row are set to zero. A row with a NaN or an infinity gets the
+// scale NaN and zeros, so its scores are NaN; a row of zeros the scale 0. Bound by reading x.
 template <int T>
 __global__ __launch_bounds__(256) void k_quantize(const char* __restrict__ x, int64_t ld, int64_t rows, int k, int kp, int lanes,
                                                   int8_t* __restrict__ q, int64_t ldq, float* __restrict__ s) {
-  constexpr int ES = size_of(T);
+  constexpr int ES = size_of(T), NE = Vec<T>::NE;
   const int64_t row = (blockIdx.x * 256ll + threadIdx.x) / lanes;
   const int l = threadIdx.x & (lanes - 1);
   if (row >= rows) return;
   const char* src = x + row * ld;
   uint32_t top = 0;
-  for (int e0 = l * 4; e0 < k; e0 += lanes * 4)
+#pragma unroll 4
+  for (int e0 = l * NE; e0 < k; e0 += lanes * NE) {
+    const Vec<T> v = load_vec<T>(src + (int64_t)e0 * ES, k - e0);
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e0 + e < k) top = max(top, __builtin_bit_cast(uint32_t, load1<T>(src + (int64_t)(e0 + e) * ES)) & 0x7fffffffu);
+    for (int e = 0; e < NE; ++e) top = max(top, __float_as_uint(fabsf(v.v[e >> 2][e & 3])));  // a NaN's bits are the largest
+  }
   for (int o = lanes >> 1; o; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
   const bool bad = top >= 0x7f800000u;
   const float scale = bad ? NAN : __builtin_bit_cast(float, top) / 127.f;
   const bool none = bad || scale == 0.f;
   if (l == 0) s[row] = scale;
   int8_t* dst = q + row * ldq;
-  for (int e0 = l * 4; e0 < kp; e0 += lanes * 4) {
+#pragma unroll 4
+  for (int e0 = l * NE; e0 < kp; e0 += lanes * NE) {
+    uint32_t w[NE / 4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int at = e0 + e;
-      if (at < kp) dst[at] = at < k && !none ? (int8_t)to8(load1<T>(src + (int64_t)at * ES), scale) : 0;
+    for (int i = 0; i < NE / 4; ++i) w[i] = 0;
+    if (!none && e0 < k) {
+      const Vec<T> v = load_vec<T>(src + (int64_t)e0 * ES, k - e0);
+#pragma unroll
+      for (int e = 0; e < NE; ++e) w[e >> 2] |= (uint32_t)(uint8_t)(int8_t)to8(v.v[e >> 2][e & 3], scale) << (8 * (e & 3));
+    }
+    if (e0 + NE <= kp) {
+#pragma unroll
+      for (int i = 0; i < NE / 4; ++i) reinterpret_cast<Unaligned4*>(dst + e0)[i].v = w[i];
+    } else {
+#pragma unroll
+      for (int e = 0; e < NE; ++e)
+        if (e0 + e < kp) dst[e0 + e] = (int8_t)(w[e >> 2] >> (8 * (e & 3)));
     }
   }
 }
@@ -106,6 +125,28 @@ struct EpiScores {
   }
 };
 
+// k up to 128: one stage, and the outputs are what counts. A workgroup of 8 waves, 16 rows and 16 FP columns each,
+// in 32 KiB of LDS, so that three of them share a compute unit and some load and multiply while others store.
+template <int TO>
+__global__ __launch_bounds__(512, 6) void k_outer8(Problem a, EpiScores<TO> epi) {
+  using S = Shape<1, 8, TO == F32 ? 4 : 8, 1>;
+  __shared__ __attribute__((aligned(1024))) char s_all[32768];
+  int tp, tq;
+  tile_of(a, &tp, &tq);
+  const int64_t p0 = (int64_t)tp * S::BP, q0 = (int64_t)tq * S::BQ;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  lds_char *lp = (lds_char*)s_all, *lq = lp + S::BP * STAGE;
+  load_stage<I8, ROW, S::BP, 8>(lp, a.p, p0, 0, a.k);
+  load_stage<I8, ROW, S::BQ, 8>(lq, a.q, q0, 0, a.k);
+  i32x4 acc[S::FP][1];
+#pragma unroll
+  for (int i = 0; i < S::FP; ++i) acc[i][0] = i32x4{0, 0, 0, 0};
+  stage_barrier();
+  mul_stage<I8, ROW, ROW, S>(lp, lq, lane_base<I8, ROW, S::BP>(), lane_base<I8, ROW, S::BQ>(), 0, wave, acc);
+  __syncthreads();
+  epi.template run<S>(acc, p0, q0 + wave * 16, 0, 0, lp + wave * 4096);
+}
+
 int64_t div_up(int64_t v, int64_t by) { return (v + by - 1) / by; }
 int64_t up(int64_t v, int64_t to) { return div_up(v, to) * to; }
 
@@ -129,7 +170,16 @@ int scores(const Operand& w, const Operand& x, int k, const float* s, const floa
   const Problem a = {w, x, k, up(k, STAGE), 0, 0};
   const EpiScores<TO> epi = {(char*)out, ldo * size_of(TO), s, t, w.rows, x.rows};
   if (x.rows <= 32) return launch<TO, NarrowQ>(a, epi, st);
-  // one or two stages of k: two small workgroups a compute unit, so that one's stores run beside the other's loads
+  if (k <= STAGE) {
+    Problem o = a;
+    o.tiles_p = (int)div_up(w.rows, TO == F32 ? 64 : 128);
+    o.tiles_q = (int)div_up(x.rows, 128);
+    BLP_CHECK((int64_t)o.tiles_p * o.tiles_q <= 0x7fffffff, BLP_E_ARG, "scores8: too many tiles for one launch");
+    k_outer8<TO><<<(unsigned)(o.tiles_p * o.tiles_q), 512, 0, st>>>(o, epi);
+    BLP_HIP(hipGetLastError());
+    return 0;
+  }
+  // two stages of k: two small workgroups a compute unit, so that one's stores run beside the other's loads
   if (k > 2 * STAGE && div_up(w.rows, 256) * div_up(x.rows, 256) >= 192) return launch<TO, Big>(a, epi, st);
   return launch<TO, Mid>(a, epi, st);
 }
@@ -171,8 +221,9 @@ extern "C" int blp_quantize_rows(int device, void* stream, int type, const void*
   DeviceGuard guard(device);
   if (guard.rc) return guard.rc;
   hipStream_t st = (hipStream_t)stream;
+  const int ne = 16 / size_of(type);
   int lanes = 1;
-  while (lanes < 64 && lanes * 4 < k) lanes <<= 1;
+  while (lanes < 64 && lanes * ne < k) lanes <<= 1;
   const unsigned grid = (unsigned)div_up(rows * lanes, 256);
   const int kp = (int)std::min<int64_t>(ldq, up(k, 16));
   if (type == F32)
