@@ -116,7 +116,7 @@ struct EpiScores {
       for (int e = 0; e < 4; ++e) tp[i][e] = t[p0 + min(i * 16 + h * 4 + e, left - 1)];
 #pragma unroll
     for (int j = 0; j < S::FQ; ++j) sq[j] = s[q0 + min(j * 16 + l, rows - 1)];
-    store_block<TO, S>(scratch, out + q0 * ld + p0 * size_of(TO), ld, left, rows, [&](int i, int j) {
+    store_block<TO, S, true>(scratch, out + q0 * ld + p0 * size_of(TO), ld, left, rows, [&](int i, int j) {
       f32x4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j][e] * sq[j] * tp[i][e];

@@ -334,13 +334,13 @@ struct __attribute__((packed, aligned(2))) Unaligned16 {  // global memory takes
 // into rows of `out` (row q of the block at out + q ld bytes; element p at p * size): by way of LDS, so that a row's
 // elements leave as whole lines, 16 bytes a lane, instead of 8 bytes from 16 rows each. Rows from nq and elements
 // from np on are not written. LDS rows are a power of two of bytes; their granules are swapped by the row's number,
-// which spreads both the writes and the reads over the banks.
+// which spreads both the writes and the reads over the banks. NT: stores that do not stay in the cache.
 __host__ __device__ constexpr int pow2_up(int v) {
   int p = 1;
   while (p < v) p <<= 1;
   return p;
 }
-template <int TO, class S, class F>
+template <int TO, class S, bool NT = false, class F>
 __device__ inline void store_block(lds_char* scratch, char* out, int64_t ld, int64_t np, int64_t nq, F value) {
   constexpr int ES = size_of(TO), ROWB = pow2_up(S::FP * 16 * ES), GR = ROWB / 16;  // bytes, granules of an LDS row
   constexpr int J = S::FQ * 16 * ROWB > 16384 ? S::FQ / 2 : S::FQ;         // blocks of 16 rows a pass
@@ -379,7 +379,7 @@ __device__ inline void store_block(lds_char* scratch, char* out, int64_t ld, int
       if (q >= nq) continue;
       char* at = out + q * ld + p * ES;
       if (p + 16 / ES <= np) {
-        reinterpret_cast<Unaligned16*>(at)->v = v;
+        if constexpr (NT) __builtin_nontemporal_store(v, &reinterpret_cast<Unaligned16*>(at)->v); else reinterpret_cast<Unaligned16*>(at)->v = v;
       } else if (p < np) {
 #pragma unroll
         for (int e = 0; e < 16 / ES; ++e)
