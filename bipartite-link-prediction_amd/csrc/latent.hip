@@ -8,6 +8,11 @@
 // recomputes them piece by piece of the catalogue into a workspace of dS, from which the two products of
 // the gradient are taken. Four products of 2 M N k operations in all; the workspace is bounded.
 //
+// Float factors go through the matrix cores as three halves each: x1 = x rounded to bfloat16, x2 = x - x1 rounded,
+// x3 = x - x1 - x2, together all 24 bits; of the nine products of two such sums the six largest are taken (the others lie
+// below 2^-25 of the product), each exact in the 32-bit accumulators. That is 6 matrix instructions of 16 cycles for
+// 16 x 16 x 32 products where the float instructions take 256 cycles.
+//
 // A row whose target lies outside [0, n_cols) is ignored: loss 0, gradient 0, and its x is never multiplied
 // (it may hold anything, NaN too).
 #include <algorithm>
@@ -21,6 +26,10 @@ using namespace blp::tile;
 
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LN2 = 0.69314718055994530942f;
+
+// The matrix instructions' type, and the planes a factor is held in.
+constexpr int mma_type(int t) { return t == F32 ? BF16 : t; }
+constexpr int planes_of(int t) { return t == F32 ? 3 : 1; }
 
 using blp::DeviceGuard;
 using Targets = blp::Ids;  // the target of row i, or -1 (ignored)
@@ -52,6 +61,36 @@ __global__ __launch_bounds__(256) void k_pack(const char* __restrict__ src, int6
       }
     }
     reinterpret_cast<i32x4*>(dst)[i] = v;
+  }
+}
+
+// The same of floats into the three planes of halves, `plane` bytes apart. An infinite or NaN factor (or one that rounds
+// to infinity) has nothing in the lower planes.
+__global__ __launch_bounds__(256) void k_pack_planes(const char* __restrict__ src, int64_t ld, int64_t rows, int k, int kp,
+                                                     Targets targets, char* __restrict__ dst, int64_t plane) {
+  const int per = kp / 8;
+  const int64_t n = rows * per, step = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += step) {
+    const int64_t r = i / per;
+    const int e0 = (int)(i - r * per) * 8;
+    bf16x8 v[3];
+    const bool keep = !targets.at || targets(r) >= 0;
+    const float* s = reinterpret_cast<const float*>(src + r * ld) + e0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = keep && e0 + e < k ? s[e] : 0.f;
+      __bf16 a = (__bf16)x;
+      if (!(fabsf((float)a) <= 3.4e38f) && fabsf(x) <= 3.4028235e38f)  // rounded up past the largest: cut off instead
+        a = __builtin_bit_cast(__bf16, (uint16_t)(__float_as_uint(x) >> 16));
+      const bool finite = fabsf(x) <= 3.4028235e38f;
+      const float b = finite ? x - (float)a : 0.f;
+      const __bf16 b1 = (__bf16)b;
+      v[0][e] = a;
+      v[1][e] = b1;
+      v[2][e] = (__bf16)(b - (float)b1);
+    }
+#pragma unroll
+    for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(dst + p * plane + i * 16) = v[p];
   }
 }
 
@@ -209,7 +248,8 @@ template <int T>
 struct EpiGrad {
   static constexpr bool SCRATCH = true;
   char* ds;
-  int64_t ld;  // elements
+  int64_t ld;     // elements
+  int64_t plane;  // floats: bytes between the planes of dS
   const float* lse;
   RowGrad g;
   Targets targets;
@@ -231,18 +271,38 @@ struct EpiGrad {
       gr[j] = t >= 0 ? g.row(row) : 0.f;
       l2[j] = t >= 0 ? -lse[row] * LOG2E : -INFINITY;
     }
-    store_block<T, S>(scratch, ds + (q0 * ld + p0) * size_of(T), ld * size_of(T), (int)min(ld - p0, (int64_t)(S::FP * 16)), rows,
-                      [&](int i, int j) {
-                        f32x4 v;
+    constexpr int MT = mma_type(T);
+    const int width = (int)min(ld - p0, (int64_t)(S::FP * 16));
+    char* at = ds + (q0 * ld + p0) * size_of(MT);
+    auto value = [&](int i, int j) {
+      f32x4 v;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                          float d = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, l2[j]));
-                          if (hit[j] == i * 16 + e) d -= 1.f;
-                          d *= gr[j];
-                          v[e] = left == S::FP * 16 || i * 16 + h * 4 + e < left ? d : 0.f;
-                        }
-                        return v;
-                      });
+      for (int e = 0; e < 4; ++e) {
+        float d = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, l2[j]));
+        if (hit[j] == i * 16 + e) d -= 1.f;
+        d *= gr[j];
+        v[e] = left == S::FP * 16 || i * 16 + h * 4 + e < left ? d : 0.f;
+      }
+      return v;
+    };
+    if constexpr (T != F32) {
+      store_block<MT, S>(scratch, at, ld * size_of(MT), width, rows, value);
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::FP; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FQ; ++j) acc[i][j] = value(i, j);
+#pragma unroll 1
+      for (int p = 0; p < 3; ++p) {
+        store_block<MT, S>(scratch, at + p * plane, ld * size_of(MT), width, rows, [&](int i, int j) { return acc[i][j]; });
+#pragma unroll
+        for (int i = 0; i < S::FP; ++i)
+#pragma unroll
+          for (int j = 0; j < S::FQ; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] -= (float)(__bf16)acc[i][j][e];
+      }
+    }
   }
 };
 
@@ -305,7 +365,7 @@ __global__ __launch_bounds__(256) void k_sum_parts(const float* __restrict__ par
 }
 
 // ---------------------------------------------------------------- narrow factors
-// Halves with k up to 128: the scores never leave the registers, in the backward pass either. A wave holds
+// Halves with k up to 128, floats up to 64: the scores never leave the registers, in the backward pass either. A wave holds
 // 16 FO rows of one side ("own") as fragments for the whole kernel and the other side ("stream") passes through
 // LDS, 64 rows a stage, two stages in turn:
 //   LSE  own x, stream w: a running (max, sum of exp2) a lane, joined over the lanes at the end
@@ -335,6 +395,7 @@ enum NarrowMode { LSE, DX, DW };
 
 struct NarrowArgs {
   Operand own, stream;
+  int64_t own_plane, stream_plane;  // floats: bytes between the planes
   int kp;
   int64_t range;  // stream rows of a split, a multiple of 64
   int own_tiles, splits;
@@ -362,13 +423,15 @@ __device__ inline int pack2(float a, float b) {
 }
 
 template <int T, int KS, int MODE, bool PER_ROW, class Epi>
-__global__ __launch_bounds__(256, KS > 2 ? 3 : 4) void k_narrow(NarrowArgs a, Epi epi) {
+__global__ __launch_bounds__(256, KS > 3 ? 2 : KS > 2 || T == F32 ? 3 : 4) void k_narrow(NarrowArgs a, Epi epi) {
+  constexpr int MT = mma_type(T), PL = planes_of(T);
   constexpr int FO = 2;                              // own fragments of 16 rows a wave
   constexpr int HALVES = KS > 2 ? 2 : 1;             // 128-byte parts of a row
   constexpr int PART = 64 * STAGE;                   // bytes of one part of a stage
-  constexpr int BUF = HALVES * PART;
-  constexpr int COPIES = 2 * HALVES + (MODE == DW);  // a wave issues for a stage
-  __shared__ __attribute__((aligned(1024))) char s_a[BUF], s_b[BUF], s_c[BUF];
+  constexpr int BUF = PL * HALVES * PART;
+  constexpr int COPIES = 2 * PL * HALVES + (MODE == DW);  // a wave issues for a stage
+  constexpr bool THREE = PL == 1;                         // buffers (floats: two, a stage of theirs lasts longer)
+  __shared__ __attribute__((aligned(1024))) char s_a[BUF], s_b[BUF], s_c[THREE ? BUF : 16];
   __shared__ __attribute__((aligned(1024))) char s_ra[MODE == DW ? 1024 : 16], s_rb[MODE == DW ? 1024 : 16],
       s_rc[MODE == DW ? 1024 : 16];
   // a die's workgroups take neighbouring own tiles of one split: the split's rows stay in its L2
@@ -383,18 +446,20 @@ __global__ __launch_bounds__(256, KS > 2 ? 3 : 4) void k_narrow(NarrowArgs a, Ep
   const float c = fmaxf(fabsf(a.scale) * LOG2E, 1.2e-38f);  // positive: -inf c is -inf for a scale of 0, too
   const Operand stream = {a.stream.base, a.stream.ld, s1};
 
-  frag_t own[FO][KS];
+  frag_t own[PL][FO][KS];
 #pragma unroll
-  for (int j = 0; j < FO; ++j) {
-    const int64_t r = own0 + j * 16 + l;
+  for (int p = 0; p < PL; ++p)
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      own[j][s] = frag_t{0, 0, 0, 0};
-      if (r < a.own.rows && s * 32 + h * 8 < a.kp)
-        own[j][s] = *reinterpret_cast<const frag_t*>(a.own.base + r * a.own.ld + (s * 32 + h * 8) * 2);
-      if (a.scale < 0.f) own[j][s] ^= (int)0x80008000;  // the scores' sign, so that c is positive
+    for (int j = 0; j < FO; ++j) {
+      const int64_t r = own0 + j * 16 + l;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        own[p][j][s] = frag_t{0, 0, 0, 0};
+        if (r < a.own.rows && s * 32 + h * 8 < a.kp)
+          own[p][j][s] = *reinterpret_cast<const frag_t*>(a.own.base + p * a.own_plane + r * a.own.ld + (s * 32 + h * 8) * 2);
+        if (a.scale < 0.f) own[p][j][s] ^= (int)0x80008000;  // the scores' sign, so that c is positive
+      }
     }
-  }
   // a lane's own rows: LSE: targets; DX: lse and targets; DW: w rows (nothing)
   int target[FO];
   float lane_l2[FO], lane_g[FO];
@@ -426,14 +491,17 @@ __global__ __launch_bounds__(256, KS > 2 ? 3 : 4) void k_narrow(NarrowArgs a, Ep
 #pragma unroll
     for (int i = 0; i < 2 * KS; ++i) out[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const uint32_t base_row = lane_base<T, ROW, 64>();
+  const uint32_t base_row = lane_base<MT, ROW, 64>();
   const uint32_t base_tr = (4 * h + (l >> 2)) * STAGE + (((l & 3) >> 1) ^ (4 * (h & 1) + (l >> 2))) * 16 + (l & 1) * 8;
 
   auto load = [&](char* buf, char* rbuf, int t) {
     const int64_t r0 = s0 + (int64_t)t * 64;
 #pragma unroll
-    for (int p = 0; p < HALVES; ++p)
-      load_stage<T, ROW, 64, 4>((lds_char*)buf + p * PART, stream, r0, p * 64, a.kp);
+    for (int p = 0; p < PL; ++p)
+#pragma unroll
+      for (int s = 0; s < HALVES; ++s)
+        load_stage<MT, ROW, 64, 4>((lds_char*)buf + (p * HALVES + s) * PART,
+                                   Operand{stream.base + p * a.stream_plane, stream.ld, s1}, r0, s * 64, a.kp);
     if constexpr (MODE == DW)  // by every wave alike, so that their counts agree
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc_at((const char*)a.rows.of(min(r0, a.stream.rows - 1) >> 6)),
                                                (__attribute__((address_space(3))) void*)(lds_char*)rbuf, 16, lane * 16, 0, 0, 0);
@@ -441,19 +509,26 @@ __global__ __launch_bounds__(256, KS > 2 ? 3 : 4) void k_narrow(NarrowArgs a, Ep
   auto compute = [&](const char* buf, const char* rbuf, int t) {
     const lds_char* lds = (const lds_char*)buf;
     const int r0 = (int)(s0 + (int64_t)t * 64);  // stream rows fit 31 bits
-    if constexpr (MODE == LSE) {
-      auto products = [&](int half, f32x4(&acc)[2][FO]) {
+    // 32 stream rows' products with the own rows
+    auto products = [&](int half, f32x4(&acc)[2][FO]) {
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int x = 0; x < PL; ++x) {
           frag_t p[2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) p[i] = read_frag<T, ROW, 64>(lds + (s >> 1) * PART, base_row, half * 2 + i, s & 1);
-#pragma unroll
           for (int i = 0; i < 2; ++i)
+            p[i] = read_frag<MT, ROW, 64>(lds + (x * HALVES + (s >> 1)) * PART, base_row, half * 2 + i, s & 1);
 #pragma unroll
-            for (int j = 0; j < FO; ++j) acc[i][j] = mma<T>(p[i], own[j][s], s ? acc[i][j] : f32x4{0.f, 0.f, 0.f, 0.f});
+          for (int y = 0; y < PL - x; ++y)  // floats: the six larger products of the planes
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int j = 0; j < FO; ++j)
+                acc[i][j] = mma<MT>(p[i], own[y][j][s], s + x + y ? acc[i][j] : f32x4{0.f, 0.f, 0.f, 0.f});
         }
-      };
+    };
+    if constexpr (MODE == LSE) {
       bool slow = t == 0 || s1 - r0 < 64;
 #pragma unroll
       for (int j = 0; j < FO; ++j) slow |= (unsigned)(target[j] - r0) < 64u;
@@ -495,7 +570,7 @@ __global__ __launch_bounds__(256, KS > 2 ? 3 : 4) void k_narrow(NarrowArgs a, Ep
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int r = first + i * 16 + e;
-              if (r == target[j]) a.hit[own0 + j * 16 + l] = acc[i][j][e] * fabsf(a.scale);
+              if (r == target[j] && r < (int)s1) a.hit[own0 + j * 16 + l] = acc[i][j][e] * fabsf(a.scale);
               if (r >= (int)s1) acc[i][j][e] = -INFINITY;  // past the range's end: zeros in LDS
               high = fmaxf(high, acc[i][j][e]);
             }
@@ -524,16 +599,7 @@ __global__ __launch_bounds__(256, KS > 2 ? 3 : 4) void k_narrow(NarrowArgs a, Ep
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         f32x4 acc[2][FO];
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          frag_t p[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) p[i] = read_frag<T, ROW, 64>(lds + (s >> 1) * PART, base_row, half * 2 + i, s & 1);
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < FO; ++j) acc[i][j] = mma<T>(p[i], own[j][s], s ? acc[i][j] : f32x4{0.f, 0.f, 0.f, 0.f});
-        }
+        products(half, acc);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           f32x4 l2, g;
@@ -570,44 +636,71 @@ __global__ __launch_bounds__(256, KS > 2 ? 3 : 4) void k_narrow(NarrowArgs a, Ep
 #pragma unroll
             for (int j = 0; j < FO; ++j) acc[i][j] *= g;
         }
-        frag_t q[FO];
+        frag_t q[PL][FO];
 #pragma unroll
-        for (int j = 0; j < FO; ++j)
-          q[j] = frag_t{pack2<T>(acc[0][j][0], acc[0][j][1]), pack2<T>(acc[0][j][2], acc[0][j][3]),
-                        pack2<T>(acc[1][j][0], acc[1][j][1]), pack2<T>(acc[1][j][2], acc[1][j][3])};
+        for (int p = 0; p < PL; ++p)
 #pragma unroll
-        for (int d = 0; d < 2 * KS; ++d) {
-          const lds_char* at = lds + (base_tr ^ ((d & 3) << 5)) + (d >> 2) * PART + half * 32 * STAGE;
-          i32x4 v;
+          for (int j = 0; j < FO; ++j)
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const s16x4 tr = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + s * 16 * STAGE));
-            const i32x2 w = __builtin_bit_cast(i32x2, tr);
-            v[2 * s] = w[0];
-            v[2 * s + 1] = w[1];
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int w = 0; w < 2; ++w) {
+                const int both = pack2<MT>(acc[i][j][2 * w], acc[i][j][2 * w + 1]);
+                q[p][j][2 * i + w] = both;
+                if (p + 1 < PL) {  // what the plane left over
+                  acc[i][j][2 * w] -= __uint_as_float((uint32_t)both << 16);
+                  acc[i][j][2 * w + 1] -= __uint_as_float((uint32_t)both & 0xffff0000u);
+                }
+              }
+#pragma unroll
+        for (int d = 0; d < 2 * KS; ++d)
+#pragma unroll
+          for (int x = 0; x < PL; ++x) {
+            const lds_char* at = lds + (base_tr ^ ((d & 3) << 5)) + (x * HALVES + (d >> 2)) * PART + half * 32 * STAGE;
+            i32x4 v;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              const s16x4 tr = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + s * 16 * STAGE));
+              const i32x2 w = __builtin_bit_cast(i32x2, tr);
+              v[2 * s] = w[0];
+              v[2 * s + 1] = w[1];
+            }
+#pragma unroll
+            for (int y = 0; y < PL - x; ++y)
+#pragma unroll
+              for (int j = 0; j < FO; ++j) out[d][j] = mma<MT>(v, q[y][j], out[d][j]);
           }
-#pragma unroll
-          for (int j = 0; j < FO; ++j) out[d][j] = mma<T>(v, q[j], out[d][j]);
-        }
       }
     }
   };
 
-  // Three buffers, two stages ahead. Stages past the range copy nothing and count for nothing: their rows are zeros
-  // (LSE masks them), so every trip takes three and the counts of outstanding copies stay the same.
+  // Three buffers, two stages ahead (floats: two, one ahead). Stages past the range copy nothing and count for nothing: their rows are zeros
+  // (LSE masks them), so every trip takes all buffers and the counts of outstanding copies stay the same.
   load(s_a, s_ra, 0);
-  load(s_b, s_rb, 1);
+  if constexpr (THREE) {
+    load(s_b, s_rb, 1);
 #pragma unroll 1
-  for (int t = 0; t < stages; t += 3) {
-    ring_barrier<COPIES>();
-    load(s_c, s_rc, t + 2);
-    compute(s_a, s_ra, t);
-    ring_barrier<COPIES>();
-    load(s_a, s_ra, t + 3);
-    compute(s_b, s_rb, t + 1);
-    ring_barrier<COPIES>();
-    load(s_b, s_rb, t + 4);
-    compute(s_c, s_rc, t + 2);
+    for (int t = 0; t < stages; t += 3) {
+      ring_barrier<COPIES>();
+      load(s_c, s_rc, t + 2);
+      compute(s_a, s_ra, t);
+      ring_barrier<COPIES>();
+      load(s_a, s_ra, t + 3);
+      compute(s_b, s_rb, t + 1);
+      ring_barrier<COPIES>();
+      load(s_b, s_rb, t + 4);
+      compute(s_c, s_rc, t + 2);
+    }
+  } else {
+#pragma unroll 1
+    for (int t = 0; t < stages; t += 2) {
+      ring_barrier<0>();
+      load(s_b, s_rb, t + 1);
+      compute(s_a, s_ra, t);
+      ring_barrier<0>();
+      load(s_a, s_ra, t + 2);
+      compute(s_b, s_rb, t + 1);
+    }
   }
   __builtin_amdgcn_s_waitcnt(0x0f70);  // nothing in flight towards LDS when the workgroup ends
 
@@ -629,7 +722,7 @@ __global__ __launch_bounds__(256, KS > 2 ? 3 : 4) void k_narrow(NarrowArgs a, Ep
     lds_char* scratch = nullptr;
     if constexpr (Epi::SCRATCH) {  // a wave's 32 rows of up to 128 halves: the ring's buffers in parts
       __syncthreads();
-      constexpr int WAVE = 16 * FO * pow2_up(64 * KS);
+      constexpr int WAVE = 16 * FO * pow2_up(32 * KS * size_of(T));
       if constexpr (WAVE * 4 <= BUF)
         scratch = (lds_char*)s_a + wave * WAVE;
       else
@@ -676,18 +769,17 @@ struct Layout {
 // One product's slices over k: enough workgroups, at least 4 stages a slice.
 struct Slices {
   int shape, n;
-  int64_t k_slice;
+  int stages;  // a slice
 };
-Slices slices_of(int64_t np, int64_t nq, int64_t k, int ke) {
+Slices slices_of(int64_t np, int64_t nq, int64_t k, int planes) {
   Slices s;
   s.shape = shape_of(np, nq);
   const int64_t tiles = std::max<int64_t>(div_up(np, bp_of(s.shape)) * div_up(nq, bq_of(s.shape)), 1);
-  const int64_t stages = div_up(k, ke);
+  const int64_t stages = div_up(k, STAGE / 2) * (planes == 1 ? 1 : SEGMENTS);
   int64_t n = tiles >= GOAL / 2 ? 1 : std::min(GOAL / tiles, std::max<int64_t>(stages / 4, 1));
   n = std::min<int64_t>(std::max<int64_t>(n, 1), 64);
-  const int64_t per = std::max<int64_t>(div_up(stages, n), 1);
-  s.n = (int)std::max<int64_t>(div_up(stages, per), 1);
-  s.k_slice = per * ke;
+  s.stages = (int)std::max<int64_t>(div_up(stages, n), 1);
+  s.n = (int)std::max<int64_t>(div_up(stages, s.stages), 1);
   return s;
 }
 
@@ -696,60 +788,64 @@ struct Splits {
   int own_tiles, n;
   int64_t range;
 };
-Splits splits_of(int64_t own, int own_rows, int64_t stream, int64_t goal) {
+Splits splits_of(int64_t own, int own_rows, int64_t stream, int64_t goal, int trip) {
   Splits s;
   s.own_tiles = (int)div_up(own, own_rows);
   const int64_t stages = div_up(stream, 64);
   const int64_t n = std::max<int64_t>(std::min(goal / std::max(s.own_tiles, 1), stages / 2), 1);
-  const int64_t per = up(std::max<int64_t>(div_up(stages, n), 1), 3);  // three stages a trip
+  const int64_t per = up(std::max<int64_t>(div_up(stages, n), 1), trip);
   s.n = (int)std::max<int64_t>(div_up(stages, per), 1);
   s.range = per * 64;
   return s;
 }
 
 struct Plan {
-  bool narrow;  // halves, k <= 128: k_narrow
-  int ks;
-  Splits nl, nx, nw;
-  int64_t o_rows;
-  int type, es, ge, ke, kp;
+  int type, es;         // the caller's type and its size
+  int planes, kp;       // the engine's: planes of halves, kp of them a row
   int64_t m, n;
   int k;
   bool grads, pack_w, pack_x;
-  int fwd;
+  bool narrow;          // k_narrow
+  int ks;
+  Splits nl, nx, nw;
+  int fwd;              // else k_product
   int64_t fwd_tiles;
   int64_t piece, pieces;
   Slices sx, sw;
-  int64_t o_x, o_w, o_part, o_hit, o_top, o_ds, o_px, o_pw, bytes;
+  int64_t o_x, o_w, o_part, o_hit, o_top, o_rows, o_ds, o_px, o_pw, bytes;
+  int64_t x_plane() const { return m * kp * 2; }
+  int64_t w_plane() const { return n * kp * 2; }
+  int64_t ds_plane() const { return m * piece * 2; }
 };
+constexpr int KE = STAGE / 2;  // halves of k a stage
 
 bool aligned(const void* p, int64_t ld_bytes, int64_t row_bytes) {
   return (((uintptr_t)p | (uintptr_t)ld_bytes | (uintptr_t)row_bytes) & 15) == 0;
 }
 
-// `pack_w`: whether the catalogue has to be packed (its rows are not whole aligned granules)
+// `pack_x`, `pack_w`: whether the rows have to be packed (they are not whole aligned granules)
 Plan plan_of(int type, int64_t m, int64_t n, int k, bool forward, bool grads, bool pack_x, bool pack_w) {
   Plan p;
   p.type = type;
   p.es = size_of(type);
-  p.ge = 16 / p.es;
-  p.ke = STAGE / p.es;
-  p.kp = (int)up(k, p.ge);
+  p.planes = planes_of(type);
+  p.kp = (int)up(k, 8);
   p.m = m;
   p.n = n;
   p.k = k;
   p.grads = grads;
-  p.pack_w = pack_w;
-  p.pack_x = grads || pack_x;
+  p.pack_w = pack_w || type == F32;
+  p.pack_x = grads || pack_x || type == F32;
   Layout l;
-  p.o_x = l.take(p.pack_x ? m * p.kp * p.es : 0);
-  p.o_w = l.take(pack_w ? n * p.kp * p.es : 0);
-  p.narrow = type != F32 && p.kp <= 128;
+  p.o_x = l.take(p.pack_x ? p.planes * p.x_plane() : 0);
+  p.o_w = l.take(p.pack_w ? p.planes * p.w_plane() : 0);
+  p.narrow = p.kp <= (type == F32 ? 64 : 128);
   if (p.narrow) {
     p.ks = (p.kp + 31) / 32;
-    p.nl = splits_of(m, 128, n, 4 * GOAL);
-    p.nx = splits_of(m, 128, n, 2 * GOAL);
-    p.nw = splits_of(n, 128, m, 2 * GOAL);
+    const int trip = type == F32 ? 2 : 3;  // stages of a trip of k_narrow's loop
+    p.nl = splits_of(m, 128, n, 4 * GOAL, trip);
+    p.nx = splits_of(m, 128, n, 2 * GOAL, trip);
+    p.nw = splits_of(n, 128, m, 2 * GOAL, trip);
     p.o_part = l.take(forward ? p.nl.n * m * 8 : 0);
     p.o_hit = l.take(forward ? m * 4 : 0);
     p.o_top = l.take(16);
@@ -766,13 +862,13 @@ Plan plan_of(int type, int64_t m, int64_t n, int k, bool forward, bool grads, bo
   p.o_top = l.take(16);
   if (grads) {
     // whole tiles of columns within the budget, the pieces as equal as that allows
-    const int64_t most = std::max<int64_t>(PIECE_BYTES / (std::max<int64_t>(m, 1) * p.es) / 256 * 256, 256);
+    const int64_t most = std::max<int64_t>(PIECE_BYTES / (std::max<int64_t>(m, 1) * 2 * p.planes) / 256 * 256, 256);
     p.pieces = div_up(n, most);
     p.piece = std::min(up(div_up(n, p.pieces), 256), up(n, 64));
     p.pieces = div_up(n, p.piece);
-    p.o_ds = l.take(m * p.piece * p.es);
-    p.sx = slices_of(k, m, std::min(p.piece, n), p.ke);
-    p.sw = slices_of(k, p.piece, m, p.ke);
+    p.o_ds = l.take(p.planes * p.ds_plane());
+    p.sx = slices_of(k, m, std::min(p.piece, n), p.planes);
+    p.sw = slices_of(k, p.piece, m, p.planes);
     p.o_px = l.take(p.sx.n > 1 || p.pieces > 1 ? (int64_t)p.sx.n * m * up(k, 4) * 4 : 0);
     p.o_pw = l.take(p.sw.n > 1 ? (int64_t)p.sw.n * p.piece * up(k, 4) * 4 : 0);
   }
@@ -780,21 +876,28 @@ Plan plan_of(int type, int64_t m, int64_t n, int k, bool forward, bool grads, bo
   return p;
 }
 
+template <int T, int LP, int LQ, class S, class Epi>
+void launch(const Problem& a, dim3 grid, const Epi& epi, hipStream_t st) {
+  k_product<mma_type(T), LP, LQ, T == F32, S, Epi><<<grid, S::THREADS, 0, st>>>(a, epi);
+}
+
+// `stages`: of a slice (0: all)
 template <int T, int LP, int LQ, class Epi>
-int product(int shape, Problem a, int slices, Epi epi, hipStream_t st) {
+int product(int shape, Problem a, int slices, int stages, Epi epi, hipStream_t st) {
   const int64_t tp = div_up(a.p.rows, bp_of(shape)), tq = div_up(a.q.rows, bq_of(shape));
   BLP_CHECK(tp * tq <= 0x7fffffff, BLP_E_ARG, "softmax loss: too many tiles for one launch");
   a.tiles_p = (int)tp;
   a.tiles_q = (int)tq;
+  a.slice = stages ? stages : (int)div_up(a.k, KE) * (T == F32 ? SEGMENTS : 1);
   const dim3 grid((unsigned)(tp * tq), (unsigned)slices);
   if (shape == BIG)
-    k_product<T, LP, LQ, Big, Epi><<<grid, Big::THREADS, 0, st>>>(a, epi);
+    launch<T, LP, LQ, Big>(a, grid, epi, st);
   else if (shape == MID)
-    k_product<T, LP, LQ, Mid, Epi><<<grid, Mid::THREADS, 0, st>>>(a, epi);
+    launch<T, LP, LQ, Mid>(a, grid, epi, st);
   else if (shape == NARROW_P)
-    k_product<T, LP, LQ, NarrowP, Epi><<<grid, NarrowP::THREADS, 0, st>>>(a, epi);
+    launch<T, LP, LQ, NarrowP>(a, grid, epi, st);
   else
-    k_product<T, LP, LQ, NarrowQ, Epi><<<grid, NarrowQ::THREADS, 0, st>>>(a, epi);
+    launch<T, LP, LQ, NarrowQ>(a, grid, epi, st);
   BLP_HIP(hipGetLastError());
   return 0;
 }
@@ -802,9 +905,13 @@ int product(int shape, Problem a, int slices, Epi epi, hipStream_t st) {
 int64_t grid_for(int64_t n) { return std::max<int64_t>(std::min<int64_t>(div_up(n, 256), 8192), 1); }
 
 template <int T>
-int pack(const char* src, int64_t ld, int64_t rows, int k, int kp, Targets t, char* dst, hipStream_t st) {
+int pack(const char* src, int64_t ld, int64_t rows, int k, int kp, Targets t, char* dst, int64_t plane, hipStream_t st) {
   if (rows == 0) return 0;
-  k_pack<size_of(T)><<<grid_for(rows * (kp * size_of(T) / 16)), 256, 0, st>>>(src, ld, rows, k, kp, t, dst);
+  const int64_t grid = grid_for(rows * (kp / 8));
+  if constexpr (T == F32)
+    k_pack_planes<<<grid, 256, 0, st>>>(src, ld, rows, k, kp, t, dst, plane);
+  else
+    k_pack<2><<<grid, 256, 0, st>>>(src, ld, rows, k, kp, t, dst);
   BLP_HIP(hipGetLastError());
   return 0;
 }
@@ -827,12 +934,12 @@ int bind(Call& c, const void* x, int64_t ldx, const void* w, int64_t ldw) {
   if (p.pack_x) {
     Targets t = c.targets;
     if (!p.grads) t.at = nullptr;
-    rc = pack<T>(c.x.base, c.x.ld, p.m, p.k, p.kp, t, c.ws + p.o_x, c.st);
-    c.x = {c.ws + p.o_x, (int64_t)p.kp * p.es, p.m};
+    rc = pack<T>(c.x.base, c.x.ld, p.m, p.k, p.kp, t, c.ws + p.o_x, p.x_plane(), c.st);
+    c.x = {c.ws + p.o_x, (int64_t)p.kp * 2, p.m};
   }
   if (!rc && p.pack_w) {
-    rc = pack<T>(c.w.base, c.w.ld, p.n, p.k, p.kp, Targets{nullptr, 0, 0}, c.ws + p.o_w, c.st);
-    c.w = {c.ws + p.o_w, (int64_t)p.kp * p.es, p.n};
+    rc = pack<T>(c.w.base, c.w.ld, p.n, p.k, p.kp, Targets{nullptr, 0, 0}, c.ws + p.o_w, p.w_plane(), c.st);
+    c.w = {c.ws + p.o_w, (int64_t)p.kp * 2, p.n};
   }
   return rc;
 }
@@ -849,14 +956,16 @@ int narrow(const Plan& p, const NarrowArgs& a, Epi epi, hipStream_t st) {
   BLP_CHECK(blocks <= 0x7fffffff, BLP_E_ARG, "softmax loss: too many tiles for one launch");
   if (blocks == 0) return 0;
   const unsigned grid = (unsigned)blocks;
-  if (p.ks == 1)
+  if (p.ks == 1) {
     k_narrow<T, 1, MODE, PER_ROW, Epi><<<grid, 256, 0, st>>>(a, epi);
-  else if (p.ks == 2)
+  } else if (p.ks == 2) {
     k_narrow<T, 2, MODE, PER_ROW, Epi><<<grid, 256, 0, st>>>(a, epi);
-  else if (p.ks == 3)
-    k_narrow<T, 3, MODE, PER_ROW, Epi><<<grid, 256, 0, st>>>(a, epi);
-  else
-    k_narrow<T, 4, MODE, PER_ROW, Epi><<<grid, 256, 0, st>>>(a, epi);
+  } else if constexpr (T != F32) {
+    if (p.ks == 3)
+      k_narrow<T, 3, MODE, PER_ROW, Epi><<<grid, 256, 0, st>>>(a, epi);
+    else
+      k_narrow<T, 4, MODE, PER_ROW, Epi><<<grid, 256, 0, st>>>(a, epi);
+  }
   BLP_HIP(hipGetLastError());
   return 0;
 }
@@ -888,15 +997,14 @@ int forward(const Call& c, float* loss, float* lse, float* total, int mean) {
   if (p.m > 0) {
     float2* part = (float2*)(c.ws + p.o_part);
     float* hit = (float*)(c.ws + p.o_hit);
-    int rc = 0;
-    if constexpr (T != F32) {
-      if (p.narrow)
-        rc = narrow<T, LSE, false>(p, NarrowArgs{c.x, c.w, p.kp, p.nl.range, p.nl.own_tiles, p.nl.n, c.scale, 1.f, c.targets, part, hit},
-                                   NoEpilogue{}, c.st);
-    }
-    if (!p.narrow) {
-      const Problem a = {c.w, c.x, p.kp, up(p.kp, p.ke), 0, 0};
-      rc = product<T, ROW, ROW>(p.fwd, a, 1, EpiLse<T>{part, hit, c.targets, p.n, p.m, c.scale}, c.st);
+    int rc;
+    if (p.narrow) {
+      const NarrowArgs a = {c.x, c.w, p.x_plane(), p.w_plane(), p.kp, p.nl.range, p.nl.own_tiles, p.nl.n, c.scale, 1.f, c.targets,
+                            part, hit, Rows{nullptr}};
+      rc = narrow<T, LSE, false>(p, a, NoEpilogue{}, c.st);
+    } else {
+      const Problem a = {c.w, c.x, p.kp, 0, 0, 0, p.w_plane(), p.x_plane()};
+      rc = product<T, ROW, ROW>(p.fwd, a, 1, 0, EpiLse<T>{part, hit, c.targets, p.n, p.m, c.scale}, c.st);
     }
     if (rc) return rc;
     k_join<<<(unsigned)div_up(p.m, 32), 256, 0, c.st>>>(part, p.narrow ? p.nl.n : p.fwd_tiles, p.m, hit, c.targets, loss, lse);
@@ -928,16 +1036,16 @@ int backward(const Call& c, const float* lse, RowGrad g, void* dx, int64_t lddx,
     BLP_HIP(hipGetLastError());
     g.top = top;
   }
-  if constexpr (T != F32) {
-    if (p.narrow) {
-      NarrowArgs a = {c.x, c.w, p.kp, 0, 0, 0, c.scale, g.extra, c.targets, nullptr, nullptr, Rows{(float*)(c.ws + p.o_rows)}};
-      k_rows<<<(unsigned)div_up(p.m, 64), 64, 0, c.st>>>(lse, g, c.targets, p.m, a.rows);
-      BLP_HIP(hipGetLastError());
-      int rc = dx ? narrow_grad<T, DX>(c, a, p.nx, g, (float*)(c.ws + p.o_px), dx, lddx, p.m) : 0;
-      std::swap(a.own, a.stream);
-      if (!rc && dw) rc = narrow_grad<T, DW>(c, a, p.nw, g, (float*)(c.ws + p.o_pw), dw, lddw, p.n);
-      return rc;
-    }
+  if (p.narrow) {
+    NarrowArgs a = {c.x, c.w, p.x_plane(), p.w_plane(), p.kp, 0, 0, 0, c.scale, g.extra, c.targets, nullptr, nullptr,
+                    Rows{(float*)(c.ws + p.o_rows)}};
+    k_rows<<<(unsigned)div_up(p.m, 64), 64, 0, c.st>>>(lse, g, c.targets, p.m, a.rows);
+    BLP_HIP(hipGetLastError());
+    int rc = dx ? narrow_grad<T, DX>(c, a, p.nx, g, (float*)(c.ws + p.o_px), dx, lddx, p.m) : 0;
+    std::swap(a.own, a.stream);
+    std::swap(a.own_plane, a.stream_plane);
+    if (!rc && dw) rc = narrow_grad<T, DW>(c, a, p.nw, g, (float*)(c.ws + p.o_pw), dw, lddw, p.n);
+    return rc;
   }
   char* ds = c.ws + p.o_ds;
   float *px = (float*)(c.ws + p.o_px), *pw = (float*)(c.ws + p.o_pw);
@@ -948,29 +1056,29 @@ int backward(const Call& c, const float* lse, RowGrad g, void* dx, int64_t lddx,
     const int64_t nj = std::min(p.piece, p.n - j0);
     const Operand wj = {c.w.base + j0 * c.w.ld, c.w.ld, nj};
     // the scores of the piece again, as dS. All of its width is written: zeros past the end
-    const Problem as = {{wj.base, wj.ld, nj}, c.x, p.kp, up(p.kp, p.ke), 0, 0};
-    EpiGrad<T> eg = {ds, p.piece, lse, g, c.targets, j0, nj, p.m, c.scale};
-    rc = product<T, ROW, ROW>(shape_of(nj, p.m), as, 1, eg, c.st);
+    const Problem as = {wj, c.x, p.kp, 0, 0, 0, p.w_plane(), p.x_plane()};
+    const EpiGrad<T> eg = {ds, p.piece, p.ds_plane(), lse, g, c.targets, j0, nj, p.m, c.scale};
+    rc = product<T, ROW, ROW>(shape_of(nj, p.m), as, 1, 0, eg, c.st);
     if (rc) break;
-    const Operand dsr = {ds, p.piece * p.es, p.m};
+    const Operand dsr = {ds, p.piece * 2, p.m};
     if (dx) {
-      const Problem ax = {{wj.base, wj.ld, p.k}, dsr, nj, p.sx.k_slice, 0, 0};
+      const Problem ax = {{wj.base, wj.ld, p.k}, dsr, nj, 0, 0, 0, p.w_plane(), p.ds_plane()};
       if (parts_x)
-        rc = product<T, COL, ROW>(p.sx.shape, ax, p.sx.n, EpiPart{px, ldp, p.k, p.m, j0 > 0}, c.st);
+        rc = product<T, COL, ROW>(p.sx.shape, ax, p.sx.n, p.sx.stages, EpiPart{px, ldp, p.k, p.m, j0 > 0}, c.st);
       else
-        rc = product<T, COL, ROW>(p.sx.shape, ax, 1, EpiOut<T>{(char*)dx, lddx * p.es, p.k, p.m, g, c.scale}, c.st);
+        rc = product<T, COL, ROW>(p.sx.shape, ax, 1, 0, EpiOut<T>{(char*)dx, lddx * p.es, p.k, p.m, g, c.scale}, c.st);
       if (rc) break;
     }
     if (dw) {
-      const Problem aw = {{c.x.base, c.x.ld, p.k}, {ds, p.piece * p.es, nj}, p.m, p.sw.k_slice, 0, 0};
+      const Problem aw = {{c.x.base, c.x.ld, p.k}, {ds, p.piece * 2, nj}, p.m, 0, 0, 0, p.x_plane(), p.ds_plane()};
       char* out = (char*)dw + j0 * lddw * p.es;
       if (p.sw.n > 1) {
-        rc = product<T, COL, COL>(p.sw.shape, aw, p.sw.n, EpiPart{pw, ldp, p.k, nj, 0}, c.st);
+        rc = product<T, COL, COL>(p.sw.shape, aw, p.sw.n, p.sw.stages, EpiPart{pw, ldp, p.k, nj, 0}, c.st);
         if (rc) break;
         k_sum_parts<T><<<grid_for(nj * (ldp / 4)), 256, 0, c.st>>>(pw, p.sw.n, ldp, p.k, nj, g, c.scale, out, lddw * p.es);
         BLP_HIP(hipGetLastError());
       } else {
-        rc = product<T, COL, COL>(p.sw.shape, aw, 1, EpiOut<T>{out, lddw * p.es, p.k, nj, g, c.scale}, c.st);
+        rc = product<T, COL, COL>(p.sw.shape, aw, 1, 0, EpiOut<T>{out, lddw * p.es, p.k, nj, g, c.scale}, c.st);
       }
     }
   }
@@ -1008,7 +1116,7 @@ int dispatch(int device, void* stream, int type, const void* x, int64_t ldx, con
   BLP_CHECK(w && (m == 0 || (x && target && loss && lse)) && ws, BLP_E_ARG, "softmax loss: null pointer");
   BLP_CHECK(ldx >= k && ldw >= k && (!dx || lddx >= k) && (!dw || lddw >= k), BLP_E_ARG,
             "softmax loss: a row stride is smaller than k");
-  BLP_CHECK(std::max(ldx, ldw) <= (1 << 20) , BLP_E_ARG, "softmax loss: row strides must be at most 2^20 elements");
+  BLP_CHECK(std::max(ldx, ldw) <= (1 << 20), BLP_E_ARG, "softmax loss: row strides must be at most 2^20 elements");
   Call c;
   c.p = plan_of(type, m, n, k, fwd, grads, !aligned(x, ldx * es, (int64_t)k * es), !aligned(w, ldw * es, (int64_t)k * es));
   BLP_CHECK(ws_bytes >= c.p.bytes, BLP_E_ARG, "softmax loss: the workspace is too small (blp_softmax_loss_workspace)");

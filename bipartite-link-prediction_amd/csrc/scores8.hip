@@ -160,14 +160,14 @@ int launch(Problem a, EpiScores<TO> epi, hipStream_t st) {
   BLP_CHECK(tp * tq <= 0x7fffffff, BLP_E_ARG, "scores8: too many tiles for one launch");
   a.tiles_p = (int)tp;
   a.tiles_q = (int)tq;
-  k_product<I8, ROW, ROW, S, EpiScores<TO>><<<(unsigned)(tp * tq), S::THREADS, 0, st>>>(a, epi);
+  k_product<I8, ROW, ROW, false, S, EpiScores<TO>><<<(unsigned)(tp * tq), S::THREADS, 0, st>>>(a, epi);
   BLP_HIP(hipGetLastError());
   return 0;
 }
 
 template <int TO>
 int scores(const Operand& w, const Operand& x, int k, const float* s, const float* t, void* out, int64_t ldo, hipStream_t st) {
-  const Problem a = {w, x, k, up(k, STAGE), 0, 0};
+  const Problem a = {w, x, k, (int)div_up(k, STAGE), 0, 0, 0, 0};
   const EpiScores<TO> epi = {(char*)out, ldo * size_of(TO), s, t, w.rows, x.rows};
   if (x.rows <= 32) return launch<TO, NarrowQ>(a, epi, st);
   if (k <= STAGE) {

@@ -222,10 +222,16 @@ __device__ inline void ring_barrier() {
 
 struct Problem {
   Operand p, q;
-  int64_t k;        // valid k, in elements
-  int64_t k_slice;  // k of one slice (blockIdx.y), a multiple of the stage
+  int64_t k;            // valid k, in elements
+  int slice;            // stages of one slice (blockIdx.y) of all segments' stages
   int tiles_p, tiles_q;
+  // Floats as three halves each (x = x1 + x2 + x3, see latent.hip): the six segments x1 w1, x1 w2, x2 w1, x2 w2, x1 w3,
+  // x3 w1 follow one another along k; the planes of an operand lie this many bytes apart.
+  int64_t p_plane, q_plane;
 };
+constexpr int SEGMENTS = 6;
+__host__ __device__ constexpr int p_plane_of(int seg) { return (0x850 >> (2 * seg)) & 3; }
+__host__ __device__ constexpr int q_plane_of(int seg) { return (0x244 >> (2 * seg)) & 3; }
 
 // The workgroup's tile: consecutive workgroups go to the 8 dies in turn, so each die gets one contiguous
 // range of tiles, and walks it in bands of 8 q tiles: the p tile stays in the die's L2 while they pass.
@@ -240,7 +246,7 @@ __device__ inline void tile_of(const Problem& a, int* tp, int* tq) {
   *tq = band * BAND + in - *tp * width;
 }
 
-template <int T, int LP, int LQ, class S, class Epi>
+template <int T, int LP, int LQ, bool SEG, class S, class Epi>
 __global__ __launch_bounds__(S::THREADS) void k_product(Problem a, Epi epi) {
   constexpr int KE = STAGE / size_of(T);
   __shared__ __attribute__((aligned(1024))) char s_p0[S::BP * STAGE], s_q0[S::BQ * STAGE];
@@ -248,7 +254,7 @@ __global__ __launch_bounds__(S::THREADS) void k_product(Problem a, Epi epi) {
   int tp, tq;
   tile_of(a, &tp, &tq);
   const int64_t p0 = (int64_t)tp * S::BP, q0 = (int64_t)tq * S::BQ;
-  const int64_t kb = (int64_t)blockIdx.y * a.k_slice, ke = min(a.k, kb + a.k_slice);
+  const int per_seg = (int)((a.k + KE - 1) / KE), sb = blockIdx.y * a.slice;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wp = wave % S::WP, wq = wave / S::WP;
   typename Acc<T>::type acc[S::FP][S::FQ];
 #pragma unroll
@@ -256,23 +262,28 @@ __global__ __launch_bounds__(S::THREADS) void k_product(Problem a, Epi epi) {
 #pragma unroll
     for (int j = 0; j < S::FQ; ++j) acc[i][j] = 0;
   const uint32_t bp = lane_base<T, LP, S::BP>(), bq = lane_base<T, LQ, S::BQ>();
-  const int stages = ke > kb ? (int)((ke - kb + KE - 1) / KE) : 0;
+  const int stages = min(a.slice, (SEG ? SEGMENTS : 1) * per_seg - sb);
   lds_char *lp0 = (lds_char*)s_p0, *lq0 = (lds_char*)s_q0, *lp1 = (lds_char*)s_p1, *lq1 = (lds_char*)s_q1;
-  if (stages > 0) {
-    load_stage<T, LP, S::BP, S::WAVES>(lp0, a.p, p0, kb, ke);
-    load_stage<T, LQ, S::BQ, S::WAVES>(lq0, a.q, q0, kb, ke);
-  }
+  auto load = [&](lds_char* lp, lds_char* lq, int t) {
+    int at = sb + t;
+    Operand p = a.p, q = a.q;
+    if constexpr (SEG) {
+      const int seg = at / per_seg;
+      at -= seg * per_seg;
+      p.base += p_plane_of(seg) * a.p_plane;
+      q.base += q_plane_of(seg) * a.q_plane;
+    }
+    load_stage<T, LP, S::BP, S::WAVES>(lp, p, p0, (int64_t)at * KE, a.k);
+    load_stage<T, LQ, S::BQ, S::WAVES>(lq, q, q0, (int64_t)at * KE, a.k);
+  };
+  if (stages > 0) load(lp0, lq0, 0);
   int t = 0;
   for (; t + 2 <= stages; t += 2) {
     stage_barrier();
-    load_stage<T, LP, S::BP, S::WAVES>(lp1, a.p, p0, kb + (int64_t)(t + 1) * KE, ke);
-    load_stage<T, LQ, S::BQ, S::WAVES>(lq1, a.q, q0, kb + (int64_t)(t + 1) * KE, ke);
+    load(lp1, lq1, t + 1);
     mul_stage<T, LP, LQ, S>(lp0, lq0, bp, bq, wp, wq, acc);
     stage_barrier();
-    if (t + 2 < stages) {
-      load_stage<T, LP, S::BP, S::WAVES>(lp0, a.p, p0, kb + (int64_t)(t + 2) * KE, ke);
-      load_stage<T, LQ, S::BQ, S::WAVES>(lq0, a.q, q0, kb + (int64_t)(t + 2) * KE, ke);
-    }
+    if (t + 2 < stages) load(lp0, lq0, t + 2);
     mul_stage<T, LP, LQ, S>(lp1, lq1, bp, bq, wp, wq, acc);
   }
   if (t < stages) {
