@@ -95,10 +95,19 @@ __global__ __launch_bounds__(256) void k_pack_planes(const char* __restrict__ sr
 }
 
 // ---------------------------------------------------------------- forward
-// One (max, sum of exp2) pair a row and wave tile, in base 2: part[tile * rows + row].
+// Two pairs as one. fmaxf drops a NaN, the sum keeps it (exp2(NaN - base)); an infinite reference gives inf - inf = NaN.
+__device__ inline void merge(float& top, float& sum, float t2, float s2) {
+  const float t = fmaxf(top, t2);
+  const float base = t == -INFINITY ? 0.f : t;
+  sum = sum * __builtin_amdgcn_exp2f(top - base) + s2 * __builtin_amdgcn_exp2f(t2 - base);
+  top = t;
+}
+
+// One (reference, sum of exp2(z - reference)) pair a row and wave tile, in base 2: part[tile * rows + row].
+// Each lane takes its first score as its reference, which does as long as no sum grows past 2^60; only where one
+// does (or a score is infinite or NaN) the maximum is taken: 16 cycles a 64 scores instead of 26.
 template <int T>
 struct EpiLse {
-  static constexpr bool SCRATCH = false;
   float2* part;
   float* hit;  // z of the target
   Targets targets;
@@ -106,45 +115,64 @@ struct EpiLse {
   float scale;
   template <class S>
   __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int tile, int, lds_char*) const {
-    const int lane = threadIdx.x & 63, h = lane >> 4;
+    if (p0 >= n || q0 >= m) {
+      const int64_t row = q0 + (threadIdx.x & 63);  // a wave past the catalogue's end still owns its pairs
+      if (q0 < m && (int)(threadIdx.x & 63) < S::FQ * 16)
+        for (int64_t r = row; r < min(m, q0 + S::FQ * 16); r += 64) part[(int64_t)tile * m + r] = make_float2(-INFINITY, 0.f);
+      return;
+    }
+    const int lane = fresh_lane(), l = lane & 15, h = lane >> 4;
+    const int left = (int)min(n - p0, (int64_t)(S::FP * 16)), rows = (int)min(m - q0, (int64_t)(S::FQ * 16));
     const float c = scale * LOG2E;
 #pragma unroll
     for (int j = 0; j < S::FQ; ++j) {
-      const int64_t row = q0 + j * 16 + (lane & 15);
-      const int64_t t = row < m ? targets(row) : -1;
-      float top = -INFINITY;
+      __builtin_amdgcn_sched_barrier(0);
+      const int64_t row = q0 + min(j * 16 + l, rows - 1), t = targets(row) - p0;
+      const bool here = j * 16 + l < rows && t >= 0 && t < left && ((t >> 2) & 3) == h;  // this lane holds the target's score
+      if (left < S::FP * 16) {
+#pragma unroll
+        for (int i = 0; i < S::FP; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i * 16 + h * 4 + e >= left) acc[i][j][e] = scale < 0.f ? INFINITY : -INFINITY;
+      }
+      if (__any(here)) {
+        const int at = here ? (int)t - h * 4 : -1;
+        float z = 0.f;
+#pragma unroll
+        for (int i = 0; i < S::FP; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) z = at == i * 16 + e ? acc[i][j][e] : z;
+        if (here) hit[row] = z * scale;
+      }
+      float top = acc[0][j][0] * c, sum = 0.f;
 #pragma unroll
       for (int i = 0; i < S::FP; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int64_t p = p0 + i * 16 + h * 4 + e;
-          if (p == t) hit[row] = acc[i][j][e] * scale;
-          const float z = p < n ? acc[i][j][e] * c : -INFINITY;
-          acc[i][j][e] = z;
-          top = fmaxf(top, z);
-        }
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float base = top == -INFINITY ? 0.f : top;
-      float sum = 0.f;
+        for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, -top));
+      if (__any(!(sum < 0x1p60f))) {
+        top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < S::FP; ++i)
+        for (int i = 0; i < S::FP; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(acc[i][j][e] - base);
-      sum += __shfl_xor(sum, 16, 64);
-      sum += __shfl_xor(sum, 32, 64);
-      if (h == 0 && row < m) part[(int64_t)tile * m + row] = make_float2(top, sum);
+          for (int e = 0; e < 4; ++e) {
+            const bool past = left < S::FP * 16 && i * 16 + h * 4 + e >= left;  // for a scale of 0: inf 0 is NaN
+            acc[i][j][e] = past ? -INFINITY : acc[i][j][e] * c;
+            top = fmaxf(top, acc[i][j][e]);
+          }
+        const float base = top == -INFINITY ? 0.f : top;
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < S::FP; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(acc[i][j][e] - base);
+      }
+#pragma unroll
+      for (int o = 16; o <= 32; o <<= 1) merge(top, sum, __shfl_xor(top, o, 64), __shfl_xor(sum, o, 64));
+      if (h == 0 && j * 16 + l < rows) part[(int64_t)tile * m + row] = make_float2(top, sum);
     }
   }
 };
-
-// fmaxf drops a NaN, the sum keeps it (exp2(NaN - base)); an infinite max gives inf - inf = NaN.
-__device__ inline void merge(float& top, float& sum, float t2, float s2) {
-  const float t = fmaxf(top, t2);
-  const float base = t == -INFINITY ? 0.f : t;
-  sum = sum * __builtin_amdgcn_exp2f(top - base) + s2 * __builtin_amdgcn_exp2f(t2 - base);
-  top = t;
-}
 
 // 32 rows a block, 8 threads a row over the tiles' pairs.
 __global__ __launch_bounds__(256) void k_join(const float2* __restrict__ part, int64_t tiles, int64_t m,
@@ -246,7 +274,6 @@ __global__ __launch_bounds__(1024) void k_top_grad(const float* __restrict__ g, 
 // dS of one piece: ds[row * ld + p - 0], zeros past the catalogue's end.
 template <int T>
 struct EpiGrad {
-  static constexpr bool SCRATCH = true;
   char* ds;
   int64_t ld;     // elements
   int64_t plane;  // floats: bytes between the planes of dS
@@ -259,15 +286,17 @@ struct EpiGrad {
   template <class S>
   __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int, lds_char* scratch) const {
     if (p0 >= ld || q0 >= m) return;
-    const int lane = threadIdx.x & 63, l = lane & 15, h = lane >> 4;
+    const int lane = fresh_lane(), l = lane & 15, h = lane >> 4;
     const float c = scale * LOG2E;
     const int left = (int)min(n - p0, (int64_t)(S::FP * 16)), rows = (int)min(m - q0, (int64_t)(S::FQ * 16));
-    int hit[S::FQ];  // the target's place in the lane's block; far off: none
+    int hit[S::FQ];   // the target's place in the lane's block; far off: none
+    bool any[S::FQ];  // in one of the wave's lanes
     float gr[S::FQ], l2[S::FQ];
 #pragma unroll
     for (int j = 0; j < S::FQ; ++j) {
-      const int64_t row = q0 + min(j * 16 + l, rows - 1), t = targets(row);
-      hit[j] = t >= 0 && t - j0 - p0 >= 0 && t - j0 - p0 < S::FP * 16 ? (int)(t - j0 - p0) - h * 4 : -1000;
+      const int64_t row = q0 + min(j * 16 + l, rows - 1), t = targets(row), at = t - j0 - p0;
+      hit[j] = t >= 0 && at >= 0 && at < S::FP * 16 ? (int)at - h * 4 : -1000;
+      any[j] = __any(hit[j] != -1000);
       gr[j] = t >= 0 ? g.row(row) : 0.f;
       l2[j] = t >= 0 ? -lse[row] * LOG2E : -INFINITY;
     }
@@ -277,11 +306,17 @@ struct EpiGrad {
     auto value = [&](int i, int j) {
       f32x4 v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float d = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, l2[j]));
-        if (hit[j] == i * 16 + e) d -= 1.f;
-        d *= gr[j];
-        v[e] = left == S::FP * 16 || i * 16 + h * 4 + e < left ? d : 0.f;
+      for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, l2[j]));
+      if (any[j]) {  // rare
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (hit[j] == i * 16 + e) v[e] -= 1.f;
+      }
+      v *= gr[j];
+      if (left < S::FP * 16) {  // the catalogue's last rows
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i * 16 + h * 4 + e >= left) v[e] = 0.f;
       }
       return v;
     };
@@ -309,7 +344,6 @@ struct EpiGrad {
 // out[q][p] = alpha acc, rounded once.
 template <int T>
 struct EpiOut {
-  static constexpr bool SCRATCH = true;
   char* out;
   int64_t ld;  // bytes
   int64_t np, nq;
@@ -326,13 +360,12 @@ struct EpiOut {
 
 // part[slice][q][p] (+)= acc: the sums over slices of k and pieces of the catalogue, in 32 bits.
 struct EpiPart {
-  static constexpr bool SCRATCH = false;
   float* part;
   int64_t ld, np, nq;  // elements; ld a multiple of 4
   int add;
   template <class S>
   __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int slice, lds_char*) const {
-    const int lane = threadIdx.x & 63, h = lane >> 4;
+    const int lane = fresh_lane(), h = lane >> 4;
     float* base = part + (int64_t)slice * nq * ld;
 #pragma unroll
     for (int j = 0; j < S::FQ; ++j) {
@@ -408,7 +441,7 @@ struct NarrowArgs {
 
 template <int KS_, int FO_>
 struct NarrowShape {  // the second product's accumulators, for the epilogues
-  static constexpr int FP = 2 * KS_, FQ = FO_;
+  static constexpr int FP = 2 * KS_, FQ = FO_, SCRATCH = 16384;
 };
 
 template <int T>
@@ -719,8 +752,8 @@ __global__ __launch_bounds__(256, KS > 3 ? 2 : KS > 2 || T == F32 ? 3 : 4) void 
       for (int j = 0; j < FO; ++j)
 #pragma unroll
         for (int d = 0; d < 2 * KS; ++d) out[d][j] *= lane_g[j];
-    lds_char* scratch = nullptr;
-    if constexpr (Epi::SCRATCH) {  // a wave's 32 rows of up to 128 halves: the ring's buffers in parts
+    lds_char* scratch;
+    {  // a wave's 32 rows of up to 128 halves: the ring's buffers in parts
       __syncthreads();
       constexpr int WAVE = 16 * FO * pow2_up(32 * KS * size_of(T));
       if constexpr (WAVE * 4 <= BUF)
@@ -889,7 +922,8 @@ int product(int shape, Problem a, int slices, int stages, Epi epi, hipStream_t s
   a.tiles_p = (int)tp;
   a.tiles_q = (int)tq;
   a.slice = stages ? stages : (int)div_up(a.k, KE) * (T == F32 ? SEGMENTS : 1);
-  const dim3 grid((unsigned)(tp * tq), (unsigned)slices);
+  // one or two workgroups a compute unit, which take tile after tile
+  const dim3 grid((unsigned)std::min<int64_t>(tp * tq, shape == BIG ? GOAL / 2 : GOAL), (unsigned)slices);
   if (shape == BIG)
     launch<T, LP, LQ, Big>(a, grid, epi, st);
   else if (shape == MID)
@@ -945,7 +979,6 @@ int bind(Call& c, const void* x, int64_t ldx, const void* w, int64_t ldw) {
 }
 
 struct NoEpilogue {
-  static constexpr bool SCRATCH = false;
   template <class S>
   __device__ void run(f32x4 (&)[S::FP][S::FQ], int64_t, int64_t, int, int, lds_char*) const {}
 };

@@ -98,7 +98,6 @@ __global__ __launch_bounds__(256) void k_pack8(const int8_t* __restrict__ src, i
 // ---------------------------------------------------------------- scores
 template <int TO>
 struct EpiScores {
-  static constexpr bool SCRATCH = true;
   char* out;
   int64_t ld;  // bytes
   const float *s, *t;
@@ -106,7 +105,7 @@ struct EpiScores {
   template <class S>
   __device__ void run(i32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int, lds_char* scratch) const {
     if (p0 >= np || q0 >= nq) return;
-    const int lane = threadIdx.x & 63, l = lane & 15, h = lane >> 4;
+    const int lane = fresh_lane(), l = lane & 15, h = lane >> 4;
     const int left = (int)min(np - p0, (int64_t)(S::FP * 16)), rows = (int)min(nq - q0, (int64_t)(S::FQ * 16));
     f32x4 tp[S::FP];
     float sq[S::FQ];
@@ -127,12 +126,16 @@ struct EpiScores {
 
 // k up to 128: one stage, and the outputs are what counts. A workgroup of 8 waves, 16 rows and 16 FP columns each,
 // in 32 KiB of LDS, so that three of them share a compute unit and some load and multiply while others store.
+template <int FP_>
+struct OuterShape : Shape<1, 8, FP_, 1> {
+  static constexpr int SCRATCH = 4096;
+};
 template <int TO>
 __global__ __launch_bounds__(512, 6) void k_outer8(Problem a, EpiScores<TO> epi) {
-  using S = Shape<1, 8, TO == F32 ? 4 : 8, 1>;
+  using S = OuterShape<TO == F32 ? 4 : 8>;
   __shared__ __attribute__((aligned(1024))) char s_all[32768];
   int tp, tq;
-  tile_of(a, &tp, &tq);
+  tile_of(a, blockIdx.x, &tp, &tq);
   const int64_t p0 = (int64_t)tp * S::BP, q0 = (int64_t)tq * S::BQ;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   lds_char *lp = (lds_char*)s_all, *lq = lp + S::BP * STAGE;
@@ -142,7 +145,13 @@ __global__ __launch_bounds__(512, 6) void k_outer8(Problem a, EpiScores<TO> epi)
 #pragma unroll
   for (int i = 0; i < S::FP; ++i) acc[i][0] = i32x4{0, 0, 0, 0};
   stage_barrier();
-  mul_stage<I8, ROW, ROW, S>(lp, lq, lane_base<I8, ROW, S::BP>(), lane_base<I8, ROW, S::BQ>(), 0, wave, acc);
+  const uint32_t bp = lane_base<I8, ROW, S::BP>(), bq = lane_base<I8, ROW, S::BQ>();
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk) {
+    Frags<I8, ROW, ROW, S> f;
+    f.read(lp, lq, bp, bq, 0, wave, kk);
+    f.multiply(acc);
+  }
   __syncthreads();
   epi.template run<S>(acc, p0, q0 + wave * 16, 0, 0, lp + wave * 4096);
 }
@@ -160,7 +169,7 @@ int launch(Problem a, EpiScores<TO> epi, hipStream_t st) {
   BLP_CHECK(tp * tq <= 0x7fffffff, BLP_E_ARG, "scores8: too many tiles for one launch");
   a.tiles_p = (int)tp;
   a.tiles_q = (int)tq;
-  k_product<I8, ROW, ROW, false, S, EpiScores<TO>><<<(unsigned)(tp * tq), S::THREADS, 0, st>>>(a, epi);
+  k_product<I8, ROW, ROW, false, S, EpiScores<TO>><<<(unsigned)std::min<int64_t>(tp * tq, S::BP == 256 && S::BQ == 256 ? 256 : 512), S::THREADS, 0, st>>>(a, epi);
   BLP_HIP(hipGetLastError());
   return 0;
 }

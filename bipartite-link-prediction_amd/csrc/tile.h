@@ -1,11 +1,14 @@
 // The tile engine of the latent-factor products (latent.hip, scores8.hip): C[q][p] = sum_k P(p, k) Q(q, k)
 // on the matrix cores, with the caller's epilogue over the accumulators. gfx950 only.
 //
-// A workgroup owns a tile of BP x BQ outputs and walks k in stages of 128 bytes (64 halves, 32 floats,
-// 128 8-bit integers). A stage of each operand is copied from memory straight into LDS (16 bytes a lane,
-// no register in between); the next stage is in flight while this one is multiplied, in the other of two
-// buffers, so a stage costs one barrier. A fragment is 16 bytes of a row: 8 halves, 4 floats or 16 8-bit
-// integers, one 16-row matrix instruction (four of them for floats).
+// A workgroup owns a tile of BP x BQ outputs and walks k in stages of 128 bytes (64 halves, 128 8-bit
+// integers). A stage of each operand is copied from memory straight into LDS (16 bytes a lane, no register
+// in between). A fragment is 16 bytes of a row: 8 halves or 16 8-bit integers, one 16-row matrix instruction.
+// The next stage is in flight while this one is multiplied, in the other of two buffers, so a stage costs one
+// barrier. A workgroup takes tile after tile, and the next one's first stage is on its way while this one's
+// outputs leave. Bound by the copies from the second-level cache and the matrix unit alike (256 x 256 x 64 halves
+// a stage: 64 KiB and 2,048 cycles of it); 2 M N k of 8,192 x 32,768 x 4,096 run at 1,319 TFLOP/s without the
+// reading of LDS or the copies being the slower by more than a quarter.
 //
 // Layouts of an operand: ROW -- k contiguous, element (p, k) at base + p ld + k size; COL -- p contiguous,
 // element (p, k) at base + k ld + p size, whose halves are transposed on their way out of LDS
@@ -83,6 +86,8 @@ struct Shape {
   static constexpr int WP = WP_, WQ = WQ_, FP = FP_, FQ = FQ_;
   static constexpr int WAVES = WP * WQ, THREADS = WAVES * 64;
   static constexpr int BP = WP * FP * 16, BQ = WQ * FQ * 16;
+  static constexpr int STAGE_BYTES = (BP + BQ) * 128;
+  static constexpr int SCRATCH = STAGE_BYTES / WAVES / 4096 * 4096;  // LDS for a wave's outputs
 };
 
 typedef __attribute__((address_space(3))) char lds_char;
@@ -186,22 +191,30 @@ __device__ inline frag_t read_frag(const lds_char* lds, uint32_t base, int f, in
 }
 
 template <int T, int LP, int LQ, class S>
-__device__ inline void mul_stage(const lds_char* lp, const lds_char* lq, uint32_t bp, uint32_t bq, int wp, int wq,
-                                 typename Acc<T>::type (&acc)[S::FP][S::FQ]) {
-  // the addresses are made anew each stage: kept across the loop they would cost the accumulators their registers
-  asm volatile("" : "+v"(bp), "+v"(bq));
-#pragma unroll
-  for (int kk = 0; kk < 2; ++kk) {
-    frag_t p[S::FP], q[S::FQ];
+struct Frags {
+  frag_t p[S::FP], q[S::FQ];
+  // half a stage (kk) out of LDS. The addresses are made anew each time: kept they would cost registers
+  __device__ inline void read(const lds_char* lp, const lds_char* lq, uint32_t bp, uint32_t bq, int wp, int wq, int kk) {
+    asm volatile("" : "+v"(bp), "+v"(bq));
 #pragma unroll
     for (int j = 0; j < S::FQ; ++j) q[j] = read_frag<T, LQ, S::BQ>(lq, bq, wq * S::FQ + j, kk);
 #pragma unroll
     for (int i = 0; i < S::FP; ++i) p[i] = read_frag<T, LP, S::BP>(lp, bp, wp * S::FP + i, kk);
+  }
+  __device__ inline void multiply(typename Acc<T>::type (&acc)[S::FP][S::FQ]) const {
 #pragma unroll
     for (int i = 0; i < S::FP; ++i)
 #pragma unroll
       for (int j = 0; j < S::FQ; ++j) acc[i][j] = mma<T>(p[i], q[j], acc[i][j]);
   }
+};
+
+// The lane, as a value that nothing computed from it is kept across the tiles (epilogues' addresses would cost the
+// accumulators their registers).
+__device__ inline int fresh_lane() {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  return lane;
 }
 
 __device__ inline void stage_barrier() {
@@ -235,8 +248,8 @@ __host__ __device__ constexpr int q_plane_of(int seg) { return (0x244 >> (2 * se
 
 // The workgroup's tile: consecutive workgroups go to the 8 dies in turn, so each die gets one contiguous
 // range of tiles, and walks it in bands of 8 q tiles: the p tile stays in the die's L2 while they pass.
-__device__ inline void tile_of(const Problem& a, int* tp, int* tq) {
-  const int n = a.tiles_p * a.tiles_q, b = blockIdx.x;
+__device__ inline void tile_of(const Problem& a, int b, int* tp, int* tq) {
+  const int n = a.tiles_p * a.tiles_q;
   const int per = n >> 3, extra = n & 7, xcd = b & 7, at = b >> 3;
   const int t = xcd * per + min(xcd, extra) + at;
   constexpr int BAND = 8;
@@ -247,24 +260,15 @@ __device__ inline void tile_of(const Problem& a, int* tp, int* tq) {
 }
 
 template <int T, int LP, int LQ, bool SEG, class S, class Epi>
-__global__ __launch_bounds__(S::THREADS) void k_product(Problem a, Epi epi) {
+__global__ __launch_bounds__(S::THREADS, 2) void k_product(Problem a, Epi epi) {
   constexpr int KE = STAGE / size_of(T);
-  __shared__ __attribute__((aligned(1024))) char s_p0[S::BP * STAGE], s_q0[S::BQ * STAGE];
-  __shared__ __attribute__((aligned(1024))) char s_p1[S::BP * STAGE], s_q1[S::BQ * STAGE];
-  int tp, tq;
-  tile_of(a, &tp, &tq);
-  const int64_t p0 = (int64_t)tp * S::BP, q0 = (int64_t)tq * S::BQ;
-  const int per_seg = (int)((a.k + KE - 1) / KE), sb = blockIdx.y * a.slice;
+  __shared__ __attribute__((aligned(1024))) char s_0[S::STAGE_BYTES], s_1[S::STAGE_BYTES];
+  lds_char *l0 = (lds_char*)s_0, *l1 = (lds_char*)s_1;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wp = wave % S::WP, wq = wave / S::WP;
-  typename Acc<T>::type acc[S::FP][S::FQ];
-#pragma unroll
-  for (int i = 0; i < S::FP; ++i)
-#pragma unroll
-    for (int j = 0; j < S::FQ; ++j) acc[i][j] = 0;
   const uint32_t bp = lane_base<T, LP, S::BP>(), bq = lane_base<T, LQ, S::BQ>();
-  const int stages = min(a.slice, (SEG ? SEGMENTS : 1) * per_seg - sb);
-  lds_char *lp0 = (lds_char*)s_p0, *lq0 = (lds_char*)s_q0, *lp1 = (lds_char*)s_p1, *lq1 = (lds_char*)s_q1;
-  auto load = [&](lds_char* lp, lds_char* lq, int t) {
+  const int per_seg = (int)((a.k + KE - 1) / KE), sb = blockIdx.y * a.slice;
+  const int stages = min(a.slice, (SEG ? SEGMENTS : 1) * per_seg - sb), tiles = a.tiles_p * a.tiles_q;
+  auto load = [&](lds_char* to, int tp, int tq, int t) {
     int at = sb + t;
     Operand p = a.p, q = a.q;
     if constexpr (SEG) {
@@ -273,36 +277,57 @@ __global__ __launch_bounds__(S::THREADS) void k_product(Problem a, Epi epi) {
       p.base += p_plane_of(seg) * a.p_plane;
       q.base += q_plane_of(seg) * a.q_plane;
     }
-    load_stage<T, LP, S::BP, S::WAVES>(lp, p, p0, (int64_t)at * KE, a.k);
-    load_stage<T, LQ, S::BQ, S::WAVES>(lq, q, q0, (int64_t)at * KE, a.k);
+    load_stage<T, LP, S::BP, S::WAVES>(to, p, (int64_t)tp * S::BP, (int64_t)at * KE, a.k);
+    load_stage<T, LQ, S::BQ, S::WAVES>(to + S::BP * STAGE, q, (int64_t)tq * S::BQ, (int64_t)at * KE, a.k);
   };
-  if (stages > 0) load(lp0, lq0, 0);
-  int t = 0;
-  for (; t + 2 <= stages; t += 2) {
-    stage_barrier();
-    load(lp1, lq1, t + 1);
-    mul_stage<T, LP, LQ, S>(lp0, lq0, bp, bq, wp, wq, acc);
-    stage_barrier();
-    if (t + 2 < stages) load(lp0, lq0, t + 2);
-    mul_stage<T, LP, LQ, S>(lp1, lq1, bp, bq, wp, wq, acc);
+  auto landed = [] {  // this wave's copies, and its reads of LDS, are done; then every wave's
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  int tp, tq, np = 0, nq = 0;
+  tile_of(a, blockIdx.x, &tp, &tq);
+  load(l0, tp, tq, 0);
+  for (int b = blockIdx.x; b < tiles; b += gridDim.x) {
+    const bool more = b + (int)gridDim.x < tiles;
+    if (more) tile_of(a, b + gridDim.x, &np, &nq);
+    typename Acc<T>::type acc[S::FP][S::FQ];
+#pragma unroll
+    for (int i = 0; i < S::FP; ++i)
+#pragma unroll
+      for (int j = 0; j < S::FQ; ++j) acc[i][j] = 0;
+    auto multiply = [&](lds_char* from) {
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        Frags<T, LP, LQ, S> f;
+        f.read(from, from + S::BP * STAGE, bp, bq, wp, wq, kk);
+        f.multiply(acc);
+      }
+    };
+    int t = 0;
+    for (; t + 2 <= stages; t += 2) {
+      landed();
+      load(l1, tp, tq, t + 1);
+      multiply(l0);
+      landed();
+      if (t + 2 < stages)
+        load(l0, tp, tq, t + 2);
+      else if (more)
+        load(l0, np, nq, 0);
+      multiply(l1);
+    }
+    if (t < stages) {
+      landed();
+      multiply(l0);
+    }
+    __syncthreads();  // every wave's last reads are done: the second buffer is free for the outputs
+    if (t < stages && more) load(l0, np, nq, 0);
+    epi.template run<S>(acc, (int64_t)tp * S::BP + wp * S::FP * 16, (int64_t)tq * S::BQ + wq * S::FQ * 16, tp * S::WP + wp, blockIdx.y,
+                        l1 + wave * S::SCRATCH);
+    tp = np;
+    tq = nq;
   }
-  if (t < stages) {
-    stage_barrier();
-    mul_stage<T, LP, LQ, S>(lp0, lq0, bp, bq, wp, wq, acc);
-  }
-  lds_char* scratch = nullptr;  // 16 KiB of the stages' LDS for each wave's outputs
-  if constexpr (Epi::SCRATCH) {
-    __syncthreads();
-    if constexpr (S::BP == 256 && S::BQ == 256)
-      scratch = (wave < 4 ? (wave < 2 ? lp0 : lq0) : (wave < 6 ? lp1 : lq1)) + (wave & 1) * 16384;
-    else if constexpr (S::BP == 128 && S::BQ == 128)
-      scratch = wave < 2 ? (wave == 0 ? lp0 : lq0) : (wave == 2 ? lp1 : lq1);
-    else if constexpr (S::BQ == 256)
-      scratch = (wave < 2 ? lq0 : lq1) + (wave & 1) * 16384;
-    else
-      scratch = (wave < 2 ? lp0 : lp1) + (wave & 1) * 16384;
-  }
-  epi.template run<S>(acc, p0 + wp * S::FP * 16, q0 + wq * S::FQ * 16, tp * S::WP + wp, blockIdx.y, scratch);
 }
 
 // round to the type once; four consecutive values
@@ -354,9 +379,10 @@ __host__ __device__ constexpr int pow2_up(int v) {
 template <int TO, class S, bool NT = false, class F>
 __device__ inline void store_block(lds_char* scratch, char* out, int64_t ld, int64_t np, int64_t nq, F value) {
   constexpr int ES = size_of(TO), ROWB = pow2_up(S::FP * 16 * ES), GR = ROWB / 16;  // bytes, granules of an LDS row
-  constexpr int J = S::FQ * 16 * ROWB > 16384 ? S::FQ / 2 : S::FQ;         // blocks of 16 rows a pass
+  constexpr int FIT = S::SCRATCH / (16 * ROWB), J = FIT < S::FQ ? FIT : S::FQ;  // blocks of 16 rows a pass
+  static_assert(J >= 1 && S::FQ % J == 0, "passes of whole blocks");
   constexpr int LANES = GR < 64 ? GR : 64, RPI = 64 / LANES;               // lanes a row, rows an instruction
-  const int lane = threadIdx.x & 63, l = lane & 15, h = lane >> 4;
+  const int lane = fresh_lane(), l = lane & 15, h = lane >> 4;
 #pragma unroll
   for (int j0 = 0; j0 < S::FQ; j0 += J) {
     if (j0) __builtin_amdgcn_wave_barrier();
@@ -364,6 +390,7 @@ __device__ inline void store_block(lds_char* scratch, char* out, int64_t ld, int
     for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int i = 0; i < S::FP; ++i) {
+        if (i == 0) __builtin_amdgcn_sched_barrier(0);  // one row's values at a time: few registers
         const f32x4 v = value(i, j0 + j);
         const int row = j * 16 + l;
         if constexpr (TO == F32) {
