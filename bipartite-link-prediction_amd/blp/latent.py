@@ -28,54 +28,73 @@ _lib.register("blp_scores8_workspace", [_P, _I64, _P, _I64, _I64, _I64, _I32, _P
 _lib.register("blp_scores8", [_I32, _P, _P, _I64, _P, _P, _I64, _P, _I64, _I64, _I32, _I32, _P, _I64, _P, _I64])
 
 _torch = None
-_TYPES = {}
+_TYPES = {}   # torch dtype -> BLP_F32 / BLP_BF16 / BLP_F16
+_INT8 = {}
+_stream = None
 
 
 def _t():
     """torch, imported on the first call: the graph engine works without it."""
-    global _torch
+    global _torch, _stream
     if _torch is None:
         import torch
 
         _TYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+        _INT8[torch.int8] = 3
+        # the current stream's handle on a device index; the public accessor makes two objects on the way
+        _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
         _torch = torch
     return _torch
 
 
+def _say(t):
+    return "%s %s on %s" % (tuple(t.shape), t.dtype, t.device) if isinstance(t, _torch.Tensor) else str(type(t))
+
+
 def _rows(t, what, dtypes):
-    """`t` as (n, k) rows: a 2-d tensor on a GPU with contiguous rows that do not overlap."""
-    torch = _t()
-    if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.dtype not in dtypes or not t.is_cuda:
+    """The row stride of `t`, checked to be (n, k) rows: a 2-d tensor on a GPU whose rows are contiguous and do not
+    overlap."""
+    if not (isinstance(t, _torch.Tensor) and t.dtype in dtypes and t.is_cuda and t.dim() == 2):
         raise ValueError("%s must be a 2-d GPU tensor of %s (got %s)" % (
-            what, " / ".join(str(d)[6:] for d in dtypes),
-            "%s %s on %s" % (tuple(t.shape), t.dtype, t.device) if isinstance(t, torch.Tensor) else type(t)))
-    if t.shape[1] < 1 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+            what, " / ".join(str(d)[6:] for d in dtypes), _say(t)))
+    n, k = t.shape
+    ld, step = t.stride()
+    if k < 1 or (k > 1 and step != 1) or (n > 1 and ld < k):
         raise ValueError("%s must have contiguous, non-overlapping rows of at least one element (shape %s, strides %s)" % (
-            what, tuple(t.shape), tuple(t.stride())))
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+            what, (n, k), (ld, step)))
+    return ld if n > 1 else k
 
 
 def _ids(t, what, device, n=None):
-    torch = _t()
-    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64) or t.device != device \
-            or not t.is_contiguous() or (n is not None and tuple(t.shape) != (n,)):
+    """1 for int64, 0 for int32 ids: a contiguous tensor on `device`, of shape (n,) where n is given."""
+    wide = isinstance(t, _torch.Tensor) and (1 if t.dtype == _torch.int64 else 0 if t.dtype == _torch.int32 else None)
+    if wide is None or wide is False or t.device != device or not t.is_contiguous() or (n is not None and t.shape != (n,)):
         raise ValueError("%s must be a contiguous int32 / int64 tensor%s on %s (got %s)" % (
-            what, "" if n is None else " of shape (%d,)" % n, device,
-            "%s %s on %s" % (tuple(t.shape), t.dtype, t.device) if isinstance(t, torch.Tensor) else type(t)))
-    return 1 if t.dtype == torch.int64 else 0
+            what, "" if n is None else " of shape (%d,)" % n, device, _say(t)))
+    return wide
 
 
-def _stream(device):
-    return _torch.cuda.current_stream(device).cuda_stream
+def _floats(t, what, device, shapes):
+    if not (isinstance(t, _torch.Tensor) and t.dtype == _torch.float32 and t.device == device and t.is_contiguous()
+            and t.shape in shapes):
+        raise ValueError("%s must be a contiguous float32 tensor of shape %s on %s (got %s)" % (
+            what, " or ".join(str(tuple(x)) for x in shapes), device, _say(t)))
+
+
+def _bytes(device, n):
+    return _torch.empty(n, dtype=_torch.uint8, device=device)
 
 
 _REDUCTIONS = ("mean", "sum", "none")
 
 
 def _loss_args(x, table, target, scale, reduction):
-    torch = _t()
-    ldx = _rows(x, "x", tuple(_TYPES))
-    ldt = _rows(table, "table", (x.dtype,))
+    _t()
+    ldx = _rows(x, "x", _TYPES)
+    if not isinstance(table, _torch.Tensor) or table.dtype != x.dtype:
+        raise ValueError("x and table must be tensors of the same type (got %s and %s)" % (_say(x), _say(table)))
+    ldt = _rows(table, "table", _TYPES)
     if table.shape[1] != x.shape[1] or table.device != x.device:
         raise ValueError("x %s and table %s must have rows of the same length on one device" % (
             tuple(x.shape), tuple(table.shape)))
@@ -84,31 +103,39 @@ def _loss_args(x, table, target, scale, reduction):
     wide = _ids(target, "target", x.device, x.shape[0])
     if reduction not in _REDUCTIONS:
         raise ValueError("reduction must be one of %s (got %r)" % (", ".join(_REDUCTIONS), reduction))
-    return torch, ldx, ldt, wide, _scale(scale)
+    return ldx, ldt, wide, _scale(scale)
 
 
-def _loss_workspace(torch, x, ldx, table, ldt, forward, grads):
+def _loss_workspace(x, ldx, table, ldt, forward, grads):
     n = ctypes.c_int64(0)
-    check(lib().blp_softmax_loss_workspace(_TYPES[x.dtype], x.data_ptr(), ldx, table.data_ptr(), ldt, x.shape[0],
-                                           table.shape[0], x.shape[1], forward, grads, ctypes.byref(n)))
-    return torch.empty(n.value, dtype=torch.uint8, device=x.device)
-
-
-def _loss_forward(x, table, target, scale, reduction, grads):
-    """-> (loss or total, lse, total, dx, dtable)"""
-    torch, ldx, ldt, wide, scale = _loss_args(x, table, target, scale, reduction)
     m, k = x.shape
-    stats = torch.empty((2 * m + 2,), dtype=torch.float32, device=x.device)
-    loss, lse, total = stats[:m], stats[m:2 * m], stats[2 * m:]
+    check(lib().blp_softmax_loss_workspace(_TYPES[x.dtype], x.data_ptr(), ldx, table.data_ptr(), ldt, m, table.shape[0], k,
+                                           forward, grads, ctypes.byref(n)))
+    return n.value
+
+
+def _loss_forward(x, table, target, scale, reduction, grads, keep=False):
+    """-> (loss or total, lse, total, dx, dtable); lse and total only where asked to `keep` them"""
+    ldx, ldt, wide, scale = _loss_args(x, table, target, scale, reduction)
+    m, k = x.shape
+    device = x.device
+    need = _loss_workspace(x, ldx, table, ldt, 1, grads)
     summed = reduction != "none"
-    dx = torch.empty((m, k), dtype=x.dtype, device=x.device) if grads else None
-    dt = torch.empty((table.shape[0], k), dtype=x.dtype, device=x.device) if grads else None
-    ws = _loss_workspace(torch, x, ldx, table, ldt, 1, 1 if grads else 0)
+    # what the caller does not get lies behind the workspace: the rows' lse, and their losses where they are summed up
+    ws = _bytes(device, need + 8 * m)
+    tail = ws.data_ptr() + need
+    lse = _torch.empty(m, dtype=_torch.float32, device=device) if keep else None
+    total = _torch.empty(2, dtype=_torch.float32, device=device) if summed else None
+    loss = None if summed else _torch.empty(m, dtype=_torch.float32, device=device)
+    dx = dt = None
+    if grads:
+        dx = _torch.empty((m, k), dtype=x.dtype, device=device)
+        dt = _torch.empty((table.shape[0], k), dtype=x.dtype, device=device)
     check(lib().blp_softmax_loss(
-        x.device.index, _stream(x.device), _TYPES[x.dtype], x.data_ptr(), ldx, table.data_ptr(), ldt, target.data_ptr(), wide,
-        m, table.shape[0], k, scale, loss.data_ptr(), lse.data_ptr(), total.data_ptr() if summed else None,
-        1 if reduction == "mean" else 0, 1 if grads else 0, dx.data_ptr() if grads else None, k,
-        dt.data_ptr() if grads else None, k, ws.data_ptr(), ws.numel()))
+        device.index, _stream(device.index), _TYPES[x.dtype], x.data_ptr(), ldx, table.data_ptr(), ldt, target.data_ptr(), wide,
+        m, table.shape[0], k, scale, tail + 4 * m if summed else loss.data_ptr(), lse.data_ptr() if keep else tail,
+        total.data_ptr() if summed else None, 1 if reduction == "mean" else 0, grads, dx.data_ptr() if grads else None, k,
+        dt.data_ptr() if grads else None, k, ws.data_ptr(), need))
     return (total[0] if summed else loss), lse, total, dx, dt
 
 
@@ -119,11 +146,12 @@ def softmax_loss(x, table, target, scale=1.0, reduction="mean"):
     row of `table` that belongs to each row of x. A target outside [0, n) (-1, as in the top-k lists'
     missing slots) ignores its row: loss 0, gradient 0, whatever x holds there. reduction "mean" (over
     the rows not ignored; 0 if there is none), "sum" or "none" (one loss a row). Returns float32;
-    differentiable in x and table. Sums and the softmax's statistics are held in 32 bits."""
+    differentiable in x and table. Sums and the softmax's statistics are held in 32 bits. Float32 factors are
+    multiplied as sums of three bfloat16 each, with 32-bit results; they have to be finite."""
     torch = _t()
     if torch.is_grad_enabled() and (getattr(x, "requires_grad", False) or getattr(table, "requires_grad", False)):
         return _function("loss").apply(x, table, target, scale, reduction)
-    return _loss_forward(x, table, target, scale, reduction, False)[0]
+    return _loss_forward(x, table, target, scale, reduction, 0)[0]
 
 
 def softmax_loss_grad(x, table, target, scale=1.0, reduction="mean"):
@@ -131,29 +159,28 @@ def softmax_loss_grad(x, table, target, scale=1.0, reduction="mean"):
     training loops that do not go through autograd."""
     if reduction == "none":
         raise ValueError("softmax_loss_grad: reduction must be mean or sum")
-    loss, _, _, dx, dt = _loss_forward(x, table, target, scale, reduction, True)
+    loss, _, _, dx, dt = _loss_forward(x, table, target, scale, reduction, 1)
     return loss, dx, dt
 
 
 def softmax_loss_backward(grad, lse, count, x, table, target, scale=1.0, need_x=True, need_table=True):
     """-> (dx, dtable) of :func:`softmax_loss`: `grad` float32, one value or one a row; `lse` (m,) the
-    forward pass's; `count` a float32 tensor that divides the gradient (mean) or None."""
-    torch, ldx, ldt, wide, scale = _loss_args(x, table, target, scale, "none")
+    forward pass's; `count` a float32 value that divides the gradient (mean) or None."""
+    ldx, ldt, wide, scale = _loss_args(x, table, target, scale, "none")
     m, k = x.shape
-    for t, what, shapes in ((grad, "grad", ((), (1,), (m,))), (lse, "lse", ((m,),)), (count, "count", ((), (1,)))):
-        if t is None and what == "count":
-            continue
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != x.device or not t.is_contiguous() \
-                or tuple(t.shape) not in shapes:
-            raise ValueError("%s must be a contiguous float32 tensor of shape %s on %s" % (what, shapes[-1], x.device))
-    stride = 1 if grad.dim() == 1 and m > 1 else 0
-    dx = torch.empty((m, k), dtype=x.dtype, device=x.device) if need_x else None
-    dt = torch.empty((table.shape[0], k), dtype=x.dtype, device=x.device) if need_table else None
-    ws = _loss_workspace(torch, x, ldx, table, ldt, 0, 1)
+    device = x.device
+    _floats(grad, "grad", device, ((), (1,), (m,)))
+    _floats(lse, "lse", device, ((m,),))
+    if count is not None:
+        _floats(count, "count", device, ((), (1,)))
+    dx = _torch.empty((m, k), dtype=x.dtype, device=device) if need_x else None
+    dt = _torch.empty((table.shape[0], k), dtype=x.dtype, device=device) if need_table else None
+    ws = _bytes(device, _loss_workspace(x, ldx, table, ldt, 0, 1))
     check(lib().blp_softmax_loss_backward(
-        x.device.index, _stream(x.device), _TYPES[x.dtype], x.data_ptr(), ldx, table.data_ptr(), ldt, target.data_ptr(), wide,
-        m, table.shape[0], k, scale, lse.data_ptr(), grad.data_ptr(), stride, None if count is None else count.data_ptr(),
-        None if dx is None else dx.data_ptr(), k, None if dt is None else dt.data_ptr(), k, ws.data_ptr(), ws.numel()))
+        device.index, _stream(device.index), _TYPES[x.dtype], x.data_ptr(), ldx, table.data_ptr(), ldt, target.data_ptr(), wide,
+        m, table.shape[0], k, scale, lse.data_ptr(), grad.data_ptr(), 1 if grad.numel() > 1 else 0,
+        None if count is None else count.data_ptr(), None if dx is None else dx.data_ptr(), k,
+        None if dt is None else dt.data_ptr(), k, ws.data_ptr(), ws.numel()))
     return dx, dt
 
 
@@ -175,15 +202,16 @@ def lookup(table, ids, scale=1.0):
 
 
 def _lookup(table, ids, scale):
-    torch = _t()
-    ld = _rows(table, "table", tuple(_TYPES))
-    if table.shape[0] < 1:
+    _t()
+    ld = _rows(table, "table", _TYPES)
+    rows, k = table.shape
+    if rows < 1:
         raise ValueError("the table must have at least one row")
-    wide = _ids(ids, "ids", table.device)
-    n, k = ids.numel(), table.shape[1]
-    out = torch.empty(tuple(ids.shape) + (k,), dtype=table.dtype, device=table.device)
-    check(lib().blp_lookup(table.device.index, _stream(table.device), _TYPES[table.dtype], table.data_ptr(), ld,
-                           table.shape[0], k, ids.data_ptr(), wide, n, _scale(scale), out.data_ptr(), k))
+    device = table.device
+    wide = _ids(ids, "ids", device)
+    out = _torch.empty((*ids.shape, k), dtype=table.dtype, device=device)
+    check(lib().blp_lookup(device.index, _stream(device.index), _TYPES[table.dtype], table.data_ptr(), ld, rows, k,
+                           ids.data_ptr(), wide, ids.numel(), _scale(scale), out.data_ptr(), k))
     return out
 
 
@@ -201,7 +229,7 @@ def lookup_grad(grad, ids, n_rows, scale=1.0, into=None):
         if not grad.is_contiguous():
             raise ValueError("grad must be contiguous")
         grad = grad.view(n, k)
-    ld = _rows(grad, "grad", tuple(_TYPES))
+    ld = _rows(grad, "grad", _TYPES)
     wide = _ids(ids, "ids", grad.device)
     n_rows = int(n_rows)
     if n_rows < 1:
@@ -214,8 +242,8 @@ def lookup_grad(grad, ids, n_rows, scale=1.0, into=None):
             raise ValueError("into must be of shape %s on %s" % ((n_rows, k), grad.device))
     b = ctypes.c_int64(0)
     check(lib().blp_lookup_grad_workspace(_TYPES[grad.dtype], n, n_rows, k, ctypes.byref(b)))
-    ws = torch.empty(b.value, dtype=torch.uint8, device=grad.device)
-    check(lib().blp_lookup_grad(grad.device.index, _stream(grad.device), _TYPES[grad.dtype], grad.data_ptr(), ld,
+    ws = _bytes(grad.device, b.value)
+    check(lib().blp_lookup_grad(grad.device.index, _stream(grad.device.index), _TYPES[grad.dtype], grad.data_ptr(), ld,
                                 ids.data_ptr(), wide, n, n_rows, k, _scale(scale), out.data_ptr(), ldo,
                                 0 if into is None else 1, ws.data_ptr(), ws.numel()))
     return out
@@ -225,14 +253,16 @@ def quantize_rows(x):
     """-> (q int8 (n, k), s float32 (n,)): s = max|x| / 127 of each row, q = x / s rounded to the nearest whole
     number (halves to the even one). A row of zeros has s = 0; a row with a NaN or an infinity s = NaN.
     The rows of q are padded to multiples of 16 bytes (its stride), as :func:`int8_scores` likes them."""
-    torch = _t()
-    ld = _rows(x, "x", tuple(_TYPES))
+    _t()
+    ld = _rows(x, "x", _TYPES)
     n, k = x.shape
-    q = torch.empty((n, (k + 15) // 16 * 16), dtype=torch.int8, device=x.device)
-    s = torch.empty((n,), dtype=torch.float32, device=x.device)
-    check(lib().blp_quantize_rows(x.device.index, _stream(x.device), _TYPES[x.dtype], x.data_ptr(), ld, n, k, q.data_ptr(),
-                                  q.shape[1], s.data_ptr()))
-    return q[:, :k], s
+    device = x.device
+    kp = (k + 15) // 16 * 16
+    q = _torch.empty((n, kp), dtype=_torch.int8, device=device)
+    s = _torch.empty(n, dtype=_torch.float32, device=device)
+    check(lib().blp_quantize_rows(device.index, _stream(device.index), _TYPES[x.dtype], x.data_ptr(), ld, n, k, q.data_ptr(),
+                                  kp, s.data_ptr()))
+    return (q if kp == k else q[:, :k]), s
 
 
 def int8_scores(q, s, table_q, table_s, dtype=None):
@@ -244,26 +274,26 @@ def int8_scores(q, s, table_q, table_s, dtype=None):
     dtype = torch.float32 if dtype is None else dtype
     if dtype not in _TYPES:
         raise ValueError("dtype must be float32, bfloat16 or float16 (got %s)" % (dtype,))
-    ldq, ldt = _rows(q, "q", (torch.int8,)), _rows(table_q, "table_q", (torch.int8,))
+    ldq, ldt = _rows(q, "q", _INT8), _rows(table_q, "table_q", _INT8)
     m, k = q.shape
     n = table_q.shape[0]
-    if table_q.shape[1] != k or table_q.device != q.device:
+    device = q.device
+    if table_q.shape[1] != k or table_q.device != device:
         raise ValueError("q %s and table_q %s must have rows of the same length on one device" % (
             tuple(q.shape), tuple(table_q.shape)))
     if k >= 1 << 17:
         raise ValueError("k must be below 131072: longer sums do not fit 32 bits")
     if n < 1:
         raise ValueError("the catalogue must have at least one row")
-    for t, what, rows in ((s, "s", m), (table_s, "table_s", n)):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != q.device or tuple(t.shape) != (rows,) \
-                or not t.is_contiguous():
-            raise ValueError("%s must be a contiguous float32 tensor of shape (%d,) on %s" % (what, rows, q.device))
-    out = torch.empty((m, n), dtype=dtype, device=q.device)
+    _floats(s, "s", device, ((m,),))
+    _floats(table_s, "table_s", device, ((n,),))
+    out = torch.empty((m, n), dtype=dtype, device=device)
+    qp, tp = q.data_ptr(), table_q.data_ptr()
     b = ctypes.c_int64(0)
-    check(lib().blp_scores8_workspace(q.data_ptr(), ldq, table_q.data_ptr(), ldt, m, n, k, ctypes.byref(b)))
-    ws = torch.empty(b.value, dtype=torch.uint8, device=q.device)
-    check(lib().blp_scores8(q.device.index, _stream(q.device), q.data_ptr(), ldq, s.data_ptr(), table_q.data_ptr(), ldt,
-                            table_s.data_ptr(), m, n, k, _TYPES[dtype], out.data_ptr(), n, ws.data_ptr(), ws.numel()))
+    check(lib().blp_scores8_workspace(qp, ldq, tp, ldt, m, n, k, ctypes.byref(b)))
+    ws = _bytes(device, b.value) if b.value else None
+    check(lib().blp_scores8(device.index, _stream(device.index), qp, ldq, s.data_ptr(), tp, ldt, table_s.data_ptr(), m, n, k,
+                            _TYPES[dtype], out.data_ptr(), n, ws.data_ptr() if b.value else None, b.value))
     return out
 
 
@@ -278,16 +308,16 @@ def _function(which):
         class SoftmaxLoss(torch.autograd.Function):
             @staticmethod
             def forward(ctx, x, table, target, scale, reduction):
-                out, lse, total, _, _ = _loss_forward(x, table, target, scale, reduction, False)
-                ctx.save_for_backward(x, table, target, lse, total)
+                out, lse, total, _, _ = _loss_forward(x, table, target, scale, reduction, 0, keep=True)
+                ctx.save_for_backward(x, table, target, lse, *(() if total is None else (total,)))
                 ctx.scale, ctx.reduction = scale, reduction
                 return out.clone()
 
             @staticmethod
             @torch.autograd.function.once_differentiable
             def backward(ctx, grad):
-                x, table, target, lse, total = ctx.saved_tensors
-                count = total[1] if ctx.reduction == "mean" else None
+                x, table, target, lse = ctx.saved_tensors[:4]
+                count = ctx.saved_tensors[4][1] if ctx.reduction == "mean" else None
                 dx, dt = softmax_loss_backward(grad.contiguous(), lse, count, x, table, target, ctx.scale,
                                                ctx.needs_input_grad[0], ctx.needs_input_grad[1])
                 return dx, dt, None, None, None

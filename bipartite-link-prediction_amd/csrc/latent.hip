@@ -773,21 +773,21 @@ constexpr int64_t GOAL = 512;                 // workgroups a launch should have
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int64_t div_up(int64_t v, int64_t by) { return (v + by - 1) / by; }
 
-enum ShapeId { BIG, MID, NARROW_P, NARROW_Q };
-using Big = Shape<2, 4, 8, 4>;       // 256 x 256
-using Mid = Shape<2, 2, 4, 4>;       // 128 x 128
-using NarrowP = Shape<1, 4, 4, 4>;   // 64 x 256
-using NarrowQ = Shape<4, 1, 4, 2>;   // 256 x 32
+enum ShapeId { BIG, MID, FLAT };
+using Big = Shape<2, 4, 8, 4>;   // 256 x 256, one workgroup a compute unit
+using Mid = Shape<2, 2, 4, 4>;   // 128 x 128, two
+using Flat = Shape<4, 1, 4, 2>;  // 256 x 32, two: few rows
+constexpr int BP_OF[] = {256, 128, 256}, BQ_OF[] = {256, 128, 32}, WP_OF[] = {2, 2, 4}, PER_CU[] = {1, 2, 2};
 
-int bp_of(int s) { return s == BIG || s == NARROW_Q ? 256 : s == MID ? 128 : 64; }
-int bq_of(int s) { return s == BIG || s == NARROW_P ? 256 : s == MID ? 128 : 32; }
-int wp_of(int s) { return s == BIG || s == MID ? 2 : s == NARROW_P ? 1 : 4; }
+int64_t tiles_of(int shape, int64_t np, int64_t nq) { return div_up(np, BP_OF[shape]) * div_up(nq, BQ_OF[shape]); }
 
-// Few rows: 32 of them a tile. Few outputs a row: 64. Else the large tile once it fills the card.
+// The shape whose rounds of tiles over the card cost least. A stage of a tile takes 1.55 us in the large shape and, two
+// workgroups side by side, 1.2 us in the middle one (8,192 x 100,000 x 1,024 halves: 980 and 860 TFLOP/s); a tile's
+// outputs about as long as 2 1/2 stages. Up to 32 rows: 32 of them a tile, bound by reading the other operand.
 int shape_of(int64_t np, int64_t nq) {
-  if (nq <= 32) return NARROW_Q;
-  if (np <= 64) return NARROW_P;
-  return div_up(np, 256) * div_up(nq, 256) >= 192 ? BIG : MID;
+  if (nq <= 32) return FLAT;
+  const double big = (double)div_up(tiles_of(BIG, np, nq), 256) * 1.55, mid = (double)div_up(tiles_of(MID, np, nq), 512) * 1.2;
+  return big <= mid ? BIG : MID;
 }
 
 struct Layout {
@@ -805,15 +805,23 @@ struct Slices {
   int stages;  // a slice
 };
 Slices slices_of(int64_t np, int64_t nq, int64_t k, int planes) {
-  Slices s;
-  s.shape = shape_of(np, nq);
-  const int64_t tiles = std::max<int64_t>(div_up(np, bp_of(s.shape)) * div_up(nq, bq_of(s.shape)), 1);
   const int64_t stages = div_up(k, STAGE / 2) * (planes == 1 ? 1 : SEGMENTS);
-  int64_t n = tiles >= GOAL / 2 ? 1 : std::min(GOAL / tiles, std::max<int64_t>(stages / 4, 1));
-  n = std::min<int64_t>(std::max<int64_t>(n, 1), 64);
-  s.stages = (int)std::max<int64_t>(div_up(stages, n), 1);
-  s.n = (int)std::max<int64_t>(div_up(stages, s.stages), 1);
-  return s;
+  Slices best = {FLAT, 1, (int)stages};
+  double least = -1;
+  for (int shape : {BIG, MID, FLAT}) {
+    if ((shape == FLAT) != (nq <= 32)) continue;
+    const int64_t tiles = std::max<int64_t>(tiles_of(shape, np, nq), 1), slots = 256 * PER_CU[shape];
+    int64_t n = std::min<int64_t>(std::max<int64_t>(std::min(slots / tiles, stages / 4), 1), 64);
+    const int64_t each = std::max<int64_t>(div_up(stages, n), 1);
+    n = std::max<int64_t>(div_up(stages, each), 1);
+    // rounds of tiles, a tile's stages and its outputs
+    const double cost = (double)div_up(tiles * n, slots) * ((double)each + 2.5) * (shape == BIG ? 1.55 : 1.2);
+    if (least < 0 || cost < least) {
+      least = cost;
+      best = {shape, (int)n, (int)each};
+    }
+  }
+  return best;
 }
 
 // The splits of the stream rows of a narrow kernel: two workgroups a compute unit, two stages each at least.
@@ -889,7 +897,7 @@ Plan plan_of(int type, int64_t m, int64_t n, int k, bool forward, bool grads, bo
     return p;
   }
   p.fwd = shape_of(n, m);
-  p.fwd_tiles = div_up(n, bp_of(p.fwd)) * wp_of(p.fwd);
+  p.fwd_tiles = div_up(n, BP_OF[p.fwd]) * WP_OF[p.fwd];
   p.o_part = l.take(forward ? p.fwd_tiles * m * 8 : 0);
   p.o_hit = l.take(forward ? m * 4 : 0);
   p.o_top = l.take(16);
@@ -917,21 +925,19 @@ void launch(const Problem& a, dim3 grid, const Epi& epi, hipStream_t st) {
 // `stages`: of a slice (0: all)
 template <int T, int LP, int LQ, class Epi>
 int product(int shape, Problem a, int slices, int stages, Epi epi, hipStream_t st) {
-  const int64_t tp = div_up(a.p.rows, bp_of(shape)), tq = div_up(a.q.rows, bq_of(shape));
+  const int64_t tp = div_up(a.p.rows, BP_OF[shape]), tq = div_up(a.q.rows, BQ_OF[shape]);
   BLP_CHECK(tp * tq <= 0x7fffffff, BLP_E_ARG, "softmax loss: too many tiles for one launch");
   a.tiles_p = (int)tp;
   a.tiles_q = (int)tq;
   a.slice = stages ? stages : (int)div_up(a.k, KE) * (T == F32 ? SEGMENTS : 1);
   // one or two workgroups a compute unit, which take tile after tile
-  const dim3 grid((unsigned)std::min<int64_t>(tp * tq, shape == BIG ? GOAL / 2 : GOAL), (unsigned)slices);
+  const dim3 grid((unsigned)std::min<int64_t>(tp * tq, 256 * PER_CU[shape]), (unsigned)slices);
   if (shape == BIG)
     launch<T, LP, LQ, Big>(a, grid, epi, st);
   else if (shape == MID)
     launch<T, LP, LQ, Mid>(a, grid, epi, st);
-  else if (shape == NARROW_P)
-    launch<T, LP, LQ, NarrowP>(a, grid, epi, st);
   else
-    launch<T, LP, LQ, NarrowQ>(a, grid, epi, st);
+    launch<T, LP, LQ, Flat>(a, grid, epi, st);
   BLP_HIP(hipGetLastError());
   return 0;
 }

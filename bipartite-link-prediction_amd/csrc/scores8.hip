@@ -204,7 +204,7 @@ int check_args(int64_t rows, int64_t cols, int k) {
 
 int64_t workspace(const void* q, int64_t ldq, const void* p, int64_t ldp, int64_t rows, int64_t cols, int k) {
   const int64_t kp = up(k, 16);
-  return std::max<int64_t>((whole(q, ldq, k) ? 0 : up(rows * kp, 256)) + (whole(p, ldp, k) ? 0 : up(cols * kp, 256)), 256);
+  return (whole(q, ldq, k) ? 0 : up(rows * kp, 256)) + (whole(p, ldp, k) ? 0 : up(cols * kp, 256));
 }
 
 int pack(Operand& o, int k, char*& ws, hipStream_t st) {
@@ -261,10 +261,11 @@ extern "C" int blp_scores8(int device, void* stream, const int8_t* q, int64_t ld
   if (rc) return rc;
   if (rows == 0) return 0;
   BLP_CHECK(out_type >= 0 && out_type <= 2, BLP_E_ARG, "scores8: type must be BLP_F32, BLP_BF16 or BLP_F16");
-  BLP_CHECK(q && s && table && ts && out && ws, BLP_E_ARG, "scores8: null pointer");
+  BLP_CHECK(q && s && table && ts && out, BLP_E_ARG, "scores8: null pointer");
   BLP_CHECK(ldq >= k && ldt >= k && ldo >= cols, BLP_E_ARG, "scores8: a row stride is smaller than the row");
   BLP_CHECK(std::max(ldq, ldt) <= (1 << 22), BLP_E_ARG, "scores8: row strides must be at most 2^22");
-  BLP_CHECK(ws_bytes >= workspace(q, ldq, table, ldt, rows, cols, k), BLP_E_ARG,
+  const int64_t need = workspace(q, ldq, table, ldt, rows, cols, k);
+  BLP_CHECK(need == 0 || (ws && ws_bytes >= need), BLP_E_ARG,
             "scores8: the workspace is too small (blp_scores8_workspace)");
   BLP_CHECK(((uintptr_t)ws & 255) == 0, BLP_E_ARG, "scores8: the workspace must be 256-byte aligned");
   DeviceGuard guard(device);
