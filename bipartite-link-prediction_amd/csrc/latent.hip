@@ -32,6 +32,7 @@ constexpr int mma_type(int t) { return t == F32 ? BF16 : t; }
 constexpr int planes_of(int t) { return t == F32 ? 3 : 1; }
 
 using blp::DeviceGuard;
+using blp::FastDiv;
 using Targets = blp::Ids;  // the target of row i, or -1 (ignored)
 
 // ---------------------------------------------------------------- packing
@@ -174,23 +175,40 @@ struct EpiLse {
   }
 };
 
-// 32 rows a block, 8 threads a row over the tiles' pairs.
+// R rows a block, 256 / R threads a row over the tiles' pairs: 32 rows read whole lines of pairs, 4 rows have 64 threads
+// each where there are too few rows to fill the card.
+template <int R>
 __global__ __launch_bounds__(256) void k_join(const float2* __restrict__ part, int64_t tiles, int64_t m,
                                               const float* __restrict__ hit, Targets targets, float* __restrict__ loss,
                                               float* __restrict__ lse) {
-  __shared__ float2 s_part[8][32];
-  const int r = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int64_t row = blockIdx.x * 32ll + r;
+  constexpr int G = 256 / R;
+  __shared__ float2 s_part[G][R];
+  const int r = threadIdx.x & (R - 1), g = threadIdx.x / R;
+  const int64_t row = blockIdx.x * (int64_t)R + r;
   float top = -INFINITY, sum = 0.f;
-  if (row < m)
-    for (int64_t t = g; t < tiles; t += 8) {
+  if (row < m) {
+    int64_t t = g;
+    for (; t + 3 * G < tiles; t += 4 * G) {
+      float2 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = part[(t + u * G) * m + row];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) merge(top, sum, v[u].x, v[u].y);
+    }
+    for (; t < tiles; t += G) {
       const float2 v = part[t * m + row];
       merge(top, sum, v.x, v.y);
     }
+  }
   s_part[g][r] = make_float2(top, sum);
-  __syncthreads();
+  for (int half = G / 2; half; half >>= 1) {
+    __syncthreads();
+    if (g < half) {
+      merge(top, sum, s_part[g + half][r].x, s_part[g + half][r].y);
+      s_part[g][r] = make_float2(top, sum);
+    }
+  }
   if (g == 0 && row < m) {
-    for (int i = 1; i < 8; ++i) merge(top, sum, s_part[i][r].x, s_part[i][r].y);
     const float l = (top + __builtin_amdgcn_logf(sum)) * LN2;  // logf: base 2
     lse[row] = l;
     loss[row] = targets(row) >= 0 ? l - hit[row] : 0.f;
@@ -382,18 +400,37 @@ struct EpiPart {
   }
 };
 
-// out = alpha sum_s part[s], in the slices' order.
-template <int T>
+// out = alpha sum_s part[s], always in the same order: G threads an output of four, thread g the slices g, g + G, ...,
+// then the threads' sums. G = 16 where the slices are many and the outputs few.
+template <int T, int G>
 __global__ __launch_bounds__(256) void k_sum_parts(const float* __restrict__ part, int slices, int64_t ld, int64_t np,
-                                                   int64_t nq, RowGrad g, float scale, char* __restrict__ out, int64_t ldo) {
+                                                   int64_t nq, FastDiv per, RowGrad g, float scale, char* __restrict__ out,
+                                                   int64_t ldo) {
+  constexpr int V = 256 / G;
+  __shared__ f32x4 s_sum[G > 1 ? 256 : 1];
   const float alpha = scale * g.all();
-  const int64_t per = ld / 4, n = nq * per, step = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += step) {
-    const int64_t q = i / per, p = (i - q * per) * 4;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < slices; ++s) v += *reinterpret_cast<const f32x4*>(part + (s * nq + q) * ld + p);
-    for (int e = 0; e < 4; ++e)
-      if (p + e < np) store1<T>(out + q * ldo + (p + e) * size_of(T), v[e] * alpha);
+  const int64_t n = nq * per.d;
+  const int v = threadIdx.x & (V - 1), gr = threadIdx.x / V;
+  for (int64_t i0 = blockIdx.x * (int64_t)V; i0 < n; i0 += (int64_t)gridDim.x * V) {
+    const int64_t i = i0 + v;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (i < n) {
+      const float* at = part + i * 4;  // ld = 4 per: rows follow one another
+#pragma unroll 4
+      for (int s = gr; s < slices; s += G) sum += *reinterpret_cast<const f32x4*>(at + s * (nq * ld));
+    }
+    if constexpr (G > 1) {
+      __syncthreads();
+      s_sum[threadIdx.x] = sum;
+      __syncthreads();
+      if (gr > 0) continue;
+      for (int k = 1; k < G; ++k) sum += s_sum[k * V + v];
+    }
+    if (i < n) {
+      const int64_t q = n < (1ll << 31) ? (int64_t)per((uint32_t)i) : i / per.d, p = (i - q * per.d) * 4;
+      for (int e = 0; e < 4; ++e)
+        if (p + e < np) store1<T>(out + q * ldo + (p + e) * size_of(T), sum[e] * alpha);
+    }
   }
 }
 
@@ -945,6 +982,21 @@ int product(int shape, Problem a, int slices, int stages, Epi epi, hipStream_t s
 int64_t grid_for(int64_t n) { return std::max<int64_t>(std::min<int64_t>(div_up(n, 256), 8192), 1); }
 
 template <int T>
+int sum_parts(const float* part, int slices, int64_t ld, int64_t np, int64_t nq, RowGrad g, float scale, void* out, int64_t ldo,
+              hipStream_t st) {
+  const FastDiv per((uint32_t)(ld / 4));
+  const int64_t n = nq * (ld / 4);
+  if (n == 0) return 0;
+  if (slices >= 16 && n < 256 * 1024)
+    k_sum_parts<T, 16><<<(unsigned)std::min<int64_t>(div_up(n, 16), 8192), 256, 0, st>>>(part, slices, ld, np, nq, per, g, scale,
+                                                                                        (char*)out, ldo * size_of(T));
+  else
+    k_sum_parts<T, 1><<<(unsigned)grid_for(n), 256, 0, st>>>(part, slices, ld, np, nq, per, g, scale, (char*)out, ldo * size_of(T));
+  BLP_HIP(hipGetLastError());
+  return 0;
+}
+
+template <int T>
 int pack(const char* src, int64_t ld, int64_t rows, int k, int kp, Targets t, char* dst, int64_t plane, hipStream_t st) {
   if (rows == 0) return 0;
   const int64_t grid = grid_for(rows * (kp / 8));
@@ -1025,9 +1077,7 @@ int narrow_grad(const Call& c, NarrowArgs a, const Splits& s, RowGrad g, float* 
   const EpiPart e = {part, ldp, p.k, rows, 0};
   const int rc = per_row ? narrow<T, MODE, true>(p, a, e, c.st) : narrow<T, MODE, false>(p, a, e, c.st);
   if (rc) return rc;
-  k_sum_parts<T><<<grid_for(rows * (ldp / 4)), 256, 0, c.st>>>(part, s.n, ldp, p.k, rows, g, c.scale, (char*)out, ldo * p.es);
-  BLP_HIP(hipGetLastError());
-  return 0;
+  return sum_parts<T>(part, s.n, ldp, p.k, rows, g, c.scale, out, ldo, c.st);
 }
 
 template <int T>
@@ -1046,7 +1096,11 @@ int forward(const Call& c, float* loss, float* lse, float* total, int mean) {
       rc = product<T, ROW, ROW>(p.fwd, a, 1, 0, EpiLse<T>{part, hit, c.targets, p.n, p.m, c.scale}, c.st);
     }
     if (rc) return rc;
-    k_join<<<(unsigned)div_up(p.m, 32), 256, 0, c.st>>>(part, p.narrow ? p.nl.n : p.fwd_tiles, p.m, hit, c.targets, loss, lse);
+    const int64_t pairs = p.narrow ? p.nl.n : p.fwd_tiles;
+    if (p.m >= 4096)
+      k_join<32><<<(unsigned)div_up(p.m, 32), 256, 0, c.st>>>(part, pairs, p.m, hit, c.targets, loss, lse);
+    else
+      k_join<4><<<(unsigned)div_up(p.m, 4), 256, 0, c.st>>>(part, pairs, p.m, hit, c.targets, loss, lse);
     BLP_HIP(hipGetLastError());
   }
   if (total) {
@@ -1061,10 +1115,7 @@ int backward(const Call& c, const float* lse, RowGrad g, void* dx, int64_t lddx,
   const Plan& p = c.p;
   if (p.m == 0) {  // no rows: the catalogue's gradient is zero
     if (dw) {
-      k_sum_parts<T><<<grid_for(p.n * up(p.k, 4) / 4), 256, 0, c.st>>>(nullptr, 0, up(p.k, 4), p.k, p.n,
-                                                                      RowGrad{nullptr, 0, nullptr, nullptr, 1.f}, 1.f,
-                                                                      (char*)dw, lddw * p.es);
-      BLP_HIP(hipGetLastError());
+      return sum_parts<T>(nullptr, 0, up(p.k, 4), p.k, p.n, RowGrad{nullptr, 0, nullptr, nullptr, 1.f}, 1.f, dw, lddw, c.st);
     }
     return 0;
   }
@@ -1114,8 +1165,7 @@ int backward(const Call& c, const float* lse, RowGrad g, void* dx, int64_t lddx,
       if (p.sw.n > 1) {
         rc = product<T, COL, COL>(p.sw.shape, aw, p.sw.n, p.sw.stages, EpiPart{pw, ldp, p.k, nj, 0}, c.st);
         if (rc) break;
-        k_sum_parts<T><<<grid_for(nj * (ldp / 4)), 256, 0, c.st>>>(pw, p.sw.n, ldp, p.k, nj, g, c.scale, out, lddw * p.es);
-        BLP_HIP(hipGetLastError());
+        rc = sum_parts<T>(pw, p.sw.n, ldp, p.k, nj, g, c.scale, out, lddw, c.st);
       } else {
         rc = product<T, COL, COL>(p.sw.shape, aw, 1, 0, EpiOut<T>{out, lddw * p.es, p.k, nj, g, c.scale}, c.st);
       }
@@ -1123,8 +1173,7 @@ int backward(const Call& c, const float* lse, RowGrad g, void* dx, int64_t lddx,
   }
   if (rc) return rc;
   if (dx && parts_x && p.m > 0) {
-    k_sum_parts<T><<<grid_for(p.m * (ldp / 4)), 256, 0, c.st>>>(px, p.sx.n, ldp, p.k, p.m, g, c.scale, (char*)dx, lddx * p.es);
-    BLP_HIP(hipGetLastError());
+    rc = sum_parts<T>(px, p.sx.n, ldp, p.k, p.m, g, c.scale, dx, lddx, c.st);
   }
   return 0;
 }
