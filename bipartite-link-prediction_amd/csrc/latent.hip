@@ -39,24 +39,20 @@ using Targets = blp::Ids;  // the target of row i, or -1 (ignored)
 // Rows as the tile engine takes them: `kp` elements a row (whole granules, zeros past k), 16-byte aligned;
 // with targets, the ignored rows as zeros. One 16-byte granule a thread; bound by the copy.
 template <int ES>
-__global__ __launch_bounds__(256) void k_pack(const char* __restrict__ src, int64_t ld, int64_t rows, int k, int kp,
+__global__ __launch_bounds__(256) void k_pack(const char* __restrict__ src, int64_t ld, int64_t rows, int k, FastDiv per,
                                               Targets targets, char* __restrict__ dst) {
   constexpr int GE = 16 / ES;
-  const int per = kp / GE;
-  const bool aligned = ((reinterpret_cast<uintptr_t>(src) | (uintptr_t)ld) & 15) == 0;
-  const int64_t n = rows * per, step = (int64_t)gridDim.x * blockDim.x;
+  const int64_t n = rows * per.d, step = (int64_t)gridDim.x * blockDim.x;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += step) {
-    const int64_t r = i / per;
-    const int e0 = (int)(i - r * per) * GE;
+    const int64_t r = n < (1ll << 31) ? (int64_t)per((uint32_t)i) : i / per.d;
+    const int e0 = (int)(i - r * per.d) * GE;
     i32x4 v = {0, 0, 0, 0};
     if (!targets.at || targets(r) >= 0) {
       const char* s = src + r * ld + (int64_t)e0 * ES;
-      if (aligned && e0 + GE <= k) {
-        v = *reinterpret_cast<const i32x4*>(s);
-      } else if constexpr (ES == 4) {
-        for (int j = 0; j < GE; ++j)
-          if (e0 + j < k) v[j] = reinterpret_cast<const int32_t*>(s)[j];
+      if (e0 + GE <= k) {
+        v = reinterpret_cast<const Unaligned16*>(s)->v;
       } else {
+        static_assert(ES == 2, "halves");
         for (int j = 0; j < GE; ++j)
           if (e0 + j < k) v[j >> 1] |= (int)((uint32_t)reinterpret_cast<const uint16_t*>(s)[j] << (16 * (j & 1)));
       }
@@ -67,13 +63,12 @@ __global__ __launch_bounds__(256) void k_pack(const char* __restrict__ src, int6
 
 // The same of floats into the three planes of halves, `plane` bytes apart. An infinite or NaN factor (or one that rounds
 // to infinity) has nothing in the lower planes.
-__global__ __launch_bounds__(256) void k_pack_planes(const char* __restrict__ src, int64_t ld, int64_t rows, int k, int kp,
+__global__ __launch_bounds__(256) void k_pack_planes(const char* __restrict__ src, int64_t ld, int64_t rows, int k, FastDiv per,
                                                      Targets targets, char* __restrict__ dst, int64_t plane) {
-  const int per = kp / 8;
-  const int64_t n = rows * per, step = (int64_t)gridDim.x * blockDim.x;
+  const int64_t n = rows * per.d, step = (int64_t)gridDim.x * blockDim.x;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += step) {
-    const int64_t r = i / per;
-    const int e0 = (int)(i - r * per) * 8;
+    const int64_t r = n < (1ll << 31) ? (int64_t)per((uint32_t)i) : i / per.d;
+    const int e0 = (int)(i - r * per.d) * 8;
     bf16x8 v[3];
     const bool keep = !targets.at || targets(r) >= 0;
     const float* s = reinterpret_cast<const float*>(src + r * ld) + e0;
@@ -1001,9 +996,9 @@ int pack(const char* src, int64_t ld, int64_t rows, int k, int kp, Targets t, ch
   if (rows == 0) return 0;
   const int64_t grid = grid_for(rows * (kp / 8));
   if constexpr (T == F32)
-    k_pack_planes<<<grid, 256, 0, st>>>(src, ld, rows, k, kp, t, dst, plane);
+    k_pack_planes<<<grid, 256, 0, st>>>(src, ld, rows, k, FastDiv((uint32_t)(kp / 8)), t, dst, plane);
   else
-    k_pack<2><<<grid, 256, 0, st>>>(src, ld, rows, k, kp, t, dst);
+    k_pack<2><<<grid, 256, 0, st>>>(src, ld, rows, k, FastDiv((uint32_t)(kp / 8)), t, dst);
   BLP_HIP(hipGetLastError());
   return 0;
 }

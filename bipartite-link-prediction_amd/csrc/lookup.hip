@@ -8,6 +8,7 @@
 // sums, which a second kernel adds up in the chunks' order. Every row of dy is read once, every row of dT
 // written once, and the result does not depend on timing.
 #include <algorithm>
+#include <type_traits>
 
 #include "blp_internal.h"
 #include "latent.h"
@@ -54,11 +55,11 @@ __global__ __launch_bounds__(256) void k_lookup(const char* __restrict__ table, 
 }
 
 // ---------------------------------------------------------------- sort
-// Stable radix sort of (id, position), least significant digit first, BITS bits a pass. A block takes
+// Stable radix sort of (id, position), least significant digit first, BITS (9 or 10) bits a pass. A block takes
 // 256 ROUNDS consecutive entries; wave w of it the w-th quarter, 64 at a time in order. The entries of one
 // digit are found with ballots (a lane's rank among them by counting the lanes below), so ranks follow
 // positions; ids outside the table get the largest key and end up last.
-constexpr int BITS = 10, BINS = 1 << BITS, SORT_WAVES = 4;
+constexpr int SORT_WAVES = 4, MOST_BITS = 10;
 
 __device__ inline uint32_t key_at(const Ids& ids, const uint32_t* keys, int64_t i) {
   if (keys) return keys[i];
@@ -67,9 +68,10 @@ __device__ inline uint32_t key_at(const Ids& ids, const uint32_t* keys, int64_t 
 }
 
 // counts[block][digit]
-template <int ROUNDS>
+template <int ROUNDS, int BITS>
 __global__ __launch_bounds__(256) void k_digit_counts(Ids ids, const uint32_t* __restrict__ keys, int64_t n, int shift,
                                                       uint32_t* __restrict__ counts) {
+  constexpr int BINS = 1 << BITS;
   __shared__ uint32_t s_count[BINS];
   for (int i = threadIdx.x; i < BINS; i += 256) s_count[i] = 0;
   __syncthreads();
@@ -84,7 +86,9 @@ __global__ __launch_bounds__(256) void k_digit_counts(Ids ids, const uint32_t* _
 }
 
 // 64 digits a block, 16 waves over the blocks' rows: counts become exclusive sums over the blocks; total[digit].
+template <int BITS>
 __global__ __launch_bounds__(1024) void k_digit_sums(uint32_t* __restrict__ counts, int blocks, uint32_t* __restrict__ total) {
+  constexpr int BINS = 1 << BITS;
   __shared__ uint32_t s_sum[16][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, d = blockIdx.x * 64 + lane;
   const int per = (blocks + 15) / 16, b0 = min(blocks, w * per), b1 = min(blocks, b0 + per);
@@ -104,11 +108,12 @@ __global__ __launch_bounds__(1024) void k_digit_sums(uint32_t* __restrict__ coun
   }
 }
 
-template <int ROUNDS>
+template <int ROUNDS, int BITS>
 __global__ __launch_bounds__(256) void k_scatter(Ids ids, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
                                                  int64_t n, int shift, const uint32_t* __restrict__ counts,
                                                  const uint32_t* __restrict__ total, uint32_t* __restrict__ keys_out,
                                                  uint32_t* __restrict__ pos_out) {
+  constexpr int BINS = 1 << BITS;
   __shared__ uint32_t s_base[BINS];
   __shared__ uint16_t s_wave[SORT_WAVES][BINS];
   __shared__ uint32_t s_sum[SORT_WAVES];
@@ -186,31 +191,31 @@ __global__ __launch_bounds__(256) void k_scatter(Ids ids, const uint32_t* __rest
   }
 }
 
-// Up to SMALL entries: one block, a bitonic sort of (id, position) pairs in LDS.
-constexpr int SMALL = 2048;
-__global__ __launch_bounds__(1024) void k_sort_small(Ids ids, int n, uint32_t* __restrict__ keys_out,
-                                                     uint32_t* __restrict__ pos_out) {
-  __shared__ unsigned long long s_v[SMALL];
-  int size = 64;
-  while (size < n) size <<= 1;
-  for (int i = threadIdx.x; i < size; i += 1024)
-    s_v[i] = i < n ? (unsigned long long)key_at(ids, nullptr, i) << 32 | (uint32_t)i : ~0ull;
+// Up to SMALL entries, in one launch: an entry's place is the number of entries with a smaller key, or with the same key
+// before it. Every block has all keys in LDS and places 64 entries, four threads an entry. n^2 comparisons: 8,192
+// entries take 6 us where the radix passes' six launches take 22.
+constexpr int SMALL = 8192;
+__global__ __launch_bounds__(256) void k_place_small(Ids ids, int n, uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out) {
+  extern __shared__ uint4 s_key[];  // n rounded up to 16, the rest the largest key
+  const int quads = (n + 15) / 16 * 4;
+  for (int i = threadIdx.x; i < quads * 4; i += 256)
+    reinterpret_cast<uint32_t*>(s_key)[i] = i < n ? key_at(ids, nullptr, i) : 0xffffffffu;
   __syncthreads();
-  for (int k2 = 2; k2 <= size; k2 <<= 1)
-    for (int j = k2 >> 1; j > 0; j >>= 1) {
-      for (int t = threadIdx.x; t < size / 2; t += 1024) {
-        const int a = ((t & ~(j - 1)) << 1) | (t & (j - 1)), b = a | j;
-        const unsigned long long x = s_v[a], y = s_v[b];
-        if ((x > y) == ((a & k2) == 0)) {
-          s_v[a] = y;
-          s_v[b] = x;
-        }
-      }
-      __syncthreads();
-    }
-  for (int i = threadIdx.x; i < n; i += 1024) {
-    keys_out[i] = (uint32_t)(s_v[i] >> 32);
-    pos_out[i] = (uint32_t)s_v[i];
+  const int i = blockIdx.x * 64 + (threadIdx.x >> 2), part = threadIdx.x & 3;
+  const uint32_t key = i < n ? reinterpret_cast<const uint32_t*>(s_key)[i] : 0xffffffffu;
+  int place = 0;
+#pragma unroll 4
+  for (int q = part; q < quads; q += 4) {
+    const uint4 v = s_key[q];
+    const int j = q * 4;
+    place += (v.x < key || (v.x == key && j < i)) + (v.y < key || (v.y == key && j + 1 < i)) +
+             (v.z < key || (v.z == key && j + 2 < i)) + (v.w < key || (v.w == key && j + 3 < i));
+  }
+  place += __shfl_xor(place, 1, 64);
+  place += __shfl_xor(place, 2, 64);
+  if (part == 0 && i < n) {
+    keys_out[place] = key;
+    pos_out[place] = (uint32_t)i;
   }
 }
 
@@ -431,7 +436,7 @@ int64_t div_up(int64_t v, int64_t by) { return (v + by - 1) / by; }
 int64_t up(int64_t v, int64_t to) { return div_up(v, to) * to; }
 
 struct Plan {
-  int passes, rounds, lanes, tiles;
+  int passes, bits, rounds, lanes, tiles;
   int64_t blocks, chunk, chunks, kv;
   int64_t o_keys[2], o_pos[2], o_counts, o_total, o_part, bytes;
 };
@@ -446,7 +451,8 @@ Plan plan_of(int type, int64_t n, int64_t rows, int k) {
   };
   int bits = 1;
   while (bits < 32 && (rows >> bits)) ++bits;
-  p.passes = n <= SMALL ? 0 : (int)div_up(bits, BITS);
+  p.passes = n <= SMALL ? 0 : (int)div_up(bits, MOST_BITS);
+  p.bits = p.passes * 9 >= bits ? 9 : 10;
   p.rounds = n <= 128 * 1024 ? 2 : 8;  // short lists: more blocks, each done sooner
   p.blocks = div_up(n, 256 * p.rounds);
   const int64_t vecs = div_up(k, 16 / size_of(type));
@@ -462,8 +468,8 @@ Plan plan_of(int type, int64_t n, int64_t rows, int k) {
     p.o_keys[i] = take(4 * n);
     p.o_pos[i] = take(4 * n);
   }
-  p.o_counts = take(p.passes ? 4 * BINS * p.blocks : 0);
-  p.o_total = take(4 * BINS);
+  p.o_counts = take(p.passes ? (4ll << p.bits) * p.blocks : 0);
+  p.o_total = take(4 << MOST_BITS);
   p.o_part = take(8 * p.chunks * p.kv);
   p.bytes = std::max<int64_t>(at, 256);
   return p;
@@ -483,18 +489,18 @@ int lookup(hipStream_t st, const void* table, int64_t ld, Ids ids, int64_t n, in
   return 0;
 }
 
-template <int ROUNDS>
+template <int ROUNDS, int BITS>
 int sort(hipStream_t st, const Plan& p, Ids ids, int64_t n, uint32_t* const* keys, uint32_t* const* pos, uint32_t* counts,
          uint32_t* total, int* last) {
   int cur = 0;
   for (int s = 0; s < p.passes; ++s) {
     const uint32_t* kin = s ? keys[cur] : nullptr;
     const int to = s ? cur ^ 1 : 0;
-    k_digit_counts<ROUNDS><<<(unsigned)p.blocks, 256, 0, st>>>(ids, kin, n, s * BITS, counts);
+    k_digit_counts<ROUNDS, BITS><<<(unsigned)p.blocks, 256, 0, st>>>(ids, kin, n, s * BITS, counts);
     BLP_HIP(hipGetLastError());
-    k_digit_sums<<<BINS / 64, 1024, 0, st>>>(counts, (int)p.blocks, total);
+    k_digit_sums<BITS><<<(1 << BITS) / 64, 1024, 0, st>>>(counts, (int)p.blocks, total);
     BLP_HIP(hipGetLastError());
-    k_scatter<ROUNDS><<<(unsigned)p.blocks, 256, 0, st>>>(ids, kin, s ? pos[cur] : nullptr, n, s * BITS, counts, total, keys[to],
+    k_scatter<ROUNDS, BITS><<<(unsigned)p.blocks, 256, 0, st>>>(ids, kin, s ? pos[cur] : nullptr, n, s * BITS, counts, total, keys[to],
                                                           pos[to]);
     BLP_HIP(hipGetLastError());
     cur = to;
@@ -512,11 +518,17 @@ int lookup_grad(hipStream_t st, const Plan& p, const void* dy, int64_t ld, Ids i
   uint32_t *counts = (uint32_t*)(ws + p.o_counts), *total = (uint32_t*)(ws + p.o_total);
   int cur = 0, rc = 0;
   if (p.passes == 0) {
-    if (n > 0) k_sort_small<<<1, 1024, 0, st>>>(ids, (int)n, keys[0], pos[0]);
+    if (n > 0) k_place_small<<<(unsigned)div_up(n, 64), 256, up(n, 16) * 4, st>>>(ids, (int)n, keys[0], pos[0]);
     BLP_HIP(hipGetLastError());
   } else {
-    rc = p.rounds == 2 ? sort<2>(st, p, ids, n, keys, pos, counts, total, &cur)
-                       : sort<8>(st, p, ids, n, keys, pos, counts, total, &cur);
+    auto run = [&](auto rounds, auto bits) {
+      return sort<decltype(rounds)::value, decltype(bits)::value>(st, p, ids, n, keys, pos, counts, total, &cur);
+    };
+    using std::integral_constant;
+    if (p.rounds == 2)
+      rc = p.bits == 9 ? run(integral_constant<int, 2>{}, integral_constant<int, 9>{}) : run(integral_constant<int, 2>{}, integral_constant<int, 10>{});
+    else
+      rc = p.bits == 9 ? run(integral_constant<int, 8>{}, integral_constant<int, 9>{}) : run(integral_constant<int, 8>{}, integral_constant<int, 10>{});
     if (rc) return rc;
   }
   const Sums a = {keys[cur], pos[cur], n, p.chunk, p.chunks, (uint32_t)ids.rows, k, p.lanes, scale, (char*)out, ldo * ES, add,

@@ -15,6 +15,7 @@ namespace {
 using namespace blp::tile;
 using namespace blp::rows;
 using blp::DeviceGuard;
+using blp::FastDiv;
 
 struct __attribute__((packed, aligned(1))) Unaligned4 {
   uint32_t v;
@@ -80,18 +81,22 @@ __global__ __launch_bounds__(256) void k_quantize(const char* __restrict__ x, in
 }
 
 // 8-bit rows as the tile engine takes them: whole granules, zeros past k.
-__global__ __launch_bounds__(256) void k_pack8(const int8_t* __restrict__ src, int64_t ld, int64_t rows, int k, int kp,
+__global__ __launch_bounds__(256) void k_pack8(const int8_t* __restrict__ src, int64_t ld, int64_t rows, int k, FastDiv per,
                                                int8_t* __restrict__ dst) {
-  const int per = kp / 16;
-  const int64_t n = rows * per, step = (int64_t)gridDim.x * blockDim.x;
+  const int64_t n = rows * per.d, step = (int64_t)gridDim.x * blockDim.x;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += step) {
-    const int64_t r = i / per;
-    const int e0 = (int)(i - r * per) * 16;
+    const int64_t r = n < (1ll << 31) ? (int64_t)per((uint32_t)i) : i / per.d;
+    const int e0 = (int)(i - r * per.d) * 16;
     const int8_t* s = src + r * ld + e0;
-    uint32_t w[4] = {0, 0, 0, 0};
-    for (int j = 0; j < 16; ++j)
-      if (e0 + j < k) w[j >> 2] |= (uint32_t)(uint8_t)s[j] << (8 * (j & 3));
-    reinterpret_cast<i32x4*>(dst)[i] = i32x4{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+    i32x4 v = {0, 0, 0, 0};
+    if (e0 + 16 <= k) {
+      v = reinterpret_cast<const Unaligned16*>(s)->v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (e0 + j < k) v[j >> 2] |= (int)((uint32_t)(uint8_t)s[j] << (8 * (j & 3)));
+    }
+    reinterpret_cast<i32x4*>(dst)[i] = v;
   }
 }
 
@@ -210,7 +215,7 @@ int64_t workspace(const void* q, int64_t ldq, const void* p, int64_t ldp, int64_
 int pack(Operand& o, int k, char*& ws, hipStream_t st) {
   const int64_t kp = up(k, 16), n = o.rows * kp / 16;
   k_pack8<<<(unsigned)std::max<int64_t>(std::min<int64_t>(div_up(n, 256), 8192), 1), 256, 0, st>>>(
-      (const int8_t*)o.base, o.ld, o.rows, k, (int)kp, (int8_t*)ws);
+      (const int8_t*)o.base, o.ld, o.rows, k, FastDiv((uint32_t)(kp / 16)), (int8_t*)ws);
   BLP_HIP(hipGetLastError());
   o = {ws, kp, o.rows};
   ws += up(o.rows * kp, 256);
