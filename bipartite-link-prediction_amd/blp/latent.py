@@ -146,7 +146,8 @@ def softmax_loss(x, table, target, scale=1.0, reduction="mean"):
     row of `table` that belongs to each row of x. A target outside [0, n) (-1, as in the top-k lists'
     missing slots) ignores its row: loss 0, gradient 0, whatever x holds there. reduction "mean" (over
     the rows not ignored; 0 if there is none), "sum" or "none" (one loss a row). Returns float32;
-    differentiable in x and table. Sums and the softmax's statistics are held in 32 bits. Float32 factors are
+    differentiable in x and table (not inside a graph capture: capture :func:`softmax_loss_grad`).
+    Sums and the softmax's statistics are held in 32 bits. Float32 factors are
     multiplied as sums of three bfloat16 each, with 32-bit results; they have to be finite."""
     torch = _t()
     if torch.is_grad_enabled() and (getattr(x, "requires_grad", False) or getattr(table, "requires_grad", False)):
@@ -194,7 +195,7 @@ def _scale(scale):
 def lookup(table, ids, scale=1.0):
     """``scale * table[ids]``: table (n, k) float32 / bfloat16 / float16, ids int32 / int64 of any shape ->
     ids.shape + (k,) in the table's type, rounded once. An id outside [0, n) (-1) gives a row of zeros.
-    Differentiable in table (:func:`lookup_grad`)."""
+    Differentiable in table (not inside a graph capture: capture :func:`lookup_grad`)."""
     torch = _t()
     if torch.is_grad_enabled() and getattr(table, "requires_grad", False):
         return _function("lookup").apply(table, ids, scale)
@@ -240,6 +241,9 @@ def lookup_grad(grad, ids, n_rows, scale=1.0, into=None):
         out, ldo = into, _rows(into, "into", (grad.dtype,))
         if tuple(into.shape) != (n_rows, k) or into.device != grad.device:
             raise ValueError("into must be of shape %s on %s" % ((n_rows, k), grad.device))
+        if n and into.data_ptr() < grad.data_ptr() + ((n - 1) * ld + k) * grad.element_size() \
+                and grad.data_ptr() < into.data_ptr() + ((n_rows - 1) * ldo + k) * grad.element_size():
+            raise ValueError("into must not overlap grad")
     b = ctypes.c_int64(0)
     check(lib().blp_lookup_grad_workspace(_TYPES[grad.dtype], n, n_rows, k, ctypes.byref(b)))
     ws = _bytes(grad.device, b.value)
@@ -297,6 +301,14 @@ def int8_scores(q, s, table_q, table_s, dtype=None):
     return out
 
 
+def _no_capture(what, instead):
+    """Autograd ties a leaf's gradient to the stream on which the leaf was first used, and waits for that stream in the
+    backward pass; inside a capture that cannot be honoured, and the process may end. The explicit calls
+    queue their work on the current stream alone."""
+    if _torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("%s: gradients through autograd cannot be captured into a graph; capture %s instead" % (what, instead))
+
+
 _fn = {}
 
 
@@ -308,6 +320,7 @@ def _function(which):
         class SoftmaxLoss(torch.autograd.Function):
             @staticmethod
             def forward(ctx, x, table, target, scale, reduction):
+                _no_capture("softmax_loss", "softmax_loss_grad")
                 out, lse, total, _, _ = _loss_forward(x, table, target, scale, reduction, 0, keep=True)
                 ctx.save_for_backward(x, table, target, lse, *(() if total is None else (total,)))
                 ctx.scale, ctx.reduction = scale, reduction
@@ -316,6 +329,7 @@ def _function(which):
             @staticmethod
             @torch.autograd.function.once_differentiable
             def backward(ctx, grad):
+                _no_capture("softmax_loss", "softmax_loss_grad")
                 x, table, target, lse = ctx.saved_tensors[:4]
                 count = ctx.saved_tensors[4][1] if ctx.reduction == "mean" else None
                 dx, dt = softmax_loss_backward(grad.contiguous(), lse, count, x, table, target, ctx.scale,
@@ -325,6 +339,7 @@ def _function(which):
         class Lookup(torch.autograd.Function):
             @staticmethod
             def forward(ctx, table, ids, scale):
+                _no_capture("lookup", "lookup_grad")
                 ctx.save_for_backward(ids)
                 ctx.scale, ctx.n_rows = scale, table.shape[0]
                 return _lookup(table, ids, scale)
@@ -332,6 +347,7 @@ def _function(which):
             @staticmethod
             @torch.autograd.function.once_differentiable
             def backward(ctx, grad):
+                _no_capture("lookup", "lookup_grad")
                 (ids,) = ctx.saved_tensors
                 return lookup_grad(grad.contiguous(), ids, ctx.n_rows, ctx.scale), None, None
 

@@ -1197,6 +1197,7 @@ int dispatch(int device, void* stream, int type, const void* x, int64_t ldx, con
   if (rc) return rc;
   const int es = size_of(type);
   BLP_CHECK(w && (m == 0 || (x && target && loss && lse)) && ws, BLP_E_ARG, "softmax loss: null pointer");
+  BLP_CHECK(fabsf(scale) <= 3.4028235e38f, BLP_E_ARG, "softmax loss: scale must be finite");
   BLP_CHECK(ldx >= k && ldw >= k && (!dx || lddx >= k) && (!dw || lddw >= k), BLP_E_ARG,
             "softmax loss: a row stride is smaller than k");
   BLP_CHECK(std::max(ldx, ldw) <= (1 << 20), BLP_E_ARG, "softmax loss: row strides must be at most 2^20 elements");

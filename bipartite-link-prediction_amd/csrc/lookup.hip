@@ -562,6 +562,7 @@ extern "C" int blp_lookup(int device, void* stream, int type, const void* table,
   if (n == 0) return 0;
   BLP_CHECK(table && ids && out, BLP_E_ARG, "lookup: null pointer");
   BLP_CHECK(ldt >= k && ldo >= k, BLP_E_ARG, "lookup: a row stride is smaller than k");
+  BLP_CHECK(fabsf(scale) <= 3.4028235e38f, BLP_E_ARG, "lookup: scale must be finite");
   DeviceGuard guard(device);
   if (guard.rc) return guard.rc;
   const Ids at = {ids, ids64, rows};
@@ -586,6 +587,7 @@ extern "C" int blp_lookup_grad(int device, void* stream, int type, const void* g
   if (rc) return rc;
   BLP_CHECK(out && ws && (n == 0 || (grad && ids)), BLP_E_ARG, "lookup: null pointer");
   BLP_CHECK((n == 0 || ldg >= k) && ldo >= k, BLP_E_ARG, "lookup: a row stride is smaller than k");
+  BLP_CHECK(fabsf(scale) <= 3.4028235e38f, BLP_E_ARG, "lookup: scale must be finite");
   const Plan p = plan_of(type, n, rows, k);
   BLP_CHECK(ws_bytes >= p.bytes, BLP_E_ARG, "lookup: the workspace is too small (blp_lookup_grad_workspace)");
   BLP_CHECK(((uintptr_t)ws & 255) == 0, BLP_E_ARG, "lookup: the workspace must be 256-byte aligned");

@@ -39,7 +39,8 @@ def check(got, want, bound):
 
 
 CASES = [(1, 1, 1), (1, 300, 50), (20, 5000, 64), (63, 7, 3), (64, 7, 8), (65, 7, 130), (300, 1, 33), (2048, 100, 16),
-         (2049, 100, 24), (5000, 3000, 64), (70001, 1500, 40), (30000, 70000, 7)]
+         (2049, 100, 24), (5000, 3000, 64), (70001, 1500, 40), (30000, 70000, 7),
+         (8192, 900, 20), (8193, 900, 20), (140001, 3000, 12)]
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
@@ -109,6 +110,17 @@ def test_added_to_a_gradient(gpu, dtype):
         check(into, *grad_reference(grad, ids, 50, 0.5, before[:, 4:24]))
         assert torch.equal(into[13], before[13, 4:24])  # a row without ids is left alone
         assert torch.equal(wide[:, :4], before[:, :4]) and torch.equal(wide[:, 24:], before[:, 24:])
+
+
+def test_overlap_is_refused(gpu):
+    torch = _torch()
+    from blp import latent
+
+    both = torch.zeros(20, 8, device="cuda")
+    ids = torch.zeros(10, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError):
+        latent.lookup_grad(both[:10], ids, 12, into=both[8:])
+    latent.lookup_grad(both[:10], ids, 10, into=both[10:])
 
 
 def test_shapes_strides_and_empty(gpu):
