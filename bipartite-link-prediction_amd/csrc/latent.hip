@@ -16,6 +16,7 @@
 // A row whose target lies outside [0, n_cols) is ignored: loss 0, gradient 0, and its x is never multiplied
 // (it may hold anything, NaN too).
 #include <algorithm>
+#include <type_traits>
 
 #include "blp_internal.h"
 #include "latent.h"
@@ -30,6 +31,8 @@ constexpr float LN2 = 0.69314718055994530942f;
 // The matrix instructions' type, and the planes a factor is held in.
 constexpr int mma_type(int t) { return t == F32 ? BF16 : t; }
 constexpr int planes_of(int t) { return t == F32 ? 3 : 1; }
+// float16 holds dS times this: a probability below 2^-24 is not lost.
+constexpr float extra_of(int t) { return t == F16 ? 16384.f : 1.f; }
 
 using blp::DeviceGuard;
 using blp::FastDiv;
@@ -89,6 +92,20 @@ __global__ __launch_bounds__(256) void k_pack_planes(const char* __restrict__ sr
     for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(dst + p * plane + i * 16) = v[p];
   }
 }
+
+// What the narrow gradients read of a row of x, in blocks of 64 rows: log2(e) lse - log2(extra) (infinite: ignored),
+// g / max|g|, the target.
+struct Rows {
+  float* at;
+  __device__ float* of(int64_t block) const { return at + block * 256; }
+  __device__ void put(int64_t row, int64_t target, float lse, float extra, float g) const {
+    float* to = of(row >> 6) + (row & 63);
+    to[0] = target >= 0 ? fmaf(lse, LOG2E, -__builtin_amdgcn_logf(extra)) : INFINITY;
+    to[64] = target >= 0 ? g : 0.f;
+    reinterpret_cast<int*>(to)[128] = (int)target;
+    to[192] = 0.f;
+  }
+};
 
 // ---------------------------------------------------------------- forward
 // Two pairs as one. fmaxf drops a NaN, the sum keeps it (exp2(NaN - base)); an infinite reference gives inf - inf = NaN.
@@ -175,7 +192,7 @@ struct EpiLse {
 template <int R>
 __global__ __launch_bounds__(256) void k_join(const float2* __restrict__ part, int64_t tiles, int64_t m,
                                               const float* __restrict__ hit, Targets targets, float* __restrict__ loss,
-                                              float* __restrict__ lse) {
+                                              float* __restrict__ lse, Rows rows, float extra) {
   constexpr int G = 256 / R;
   __shared__ float2 s_part[G][R];
   const int r = threadIdx.x & (R - 1), g = threadIdx.x / R;
@@ -205,8 +222,12 @@ __global__ __launch_bounds__(256) void k_join(const float2* __restrict__ part, i
   }
   if (g == 0 && row < m) {
     const float l = (top + __builtin_amdgcn_logf(sum)) * LN2;  // logf: base 2
+    const int64_t t = targets(row);
     lse[row] = l;
-    loss[row] = targets(row) >= 0 ? l - hit[row] : 0.f;
+    loss[row] = t >= 0 ? l - hit[row] : 0.f;
+    if (rows.at) rows.put(row, t, l, extra, 1.f);
+  } else if (g == 0 && rows.at && row < (m + 63) / 64 * 64) {
+    rows.put(row, -1, 0.f, extra, 0.f);
   }
 }
 
@@ -441,19 +462,10 @@ __global__ __launch_bounds__(256) void k_sum_parts(const float* __restrict__ par
 // Per 64 scores a wave spends about 26 (LSE) and 22 (DX, DW) cycles in the vector unit, 16 of them in exp2, and
 // k / 8 (k / 4) in the matrix unit: exp2 is what bounds these kernels, and computing it again in DX and DW costs less
 // than writing dS once and reading it twice.
-struct Rows {  // per 64 rows of x: log2(e) lse - log2(extra) (infinite: ignored), g / max|g|, target, in blocks of 3 x 64
-  float* at;
-  __device__ float* of(int64_t block) const { return at + block * 256; }
-};
-
 __global__ __launch_bounds__(64) void k_rows(const float* __restrict__ lse, RowGrad g, Targets targets, int64_t m, Rows rows) {
   const int64_t i = blockIdx.x * 64ll + threadIdx.x;
   const int64_t t = i < m ? targets(i) : -1;
-  float* at = rows.of(blockIdx.x) + threadIdx.x;
-  at[0] = t >= 0 ? fmaf(lse[i], LOG2E, -__builtin_amdgcn_logf(g.extra)) : INFINITY;
-  at[64] = t >= 0 ? g.row(i) / g.extra : 0.f;
-  reinterpret_cast<int*>(at)[128] = (int)t;
-  at[192] = 0.f;
+  rows.put(i, t, t >= 0 ? lse[i] : 0.f, g.extra, t >= 0 ? g.row(i) / g.extra : 0.f);
 }
 
 enum NarrowMode { LSE, DX, DW };
@@ -487,21 +499,27 @@ __device__ inline int pack2(float a, float b) {
   }
 }
 
+// LDS of a workgroup: a stage's rows, and three buffers of them (floats: two, a stage of theirs lasts longer).
+template <int T, int KS>
+struct NarrowLds {
+  static constexpr int HALVES = KS > 2 ? 2 : 1;  // 128-byte parts of a row
+  static constexpr int PART = 64 * STAGE;        // bytes of one part of a stage
+  static constexpr int BUF = planes_of(T) * HALVES * PART;
+  static constexpr bool THREE = T != F32;
+};
+
 template <int T, int KS, int MODE, bool PER_ROW, class Epi>
-__global__ __launch_bounds__(256, KS > 3 ? 2 : KS > 2 || T == F32 ? 3 : 4) void k_narrow(NarrowArgs a, Epi epi) {
+__device__ __attribute__((always_inline)) inline void narrow_body(const NarrowArgs& a, const Epi& epi, int block, char* s_a, char* s_b,
+                                                                  char* s_c, char* s_ra, char* s_rb, char* s_rc) {
   constexpr int MT = mma_type(T), PL = planes_of(T);
-  constexpr int FO = 2;                              // own fragments of 16 rows a wave
-  constexpr int HALVES = KS > 2 ? 2 : 1;             // 128-byte parts of a row
-  constexpr int PART = 64 * STAGE;                   // bytes of one part of a stage
-  constexpr int BUF = PL * HALVES * PART;
+  constexpr int FO = 2;  // own fragments of 16 rows a wave
+  constexpr int HALVES = NarrowLds<T, KS>::HALVES, PART = NarrowLds<T, KS>::PART, BUF = NarrowLds<T, KS>::BUF;
+  constexpr bool THREE = NarrowLds<T, KS>::THREE;
   constexpr int COPIES = 2 * PL * HALVES + (MODE == DW);  // a wave issues for a stage
-  constexpr bool THREE = PL == 1;                         // buffers (floats: two, a stage of theirs lasts longer)
-  __shared__ __attribute__((aligned(1024))) char s_a[BUF], s_b[BUF], s_c[THREE ? BUF : 16];
-  __shared__ __attribute__((aligned(1024))) char s_ra[MODE == DW ? 1024 : 16], s_rb[MODE == DW ? 1024 : 16],
-      s_rc[MODE == DW ? 1024 : 16];
   // a die's workgroups take neighbouring own tiles of one split: the split's rows stay in its L2
-  const int n_blocks = a.own_tiles * a.splits, per = n_blocks >> 3, more = n_blocks & 7, xcd = blockIdx.x & 7;
-  const int id = xcd * per + min(xcd, more) + (blockIdx.x >> 3);
+  const int n_blocks = a.own_tiles * a.splits, per = n_blocks >> 3, more = n_blocks & 7, xcd = block & 7;
+  if (block >= n_blocks) return;
+  const int id = xcd * per + min(xcd, more) + (block >> 3);
   const int split = id / a.own_tiles, own_tile = id - split * a.own_tiles;
   const int lane = threadIdx.x & 63, l = lane & 15, h = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -798,6 +816,43 @@ __global__ __launch_bounds__(256, KS > 3 ? 2 : KS > 2 || T == F32 ? 3 : 4) void 
   }
 }
 
+template <int T, int KS>
+__global__ __launch_bounds__(256, KS > 2 || T == F32 ? 3 : 4) void k_narrow_lse(NarrowArgs a) {
+  using L = NarrowLds<T, KS>;
+  __shared__ __attribute__((aligned(1024))) char s_a[L::BUF], s_b[L::BUF], s_c[L::THREE ? L::BUF : 16];
+  narrow_body<T, KS, LSE, false>(a, 0, blockIdx.x, s_a, s_b, s_c, nullptr, nullptr, nullptr);
+}
+
+// A gradient's outputs: splits' partial sums, or rounded in place.
+template <int T>
+struct EpiGradient {
+  bool parts;
+  EpiPart part;
+  EpiOut<T> out;
+  template <class S>
+  __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int tile, int slice, lds_char* scratch) const {
+    if (parts)
+      part.template run<S>(acc, p0, q0, tile, slice, scratch);
+    else
+      out.template run<S>(acc, p0, q0, tile, slice, scratch);
+  }
+};
+
+// Both gradients in one launch: the workgroups of one fill the compute units that the other's leave (10,000 x 100,000
+// x 64: 782 workgroups of dw alone keep three quarters of the card's slots busy).
+template <int T, int KS, bool PER_ROW>
+__global__ __launch_bounds__(256, KS > 3 ? 2 : KS > 2 || T == F32 ? 3 : 4) void k_narrow_grads(NarrowArgs w, EpiGradient<T> ew,
+                                                                                              int w_blocks, NarrowArgs x,
+                                                                                              EpiGradient<T> ex) {
+  using L = NarrowLds<T, KS>;
+  __shared__ __attribute__((aligned(1024))) char s_a[L::BUF], s_b[L::BUF], s_c[L::THREE ? L::BUF : 16];
+  __shared__ __attribute__((aligned(1024))) char s_ra[1024], s_rb[1024], s_rc[L::THREE ? 1024 : 16];
+  if ((int)blockIdx.x < w_blocks)
+    narrow_body<T, KS, DW, PER_ROW>(w, ew, blockIdx.x, s_a, s_b, s_c, s_ra, s_rb, s_rc);
+  else
+    narrow_body<T, KS, DX, PER_ROW>(x, ex, blockIdx.x - w_blocks, s_a, s_b, s_c, s_ra, s_rb, s_rc);
+}
+
 // ---------------------------------------------------------------- host side
 constexpr int64_t PIECE_BYTES = 512ll << 20;  // dS of one piece of the catalogue
 constexpr int64_t GOAL = 512;                 // workgroups a launch should have
@@ -1031,48 +1086,60 @@ int bind(Call& c, const void* x, int64_t ldx, const void* w, int64_t ldw) {
   return rc;
 }
 
-struct NoEpilogue {
-  template <class S>
-  __device__ void run(f32x4 (&)[S::FP][S::FQ], int64_t, int64_t, int, int, lds_char*) const {}
-};
-
-template <int T, int MODE, bool PER_ROW, class Epi>
-int narrow(const Plan& p, const NarrowArgs& a, Epi epi, hipStream_t st) {
-  const int64_t blocks = (int64_t)a.own_tiles * a.splits;
-  BLP_CHECK(blocks <= 0x7fffffff, BLP_E_ARG, "softmax loss: too many tiles for one launch");
-  if (blocks == 0) return 0;
-  const unsigned grid = (unsigned)blocks;
-  if (p.ks == 1) {
-    k_narrow<T, 1, MODE, PER_ROW, Epi><<<grid, 256, 0, st>>>(a, epi);
-  } else if (p.ks == 2) {
-    k_narrow<T, 2, MODE, PER_ROW, Epi><<<grid, 256, 0, st>>>(a, epi);
+template <int T, class F>
+void with_steps(int ks, F f) {
+  if (ks == 1) {
+    f(std::integral_constant<int, 1>{});
+  } else if (ks == 2) {
+    f(std::integral_constant<int, 2>{});
   } else if constexpr (T != F32) {
-    if (p.ks == 3)
-      k_narrow<T, 3, MODE, PER_ROW, Epi><<<grid, 256, 0, st>>>(a, epi);
+    if (ks == 3)
+      f(std::integral_constant<int, 3>{});
     else
-      k_narrow<T, 4, MODE, PER_ROW, Epi><<<grid, 256, 0, st>>>(a, epi);
+      f(std::integral_constant<int, 4>{});
   }
+}
+
+template <int T>
+int narrow_lse(const Call& c, float2* part, float* hit) {
+  const Plan& p = c.p;
+  const NarrowArgs a = {c.x, c.w, p.x_plane(), p.w_plane(), p.kp, p.nl.range, p.nl.own_tiles, p.nl.n, c.scale, 1.f, c.targets,
+                        part, hit, Rows{nullptr}};
+  const int64_t blocks = (int64_t)p.nl.own_tiles * p.nl.n;
+  BLP_CHECK(blocks <= 0x7fffffff, BLP_E_ARG, "softmax loss: too many tiles for one launch");
+  with_steps<T>(p.ks, [&](auto ks) { k_narrow_lse<T, decltype(ks)::value><<<(unsigned)blocks, 256, 0, c.st>>>(a); });
   BLP_HIP(hipGetLastError());
   return 0;
 }
 
-// One gradient of the narrow path: straight into `out`, or by way of the splits' partial sums.
-template <int T, int MODE>
-int narrow_grad(const Call& c, NarrowArgs a, const Splits& s, RowGrad g, float* part, void* out, int64_t ldo, int64_t rows) {
+template <int T>
+int narrow_grads(const Call& c, RowGrad g, void* dx, int64_t lddx, void* dw, int64_t lddw) {
   const Plan& p = c.p;
   const int64_t ldp = up(p.k, 4);
-  a.own_tiles = s.own_tiles;
-  a.splits = s.n;
-  a.range = s.range;
+  float *px = (float*)(c.ws + p.o_px), *pw = (float*)(c.ws + p.o_pw);
+  const Rows rows = {(float*)(c.ws + p.o_rows)};
+  const NarrowArgs x = {c.x, c.w, p.x_plane(), p.w_plane(), p.kp, p.nx.range, dx ? p.nx.own_tiles : 0, p.nx.n, c.scale, g.extra,
+                        c.targets, nullptr, nullptr, rows};
+  const NarrowArgs w = {c.w, c.x, p.w_plane(), p.x_plane(), p.kp, p.nw.range, dw ? p.nw.own_tiles : 0, p.nw.n, c.scale, g.extra,
+                        c.targets, nullptr, nullptr, rows};
+  const EpiGradient<T> ex = {p.nx.n > 1, {px, ldp, p.k, p.m, 0}, {(char*)dx, lddx * p.es, p.k, p.m, g, c.scale}};
+  const EpiGradient<T> ew = {p.nw.n > 1, {pw, ldp, p.k, p.n, 0}, {(char*)dw, lddw * p.es, p.k, p.n, g, c.scale}};
+  const int64_t bw = up((int64_t)w.own_tiles * w.splits, 8), bx = (int64_t)x.own_tiles * x.splits;  // eights: x keeps its dies
+  BLP_CHECK(bw + bx <= 0x7fffffff, BLP_E_ARG, "softmax loss: too many tiles for one launch");
+  if (bw + bx == 0) return 0;
   const bool per_row = g.g && g.stride;
-  if (s.n == 1) {
-    const EpiOut<T> e = {(char*)out, ldo * p.es, p.k, rows, g, c.scale};
-    return per_row ? narrow<T, MODE, true>(p, a, e, c.st) : narrow<T, MODE, false>(p, a, e, c.st);
-  }
-  const EpiPart e = {part, ldp, p.k, rows, 0};
-  const int rc = per_row ? narrow<T, MODE, true>(p, a, e, c.st) : narrow<T, MODE, false>(p, a, e, c.st);
-  if (rc) return rc;
-  return sum_parts<T>(part, s.n, ldp, p.k, rows, g, c.scale, out, ldo, c.st);
+  with_steps<T>(p.ks, [&](auto ks) {
+    constexpr int KS = decltype(ks)::value;
+    if (per_row)
+      k_narrow_grads<T, KS, true><<<(unsigned)(bw + bx), 256, 0, c.st>>>(w, ew, (int)bw, x, ex);
+    else
+      k_narrow_grads<T, KS, false><<<(unsigned)(bw + bx), 256, 0, c.st>>>(w, ew, (int)bw, x, ex);
+  });
+  BLP_HIP(hipGetLastError());
+  int rc = 0;
+  if (dx && p.nx.n > 1) rc = sum_parts<T>(px, p.nx.n, ldp, p.k, p.m, g, c.scale, dx, lddx, c.st);
+  if (!rc && dw && p.nw.n > 1) rc = sum_parts<T>(pw, p.nw.n, ldp, p.k, p.n, g, c.scale, dw, lddw, c.st);
+  return rc;
 }
 
 template <int T>
@@ -1083,19 +1150,19 @@ int forward(const Call& c, float* loss, float* lse, float* total, int mean) {
     float* hit = (float*)(c.ws + p.o_hit);
     int rc;
     if (p.narrow) {
-      const NarrowArgs a = {c.x, c.w, p.x_plane(), p.w_plane(), p.kp, p.nl.range, p.nl.own_tiles, p.nl.n, c.scale, 1.f, c.targets,
-                            part, hit, Rows{nullptr}};
-      rc = narrow<T, LSE, false>(p, a, NoEpilogue{}, c.st);
+      rc = narrow_lse<T>(c, part, hit);
     } else {
       const Problem a = {c.w, c.x, p.kp, 0, 0, 0, p.w_plane(), p.x_plane()};
       rc = product<T, ROW, ROW>(p.fwd, a, 1, 0, EpiLse<T>{part, hit, c.targets, p.n, p.m, c.scale}, c.st);
     }
     if (rc) return rc;
     const int64_t pairs = p.narrow ? p.nl.n : p.fwd_tiles;
+    const Rows rows = {p.narrow && p.grads ? (float*)(c.ws + p.o_rows) : nullptr};
+    const int64_t all = rows.at ? up(p.m, 64) : p.m;
     if (p.m >= 4096)
-      k_join<32><<<(unsigned)div_up(p.m, 32), 256, 0, c.st>>>(part, pairs, p.m, hit, c.targets, loss, lse);
+      k_join<32><<<(unsigned)div_up(all, 32), 256, 0, c.st>>>(part, pairs, p.m, hit, c.targets, loss, lse, rows, extra_of(T));
     else
-      k_join<4><<<(unsigned)div_up(p.m, 4), 256, 0, c.st>>>(part, pairs, p.m, hit, c.targets, loss, lse);
+      k_join<4><<<(unsigned)div_up(all, 4), 256, 0, c.st>>>(part, pairs, p.m, hit, c.targets, loss, lse, rows, extra_of(T));
     BLP_HIP(hipGetLastError());
   }
   if (total) {
@@ -1106,7 +1173,7 @@ int forward(const Call& c, float* loss, float* lse, float* total, int mean) {
 }
 
 template <int T>
-int backward(const Call& c, const float* lse, RowGrad g, void* dx, int64_t lddx, void* dw, int64_t lddw) {
+int backward(const Call& c, bool fwd, const float* lse, RowGrad g, void* dx, int64_t lddx, void* dw, int64_t lddw) {
   const Plan& p = c.p;
   if (p.m == 0) {  // no rows: the catalogue's gradient is zero
     if (dw) {
@@ -1114,7 +1181,7 @@ int backward(const Call& c, const float* lse, RowGrad g, void* dx, int64_t lddx,
     }
     return 0;
   }
-  g.extra = T == F16 ? 16384.f : 1.f;  // halves: a probability below 2^-24 is not lost
+  g.extra = extra_of(T);
   if (g.g && g.stride) {
     float* top = (float*)(c.ws + p.o_top);
     k_top_grad<<<1, 1024, 0, c.st>>>(g.g, c.targets, p.m, top);
@@ -1122,15 +1189,11 @@ int backward(const Call& c, const float* lse, RowGrad g, void* dx, int64_t lddx,
     g.top = top;
   }
   if (p.narrow) {
-    NarrowArgs a = {c.x, c.w, p.x_plane(), p.w_plane(), p.kp, 0, 0, 0, c.scale, g.extra, c.targets, nullptr, nullptr,
-                    Rows{(float*)(c.ws + p.o_rows)}};
-    k_rows<<<(unsigned)div_up(p.m, 64), 64, 0, c.st>>>(lse, g, c.targets, p.m, a.rows);
-    BLP_HIP(hipGetLastError());
-    int rc = dx ? narrow_grad<T, DX>(c, a, p.nx, g, (float*)(c.ws + p.o_px), dx, lddx, p.m) : 0;
-    std::swap(a.own, a.stream);
-    std::swap(a.own_plane, a.stream_plane);
-    if (!rc && dw) rc = narrow_grad<T, DW>(c, a, p.nw, g, (float*)(c.ws + p.o_pw), dw, lddw, p.n);
-    return rc;
+    if (!fwd) {  // the forward pass's last step leaves them otherwise
+      k_rows<<<(unsigned)div_up(p.m, 64), 64, 0, c.st>>>(lse, g, c.targets, p.m, Rows{(float*)(c.ws + p.o_rows)});
+      BLP_HIP(hipGetLastError());
+    }
+    return narrow_grads<T>(c, g, dx, lddx, dw, lddw);
   }
   char* ds = c.ws + p.o_ds;
   float *px = (float*)(c.ws + p.o_px), *pw = (float*)(c.ws + p.o_pw);
@@ -1186,7 +1249,7 @@ int run(Call& c, const void* x, int64_t ldx, const void* w, int64_t ldw, float* 
         bool fwd, RowGrad g, void* dx, int64_t lddx, void* dw, int64_t lddw) {
   int rc = bind<T>(c, x, ldx, w, ldw);
   if (!rc && fwd) rc = forward<T>(c, loss, lse, total, mean);
-  if (!rc && c.p.grads) rc = backward<T>(c, lse, g, dx, lddx, dw, lddw);
+  if (!rc && c.p.grads) rc = backward<T>(c, fwd, lse, g, dx, lddx, dw, lddw);
   return rc;
 }
 
