@@ -56,10 +56,10 @@ __global__ __launch_bounds__(256) void k_lookup(const char* __restrict__ table, 
 
 // ---------------------------------------------------------------- sort
 // Stable radix sort of (id, position), least significant digit first, BITS (9 or 10) bits a pass. A block takes
-// 256 ROUNDS consecutive entries; wave w of it the w-th quarter, 64 at a time in order. The entries of one
+// 512 ROUNDS consecutive entries; wave w of it the w-th eighth, 64 at a time in order. The entries of one
 // digit are found with ballots (a lane's rank among them by counting the lanes below), so ranks follow
 // positions; ids outside the table get the largest key and end up last.
-constexpr int SORT_WAVES = 4, MOST_BITS = 10;
+constexpr int SORT_WAVES = 8, SORT_THREADS = 64 * SORT_WAVES, MOST_BITS = 10;
 
 __device__ inline uint32_t key_at(const Ids& ids, const uint32_t* keys, int64_t i) {
   if (keys) return keys[i];
@@ -69,47 +69,60 @@ __device__ inline uint32_t key_at(const Ids& ids, const uint32_t* keys, int64_t 
 
 // counts[block][digit]
 template <int ROUNDS, int BITS>
-__global__ __launch_bounds__(256) void k_digit_counts(Ids ids, const uint32_t* __restrict__ keys, int64_t n, int shift,
-                                                      uint32_t* __restrict__ counts) {
+__global__ __launch_bounds__(SORT_THREADS) void k_digit_counts(Ids ids, const uint32_t* __restrict__ keys, int64_t n, int shift,
+                                                               uint32_t* __restrict__ counts) {
   constexpr int BINS = 1 << BITS;
   __shared__ uint32_t s_count[BINS];
-  for (int i = threadIdx.x; i < BINS; i += 256) s_count[i] = 0;
+  for (int i = threadIdx.x; i < BINS; i += SORT_THREADS) s_count[i] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * (256 * ROUNDS);
+  const int64_t base = (int64_t)blockIdx.x * (SORT_THREADS * ROUNDS);
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
-    const int64_t i = base + r * 256 + threadIdx.x;
+    const int64_t i = base + r * SORT_THREADS + threadIdx.x;
     if (i < n) atomicAdd(&s_count[(key_at(ids, keys, i) >> shift) & (BINS - 1)], 1u);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < BINS; i += 256) counts[(int64_t)blockIdx.x * BINS + i] = s_count[i];
+  for (int i = threadIdx.x; i < BINS; i += SORT_THREADS) counts[(int64_t)blockIdx.x * BINS + i] = s_count[i];
 }
 
-// 64 digits a block, 16 waves over the blocks' rows: counts become exclusive sums over the blocks; total[digit].
+// 16 digits a block, 64 threads each over the blocks' rows: counts become exclusive sums over the blocks; total[digit].
 template <int BITS>
 __global__ __launch_bounds__(1024) void k_digit_sums(uint32_t* __restrict__ counts, int blocks, uint32_t* __restrict__ total) {
   constexpr int BINS = 1 << BITS;
-  __shared__ uint32_t s_sum[16][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, d = blockIdx.x * 64 + lane;
-  const int per = (blocks + 15) / 16, b0 = min(blocks, w * per), b1 = min(blocks, b0 + per);
+  __shared__ uint32_t s_sum[64][17];
+  const int c = threadIdx.x & 15, w = threadIdx.x >> 4, d = blockIdx.x * 16 + c;
+  const int per = (blocks + 63) / 64, b0 = min(blocks, w * per), b1 = min(blocks, b0 + per);
   uint32_t sum = 0;
 #pragma unroll 8
   for (int b = b0; b < b1; ++b) sum += counts[(int64_t)b * BINS + d];
-  s_sum[w][lane] = sum;
+  s_sum[w][c] = sum;
   __syncthreads();
-  uint32_t run = 0;
-  for (int i = 0; i < w; ++i) run += s_sum[i][lane];
-  if (w == 15) total[d] = run + sum;
+  if (threadIdx.x < 512) {  // a wave scans two digits' 64 sums, one after the other
+    const int lane = threadIdx.x & 63, v = threadIdx.x >> 6;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t x = s_sum[lane][v * 2 + k];
+      uint32_t s = x;
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t t = __shfl_up(s, o, 64);
+        if (lane >= o) s += t;
+      }
+      s_sum[lane][v * 2 + k] = s - x;
+      if (lane == 63) total[blockIdx.x * 16 + v * 2 + k] = s;
+    }
+  }
+  __syncthreads();
+  uint32_t run = s_sum[w][c];
 #pragma unroll 8
   for (int b = b0; b < b1; ++b) {
-    const uint32_t c = counts[(int64_t)b * BINS + d];
+    const uint32_t x = counts[(int64_t)b * BINS + d];
     counts[(int64_t)b * BINS + d] = run;
-    run += c;
+    run += x;
   }
 }
 
 template <int ROUNDS, int BITS>
-__global__ __launch_bounds__(256) void k_scatter(Ids ids, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
+__global__ __launch_bounds__(SORT_THREADS) void k_scatter(Ids ids, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
                                                  int64_t n, int shift, const uint32_t* __restrict__ counts,
                                                  const uint32_t* __restrict__ total, uint32_t* __restrict__ keys_out,
                                                  uint32_t* __restrict__ pos_out) {
@@ -118,7 +131,7 @@ __global__ __launch_bounds__(256) void k_scatter(Ids ids, const uint32_t* __rest
   __shared__ uint16_t s_wave[SORT_WAVES][BINS];
   __shared__ uint32_t s_sum[SORT_WAVES];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t base = (int64_t)blockIdx.x * (256 * ROUNDS) + w * (64 * ROUNDS);
+  const int64_t base = (int64_t)blockIdx.x * (SORT_THREADS * ROUNDS) + w * (64 * ROUNDS);
   uint32_t key[ROUNDS], at[ROUNDS];
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
@@ -126,13 +139,13 @@ __global__ __launch_bounds__(256) void k_scatter(Ids ids, const uint32_t* __rest
     key[r] = key_at(ids, keys, i);
     at[r] = pos ? pos[i] : (uint32_t)i;
   }
-  for (int i = threadIdx.x; i < SORT_WAVES * BINS / 2; i += 256) reinterpret_cast<uint32_t*>(&s_wave[0][0])[i] = 0;
-  // where each digit starts: exclusive sums of the totals, four digits a thread
-  uint32_t c[BINS / 256], sum = 0;
+  for (int i = threadIdx.x; i < SORT_WAVES * BINS / 2; i += SORT_THREADS) reinterpret_cast<uint32_t*>(&s_wave[0][0])[i] = 0;
+  // where each digit starts: exclusive sums of the totals, BINS / 512 digits a thread
+  uint32_t c[BINS / SORT_THREADS], sum = 0;
 #pragma unroll
-  for (int j = 0; j < BINS / 256; ++j) {
+  for (int j = 0; j < BINS / SORT_THREADS; ++j) {
     c[j] = sum;
-    sum += total[threadIdx.x * (BINS / 256) + j];
+    sum += total[threadIdx.x * (BINS / SORT_THREADS) + j];
   }
   uint32_t s = sum;
   for (int o = 1; o < 64; o <<= 1) {
@@ -144,8 +157,8 @@ __global__ __launch_bounds__(256) void k_scatter(Ids ids, const uint32_t* __rest
   uint32_t before = s - sum;
   for (int i = 0; i < w; ++i) before += s_sum[i];
 #pragma unroll
-  for (int j = 0; j < BINS / 256; ++j) {
-    const int d = threadIdx.x * (BINS / 256) + j;
+  for (int j = 0; j < BINS / SORT_THREADS; ++j) {
+    const int d = threadIdx.x * (BINS / SORT_THREADS) + j;
     s_base[d] = before + c[j] + counts[(int64_t)blockIdx.x * BINS + d];
   }
   // ranks within the wave
@@ -170,8 +183,8 @@ __global__ __launch_bounds__(256) void k_scatter(Ids ids, const uint32_t* __rest
   }
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < BINS / 256; ++j) {  // the waves' counts become exclusive sums over the waves
-    const int d = threadIdx.x * (BINS / 256) + j;
+  for (int j = 0; j < BINS / SORT_THREADS; ++j) {  // the waves' counts become exclusive sums over the waves
+    const int d = threadIdx.x * (BINS / SORT_THREADS) + j;
     uint32_t run = 0;
     for (int i = 0; i < SORT_WAVES; ++i) {
       const uint32_t t = s_wave[i][d];
@@ -361,11 +374,11 @@ __device__ inline bool heavy(const Sums& a, int64_t chunk, uint32_t key) {
   return far < a.n && a.keys[far] == key;
 }
 
-// The rows that cross chunks. The first blocks: a group of lanes a chunk, the partial sums of the row that
-// begins there in the chunks' order. The others: HEAVY chunks each, in which one heavy row can begin; its
-// partial sums go to the groups in turn, then the groups' sums are added in order. In 64 bits.
+// The rows that cross chunks, in 64 bits. The first blocks, which last longest: HEAVY chunks each, in which one heavy row
+// can begin; its partial sums go to the groups of lanes in turn, then the groups' sums are added in order. The
+// others: a group of lanes a chunk, the partial sums of the row that begins there in the chunks' order.
 template <int T>
-__global__ __launch_bounds__(256) void k_join_chunks(Sums a, unsigned light_blocks) {
+__global__ __launch_bounds__(256) void k_join_chunks(Sums a, unsigned heavy_blocks) {
   constexpr int NE = Vec<T>::NE;
   __shared__ double s_sum[256 * NE];
   __shared__ int s_at;
@@ -375,8 +388,8 @@ __global__ __launch_bounds__(256) void k_join_chunks(Sums a, unsigned light_bloc
 #pragma unroll
   for (int j = 0; j < NE; ++j) sum[j] = 0.0;
   uint32_t key;
-  if (blockIdx.x < light_blocks) {
-    const int64_t chunk = (int64_t)blockIdx.x * groups + g;
+  if (blockIdx.x >= heavy_blocks) {
+    const int64_t chunk = (int64_t)(blockIdx.x - heavy_blocks) * groups + g;
     if (chunk >= a.chunks || e0 >= a.k || !crosses(a, chunk, &key) || heavy(a, chunk, key)) return;
     int64_t c = chunk;
     do {
@@ -393,7 +406,7 @@ __global__ __launch_bounds__(256) void k_join_chunks(Sums a, unsigned light_bloc
   }
   if (threadIdx.x == 0) s_at = -1;
   __syncthreads();
-  const int64_t first = (blockIdx.x - light_blocks) * (int64_t)HEAVY;
+  const int64_t first = blockIdx.x * (int64_t)HEAVY;
   if (threadIdx.x < HEAVY && first + threadIdx.x < a.chunks && crosses(a, first + threadIdx.x, &key) &&
       heavy(a, first + threadIdx.x, key))
     s_at = threadIdx.x;
@@ -453,8 +466,8 @@ Plan plan_of(int type, int64_t n, int64_t rows, int k) {
   while (bits < 32 && (rows >> bits)) ++bits;
   p.passes = n <= SMALL ? 0 : (int)div_up(bits, MOST_BITS);
   p.bits = p.passes * 9 >= bits ? 9 : 10;
-  p.rounds = n <= 128 * 1024 ? 2 : 8;  // short lists: more blocks, each done sooner
-  p.blocks = div_up(n, 256 * p.rounds);
+  p.rounds = n <= 128 * 1024 ? 1 : 4;  // short lists: more blocks, each done sooner
+  p.blocks = div_up(n, SORT_THREADS * p.rounds);
   const int64_t vecs = div_up(k, 16 / size_of(type));
   p.lanes = 1;
   while (p.lanes < 64 && p.lanes < vecs) p.lanes <<= 1;
@@ -496,11 +509,11 @@ int sort(hipStream_t st, const Plan& p, Ids ids, int64_t n, uint32_t* const* key
   for (int s = 0; s < p.passes; ++s) {
     const uint32_t* kin = s ? keys[cur] : nullptr;
     const int to = s ? cur ^ 1 : 0;
-    k_digit_counts<ROUNDS, BITS><<<(unsigned)p.blocks, 256, 0, st>>>(ids, kin, n, s * BITS, counts);
+    k_digit_counts<ROUNDS, BITS><<<(unsigned)p.blocks, SORT_THREADS, 0, st>>>(ids, kin, n, s * BITS, counts);
     BLP_HIP(hipGetLastError());
-    k_digit_sums<BITS><<<(1 << BITS) / 64, 1024, 0, st>>>(counts, (int)p.blocks, total);
+    k_digit_sums<BITS><<<(1 << BITS) / 16, 1024, 0, st>>>(counts, (int)p.blocks, total);
     BLP_HIP(hipGetLastError());
-    k_scatter<ROUNDS, BITS><<<(unsigned)p.blocks, 256, 0, st>>>(ids, kin, s ? pos[cur] : nullptr, n, s * BITS, counts, total, keys[to],
+    k_scatter<ROUNDS, BITS><<<(unsigned)p.blocks, SORT_THREADS, 0, st>>>(ids, kin, s ? pos[cur] : nullptr, n, s * BITS, counts, total, keys[to],
                                                           pos[to]);
     BLP_HIP(hipGetLastError());
     cur = to;
@@ -525,10 +538,10 @@ int lookup_grad(hipStream_t st, const Plan& p, const void* dy, int64_t ld, Ids i
       return sort<decltype(rounds)::value, decltype(bits)::value>(st, p, ids, n, keys, pos, counts, total, &cur);
     };
     using std::integral_constant;
-    if (p.rounds == 2)
-      rc = p.bits == 9 ? run(integral_constant<int, 2>{}, integral_constant<int, 9>{}) : run(integral_constant<int, 2>{}, integral_constant<int, 10>{});
+    if (p.rounds == 1)
+      rc = p.bits == 9 ? run(integral_constant<int, 1>{}, integral_constant<int, 9>{}) : run(integral_constant<int, 1>{}, integral_constant<int, 10>{});
     else
-      rc = p.bits == 9 ? run(integral_constant<int, 8>{}, integral_constant<int, 9>{}) : run(integral_constant<int, 8>{}, integral_constant<int, 10>{});
+      rc = p.bits == 9 ? run(integral_constant<int, 4>{}, integral_constant<int, 9>{}) : run(integral_constant<int, 4>{}, integral_constant<int, 10>{});
     if (rc) return rc;
   }
   const Sums a = {keys[cur], pos[cur], n, p.chunk, p.chunks, (uint32_t)ids.rows, k, p.lanes, scale, (char*)out, ldo * ES, add,
@@ -538,8 +551,8 @@ int lookup_grad(hipStream_t st, const Plan& p, const void* dy, int64_t ld, Ids i
   k_chunk_sums<T><<<dim3(sum_blocks + clear_blocks, p.tiles), 256, 0, st>>>(a, (const char*)dy, ld * ES, sum_blocks);
   BLP_HIP(hipGetLastError());
   if (p.chunks > 1) {
-    const unsigned light = (unsigned)div_up(p.chunks, 256 / p.lanes), rest = (unsigned)div_up(p.chunks, HEAVY);
-    k_join_chunks<T><<<dim3(light + rest, p.tiles), 256, 0, st>>>(a, light);
+    const unsigned light = (unsigned)div_up(p.chunks, 256 / p.lanes), heavies = (unsigned)div_up(p.chunks, HEAVY);
+    k_join_chunks<T><<<dim3(light + heavies, p.tiles), 256, 0, st>>>(a, heavies);
     BLP_HIP(hipGetLastError());
   }
   return 0;
