@@ -606,7 +606,7 @@ __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowAr
       }
     }
   }
-  // LSE: the running maximum of the products (not yet times c), its -top c (0 while it is infinite), the sum
+  // LSE: the reference of the sum, a score or a maximum (not yet times c), its -top c (0 while it is infinite), the sum
   float top[FO], shift[FO], sum[FO];
   f32x4 out[2 * KS][FO];            // DX, DW
 #pragma unroll
@@ -655,11 +655,12 @@ __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowAr
         }
     };
     if constexpr (MODE == LSE) {
-      bool slow = t == 0 || s1 - r0 < 64;
+      bool here = false, slow = s1 - r0 < 64;
 #pragma unroll
-      for (int j = 0; j < FO; ++j) slow |= (unsigned)(target[j] - r0) < 64u;
+      for (int j = 0; j < FO; ++j) here |= (unsigned)(target[j] - r0) < 64u;
+      const bool any = __any(here);
       if (!__any(slow)) {
-        // The stale maximum does as long as no sum grows past 2^60 (or is NaN): no maximum to take.
+        // Each lane's first score is its reference, and does as long as no sum grows past 2^60 (or is NaN): no maximum to take.
         float add[FO];
 #pragma unroll
         for (int j = 0; j < FO; ++j) add[j] = 0.f;
@@ -667,6 +668,26 @@ __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowAr
         for (int half = 0; half < 2; ++half) {
           f32x4 acc[2][FO];
           products(half, acc);
+          if (half == 0 && t == 0) {
+#pragma unroll
+            for (int j = 0; j < FO; ++j) {
+              top[j] = acc[0][j][0];
+              shift[j] = -top[j] * c;
+            }
+          }
+          if (any) {  // the targets' scores: rare
+            const int first = r0 + half * 32 + h * 4;
+#pragma unroll
+            for (int j = 0; j < FO; ++j) {
+              const int at = target[j] - first;
+              float z = 0.f;
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z = at == i * 16 + e ? acc[i][j][e] : z;
+              if ((unsigned)at < 32u && (at & 12) == 0) a.hit[own0 + j * 16 + l] = z * fabsf(a.scale);
+            }
+          }
 #pragma unroll
           for (int j = 0; j < FO; ++j)
 #pragma unroll
@@ -681,8 +702,15 @@ __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowAr
           for (int j = 0; j < FO; ++j) sum[j] += add[j];
           return;
         }
+        if (t == 0) {  // no reference yet that holds
+#pragma unroll
+          for (int j = 0; j < FO; ++j) {
+            top[j] = -INFINITY;
+            shift[j] = 0.f;
+          }
+        }
       }
-      // The first and the last stage, targets' scores, and rows that rise far: rare.
+      // The range's last stage, and rows that rise far: rare.
 #pragma unroll 1
       for (int half = 0; half < 2; ++half) {
         f32x4 acc[2][FO];
