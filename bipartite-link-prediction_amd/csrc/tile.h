@@ -6,9 +6,9 @@
 // in between). A fragment is 16 bytes of a row: 8 halves or 16 8-bit integers, one 16-row matrix instruction.
 // The next stage is in flight while this one is multiplied, in the other of two buffers, so a stage costs one
 // barrier. A workgroup takes tile after tile, and the next one's first stage is on its way while this one's
-// outputs leave. Bound by the copies from the second-level cache and the matrix unit alike (256 x 256 x 64 halves
-// a stage: 64 KiB and 2,048 cycles of it); 2 M N k of 8,192 x 32,768 x 4,096 run at 1,319 TFLOP/s without the
-// reading of LDS or the copies being the slower by more than a quarter.
+// outputs leave. A stage of 256 x 256 x 64 halves is 64 KiB of copies and 2,048 cycles of the matrix unit; 8,192 x
+// 32,768 x 4,096 random halves run at 1,061 TFLOP/s, at 1,346 without the copies, and the copies alone take as long as
+// 1,717 would (constant halves, which draw less power: 1,319): bound by power and the second-level cache together.
 //
 // Layouts of an operand: ROW -- k contiguous, element (p, k) at base + p ld + k size; COL -- p contiguous,
 // element (p, k) at base + k ld + p size, whose halves are transposed on their way out of LDS
@@ -59,21 +59,16 @@ struct Acc<I8> {
 
 template <int T>
 __device__ inline typename Acc<T>::type mma(frag_t p, frag_t q, typename Acc<T>::type c) {
-  if constexpr (T == BF16) {
+  static_assert(T == BF16 || T == F16 || T == I8, "floats are multiplied as halves (latent.hip)");
+  if constexpr (T == BF16)
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
-  } else if constexpr (T == F16) {
+  else if constexpr (T == F16)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, p), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
-  } else if constexpr (T == I8) {
+  else
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(p, q, c, 0, 0, 0);
-  } else {
-    const f32x4 a = __builtin_bit_cast(f32x4, p), b = __builtin_bit_cast(f32x4, q);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
-    return c;
-  }
 }
 
-// One operand of a product, in bytes (`rows`: valid p; `k`: valid k, both in elements).
+// One operand of a product: `ld` in bytes, `rows` the valid p in elements.
 struct Operand {
   const char* base;
   int64_t ld;
@@ -97,19 +92,15 @@ __device__ inline __amdgpu_buffer_rsrc_t rsrc_at(const char* p) {
 }
 constexpr uint32_t OUT_OF_RANGE = 0x80000000u;
 
-// COL tiles: which granules of a row trade places, by k. Halves: the 16 lanes of a transposing read take
-// 4 rows (k & 3) of 32 bytes, the next 16 the rows 8 further; floats: 16 lanes take 64 bytes of one row,
-// the next 16 the row 4 further.
-template <int T>
-__device__ inline int col_swz(int k) {
-  return T == F32 ? ((k >> 2) & 3) << 2 : ((k & 3) | ((k >> 3) & 1) << 2) << 1;
-}
+// COL tiles (halves): which granules of a row trade places, by k: the 16 lanes of a transposing read take 4 rows (k & 3)
+// of 32 bytes, the next 16 the rows 8 further.
+__device__ inline int col_swz(int k) { return ((k & 3) | ((k >> 3) & 1) << 2) << 1; }
 
 // Copy stage [k0, k0 + STAGE/size) of a tile of R rows starting at row r0 into LDS (asynchronous: counted
 // by vmcnt). Every wave copies R / WAVES rows' worth of granules.
 template <int T, int LAYOUT, int R, int WAVES>
 __device__ inline void load_stage(lds_char* lds, const Operand& o, int64_t r0, int64_t k0, int64_t kend) {
-  constexpr int ES = size_of(T), KE = STAGE / ES, GE = 16 / ES;
+  constexpr int ES = size_of(T), GE = 16 / ES;
   constexpr int PASS = WAVES * 64;                    // granules a pass of the workgroup copies
   constexpr int GRANULES = R * STAGE / 16;
   static_assert(GRANULES % PASS == 0, "tile too small for the workgroup");
@@ -138,13 +129,12 @@ __device__ inline void load_stage(lds_char* lds, const Operand& o, int64_t r0, i
 #pragma unroll
     for (int i = 0; i < GRANULES / PASS; ++i) {
       const int g = (i * WAVES + wave) * 64 + lane;
-      const int k = g / GR, c = (g % GR) ^ (col_swz<T>(k) & (GR - 1));
+      const int k = g / GR, c = (g % GR) ^ (col_swz(k) & (GR - 1));
       const bool ok = k0 + k < kend && c * GE < left;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           rs, (__attribute__((address_space(3))) void*)(lds + (i * PASS + wave * 64) * 16), 16,
           ok ? (uint32_t)k * ld + c * 16 : OUT_OF_RANGE, 0, 0, 0);
     }
-    (void)KE;
   }
 }
 
@@ -155,12 +145,9 @@ __device__ inline uint32_t lane_base() {
   const int lane = threadIdx.x & 63, i = lane & 15, h = lane >> 4;
   if constexpr (LAYOUT == ROW) {
     return i * STAGE + (h ^ (i & 7)) * 16;
-  } else if constexpr (T == F32) {
-    const int k = h * 4;
-    return k * R * 4 + ((i >> 2) ^ (col_swz<T>(k) & (R / 4 - 1))) * 16 + (i & 3) * 4;
   } else {
     const int k = h * 8 + (i >> 2);
-    return k * R * 2 + (((i & 3) >> 1) ^ (col_swz<T>(k) & (R / 8 - 1))) * 16 + (i & 1) * 8;
+    return k * R * 2 + (((i & 3) >> 1) ^ (col_swz(k) & (R / 8 - 1))) * 16 + (i & 1) * 8;
   }
 }
 
@@ -169,14 +156,8 @@ template <int T, int LAYOUT, int R>
 __device__ inline frag_t read_frag(const lds_char* lds, uint32_t base, int f, int kk) {
   if constexpr (LAYOUT == ROW) {
     return *(const __attribute__((address_space(3))) frag_t*)(lds + (base ^ (kk * 64)) + f * 16 * STAGE);
-  } else if constexpr (T == F32) {
-    const lds_char* at = lds + (base ^ (f << 6)) + kk * 16 * R * 4;
-    f32x4 v;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = *(const __attribute__((address_space(3))) float*)(at + j * R * 4);
-    return __builtin_bit_cast(frag_t, v);
   } else {
-    static_assert(T == BF16 || T == F16, "column layout: halves and floats");
+    static_assert(T == BF16 || T == F16, "column layout: halves");
     const lds_char* at = lds + (base ^ (f << 5)) + kk * 32 * R * 2;
     i32x4 v;
 #pragma unroll
