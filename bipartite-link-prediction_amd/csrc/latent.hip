@@ -17,6 +17,7 @@
 // A row whose target lies outside [0, n_cols) is ignored: loss 0, gradient 0, and its x is never multiplied
 // (it may hold anything, NaN too).
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "blp_internal.h"
@@ -305,8 +306,9 @@ struct RowGrad {
   float extra;         // the halves' factor
   __device__ float row(int64_t i) const {  // in [-1, 1] times extra
     if (!g || !stride) return extra;
-    const float t = *top;
-    return t > 0.f ? g[i] / t * extra : t != t ? t : 0.f;
+    const float t = *top, v = g[i];
+    if (!(fabsf(v) <= FLT_MAX)) return v;  // an infinite or NaN gradient: its row's, and the catalogue's
+    return t > 0.f ? v / t * extra : 0.f;
   }
   __device__ float all() const {
     const float f = (g ? (stride ? *top : *g) : 1.f) / extra;
@@ -314,24 +316,22 @@ struct RowGrad {
   }
 };
 
+// top = max |g| of the finite row gradients (1 if there is none).
 __global__ __launch_bounds__(1024) void k_top_grad(const float* __restrict__ g, Targets targets, int64_t m,
                                                    float* __restrict__ top) {
   __shared__ float s_top[16];
-  float t = 0.f;
-  bool nan = false;
+  float t = -1.f;
   for (int64_t i = threadIdx.x; i < m; i += 1024)
     if (targets(i) >= 0) {
       const float v = fabsf(g[i]);
-      nan |= !(v <= 3.0e38f);
-      t = fmaxf(t, v);
+      if (v <= FLT_MAX) t = fmaxf(t, v);
     }
-  if (nan) t = INFINITY;
   for (int o = 32; o; o >>= 1) t = fmaxf(t, __shfl_xor(t, o, 64));
   if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = t;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 16; ++i) t = fmaxf(t, s_top[i]);
-    *top = t <= 3.0e38f ? t : NAN;  // an infinite or NaN gradient: everything it reaches is NaN
+    *top = t < 0.f ? 1.f : t;
   }
 }
 

@@ -311,6 +311,32 @@ def test_infinite_and_nan_scores_stay_in_their_rows(gpu):
     np.testing.assert_allclose(loss.cpu().numpy(), np.log(1000.0), rtol=0, atol=20000 * 4 * U)
 
 
+@pytest.mark.parametrize("k", [40, 200])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_infinite_and_nan_row_gradients_stay_in_their_rows(gpu, dtype, k):
+    """Row gradients that are infinite or NaN: their rows of dx and all of dtable; the other rows of dx are those of
+    row gradients of 0 in these places. Finite ones next to the largest float are taken as they are."""
+    torch = _torch()
+    from blp import latent
+
+    x, w, t = make(150, 700, k, getattr(torch, dtype), seed=8)
+    t[9] = -1
+    g = torch.randn(150, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    lse = torch.logsumexp(x.float() @ w.float().t().contiguous(), 1)
+    bad = {3: float("inf"), 9: float("nan"), 77: float("nan"), 149: float("-inf")}
+    zeroed = g.clone()
+    for i, v in bad.items():
+        g[i], zeroed[i] = v, 0.0
+    want, _ = latent.softmax_loss_backward(zeroed, lse, None, x, w, t)
+    dx, dw = latent.softmax_loss_backward(g, lse, None, x, w, t)
+    keep = [i for i in range(150) if i not in (3, 77, 149)]  # row 9 is ignored
+    assert torch.equal(dx[keep], want[keep]) and want[keep].isfinite().all()
+    assert not dx[[3, 77, 149]].isfinite().any() and not dw.isfinite().any()
+    if dtype != "float16":  # whose gradients end at 65,504
+        dw = latent.softmax_loss_backward(torch.full_like(g, 3.2e38), lse, None, x * 2.0 ** -20, w, t)[1]
+        assert dw.isfinite().all() and dw.any()
+
+
 def test_strided_and_unaligned_rows(gpu):
     """Slices of wider tensors: row strides, and starts that no 16-byte load can take."""
     torch = _torch()
