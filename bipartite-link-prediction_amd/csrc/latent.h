@@ -27,6 +27,7 @@ struct Ids {
   const void* at;
   int wide;
   int64_t rows;
+  const void* from(int64_t i) const { return (const char*)at + i * (wide ? 8 : 4); }
   __device__ int64_t operator()(int64_t i) const {
     const int64_t t = wide ? reinterpret_cast<const int64_t*>(at)[i] : reinterpret_cast<const int32_t*>(at)[i];
     return t >= 0 && t < rows ? t : -1;

@@ -931,6 +931,7 @@ __global__ __launch_bounds__(256, KS > 3 ? 2 : KS > 2 || T == F32 ? 3 : 4) void 
 
 // ---------------------------------------------------------------- host side
 constexpr int64_t PIECE_BYTES = 512ll << 20;  // dS of one piece of the catalogue
+constexpr int64_t PAIR_BYTES = 256ll << 20;   // the forward pass's pairs of the rows taken at a time
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int64_t div_up(int64_t v, int64_t by) { return (v + by - 1) / by; }
@@ -1021,7 +1022,7 @@ struct Plan {
   int ks;
   Splits nl, nx, nw;
   int fwd;              // else k_product
-  int64_t fwd_tiles;
+  int64_t fwd_tiles, fwd_rows;
   int64_t piece, pieces;
   Slices sx, sw;
   int64_t o_x, o_w, o_part, o_hit, o_top, o_rows, o_ds, o_px, o_pw, bytes;
@@ -1061,6 +1062,7 @@ Plan plan_of(int type, int64_t m, int64_t n, int k, bool forward, bool grads, bo
     p.nx = splits_of(m, n, trip, grad_us, 4.0 * m * up(k, 4));
     p.nw = splits_of(n, m, trip, grad_us, 4.0 * n * up(k, 4));
     p.o_part = l.take(forward ? p.nl.n * m * 8 : 0);
+    p.fwd_rows = m;
     p.o_hit = l.take(forward ? m * 4 : 0);
     p.o_top = l.take(16);
     p.o_rows = l.take(grads ? div_up(m, 64) * 1024 : 0);
@@ -1071,8 +1073,10 @@ Plan plan_of(int type, int64_t m, int64_t n, int k, bool forward, bool grads, bo
   }
   p.fwd = shape_of(n, m);
   p.fwd_tiles = div_up(n, BP_OF[p.fwd]) * WP_OF[p.fwd];
-  p.o_part = l.take(forward ? p.fwd_tiles * m * 8 : 0);
-  p.o_hit = l.take(forward ? m * 4 : 0);
+  // whole tiles of rows; at least 512, so that short lists are joined, and their total taken, in one launch
+  p.fwd_rows = std::min(m, std::max<int64_t>(PAIR_BYTES / (p.fwd_tiles * 8) / 256 * 256, 512));
+  p.o_part = l.take(forward ? p.fwd_tiles * p.fwd_rows * 8 : 0);
+  p.o_hit = l.take(forward ? p.fwd_rows * 4 : 0);
   p.o_top = l.take(16);
   if (grads) {
     // whole tiles of columns within the budget, the pieces as equal as that allows
@@ -1226,22 +1230,27 @@ int forward(const Call& c, float* loss, float* lse, Total total, uint32_t* done)
   if (p.m > 0) {
     float2* part = (float2*)(c.ws + p.o_part);
     float* hit = (float*)(c.ws + p.o_hit);
-    int rc;
-    if (p.narrow) {
-      rc = narrow_lse<T>(c, part, hit);
-    } else {
-      const Problem a = {c.w, c.x, p.kp, 0, 0, 0, p.w_plane(), p.x_plane()};
-      rc = product<T, ROW, ROW>(p.fwd, a, 1, 0, EpiLse<T>{part, hit, c.targets, p.n, p.m, c.scale}, c.st);
+    // as many rows at a time as the pairs have room for (narrow factors: all)
+    for (int64_t r0 = 0; r0 < p.m; r0 += p.fwd_rows) {
+      const int64_t m = std::min(p.fwd_rows, p.m - r0);
+      const Targets targets = {c.targets.from(r0), c.targets.wide, c.targets.rows};
+      int rc;
+      if (p.narrow) {
+        rc = narrow_lse<T>(c, part, hit);
+      } else {
+        const Problem a = {c.w, {c.x.base + r0 * c.x.ld, c.x.ld, m}, p.kp, 0, 0, 0, p.w_plane(), p.x_plane()};
+        rc = product<T, ROW, ROW>(p.fwd, a, 1, 0, EpiLse<T>{part, hit, targets, p.n, m, c.scale}, c.st);
+      }
+      if (rc) return rc;
+      const int64_t pairs = p.narrow ? p.nl.n : p.fwd_tiles;
+      const Rows rows = {p.narrow && p.grads ? (float*)(c.ws + p.o_rows) : nullptr};
+      const int64_t all = rows.at ? up(m, 64) : m;
+      if (m >= 4096)
+        k_join<32><<<(unsigned)div_up(all, 32), 256, 0, c.st>>>(part, pairs, m, hit, targets, loss + r0, lse + r0, rows, extra_of(T), total, done);
+      else
+        k_join<4><<<(unsigned)div_up(all, 4), 256, 0, c.st>>>(part, pairs, m, hit, targets, loss + r0, lse + r0, rows, extra_of(T), total, done);
+      BLP_HIP(hipGetLastError());
     }
-    if (rc) return rc;
-    const int64_t pairs = p.narrow ? p.nl.n : p.fwd_tiles;
-    const Rows rows = {p.narrow && p.grads ? (float*)(c.ws + p.o_rows) : nullptr};
-    const int64_t all = rows.at ? up(p.m, 64) : p.m;
-    if (p.m >= 4096)
-      k_join<32><<<(unsigned)div_up(all, 32), 256, 0, c.st>>>(part, pairs, p.m, hit, c.targets, loss, lse, rows, extra_of(T), total, done);
-    else
-      k_join<4><<<(unsigned)div_up(all, 4), 256, 0, c.st>>>(part, pairs, p.m, hit, c.targets, loss, lse, rows, extra_of(T), total, done);
-    BLP_HIP(hipGetLastError());
   }
   if (total.at && !(done && p.m > 0)) {
     k_total<<<1, 1024, 0, c.st>>>(loss, c.targets, p.m, total);

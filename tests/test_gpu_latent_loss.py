@@ -261,6 +261,23 @@ def test_against_differences(gpu):
             assert abs((hi - lo) / (2 * step) - float(got[i, j])) < 10 * step ** 2 + 1e-10 + 1e-5 * float(got.abs().max())
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_more_rows_than_the_pairs_have_room_for(gpu, dtype):
+    """391 tiles of the catalogue leave 782 pairs a row, of which 256 MiB hold 42,752 rows."""
+    torch = _torch()
+    from blp import latent
+
+    m, n, k = 43100, 100000, 136
+    x, w, t = make(m, n, k, getattr(torch, dtype), seed=11, ignored=0.1)
+    at = torch.cat([torch.arange(0, 43), torch.arange(42700, 42800), torch.arange(m - 20, m), torch.arange(0, m, 997)]).cuda()
+    ref = reference(x[at], w, t[at], 1.0)
+    for tt in (t, t.to(torch.int32)):
+        loss = latent.softmax_loss(x, w, tt, reduction="none")
+        near(loss[at], ref["loss"], ref["b_loss"])
+        total = latent.softmax_loss(x, w, tt, reduction="sum")
+        assert abs(float(total) - float(loss.double().sum())) <= U * float(total)
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
 def test_ignored_rows_hold_anything(gpu, dtype):
     torch = _torch()

@@ -48,6 +48,15 @@ def workspace(type, rows, cols, k, forward=1, grads=1, x=ONE, ldx=None, w=ONE, l
     return n.value
 
 
+def test_softmax_loss_forward_workspace_is_bounded():
+    """The forward pass alone: its pairs of as many rows as 256 MiB hold, a float a row, and the factors where packed."""
+    for type, planes in ((0, 3), (1, 1), (2, 1)):
+        for rows, cols, k in ((1 << 20, 1 << 20, 256), (1 << 24, 100000, 136), (300, 1 << 30, 136), (1 << 20, 40, 1000)):
+            factors = 2 * planes * (rows + cols) * k if type == 0 else 0
+            pairs = max(256 << 20, 8 * 512 * (cols // 32 + 4))
+            assert workspace(type, rows, cols, k, grads=0, x=1 << 20, w=1 << 20) <= factors + pairs + 4 * rows + 4096
+
+
 def test_softmax_loss_workspace_is_bounded():
     """The workspace never grows with rows x columns past one piece of the catalogue and the partial sums."""
     for type, es in ((0, 4), (1, 2), (2, 2)):
