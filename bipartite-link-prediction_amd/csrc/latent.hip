@@ -640,6 +640,7 @@ __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowAr
   auto compute = [&](const char* buf, const char* rbuf, int t) {
     const lds_char* lds = (const lds_char*)buf;
     const int r0 = (int)(s0 + (int64_t)t * 64);  // stream rows fit 31 bits
+    if (r0 >= (int)s1) return;
     // 32 stream rows' products with the own rows
     auto products = [&](int half, f32x4(&acc)[2][FO]) {
 #pragma unroll
@@ -754,7 +755,7 @@ __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowAr
         const int t64 = ((const __attribute__((address_space(3))) int*)rp)[128 + lane];
         mine = (unsigned)(t64 - (int)own0) < 16u * FO;
       }
-      const bool any = __any(mine);
+      const bool any = __any(mine), cut = (int)s1 - r0 < 64;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         f32x4 acc[2][FO];
@@ -775,6 +776,13 @@ __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowAr
               else
                 acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, -l2[e]));
             }
+          if (MODE == DX && cut) {  // past the range's end: exp2(-lse) of any size, times rows of zeros
+#pragma unroll
+            for (int j = 0; j < FO; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (r0 + half * 32 + i * 16 + h * 4 + e >= (int)s1) acc[i][j][e] = 0.f;
+          }
           if (any) {  // rare
             if constexpr (MODE == DX) {
 #pragma unroll
@@ -833,8 +841,7 @@ __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowAr
     }
   };
 
-  // Three buffers, two stages ahead (floats: two, one ahead). Stages past the range copy nothing and count for nothing: their rows are zeros
-  // (LSE masks them), so every trip takes all buffers and the counts of outstanding copies stay the same.
+  // Three buffers, two stages ahead (floats: two, one ahead). Stages past the range copy zeros and are not computed, so every trip takes all buffers and the counts of outstanding copies stay the same.
   load(s_a, s_ra, 0);
   if constexpr (THREE) {
     load(s_b, s_rb, 1);

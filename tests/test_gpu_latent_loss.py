@@ -199,6 +199,28 @@ def test_confident_rows(gpu, dtype):
         near(dw, ref["dw"], ref["b_dw"])
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("m,n,k", [(70, 77, 40), (150, 700, 64), (1537, 3001, 33), (150, 700, 200), (70, 3001, 128)])
+def test_catalogues_of_low_scores(gpu, m, n, k, dtype):
+    """Every score far below zero, so exp(0 - lse) of the rows past the catalogue's end (zeros) is infinite in the type."""
+    torch = _torch()
+    from blp import latent
+
+    dtype = getattr(torch, dtype)
+    g = torch.Generator().manual_seed(k)
+    x = (0.5 + torch.rand(m, k, generator=g)).to(dtype).cuda()
+    w = (-(0.5 + torch.rand(n, k, generator=g)) * (200 / k)).to(dtype).cuda()
+    t = torch.randint(0, n, (m,), generator=g).cuda()
+    ref = reference(x, w, t, 1.0)
+    total, dx, dw = latent.softmax_loss_grad(x, w, t)
+    near(total, ref["loss"].sum() / ref["count"], ref["b_loss"].mean() * m / ref["count"] + U * abs(float(total)))
+    near(dx, ref["dx"], ref["b_dx"])
+    near(dw, ref["dw"], ref["b_dw"])
+    lse = torch.logsumexp(x.double() @ w.double().t().contiguous(), 1).float()
+    dx, dw = latent.softmax_loss_backward(torch.full((m,), 1 / m, device="cuda"), lse, None, x, w, t)
+    assert dx.isfinite().all() and dw.isfinite().all()
+
+
 def test_scores_that_rise_along_the_catalogue(gpu):
     """Sorted scores, over 300 in all: the running reference is overtaken again and again, by more than 2^60 at a time."""
     torch = _torch()
