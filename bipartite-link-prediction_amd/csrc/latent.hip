@@ -1331,10 +1331,12 @@ int backward(const Call& c, bool fwd, const float* lse, RowGrad g, void* dx, int
   return 0;
 }
 
+constexpr int64_t MOST_ROWS = (1ll << 31) - (1 << 16);  // the row numbers of stages past the end fit 31 bits
+
 int check_args(int type, int64_t rows, int64_t cols, int k) {
   BLP_CHECK(type >= 0 && type <= 2, BLP_E_ARG, "softmax loss: type must be BLP_F32, BLP_BF16 or BLP_F16");
-  BLP_CHECK(rows >= 0 && rows < (1ll << 31), BLP_E_ARG, "softmax loss: rows must be in [0, 2^31)");
-  BLP_CHECK(cols >= 1 && cols < (1ll << 31), BLP_E_ARG, "softmax loss: the catalogue must have 1 to 2^31 - 1 rows");
+  BLP_CHECK(rows >= 0 && rows <= MOST_ROWS, BLP_E_ARG, "softmax loss: rows must be in [0, 2^31 - 2^16]");
+  BLP_CHECK(cols >= 1 && cols <= MOST_ROWS, BLP_E_ARG, "softmax loss: the catalogue must have 1 to 2^31 - 2^16 rows");
   BLP_CHECK(k >= 1 && k <= (1 << 20), BLP_E_ARG, "softmax loss: k must be in [1, 2^20]");
   return 0;
 }

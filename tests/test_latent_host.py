@@ -35,6 +35,11 @@ def test_softmax_loss_refuses(args, what):
     refused(loss(**args), what)
 
 
+@pytest.mark.parametrize("args,what", [({"rows": (1 << 31) - (1 << 16) + 1}, "rows"), ({"cols": (1 << 31) - (1 << 16) + 1}, "catalogue")])
+def test_softmax_loss_refuses_rows_whose_stages_pass_31_bits(args, what):
+    refused(loss(**args), what)
+
+
 def test_softmax_loss_backward_refuses():
     refused(lib().blp_softmax_loss_backward(0, None, 0, ONE, 8, ONE, 8, ONE, 0, 4, 4, 8, 1.0, ONE, ONE, 2, None, ONE, 8, ONE, 8, ONE,
                                             1 << 40), "grad_stride")
