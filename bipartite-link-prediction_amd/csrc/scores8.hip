@@ -121,10 +121,19 @@ struct EpiScores {
       for (int e = 0; e < 4; ++e) tp[i][e] = t[p0 + min(i * 16 + h * 4 + e, left - 1)];
 #pragma unroll
     for (int j = 0; j < S::FQ; ++j) sq[j] = s[q0 + min(j * 16 + l, rows - 1)];
+    bool far = false;
+#pragma unroll
+    for (int j = 0; j < S::FQ; ++j) far |= fabsf(sq[j]) > 0x1p96f;
+    far = __any(far);
     store_block<TO, S, true>(scratch, out + q0 * ld + p0 * size_of(TO), ld, left, rows, [&](int i, int j) {
       f32x4 v;
+      if (far) {  // |sum| < 2^31, times s it may pass the largest float though the score does not: in 64 bits
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j][e] * sq[j] * tp[i][e];
+        for (int e = 0; e < 4; ++e) v[e] = (float)((double)acc[i][j][e] * sq[j] * tp[i][e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j][e] * sq[j] * tp[i][e];
+      }
       return v;
     });
   }

@@ -28,7 +28,10 @@ def check_scores(got, q, s, p, t):
 
     want = (q.double() @ p.double().t().contiguous()) * s.double()[:, None] * t.double()[None, :]
     h = torch.finfo(got.dtype).eps / 2
-    tiny = 2.0 ** -25 if got.dtype == torch.float16 else 0.0
+    # Below the type's smallest normal number roundings are off by half of its last place at most, whatever the value:
+    # float16 2^-24 / 2; float32 2^-149 / 2 (the product with t; sum times s is a multiple of s, so it is a multiple of
+    # 2^-149 and exact there); bfloat16 2^-133 / 2 after that float32 rounding.
+    tiny = {torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150, torch.bfloat16: 2.0 ** -134 + 2.0 ** -150}[got.dtype]
     off = (got.double() - want).abs() - (want.abs() * (3 * 2.0 ** -24 + h) * 1.001 + tiny)
     assert got.shape == want.shape and bool((off <= 0).all()), float(off.max())
 
@@ -84,6 +87,27 @@ def test_scores(gpu, m, n, k, out):
     t = torch.rand(n, device="cuda", generator=g) * 1e-2
     got = latent.int8_scores(q, s, p, t, dtype=getattr(torch, out))
     check_scores(got, q, s, p, t)
+
+
+@pytest.mark.parametrize("out", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("m,n,k", [(5, 700, 64), (40, 300, 200), (300, 301, 1000)])
+def test_scales_far_apart(gpu, m, n, k, out):
+    """Large scales of rows against small ones of the catalogue: sum times row scale passes the largest float, the score
+    does not."""
+    torch = _torch()
+    from blp import latent
+
+    g = torch.Generator(device="cuda").manual_seed(m)
+    q = torch.randint(-128, 128, (m, k), device="cuda", generator=g).to(torch.int8)
+    p = torch.randint(-128, 128, (n, k), device="cuda", generator=g).to(torch.int8)
+    q[0], p[0] = 127, 127
+    s = (0.5 + torch.rand(m, device="cuda", generator=g)) * 2.0 ** 126
+    t = (0.5 + torch.rand(n, device="cuda", generator=g)) * 2.0 ** -120
+    s[-1], s[-2] = 2.0 ** -40, -2.0 ** 120
+    if out == "float16":
+        t *= 2.0 ** -6
+        p[:, 1:] = 0
+    check_scores(latent.int8_scores(q, s, p, t, dtype=getattr(torch, out)), q, s, p, t)
 
 
 def test_longest_sums(gpu):
