@@ -61,18 +61,22 @@ __global__ __launch_bounds__(256) void k_lookup(const char* __restrict__ table, 
 // 512 ROUNDS consecutive entries; wave w of it the w-th eighth, 64 at a time in order. The entries of one
 // digit are found with ballots (a lane's rank among them by counting the lanes below), so ranks follow
 // positions; ids outside the table get the largest key and end up last. 1 M ids of 100,000 rows, two passes: counts 2 x 5 us,
-// sums 2 x 5 us, entries 2 x 17 us (16 MB each, scattered words: 0.9 TB/s).
+// sums 2 x 5 us, entries 2 x 11 us (8 MB in, 8 MB out in scattered entries; keys and positions apart: 17 us).
 constexpr int SORT_WAVES = 8, SORT_THREADS = 64 * SORT_WAVES, MOST_BITS = 10;
 
-__device__ inline uint32_t key_at(const Ids& ids, const uint32_t* keys, int64_t i) {
-  if (keys) return keys[i];
+struct Entry {  // eight bytes together: a scattered entry is one write
+  uint32_t key, pos;
+};
+
+__device__ inline uint32_t key_at(const Ids& ids, const Entry* in, int64_t i) {
+  if (in) return in[i].key;
   const int64_t id = ids(i);
   return id >= 0 ? (uint32_t)id : (uint32_t)ids.rows;
 }
 
 // counts[block][digit]
 template <int ROUNDS, int BITS>
-__global__ __launch_bounds__(SORT_THREADS) void k_digit_counts(Ids ids, const uint32_t* __restrict__ keys, int64_t n, int shift,
+__global__ __launch_bounds__(SORT_THREADS) void k_digit_counts(Ids ids, const Entry* __restrict__ in, int64_t n, int shift,
                                                                uint32_t* __restrict__ counts) {
   constexpr int BINS = 1 << BITS;
   __shared__ uint32_t s_count[BINS];
@@ -82,7 +86,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_digit_counts(Ids ids, const ui
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
     const int64_t i = base + r * SORT_THREADS + threadIdx.x;
-    if (i < n) atomicAdd(&s_count[(key_at(ids, keys, i) >> shift) & (BINS - 1)], 1u);
+    if (i < n) atomicAdd(&s_count[(key_at(ids, in, i) >> shift) & (BINS - 1)], 1u);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += SORT_THREADS) counts[(int64_t)blockIdx.x * BINS + i] = s_count[i];
@@ -125,22 +129,20 @@ __global__ __launch_bounds__(1024) void k_digit_sums(uint32_t* __restrict__ coun
 }
 
 template <int ROUNDS, int BITS>
-__global__ __launch_bounds__(SORT_THREADS) void k_scatter(Ids ids, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
-                                                 int64_t n, int shift, const uint32_t* __restrict__ counts,
-                                                 const uint32_t* __restrict__ total, uint32_t* __restrict__ keys_out,
-                                                 uint32_t* __restrict__ pos_out) {
+__global__ __launch_bounds__(SORT_THREADS) void k_scatter(Ids ids, const Entry* __restrict__ in, int64_t n, int shift,
+                                                          const uint32_t* __restrict__ counts,
+                                                          const uint32_t* __restrict__ total, Entry* __restrict__ out) {
   constexpr int BINS = 1 << BITS;
   __shared__ uint32_t s_base[BINS];
   __shared__ uint16_t s_wave[SORT_WAVES][BINS];
   __shared__ uint32_t s_sum[SORT_WAVES];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t base = (int64_t)blockIdx.x * (SORT_THREADS * ROUNDS) + w * (64 * ROUNDS);
-  uint32_t key[ROUNDS], at[ROUNDS];
+  Entry entry[ROUNDS];
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
     const int64_t i = min(base + r * 64 + lane, n - 1);
-    key[r] = key_at(ids, keys, i);
-    at[r] = pos ? pos[i] : (uint32_t)i;
+    entry[r] = in ? in[i] : Entry{key_at(ids, nullptr, i), (uint32_t)i};
   }
   for (int i = threadIdx.x; i < SORT_WAVES * BINS / 2; i += SORT_THREADS) reinterpret_cast<uint32_t*>(&s_wave[0][0])[i] = 0;
   // where each digit starts: exclusive sums of the totals, BINS / 512 digits a thread
@@ -168,19 +170,19 @@ __global__ __launch_bounds__(SORT_THREADS) void k_scatter(Ids ids, const uint32_
   uint16_t rank[ROUNDS];
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
-    const bool in = base + r * 64 + lane < n;
-    const uint32_t d = (key[r] >> shift) & (BINS - 1);
-    unsigned long long same = __ballot(in);
+    const bool ok = base + r * 64 + lane < n;
+    const uint32_t d = (entry[r].key >> shift) & (BINS - 1);
+    unsigned long long same = __ballot(ok);
 #pragma unroll
     for (int b = 0; b < BITS; ++b) {
       const unsigned long long m = __ballot((d >> b) & 1);
       same &= ((d >> b) & 1) ? m : ~m;
     }
     const int below = __popcll(same & ((1ull << lane) - 1));
-    if (in) rank[r] = (uint16_t)(s_wave[w][d] + below);
+    if (ok) rank[r] = (uint16_t)(s_wave[w][d] + below);
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    if (in && below == 0) s_wave[w][d] += (uint16_t)__popcll(same);
+    if (ok && below == 0) s_wave[w][d] += (uint16_t)__popcll(same);
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
@@ -199,10 +201,8 @@ __global__ __launch_bounds__(SORT_THREADS) void k_scatter(Ids ids, const uint32_
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
     if (base + r * 64 + lane < n) {
-      const uint32_t d = (key[r] >> shift) & (BINS - 1);
-      const uint32_t to = s_base[d] + s_wave[w][d] + rank[r];
-      keys_out[to] = key[r];
-      pos_out[to] = at[r];
+      const uint32_t d = (entry[r].key >> shift) & (BINS - 1);
+      out[s_base[d] + s_wave[w][d] + rank[r]] = entry[r];
     }
   }
 }
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_scatter(Ids ids, const uint32_
 // before it. Every block has all keys in LDS and places 64 entries, four threads an entry. n^2 comparisons: 8,192
 // entries take 6 us where the radix passes' six launches take 22.
 constexpr int SMALL = 8192;
-__global__ __launch_bounds__(256) void k_place_small(Ids ids, int n, uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out) {
+__global__ __launch_bounds__(256) void k_place_small(Ids ids, int n, Entry* __restrict__ out) {
   extern __shared__ uint4 s_key[];  // n rounded up to 16, the rest the largest key
   const int quads = (n + 15) / 16 * 4;
   for (int i = threadIdx.x; i < quads * 4; i += 256)
@@ -229,14 +229,11 @@ __global__ __launch_bounds__(256) void k_place_small(Ids ids, int n, uint32_t* _
   }
   place += __shfl_xor(place, 1, 64);
   place += __shfl_xor(place, 2, 64);
-  if (part == 0 && i < n) {
-    keys_out[place] = key;
-    pos_out[place] = (uint32_t)i;
-  }
+  if (part == 0 && i < n) out[place] = Entry{key, (uint32_t)i};
 }
 
 // ---------------------------------------------------------------- sums
-constexpr int HEAVY = 32;  // chunks: a row that crosses more of them is added up by a whole block
+constexpr int HEAVY = 16;  // chunks: a row that crosses more of them is added up by a whole block
 
 template <int T>
 __device__ inline void put(char* out, int64_t ldo, uint32_t key, int e0, int k, const Vec<T>& sum, float scale, int add) {
@@ -262,7 +259,7 @@ __device__ inline void put_part(float* part, int64_t slot, int64_t kv, int vec, 
 }
 
 struct Sums {
-  const uint32_t *keys, *pos;
+  const Entry* in;           // sorted
   int64_t n, chunk, chunks;  // entries, entries a chunk
   uint32_t rows;
   int k, lanes;              // lanes of a chunk: a power of two up to 64; blockIdx.y: their column tile
@@ -274,8 +271,9 @@ struct Sums {
   int64_t kv;  // floats of a partial sum
 };
 
-// Bound by reading dy, in whole rows but in sorted order: 1 M x 64 float32 0.28 GB in 55 us, 5.2 TB/s.
-// The blocks past `sum_blocks` clear the rows without ids: 64 rows a wave, each lane looks its row up in the
+// Bound by reading dy, in whole rows but in sorted order: 1 M x 64 float32 0.28 GB in 55 to 60 us, 4.7 to
+// 5.2 TB/s.
+// The first `clear_blocks` blocks clear the rows without ids: 64 rows a wave, each lane looks its row up in the
 // sorted ids.
 template <int T>
 __device__ void clear_rows(const Sums& a, int64_t wave) {
@@ -286,12 +284,12 @@ __device__ void clear_rows(const Sums& a, int64_t wave) {
     int64_t lo = 0, hi = a.n;
     while (lo < hi) {
       const int64_t mid = (lo + hi) >> 1;
-      if (a.keys[mid] < (uint32_t)r)
+      if (a.in[mid].key < (uint32_t)r)
         lo = mid + 1;
       else
         hi = mid;
     }
-    absent = lo == a.n || a.keys[lo] != (uint32_t)r;
+    absent = lo == a.n || a.in[lo].key != (uint32_t)r;
   }
   unsigned long long left = __ballot(absent);
   const int vecs = (a.k + Vec<T>::NE - 1) / Vec<T>::NE;
@@ -310,37 +308,34 @@ __device__ void clear_rows(const Sums& a, int64_t wave) {
 }
 
 template <int T>
-__global__ __launch_bounds__(256) void k_chunk_sums(Sums a, const char* __restrict__ dy, int64_t ld, unsigned sum_blocks) {
+__global__ __launch_bounds__(256) void k_chunk_sums(Sums a, const char* __restrict__ dy, int64_t ld, unsigned clear_blocks) {
   constexpr int NE = Vec<T>::NE, U = 8;
-  if (blockIdx.x >= sum_blocks) {
-    if (blockIdx.y == 0) clear_rows<T>(a, (blockIdx.x - sum_blocks) * 4ll + (threadIdx.x >> 6));
+  if (blockIdx.x < clear_blocks) {
+    if (blockIdx.y == 0) clear_rows<T>(a, blockIdx.x * 4ll + (threadIdx.x >> 6));
     return;
   }
-  const int64_t chunk = (blockIdx.x * 256ll + threadIdx.x) / a.lanes;
+  const int64_t chunk = ((blockIdx.x - clear_blocks) * 256ll + threadIdx.x) / a.lanes;
   const int vec = blockIdx.y * a.lanes + (threadIdx.x & (a.lanes - 1)), e0 = vec * NE, k = a.k;
   const int64_t b = chunk * a.chunk, e = min(a.n, b + a.chunk);
   const uint32_t rows = a.rows;
   if (b >= a.n || e0 >= k) return;
   const char* src = dy + (int64_t)e0 * size_of(T);
-  uint32_t cur = a.keys[b];
-  bool head = b > 0 && a.keys[b - 1] == cur;  // the running row began in an earlier chunk
+  uint32_t cur = a.in[b].key;
+  bool head = b > 0 && a.in[b - 1].key == cur;  // the running row began in an earlier chunk
   Vec<T> sum{};
   for (int64_t i = b; i < e; i += U) {
-    uint32_t key[U], pos[U];
+    Entry in[U];
     Vec<T> v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      key[u] = i + u < e ? a.keys[i + u] : rows;
-      pos[u] = i + u < e ? a.pos[i + u] : 0;
-    }
+    for (int u = 0; u < U; ++u) in[u] = i + u < e ? a.in[i + u] : Entry{rows, 0};
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       v[u] = Vec<T>{};
-      if (key[u] < rows) v[u] = load_vec<T>(src + (int64_t)pos[u] * ld, k - e0);
+      if (in[u].key < rows) v[u] = load_vec<T>(src + (int64_t)in[u].pos * ld, k - e0);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (i + u < e && key[u] != cur) {  // `cur` ended before this entry
+      if (i + u < e && in[u].key != cur) {  // `cur` ended before this entry
         if (cur < rows) {
           if (head)
             put_part<T>(a.part, 2 * chunk, a.kv, vec, sum);
@@ -348,7 +343,7 @@ __global__ __launch_bounds__(256) void k_chunk_sums(Sums a, const char* __restri
             put<T>(a.out, a.ldo, cur, e0, k, sum, a.scale, a.add);
         }
         head = false;
-        cur = key[u];
+        cur = in[u].key;
         sum = Vec<T>{};
       }
 #pragma unroll
@@ -356,7 +351,7 @@ __global__ __launch_bounds__(256) void k_chunk_sums(Sums a, const char* __restri
     }
   }
   if (cur >= rows) return;
-  const bool goes_on = e < a.n && a.keys[e] == cur;
+  const bool goes_on = e < a.n && a.in[e].key == cur;
   if (head)
     put_part<T>(a.part, 2 * chunk, a.kv, vec, sum);
   else if (goes_on)
@@ -365,28 +360,28 @@ __global__ __launch_bounds__(256) void k_chunk_sums(Sums a, const char* __restri
     put<T>(a.out, a.ldo, cur, e0, k, sum, a.scale, a.add);
 }
 
-// Whether a row begins in `chunk` and goes on in the next; its key. (A chunk's last row, so at most one.)
-__device__ inline bool crosses(const Sums& a, int64_t chunk, uint32_t* key) {
-  const int64_t b = chunk * a.chunk, e = b + a.chunk;
-  if (e >= a.n) return false;
-  *key = a.keys[e - 1];
-  if (*key >= a.rows || a.keys[e] != *key) return false;
-  return !(b > 0 && a.keys[b] == *key && a.keys[b - 1] == *key);
-}
-__device__ inline bool heavy(const Sums& a, int64_t chunk, uint32_t key) {
-  const int64_t far = (chunk + HEAVY + 1) * a.chunk;
-  return far < a.n && a.keys[far] == key;
+// Whether a row begins in `chunk` and goes on in the next (a chunk's last row, so at most one), and whether it is heavy.
+enum Crossing { NONE, LIGHT, HEAVY_ROW };
+__device__ inline Crossing crossing(const Sums& a, int64_t chunk, uint32_t* key) {
+  const int64_t b = chunk * a.chunk, e = b + a.chunk, far = (chunk + HEAVY + 1) * a.chunk;
+  if (e >= a.n) return NONE;
+  const uint32_t last = a.in[e - 1].key, next = a.in[e].key, first = a.in[b].key, before = a.in[max(b - 1, (int64_t)0)].key,
+                 away = a.in[min(far, a.n - 1)].key;  // one wait for all five
+  *key = last;
+  if (last >= a.rows || next != last || (b > 0 && first == last && before == last)) return NONE;
+  return far < a.n && away == last ? HEAVY_ROW : LIGHT;
 }
 
 // The rows that cross chunks, in 64 bits. The first blocks, which last longest: HEAVY chunks each, in which one heavy row
 // can begin; its partial sums go to the groups of lanes in turn, then the groups' sums are added in order. The
-// others: a group of lanes a chunk, the partial sums of the row that begins there in the chunks' order. 17 us in the case
-// above, bound by the longest row's chain of adds.
+// others: a group of lanes a chunk, the partial sums of the row that begins there in the chunks' order. 14 us in the case
+// above: six or seven waits for memory, one after the other.
 template <int T>
 __global__ __launch_bounds__(256) void k_join_chunks(Sums a, unsigned heavy_blocks) {
-  constexpr int NE = Vec<T>::NE;
+  constexpr int NE = Vec<T>::NE, U = 4;
   __shared__ double s_sum[256 * NE];
   __shared__ int s_at;
+  __shared__ uint32_t s_key;
   const int groups = 256 / a.lanes, g = threadIdx.x / a.lanes, l = threadIdx.x & (a.lanes - 1);
   const int vec = blockIdx.y * a.lanes + l, e0 = vec * NE;
   double sum[NE];
@@ -395,14 +390,26 @@ __global__ __launch_bounds__(256) void k_join_chunks(Sums a, unsigned heavy_bloc
   uint32_t key;
   if (blockIdx.x >= heavy_blocks) {
     const int64_t chunk = (int64_t)(blockIdx.x - heavy_blocks) * groups + g;
-    if (chunk >= a.chunks || e0 >= a.k || !crosses(a, chunk, &key) || heavy(a, chunk, key)) return;
-    int64_t c = chunk;
-    do {
-      const f32x4* at = reinterpret_cast<const f32x4*>(a.part + (2 * c + (c == chunk ? 1 : 0)) * a.kv + (int64_t)e0);
+    if (chunk >= a.chunks || e0 >= a.k || crossing(a, chunk, &key) != LIGHT) return;
+    bool more = true;
+    for (int64_t c = chunk; more; c += U) {  // U chunks' loads at a time, their keys' beside their sums'
+      bool mine[U];
+      f32x4 v[U][NE / 4];
 #pragma unroll
-      for (int j = 0; j < NE; ++j) sum[j] += (double)at[j >> 2][j & 3];
-      ++c;
-    } while (c * a.chunk < a.n && a.keys[c * a.chunk] == key);
+      for (int u = 0; u < U; ++u) {
+        const int64_t at = min(c + u, a.chunks - 1);
+        mine[u] = c + u == chunk || (c + u < a.chunks && a.in[at * a.chunk].key == key);
+        const f32x4* part = reinterpret_cast<const f32x4*>(a.part + (2 * at + (at == chunk ? 1 : 0)) * a.kv + (int64_t)e0);
+#pragma unroll
+        for (int j = 0; j < NE / 4; ++j) v[u][j] = part[j];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        more = more && mine[u];
+#pragma unroll
+        for (int j = 0; j < NE; ++j) sum[j] += more ? (double)v[u][j >> 2][j & 3] : 0.0;
+      }
+    }
     Vec<T> r;
 #pragma unroll
     for (int j = 0; j < NE; ++j) r.v[j >> 2][j & 3] = (float)sum[j];
@@ -412,23 +419,24 @@ __global__ __launch_bounds__(256) void k_join_chunks(Sums a, unsigned heavy_bloc
   if (threadIdx.x == 0) s_at = -1;
   __syncthreads();
   const int64_t first = blockIdx.x * (int64_t)HEAVY;
-  if (threadIdx.x < HEAVY && first + threadIdx.x < a.chunks && crosses(a, first + threadIdx.x, &key) &&
-      heavy(a, first + threadIdx.x, key))
+  if (threadIdx.x < HEAVY && first + threadIdx.x < a.chunks && crossing(a, first + threadIdx.x, &key) == HEAVY_ROW) {
     s_at = threadIdx.x;
+    s_key = key;
+  }
   __syncthreads();
   if (s_at < 0) return;
   const int64_t chunk = first + s_at;
-  key = a.keys[(chunk + 1) * a.chunk - 1];
-  int64_t lo = chunk + 1, hi = a.chunks;  // the first chunk that does not begin with the row
+  key = s_key;
+  int64_t lo = chunk + 1, hi = a.chunks;  // the first chunk that does not begin with the row: 256 probes at a time
   while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (a.keys[mid * a.chunk] == key)
-      lo = mid + 1;
-    else
-      hi = mid;
+    const int64_t step = (hi - lo + 255) >> 8, at = lo + threadIdx.x * step;
+    const int begin = __syncthreads_count(at < hi && a.in[at * a.chunk].key == key);
+    if (begin == 0) break;
+    hi = min(hi, lo + begin * step);
+    lo += (begin - 1) * step + 1;
   }
   if (e0 < a.k) {
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t c = chunk + g; c < lo; c += groups) {
       const f32x4* at = reinterpret_cast<const f32x4*>(a.part + (2 * c + (c == chunk ? 1 : 0)) * a.kv + (int64_t)e0);
 #pragma unroll
@@ -456,7 +464,7 @@ int64_t up(int64_t v, int64_t to) { return div_up(v, to) * to; }
 struct Plan {
   int passes, bits, rounds, lanes, tiles;
   int64_t blocks, chunk, chunks, kv;
-  int64_t o_keys[2], o_pos[2], o_counts, o_total, o_part, bytes;
+  int64_t o_in[2], o_counts, o_total, o_part, bytes;
 };
 
 Plan plan_of(int type, int64_t n, int64_t rows, int k) {
@@ -482,10 +490,7 @@ Plan plan_of(int type, int64_t n, int64_t rows, int k) {
   while (p.chunk > 8 && div_up(n, p.chunk) * p.lanes * p.tiles / 64 < 4096) p.chunk >>= 1;
   p.chunks = div_up(n, p.chunk);
   p.kv = up(k, 16 / size_of(type));
-  for (int i = 0; i < 2; ++i) {
-    p.o_keys[i] = take(4 * n);
-    p.o_pos[i] = take(4 * n);
-  }
+  for (int i = 0; i < 2; ++i) p.o_in[i] = take(8 * n);
   p.o_counts = take(p.passes ? (4ll << p.bits) * p.blocks : 0);
   p.o_total = take(4 << MOST_BITS);
   p.o_part = take(8 * p.chunks * p.kv);
@@ -508,18 +513,16 @@ int lookup(hipStream_t st, const void* table, int64_t ld, Ids ids, int64_t n, in
 }
 
 template <int ROUNDS, int BITS>
-int sort(hipStream_t st, const Plan& p, Ids ids, int64_t n, uint32_t* const* keys, uint32_t* const* pos, uint32_t* counts,
-         uint32_t* total, int* last) {
+int sort(hipStream_t st, const Plan& p, Ids ids, int64_t n, Entry* const* sorted, uint32_t* counts, uint32_t* total, int* last) {
   int cur = 0;
   for (int s = 0; s < p.passes; ++s) {
-    const uint32_t* kin = s ? keys[cur] : nullptr;
+    const Entry* in = s ? sorted[cur] : nullptr;
     const int to = s ? cur ^ 1 : 0;
-    k_digit_counts<ROUNDS, BITS><<<(unsigned)p.blocks, SORT_THREADS, 0, st>>>(ids, kin, n, s * BITS, counts);
+    k_digit_counts<ROUNDS, BITS><<<(unsigned)p.blocks, SORT_THREADS, 0, st>>>(ids, in, n, s * BITS, counts);
     BLP_HIP(hipGetLastError());
     k_digit_sums<BITS><<<(1 << BITS) / 16, 1024, 0, st>>>(counts, (int)p.blocks, total);
     BLP_HIP(hipGetLastError());
-    k_scatter<ROUNDS, BITS><<<(unsigned)p.blocks, SORT_THREADS, 0, st>>>(ids, kin, s ? pos[cur] : nullptr, n, s * BITS, counts, total, keys[to],
-                                                          pos[to]);
+    k_scatter<ROUNDS, BITS><<<(unsigned)p.blocks, SORT_THREADS, 0, st>>>(ids, in, n, s * BITS, counts, total, sorted[to]);
     BLP_HIP(hipGetLastError());
     cur = to;
   }
@@ -531,16 +534,15 @@ template <int T>
 int lookup_grad(hipStream_t st, const Plan& p, const void* dy, int64_t ld, Ids ids, int64_t n, int k, float scale, void* out,
                 int64_t ldo, int add, char* ws) {
   const int ES = size_of(T);
-  uint32_t* keys[2] = {(uint32_t*)(ws + p.o_keys[0]), (uint32_t*)(ws + p.o_keys[1])};
-  uint32_t* pos[2] = {(uint32_t*)(ws + p.o_pos[0]), (uint32_t*)(ws + p.o_pos[1])};
+  Entry* sorted[2] = {(Entry*)(ws + p.o_in[0]), (Entry*)(ws + p.o_in[1])};
   uint32_t *counts = (uint32_t*)(ws + p.o_counts), *total = (uint32_t*)(ws + p.o_total);
   int cur = 0, rc = 0;
   if (p.passes == 0) {
-    if (n > 0) k_place_small<<<(unsigned)div_up(n, 64), 256, up(n, 16) * 4, st>>>(ids, (int)n, keys[0], pos[0]);
+    if (n > 0) k_place_small<<<(unsigned)div_up(n, 64), 256, up(n, 16) * 4, st>>>(ids, (int)n, sorted[0]);
     BLP_HIP(hipGetLastError());
   } else {
     auto run = [&](auto rounds, auto bits) {
-      return sort<decltype(rounds)::value, decltype(bits)::value>(st, p, ids, n, keys, pos, counts, total, &cur);
+      return sort<decltype(rounds)::value, decltype(bits)::value>(st, p, ids, n, sorted, counts, total, &cur);
     };
     using std::integral_constant;
     if (p.rounds == 1)
@@ -549,11 +551,11 @@ int lookup_grad(hipStream_t st, const Plan& p, const void* dy, int64_t ld, Ids i
       rc = p.bits == 9 ? run(integral_constant<int, 4>{}, integral_constant<int, 9>{}) : run(integral_constant<int, 4>{}, integral_constant<int, 10>{});
     if (rc) return rc;
   }
-  const Sums a = {keys[cur], pos[cur], n, p.chunk, p.chunks, (uint32_t)ids.rows, k, p.lanes, scale, (char*)out, ldo * ES, add,
+  const Sums a = {sorted[cur], n, p.chunk, p.chunks, (uint32_t)ids.rows, k, p.lanes, scale, (char*)out, ldo * ES, add,
                   (float*)(ws + p.o_part), p.kv};
   const unsigned sum_blocks = (unsigned)div_up(p.chunks * p.lanes, 256), clear_blocks = add ? 0 : (unsigned)div_up(ids.rows, 256);
   if (sum_blocks + clear_blocks == 0) return 0;
-  k_chunk_sums<T><<<dim3(sum_blocks + clear_blocks, p.tiles), 256, 0, st>>>(a, (const char*)dy, ld * ES, sum_blocks);
+  k_chunk_sums<T><<<dim3(sum_blocks + clear_blocks, p.tiles), 256, 0, st>>>(a, (const char*)dy, ld * ES, clear_blocks);
   BLP_HIP(hipGetLastError());
   if (p.chunks > 1) {
     const unsigned light = (unsigned)div_up(p.chunks, 256 / p.lanes), heavies = (unsigned)div_up(p.chunks, HEAVY);
