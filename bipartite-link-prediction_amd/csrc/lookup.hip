@@ -208,28 +208,40 @@ __global__ __launch_bounds__(SORT_THREADS) void k_scatter(Ids ids, const Entry* 
 }
 
 // Up to SMALL entries, in one launch: an entry's place is the number of entries with a smaller key, or with the same key
-// before it. Every block has all keys in LDS and places 64 entries, four threads an entry. n^2 comparisons: 8,192
-// entries take 6 us where the radix passes' six launches take 22.
-constexpr int SMALL = 8192;
-__global__ __launch_bounds__(256) void k_place_small(Ids ids, int n, Entry* __restrict__ out) {
+// before it. Every block has all keys in LDS; a wave places EACH entries, its lanes passing over the keys by vectors.
+// n^2 comparisons: 2,000 entries take 6 us and 8,192 take 13, where the radix passes' six launches take 20 and more.
+constexpr int SMALL = 8192, EACH = 4, PLACED = 8 * EACH;
+__global__ __launch_bounds__(512) void k_place_small(Ids ids, int n, Entry* __restrict__ out) {
   extern __shared__ uint4 s_key[];  // n rounded up to 16, the rest the largest key
+  uint32_t* const word = reinterpret_cast<uint32_t*>(s_key);
   const int quads = (n + 15) / 16 * 4;
-  for (int i = threadIdx.x; i < quads * 4; i += 256)
-    reinterpret_cast<uint32_t*>(s_key)[i] = i < n ? key_at(ids, nullptr, i) : 0xffffffffu;
+  for (int i = threadIdx.x; i < quads * 4; i += 512) word[i] = i < n ? key_at(ids, nullptr, i) : 0xffffffffu;
   __syncthreads();
-  const int i = blockIdx.x * 64 + (threadIdx.x >> 2), part = threadIdx.x & 3;
-  const uint32_t key = i < n ? reinterpret_cast<const uint32_t*>(s_key)[i] : 0xffffffffu;
-  int place = 0;
-#pragma unroll 4
-  for (int q = part; q < quads; q += 4) {
-    const uint4 v = s_key[q];
-    const int j = q * 4;
-    place += (v.x < key || (v.x == key && j < i)) + (v.y < key || (v.y == key && j + 1 < i)) +
-             (v.z < key || (v.z == key && j + 2 < i)) + (v.w < key || (v.w == key && j + 3 < i));
+  const int lane = threadIdx.x & 63, first = blockIdx.x * PLACED + (threadIdx.x >> 6) * EACH;
+  if (first >= n) return;
+  uint32_t key[EACH];
+  int place[EACH];
+#pragma unroll
+  for (int u = 0; u < EACH; ++u) {  // first is a multiple of four: the entries lie in one vector
+    key[u] = word[first + u];
+    place[u] = lane < u && word[first + lane] == key[u];  // within the vector
   }
-  place += __shfl_xor(place, 1, 64);
-  place += __shfl_xor(place, 2, 64);
-  if (part == 0 && i < n) out[place] = Entry{key, (uint32_t)i};
+#pragma unroll 2
+  for (int q = lane; q < quads; q += 64) {
+    const uint4 v = s_key[q];
+    const uint32_t same = q < (first >> 2);  // before the entries the same key counts, too
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+      const uint32_t below = key[u] + same;
+      place[u] += (v.x < below) + (v.y < below) + (v.z < below) + (v.w < below);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < EACH; ++u) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) place[u] += __shfl_xor(place[u], o, 64);
+    if (lane == u && first + u < n) out[place[u]] = Entry{key[u], (uint32_t)(first + u)};
+  }
 }
 
 // ---------------------------------------------------------------- sums
@@ -271,40 +283,66 @@ struct Sums {
   int64_t kv;  // floats of a partial sum
 };
 
-// Bound by reading dy, in whole rows but in sorted order: 1 M x 64 float32 0.28 GB in 55 to 60 us, 4.7 to
-// 5.2 TB/s.
-// The first `clear_blocks` blocks clear the rows without ids: 64 rows a wave, each lane looks its row up in the
-// sorted ids.
+// Bound by reading dy, in whole rows but in sorted order: 1 M x 64 float32 0.28 GB in 60 us, 4.7
+// TB/s; 16,384 x 1,024 bf16 0.09 GB in 20 us.
+// The first `clear_blocks` blocks clear the rows without ids: 64 rows a wave, whose entries it looks up, 64 probes at
+// a time.
 template <int T>
 __device__ void clear_rows(const Sums& a, int64_t wave) {
   const int lane = threadIdx.x & 63;
-  const int64_t r = wave * 64 + lane;
-  bool absent = false;
-  if (r < a.rows) {
-    int64_t lo = 0, hi = a.n;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (a.in[mid].key < (uint32_t)r)
-        lo = mid + 1;
-      else
-        hi = mid;
+  const int64_t r0 = wave * 64;
+  if (r0 >= a.rows) return;
+  int64_t lo[2] = {0, 0}, hi[2] = {a.n, a.n};  // the first entries of row r0 and of row r0 + 64
+  while (lo[0] < hi[0] || lo[1] < hi[1]) {
+    unsigned long long less[2];
+    int64_t step[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      step[i] = (hi[i] - lo[i] + 63) >> 6;
+      const int64_t at = lo[i] + lane * step[i];
+      less[i] = __ballot(at < hi[i] && a.in[at].key < (uint32_t)(r0 + i * 64));
     }
-    absent = lo == a.n || a.in[lo].key != (uint32_t)r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int c = __popcll(less[i]);
+      hi[i] = min(hi[i], lo[i] + c * step[i]);
+      if (c) lo[i] += (c - 1) * step[i] + 1;
+    }
   }
-  unsigned long long left = __ballot(absent);
+  uint32_t low = 0, high = 0;  // which of the 64 rows have entries
+  if (lo[1] - lo[0] <= 512) {
+    for (int64_t i = lo[0] + lane; i < lo[1]; i += 64) {
+      const uint32_t r = a.in[i].key - (uint32_t)r0;
+      (r < 32 ? low : high) |= 1u << (r & 31);
+    }
+    for (int o = 1; o < 64; o <<= 1) {
+      low |= __shfl_xor(low, o, 64);
+      high |= __shfl_xor(high, o, 64);
+    }
+  } else {
+    const uint32_t r = (uint32_t)(r0 + lane);
+    int64_t first = lo[0], end = lo[1];
+    while (first < end) {
+      const int64_t mid = (first + end) >> 1;
+      if (a.in[mid].key < r)
+        first = mid + 1;
+      else
+        end = mid;
+    }
+    const unsigned long long there = __ballot(first < lo[1] && a.in[first].key == r);
+    low = (uint32_t)there;
+    high = (uint32_t)(there >> 32);
+  }
+  unsigned long long left = ~((unsigned long long)high << 32 | low);
+  if (a.rows - r0 < 64) left &= (1ull << (a.rows - r0)) - 1;
   const int vecs = (a.k + Vec<T>::NE - 1) / Vec<T>::NE;
   // short rows: several at a time
-  const int each = a.lanes, groups = 64 / each, g = lane / each, l = lane & (each - 1);
-  while (left) {
-    unsigned long long mine = left;
-    for (int i = 0; i < g && mine; ++i) mine &= mine - 1;
-    if (mine) {
-      char* at = a.out + (wave * 64 + __builtin_ctzll(mine)) * a.ldo;
-      for (int v = l; v < vecs; v += each)
-        store_vec<T>(at + (int64_t)v * 16, a.k - v * Vec<T>::NE, Vec<T>{});
-    }
-    for (int i = 0; i < groups && left; ++i) left &= left - 1;
-  }
+  const int each = a.lanes, groups = 64 / each, l = lane & (each - 1);
+  char* at = a.out + (r0 + lane / each) * a.ldo;
+  left >>= lane / each;
+  for (int r = 0; r < 64; r += groups, at += groups * a.ldo, left >>= groups & 63)
+    if (left & 1)
+      for (int v = l; v < vecs; v += each) store_vec<T>(at + (int64_t)v * 16, a.k - v * Vec<T>::NE, Vec<T>{});
 }
 
 template <int T>
@@ -538,7 +576,7 @@ int lookup_grad(hipStream_t st, const Plan& p, const void* dy, int64_t ld, Ids i
   uint32_t *counts = (uint32_t*)(ws + p.o_counts), *total = (uint32_t*)(ws + p.o_total);
   int cur = 0, rc = 0;
   if (p.passes == 0) {
-    if (n > 0) k_place_small<<<(unsigned)div_up(n, 64), 256, up(n, 16) * 4, st>>>(ids, (int)n, sorted[0]);
+    if (n > 0) k_place_small<<<(unsigned)div_up(n, PLACED), 512, up(n, 16) * 4, st>>>(ids, (int)n, sorted[0]);
     BLP_HIP(hipGetLastError());
   } else {
     auto run = [&](auto rounds, auto bits) {
