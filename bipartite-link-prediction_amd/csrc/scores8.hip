@@ -139,10 +139,10 @@ struct EpiScores {
   }
 };
 
-// k up to 128: one stage, and the outputs are what counts. A workgroup of 8 waves, 16 rows and 16 FP columns each,
-// in 32 KiB of LDS, so that three of them share a compute unit and some load and multiply while others store. Bound by the stores: 10,000 x 100,000 bf16,
-// 2.0 GB, 0.44 to 0.53 ms, 0.44 (4.6 TB/s) with rows of whole 128-byte lines; larger k go through k_product (4,096 x 16,384 x
-// 4,096: 241 us, 2,278 TOP/s).
+// k up to 128: one stage, and the outputs are what counts. A workgroup of 8 waves, 16 rows and 16 FP columns each, in 32
+// KiB of LDS, so that three of them share a compute unit and some load and multiply while others store. Bound by the
+// stores: 10,000 x 100,000 bf16, 2.0 GB, 0.45 to 0.48 ms (4.2 to 4.4 TB/s; a fill reaches 6.8). Larger k go through
+// k_product (4,096 x 16,384 x 4,096: 241 us, 2,278 TOP/s).
 template <int FP_>
 struct OuterShape : Shape<1, 8, FP_, 1> {
   static constexpr int SCRATCH = 4096;
@@ -173,6 +173,151 @@ __global__ __launch_bounds__(512, 6) void k_outer8(Problem a, EpiScores<TO> epi)
   epi.template run<S>(acc, p0, q0 + wave * 16, 0, 0, lp + wave * 4096);
 }
 
+// The same where rows of outputs do not begin at whole vectors: k_outer8's stores of 16 bytes would straddle lines and run at
+// half the rate (2.1 TB/s; this one: 3.2 in bf16, 4.8 in float32). A workgroup passes along a strip of columns, W of them a step, with its 128 rows of q in
+// registers; the scores go through LDS, where row r begins at its place within its line, so that LINES whole lines of
+// every row leave, aligned, a step; what is left of the last one is carried to the next step. Only a strip's ends are
+// partial lines.
+template <int TO>
+struct Strip {
+  static constexpr int LINES = TO == F32 ? 2 : 1, W = LINES * 128 / size_of(TO), PITCH = (LINES + 1) * 128 + 16;
+};
+template <int TO, int KK>
+__global__ __launch_bounds__(512) void k_strip8(Operand w, Operand x, int k, EpiScores<TO> epi, int strips, int steps) {
+  constexpr int ES = size_of(TO), EG = 16 / ES, LINES = Strip<TO>::LINES, W = Strip<TO>::W, FP = W / 16, PITCH = Strip<TO>::PITCH;
+  constexpr int GR = LINES * 8, RPI = 64 / GR;  // granules of a row a step, rows a store instruction
+  __shared__ __attribute__((aligned(1024))) char s_p[W * STAGE], s_q[W * STAGE];
+  __shared__ __attribute__((aligned(16))) char s_rows[8][16 * PITCH];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l = lane & 15, h = lane >> 4;
+  // a die's workgroups take neighbouring rows of one strip: the strip's part of the catalogue stays in its L2
+  const int n = gridDim.x, groups = n / strips, per = n >> 3, more = n & 7, xcd = blockIdx.x & 7;
+  const int id = xcd * per + min(xcd, more) + (blockIdx.x >> 3);
+  const int strip = id / groups;
+  const int64_t q0 = ((int64_t)(id - strip * groups) * 8 + wave) * 16, c0 = (int64_t)strip * steps * W;
+  const int total = (int)min((int64_t)steps * W, w.rows - c0), rows = (int)max(min(x.rows - q0, (int64_t)16), (int64_t)0);
+  lds_char* const lds = (lds_char*)s_rows[wave];
+
+  const int64_t qr = min(q0 + l, x.rows - 1);
+  frag_t q[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) {
+    q[kk] = frag_t{0, 0, 0, 0};
+    if (kk * 64 + h * 16 < k) q[kk] = *reinterpret_cast<const frag_t*>(x.base + qr * x.ld + kk * 64 + h * 16);
+  }
+  const float sq = epi.s[qr];
+  const bool far = __any(fabsf(sq) > 0x1p96f);
+  char* const out = epi.out + q0 * epi.ld + c0 * ES;  // row r's first output: out + r ld
+  auto place = [&](int r) { return (int)((uintptr_t)(out + r * epi.ld) & 127); };
+  lds_char* const mine = lds + l * PITCH + place(l) + h * 4 * ES;
+  int at[16 / RPI];  // the granule's place among its row's outputs, in elements
+  char* to[16 / RPI];
+#pragma unroll
+  for (int i = 0; i < 16 / RPI; ++i) {
+    const int r = i * RPI + lane / GR;
+    to[i] = r < rows ? out + r * epi.ld - place(r) + (lane & (GR - 1)) * 16 : nullptr;
+    at[i] = (lane & (GR - 1)) * EG - place(r) / ES;
+  }
+  f32x4 t[FP];
+  auto scales = [&](int c) {
+#pragma unroll
+    for (int f = 0; f < FP; ++f) {
+      const int first = c + f * 16 + h * 4;
+      if (c + W <= total) {
+        struct __attribute__((packed, aligned(4))) Four {
+          f32x4 v;
+        };
+        t[f] = reinterpret_cast<const Four*>(epi.t + c0 + first)->v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[f][e] = epi.t[c0 + min(first + e, total - 1)];
+      }
+    }
+  };
+  auto emit = [&](int c) {  // the outputs from column c on that lie in the first LINES lines
+#pragma unroll
+    for (int i = 0; i < 16 / RPI; ++i) {
+      const i32x4 v = *(const __attribute__((address_space(3))) i32x4*)(lds + (i * RPI + lane / GR) * PITCH + (lane & (GR - 1)) * 16);
+      char* const o = to[i] + (int64_t)c * ES;
+      const int first = at[i] + c;  // of the lane's granule
+      if (to[i] && first >= 0 && first + EG <= total) {
+        __builtin_nontemporal_store(v, reinterpret_cast<i32x4*>(o));
+      } else if (to[i] && first + EG > 0 && first < total) {
+#pragma unroll
+        for (int e = 0; e < EG; ++e)
+          if (first + e >= 0 && first + e < total) {
+            if constexpr (ES == 4)
+              reinterpret_cast<int*>(o)[e] = v[e];
+            else
+              reinterpret_cast<uint16_t*>(o)[e] = (uint16_t)((uint32_t)v[e >> 1] >> (16 * (e & 1)));
+          }
+      }
+    }
+  };
+  const uint32_t base = lane_base<I8, ROW, W>();
+  auto load = [&](char* buf, int c) { load_stage<I8, ROW, W, 8>((lds_char*)buf, w, c0 + c, 0, k); };
+  auto step = [&](const char* buf, int c) {
+    if (c >= total) return;
+    i32x4 acc[FP];
+#pragma unroll
+    for (int f = 0; f < FP; ++f) {
+      acc[f] = i32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) acc[f] = mma<I8>(read_frag<I8, ROW, W>((const lds_char*)buf, base, f, kk), q[kk], acc[f]);
+    }
+#pragma unroll
+    for (int f = 0; f < FP; ++f) {
+      f32x4 v;
+      if (far) {  // |sum| < 2^31, times s it may pass the largest float though the score does not: in 64 bits
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (float)((double)acc[f][e] * sq * t[f][e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (float)acc[f][e] * sq * t[f][e];
+      }
+      if constexpr (TO == F32) {
+        struct __attribute__((packed, aligned(4))) Out {
+          f32x4 v;
+        };
+        ((__attribute__((address_space(3))) Out*)(mine + f * 16 * ES))->v = v;
+      } else {
+        struct __attribute__((packed, aligned(2))) Out {
+          i32x2 v;
+        };
+        i32x2 b;
+        if constexpr (TO == BF16)
+          b = __builtin_bit_cast(i32x2, __builtin_convertvector(v, bf16x4));
+        else
+          b = __builtin_bit_cast(i32x2, __builtin_convertvector(v, f16x4));
+        ((__attribute__((address_space(3))) Out*)(mine + f * 16 * ES))->v = b;
+      }
+    }
+    scales(min(c + W, total - 1));
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    emit(c);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // the last line, not yet whole, becomes the first
+      lds_char* const r = lds + (i * 8 + (lane >> 3)) * PITCH + (lane & 7) * 16;
+      *(__attribute__((address_space(3))) i32x4*)r = *(const __attribute__((address_space(3))) i32x4*)(r + LINES * 128);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  load(s_p, 0);
+  scales(0);
+  int c = 0;
+  for (; c < total; c += 2 * W) {  // rows past the catalogue's end and steps past the strip's copy zeros, or are not taken
+    stage_barrier();
+    load(s_q, c + W);
+    step(s_p, c);
+    stage_barrier();
+    load(s_p, c + 2 * W);
+    step(s_q, c + W);
+  }
+  emit((total + W - 1) / W * W);  // what the carried line holds
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // nothing in flight towards LDS when the workgroup ends
+}
+
 int64_t div_up(int64_t v, int64_t by) { return (v + by - 1) / by; }
 int64_t up(int64_t v, int64_t to) { return div_up(v, to) * to; }
 
@@ -197,6 +342,19 @@ int scores(const Operand& w, const Operand& x, int k, const float* s, const floa
   const EpiScores<TO> epi = {(char*)out, ldo * size_of(TO), s, t, w.rows, x.rows};
   if (x.rows <= 32) return launch<TO, NarrowQ>(a, epi, st);
   if (k <= STAGE) {
+    // rows that do not begin at whole vectors: strips, once the outputs do not stay in the caches (30 MB of bf16: 20 us to
+    // k_outer8's 15; 60 MB: 28 to 30; 2 GB: 0.62 ms to 0.95; 4 GB of float32: 0.83 ms to 1.87)
+    if ((((uintptr_t)out | (uintptr_t)epi.ld) & 15) != 0 && x.rows * epi.ld >= 48ll << 20) {
+      constexpr int W = Strip<TO>::W;
+      const int64_t groups = div_up(x.rows, 128), all = div_up(w.rows, W);
+      const int64_t want = std::max<int64_t>(std::min<int64_t>(div_up(2560, groups), all / 4), 1);  // 10 workgroups a compute unit
+      const int64_t steps = std::min<int64_t>(div_up(all, want), (1 << 29) / W);  // a strip's columns are counted in 31 bits
+      const int64_t strips = div_up(all, steps);
+      BLP_CHECK(groups * strips <= 0x7fffffff, BLP_E_ARG, "scores8: too many tiles for one launch");
+      (k <= 64 ? k_strip8<TO, 1> : k_strip8<TO, 2>)<<<(unsigned)(groups * strips), 512, 0, st>>>(w, x, k, epi, (int)strips, (int)steps);
+      BLP_HIP(hipGetLastError());
+      return 0;
+    }
     Problem o = a;
     o.tiles_p = (int)div_up(w.rows, TO == F32 ? 64 : 128);
     o.tiles_q = (int)div_up(x.rows, 128);
@@ -280,6 +438,7 @@ extern "C" int blp_scores8(int device, void* stream, const int8_t* q, int64_t ld
   BLP_CHECK(out_type >= 0 && out_type <= 2, BLP_E_ARG, "scores8: type must be BLP_F32, BLP_BF16 or BLP_F16");
   BLP_CHECK(q && s && table && ts && out, BLP_E_ARG, "scores8: null pointer");
   BLP_CHECK(ldq >= k && ldt >= k && ldo >= cols, BLP_E_ARG, "scores8: a row stride is smaller than the row");
+  BLP_CHECK((uintptr_t)out % size_of(out_type) == 0, BLP_E_ARG, "scores8: out must be aligned to its elements");
   BLP_CHECK(std::max(ldq, ldt) <= (1 << 22), BLP_E_ARG, "scores8: row strides must be at most 2^22");
   const int64_t need = workspace(q, ldq, table, ldt, rows, cols, k);
   BLP_CHECK(need == 0 || (ws && ws_bytes >= need), BLP_E_ARG,

@@ -110,6 +110,45 @@ def test_scales_far_apart(gpu, m, n, k, out):
     check_scores(latent.int8_scores(q, s, p, t, dtype=getattr(torch, out)), q, s, p, t)
 
 
+@pytest.mark.parametrize("out", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("m,n,k", [(300, 90001, 50), (129, 210002, 128), (37, 700003, 64), (1000, 27004, 100)])
+def test_many_scores_in_rows_of_odd_lengths(gpu, m, n, k, out):
+    """Past 48 MB of outputs whose rows begin anywhere in a line."""
+    torch = _torch()
+    from blp import latent
+
+    g = torch.Generator(device="cuda").manual_seed(n)
+    q = torch.randint(-128, 128, (m, k), device="cuda", generator=g).to(torch.int8)
+    p = torch.randint(-128, 128, (n, k), device="cuda", generator=g).to(torch.int8)
+    s = torch.rand(m, device="cuda", generator=g) * 1e-3
+    t = torch.rand(n, device="cuda", generator=g) * 1e-2
+    s[1] = 2.0 ** 100
+    t[: n // 2] *= 2.0 ** -100 if out != "float16" else 1.0
+    got = latent.int8_scores(q, s, p, t, dtype=getattr(torch, out))
+    if out == "float16":  # row 1 passes its largest number
+        got, q, s = got[2:], q[2:], s[2:]
+    check_scores(got, q, s, p, t)
+
+
+def test_rows_of_odd_lengths_leave_their_surroundings(gpu):
+    """Into rows of a wider buffer: only the scores change."""
+    torch = _torch()
+    from blp import latent
+    from blp._lib import check, lib
+
+    m, n, k, ld = 140, 200001, 64, 200013
+    q, s = latent.quantize_rows(torch.randn(m, k, device="cuda"))
+    p, t = latent.quantize_rows(torch.randn(n, k, device="cuda"))
+    for dtype, code in ((torch.float32, 0), (torch.bfloat16, 1)):
+        want = latent.int8_scores(q, s, p, t, dtype=dtype)
+        buf = torch.full((m + 2, ld), 77.0, device="cuda", dtype=dtype)
+        check(lib().blp_scores8(0, torch.cuda.current_stream().cuda_stream, q.data_ptr(), k, s.data_ptr(), p.data_ptr(), k,
+                                t.data_ptr(), m, n, k, code, buf[1:, 5:].data_ptr(), ld, None, 0))
+        assert torch.equal(buf[1:-1, 5:5 + n], want)
+        buf[1:-1, 5:5 + n] = 77.0
+        assert bool((buf == 77.0).all())
+
+
 def test_longest_sums(gpu):
     """The largest k: sums next to 2^31."""
     torch = _torch()

@@ -115,6 +115,8 @@ def test_scores8_refuses():
                        ({"out": None}, "null"), ({"ldq": 15}, "stride"), ({"ldt": 15}, "stride"), ({"ldo": 2}, "stride"),
                        ({"ldq": (1 << 22) + 1}, "strides"), ({"k": 15}, "workspace"), ({"q": ONE + 1}, "workspace")):
         refused(scores(**args), what)
+    for type, out in ((0, ONE + 2), (1, ONE + 1), (2, ONE + 1)):
+        refused(scores(type=type, out=out), "aligned to its elements")
     assert scores(rows=0) == 0
 
 
