@@ -139,6 +139,46 @@ struct EpiScores {
   }
 };
 
+// A slice's sums of k as they are: part[slice][q][p].
+struct EpiSums {
+  int32_t* part;
+  int64_t ld, nq;  // elements; ld a multiple of 4
+  template <class S>
+  __device__ void run(i32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int slice, lds_char*) const {
+    const int lane = fresh_lane(), h = lane >> 4;
+    int32_t* base = part + (int64_t)slice * nq * ld;
+#pragma unroll
+    for (int j = 0; j < S::FQ; ++j) {
+      const int64_t q = q0 + j * 16 + (lane & 15);
+      if (q >= nq) continue;
+#pragma unroll
+      for (int i = 0; i < S::FP; ++i) {
+        const int64_t p = p0 + i * 16 + h * 4;
+        if (p < ld) *reinterpret_cast<i32x4*>(base + q * ld + p) = acc[i][j];
+      }
+    }
+  }
+};
+
+// The slices' sums as scores, four a thread.
+template <int TO>
+__global__ __launch_bounds__(256) void k_join8(const int32_t* __restrict__ part, int slices, int64_t ld, FastDiv per, EpiScores<TO> epi) {
+  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+  const int64_t row = per(i), p = ((int64_t)i - row * per.d) * 4;
+  if (row >= epi.nq) return;
+  i32x4 sum = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int s = 0; s < slices; ++s) sum += *reinterpret_cast<const i32x4*>(part + ((int64_t)s * epi.nq + row) * ld + p);
+  const double sq = epi.s[row];
+  char* at = epi.out + row * epi.ld + p * size_of(TO);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (p + e < epi.np) {
+      const float v = fabs(sq) > 0x1p96 ? (float)((double)sum[e] * sq * epi.t[p + e]) : (float)sum[e] * (float)sq * epi.t[p + e];
+      store1<TO>(at + e * size_of(TO), v);
+    }
+}
+
 // k up to 128: one stage, and the outputs are what counts. A workgroup of 8 waves, 16 rows and 16 FP columns each, in 32
 // KiB of LDS, so that three of them share a compute unit and some load and multiply while others store. Bound by the
 // stores: 10,000 x 100,000 bf16, 2.0 GB, 0.45 to 0.48 ms (4.2 to 4.4 TB/s; a fill reaches 6.8). Larger k go through
@@ -325,23 +365,63 @@ using Big = Shape<2, 4, 8, 4>;      // 256 x 256
 using Mid = Shape<2, 2, 4, 4>;      // 128 x 128
 using NarrowQ = Shape<4, 1, 4, 2>;  // 256 x 32
 
-template <int TO, class S>
-int launch(Problem a, EpiScores<TO> epi, hipStream_t st) {
+// The tiles of longer rows, and how many slices of k: a tile's stages take about 1 us each (large tiles: 1.8), its outputs
+// 2.5 stages; slices take one more launch and their sums' way through memory. 10 x 1,266 x 6,462: 5 tiles of 51 stages,
+// 52 us in one slice and 19 in 17, each with the packing of its rows.
+enum Tiles { NARROW, MID, BIG };
+struct Split {
+  Tiles tiles;
+  int n, stages;  // slices, stages of each
+  int64_t bytes;  // of their sums
+};
+Split split_of(int64_t rows, int64_t cols, int k) {
+  const int64_t stages = div_up(k, STAGE);
+  Split best = {MID, 1, (int)stages, 0};
+  // two stages of k: two small workgroups a compute unit, so that one's stores run beside the other's loads
+  if (rows <= 32)
+    best.tiles = NARROW;
+  else if (k > 2 * STAGE && div_up(cols, 256) * div_up(rows, 256) >= 192)
+    best.tiles = BIG;
+  const int64_t tiles = div_up(cols, best.tiles == MID ? 128 : 256) * div_up(rows, best.tiles == NARROW ? 32 : best.tiles == MID ? 128 : 256);
+  const int64_t slots = best.tiles == BIG ? 256 : 512;
+  double least = -1;
+  for (int64_t n = 1; n <= 32 && n * tiles <= slots && n <= std::max<int64_t>(stages / 2, 1); ++n) {
+    const int64_t each = div_up(stages, n), slices = div_up(stages, each), bytes = slices * rows * up(cols, 4) * 4;
+    const double cost = ((double)each + 2.5) * (best.tiles == BIG ? 1.8 : 1.0) + (slices > 1 ? 4.0 + 2.0 * bytes / 4e6 : 0.0);
+    if (least < 0 || cost < least) {
+      least = cost;
+      best.n = (int)slices;
+      best.stages = (int)each;
+      best.bytes = slices > 1 ? bytes : 0;
+    }
+  }
+  return best;
+}
+
+template <class S, class Epi>
+int launch(Problem a, int slices, int stages, Epi epi, hipStream_t st) {
   const int64_t tp = div_up(a.p.rows, S::BP), tq = div_up(a.q.rows, S::BQ);
   BLP_CHECK(tp * tq <= 0x7fffffff, BLP_E_ARG, "scores8: too many tiles for one launch");
   a.tiles_p = (int)tp;
   a.tiles_q = (int)tq;
-  k_product<I8, ROW, ROW, false, S, EpiScores<TO>><<<(unsigned)std::min<int64_t>(tp * tq, S::BP == 256 && S::BQ == 256 ? 256 : 512), S::THREADS, 0, st>>>(a, epi);
+  a.slice = stages;
+  const dim3 grid((unsigned)std::min<int64_t>(tp * tq, S::BP == 256 && S::BQ == 256 ? 256 : 512), (unsigned)slices);
+  k_product<I8, ROW, ROW, false, S, Epi><<<grid, S::THREADS, 0, st>>>(a, epi);
   BLP_HIP(hipGetLastError());
   return 0;
 }
+template <class Epi>
+int launch(const Problem& a, const Split& s, Epi epi, hipStream_t st) {
+  if (s.tiles == NARROW) return launch<NarrowQ>(a, s.n, s.stages, epi, st);
+  if (s.tiles == BIG) return launch<Big>(a, s.n, s.stages, epi, st);
+  return launch<Mid>(a, s.n, s.stages, epi, st);
+}
 
 template <int TO>
-int scores(const Operand& w, const Operand& x, int k, const float* s, const float* t, void* out, int64_t ldo, hipStream_t st) {
+int scores(const Operand& w, const Operand& x, int k, const float* s, const float* t, void* out, int64_t ldo, char* ws, hipStream_t st) {
   const Problem a = {w, x, k, (int)div_up(k, STAGE), 0, 0, 0, 0};
   const EpiScores<TO> epi = {(char*)out, ldo * size_of(TO), s, t, w.rows, x.rows};
-  if (x.rows <= 32) return launch<TO, NarrowQ>(a, epi, st);
-  if (k <= STAGE) {
+  if (k <= STAGE && x.rows > 32) {
     // rows that do not begin at whole vectors: strips, once the outputs do not stay in the caches (30 MB of bf16: 20 us to
     // k_outer8's 15; 60 MB: 28 to 30; 2 GB: 0.62 ms to 0.95; 4 GB of float32: 0.83 ms to 1.87)
     if ((((uintptr_t)out | (uintptr_t)epi.ld) & 15) != 0 && x.rows * epi.ld >= 48ll << 20) {
@@ -363,9 +443,14 @@ int scores(const Operand& w, const Operand& x, int k, const float* s, const floa
     BLP_HIP(hipGetLastError());
     return 0;
   }
-  // two stages of k: two small workgroups a compute unit, so that one's stores run beside the other's loads
-  if (k > 2 * STAGE && div_up(w.rows, 256) * div_up(x.rows, 256) >= 192) return launch<TO, Big>(a, epi, st);
-  return launch<TO, Mid>(a, epi, st);
+  const Split split = split_of(x.rows, w.rows, k);
+  if (split.n == 1) return launch(a, split, epi, st);
+  const int64_t ld = up(w.rows, 4);
+  const int rc = launch(a, split, EpiSums{(int32_t*)ws, ld, x.rows}, st);
+  if (rc) return rc;
+  k_join8<TO><<<(unsigned)div_up(x.rows * ld / 4, 256), 256, 0, st>>>((const int32_t*)ws, split.n, ld, FastDiv((uint32_t)(ld / 4)), epi);
+  BLP_HIP(hipGetLastError());
+  return 0;
 }
 
 bool whole(const void* p, int64_t ld, int k) { return (((uintptr_t)p | (uintptr_t)ld | (uintptr_t)k) & 15) == 0; }
@@ -379,7 +464,7 @@ int check_args(int64_t rows, int64_t cols, int k) {
 
 int64_t workspace(const void* q, int64_t ldq, const void* p, int64_t ldp, int64_t rows, int64_t cols, int k) {
   const int64_t kp = up(k, 16);
-  return (whole(q, ldq, k) ? 0 : up(rows * kp, 256)) + (whole(p, ldp, k) ? 0 : up(cols * kp, 256));
+  return (whole(q, ldq, k) ? 0 : up(rows * kp, 256)) + (whole(p, ldp, k) ? 0 : up(cols * kp, 256)) + split_of(rows, cols, k).bytes;
 }
 
 int pack(Operand& o, int k, char*& ws, hipStream_t st) {
@@ -453,7 +538,7 @@ extern "C" int blp_scores8(int device, void* stream, const int8_t* q, int64_t ld
   if (!rc && !whole(table, ldt, k)) rc = pack(w, k, at, st);
   if (rc) return rc;
   const int kp = (int)up(k, 16);
-  if (out_type == F32) return scores<F32>(w, x, kp, s, ts, out, ldo, st);
-  if (out_type == BF16) return scores<BF16>(w, x, kp, s, ts, out, ldo, st);
-  return scores<F16>(w, x, kp, s, ts, out, ldo, st);
+  if (out_type == F32) return scores<F32>(w, x, kp, s, ts, out, ldo, at, st);
+  if (out_type == BF16) return scores<BF16>(w, x, kp, s, ts, out, ldo, at, st);
+  return scores<F16>(w, x, kp, s, ts, out, ldo, at, st);
 }

@@ -149,6 +149,24 @@ def test_rows_of_odd_lengths_leave_their_surroundings(gpu):
         assert bool((buf == 77.0).all())
 
 
+@pytest.mark.parametrize("out", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("m,n,k", [(10, 1266, 6462), (1, 3, 5000), (100, 1001, 4100), (321, 2047, 6120), (40, 513, 272), (1, 40001, 513)])
+def test_long_rows_of_few_tiles(gpu, m, n, k, out):
+    """Where k is taken in slices, whose sums are joined."""
+    torch = _torch()
+    from blp import latent
+
+    g = torch.Generator(device="cuda").manual_seed(k)
+    q = torch.randint(-128, 128, (m, k), device="cuda", generator=g).to(torch.int8)
+    p = torch.randint(-128, 128, (n, k), device="cuda", generator=g).to(torch.int8)
+    s = torch.rand(m, device="cuda", generator=g) * 1e-3
+    t = torch.rand(n, device="cuda", generator=g) * 1e-2
+    if out != "float16":
+        s[-1] = 2.0 ** 110
+        t[n // 2:] *= 2.0 ** -110
+    check_scores(latent.int8_scores(q, s, p, t, dtype=getattr(torch, out)), q, s, p, t)
+
+
 def test_longest_sums(gpu):
     """The largest k: sums next to 2^31."""
     torch = _torch()
