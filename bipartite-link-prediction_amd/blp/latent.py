@@ -82,8 +82,8 @@ def _floats(t, what, device, shapes):
             what, " or ".join(str(tuple(x)) for x in shapes), device, _say(t)))
 
 
-def _bytes(device, n):
-    return _torch.empty(n, dtype=_torch.uint8, device=device)
+def _bytes(like, n):
+    return like.new_empty(n, dtype=_torch.uint8)
 
 
 _REDUCTIONS = ("mean", "sum", "none")
@@ -122,15 +122,14 @@ def _loss_forward(x, table, target, scale, reduction, grads, keep=False):
     need = _loss_workspace(x, ldx, table, ldt, 1, grads)
     summed = reduction != "none"
     # what the caller does not get lies behind the workspace: the rows' lse, and their losses where they are summed up
-    ws = _bytes(device, need + 8 * m)
+    ws = _bytes(x, need + 8 * m)
     tail = ws.data_ptr() + need
-    lse = _torch.empty(m, dtype=_torch.float32, device=device) if keep else None
-    total = _torch.empty(2, dtype=_torch.float32, device=device) if summed else None
-    loss = None if summed else _torch.empty(m, dtype=_torch.float32, device=device)
+    lse = x.new_empty(m, dtype=_torch.float32) if keep else None
+    total = x.new_empty(2, dtype=_torch.float32) if summed else None
+    loss = None if summed else x.new_empty(m, dtype=_torch.float32)
     dx = dt = None
     if grads:
-        dx = _torch.empty((m, k), dtype=x.dtype, device=device)
-        dt = _torch.empty((table.shape[0], k), dtype=x.dtype, device=device)
+        dx, dt = x.new_empty(m, k), x.new_empty(table.shape[0], k)
     check(lib().blp_softmax_loss(
         device.index, _stream(device.index), _TYPES[x.dtype], x.data_ptr(), ldx, table.data_ptr(), ldt, target.data_ptr(), wide,
         m, table.shape[0], k, scale, tail + 4 * m if summed else loss.data_ptr(), lse.data_ptr() if keep else tail,
@@ -174,9 +173,9 @@ def softmax_loss_backward(grad, lse, count, x, table, target, scale=1.0, need_x=
     _floats(lse, "lse", device, ((m,),))
     if count is not None:
         _floats(count, "count", device, ((), (1,)))
-    dx = _torch.empty((m, k), dtype=x.dtype, device=device) if need_x else None
-    dt = _torch.empty((table.shape[0], k), dtype=x.dtype, device=device) if need_table else None
-    ws = _bytes(device, _loss_workspace(x, ldx, table, ldt, 0, 1))
+    dx = x.new_empty(m, k) if need_x else None
+    dt = x.new_empty(table.shape[0], k) if need_table else None
+    ws = _bytes(x, _loss_workspace(x, ldx, table, ldt, 0, 1))
     check(lib().blp_softmax_loss_backward(
         device.index, _stream(device.index), _TYPES[x.dtype], x.data_ptr(), ldx, table.data_ptr(), ldt, target.data_ptr(), wide,
         m, table.shape[0], k, scale, lse.data_ptr(), grad.data_ptr(), 1 if grad.numel() > 1 else 0,
@@ -210,7 +209,7 @@ def _lookup(table, ids, scale):
         raise ValueError("the table must have at least one row")
     device = table.device
     wide = _ids(ids, "ids", device)
-    out = _torch.empty((*ids.shape, k), dtype=table.dtype, device=device)
+    out = table.new_empty(*ids.shape, k)
     check(lib().blp_lookup(device.index, _stream(device.index), _TYPES[table.dtype], table.data_ptr(), ld, rows, k,
                            ids.data_ptr(), wide, ids.numel(), _scale(scale), out.data_ptr(), k))
     return out
@@ -236,7 +235,7 @@ def lookup_grad(grad, ids, n_rows, scale=1.0, into=None):
     if n_rows < 1:
         raise ValueError("n_rows must be at least 1")
     if into is None:
-        out, ldo = torch.empty((n_rows, k), dtype=grad.dtype, device=grad.device), k
+        out, ldo = grad.new_empty(n_rows, k), k
     else:
         out, ldo = into, _rows(into, "into", (grad.dtype,))
         if tuple(into.shape) != (n_rows, k) or into.device != grad.device:
@@ -246,7 +245,7 @@ def lookup_grad(grad, ids, n_rows, scale=1.0, into=None):
             raise ValueError("into must not overlap grad")
     b = ctypes.c_int64(0)
     check(lib().blp_lookup_grad_workspace(_TYPES[grad.dtype], n, n_rows, k, ctypes.byref(b)))
-    ws = _bytes(grad.device, b.value)
+    ws = _bytes(grad, b.value)
     check(lib().blp_lookup_grad(grad.device.index, _stream(grad.device.index), _TYPES[grad.dtype], grad.data_ptr(), ld,
                                 ids.data_ptr(), wide, n, n_rows, k, _scale(scale), out.data_ptr(), ldo,
                                 0 if into is None else 1, ws.data_ptr(), ws.numel()))
@@ -262,8 +261,8 @@ def quantize_rows(x):
     n, k = x.shape
     device = x.device
     kp = (k + 15) // 16 * 16
-    q = _torch.empty((n, kp), dtype=_torch.int8, device=device)
-    s = _torch.empty(n, dtype=_torch.float32, device=device)
+    q = x.new_empty(n, kp, dtype=_torch.int8)
+    s = x.new_empty(n, dtype=_torch.float32)
     check(lib().blp_quantize_rows(device.index, _stream(device.index), _TYPES[x.dtype], x.data_ptr(), ld, n, k, q.data_ptr(),
                                   kp, s.data_ptr()))
     return (q if kp == k else q[:, :k]), s
@@ -291,11 +290,11 @@ def int8_scores(q, s, table_q, table_s, dtype=None):
         raise ValueError("the catalogue must have at least one row")
     _floats(s, "s", device, ((m,),))
     _floats(table_s, "table_s", device, ((n,),))
-    out = torch.empty((m, n), dtype=dtype, device=device)
+    out = q.new_empty(m, n, dtype=dtype)
     qp, tp = q.data_ptr(), table_q.data_ptr()
     b = ctypes.c_int64(0)
     check(lib().blp_scores8_workspace(qp, ldq, tp, ldt, m, n, k, ctypes.byref(b)))
-    ws = _bytes(device, b.value) if b.value else None
+    ws = _bytes(q, b.value) if b.value else None
     check(lib().blp_scores8(device.index, _stream(device.index), qp, ldq, s.data_ptr(), tp, ldt, table_s.data_ptr(), m, n, k,
                             _TYPES[dtype], out.data_ptr(), n, ws.data_ptr() if b.value else None, b.value))
     return out

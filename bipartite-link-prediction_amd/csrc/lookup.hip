@@ -245,7 +245,7 @@ __global__ __launch_bounds__(512) void k_place_small(Ids ids, int n, Entry* __re
 }
 
 // ---------------------------------------------------------------- sums
-constexpr int HEAVY = 16;  // chunks: a row that crosses more of them is added up by a whole block
+constexpr int HEAVY = 8;  // chunks: a row that crosses more of them is added up by a whole block
 
 template <int T>
 __device__ inline void put(char* out, int64_t ldo, uint32_t key, int e0, int k, const Vec<T>& sum, float scale, int add) {
@@ -412,7 +412,7 @@ __device__ inline Crossing crossing(const Sums& a, int64_t chunk, uint32_t* key)
 
 // The rows that cross chunks, in 64 bits. The first blocks, which last longest: HEAVY chunks each, in which one heavy row
 // can begin; its partial sums go to the groups of lanes in turn, then the groups' sums are added in order. The
-// others: a group of lanes a chunk, the partial sums of the row that begins there in the chunks' order. 14 us in the case
+// others: a group of lanes a chunk, the partial sums of the row that begins there in the chunks' order. 13 us in the case
 // above: six or seven waits for memory, one after the other.
 template <int T>
 __global__ __launch_bounds__(256) void k_join_chunks(Sums a, unsigned heavy_blocks) {
