@@ -176,6 +176,32 @@ def test_autograd_and_replay(gpu):
         assert torch.equal(out, latent.lookup_grad(grad, big, 100))
 
 
+@pytest.mark.parametrize("n,rows", [(20000, 700), (300000, 2500)])
+def test_long_lists_captured_and_replayed(gpu, n, rows):
+    torch = _torch()
+    from blp import latent
+
+    grad, ids = torch.randn(n, 20, device="cuda"), torch.randint(-1, rows, (n,), device="cuda")
+    into = torch.randn(rows, 20, device="cuda")
+    held = into.clone()
+
+    def step(into):
+        return latent.lookup_grad(grad, ids, rows, 0.5), latent.lookup_grad(grad, ids, rows, 0.5, into=into)
+
+    step(into.clone())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(into)
+    for i in range(4):
+        grad.normal_()
+        ids.copy_((torch.rand(n, device="cuda") ** 3 * (rows + 1)).long() - 1)
+        into.copy_(held)
+        graph.replay()
+        for p, q in zip(out, step(held.clone())):
+            assert torch.equal(p, q)
+
+
 def test_refusals(gpu):
     torch = _torch()
     from blp import latent

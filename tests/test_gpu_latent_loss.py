@@ -432,6 +432,57 @@ def test_captured_and_replayed(gpu):
                 assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("dtype,m,n,k", [("bfloat16", 600, 3000, 200), ("float32", 600, 1300, 40), ("float32", 300, 900, 100),
+                                         ("float16", 20, 3000, 500)])
+def test_every_path_captured_and_replayed(gpu, dtype, m, n, k):
+    """Forward and backward with row gradients, beside the step in one call; eager calls between the replays."""
+    torch = _torch()
+    from blp import latent
+
+    dtype = getattr(torch, dtype)
+    x, w, t = make(m, n, k, dtype, seed=1, ignored=0.1)
+    g = torch.randn(m, device="cuda")
+    lse = torch.logsumexp(x.float() @ w.float().t().contiguous(), 1)
+
+    def step():
+        return (latent.softmax_loss(x, w, t, reduction="none"), *latent.softmax_loss_grad(x, w, t, reduction="sum"),
+                *latent.softmax_loss_backward(g, lse, None, x, w, t, need_x=True))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        for dst, src in zip((x, w, t), make(m, n, k, dtype, seed=30 + i, ignored=0.1)):
+            dst.copy_(src)
+        g.normal_()
+        lse.copy_(torch.logsumexp(x.float() @ w.float().t().contiguous(), 1))
+        graph.replay()
+        for p, q in zip(out, step()):
+            assert torch.equal(p, q)
+
+
+def test_two_calls_at_once(gpu):
+    """The same step on two streams side by side, many times over: each call has its own workspace."""
+    torch = _torch()
+    from blp import latent
+
+    sets = [make(500, 2000, k, torch.bfloat16, seed=40 + k) for k in (64, 200)]
+    want = [latent.softmax_loss_grad(*a) for a in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[] for _ in sets]
+    for _ in range(20):
+        for s, a, to in zip(streams, sets, got):
+            with torch.cuda.stream(s):
+                to.append(latent.softmax_loss_grad(*a))
+    torch.cuda.synchronize()
+    for w, all_of in zip(want, got):
+        for out in all_of:
+            assert all(torch.equal(p, q) for p, q in zip(out, w))
+
+
 def test_refusals(gpu):
     torch = _torch()
     from blp import latent

@@ -222,6 +222,24 @@ def test_replayed(gpu):
         assert torch.equal(out, latent.int8_scores(*latent.quantize_rows(x), p, t))
 
 
+@pytest.mark.parametrize("m,n,k", [(10, 1266, 6462), (300, 90001, 64), (600, 3000, 300)])
+def test_every_path_replayed(gpu, m, n, k):
+    torch = _torch()
+    from blp import latent
+
+    x = torch.randn(m, k, device="cuda")
+    p, t = latent.quantize_rows(torch.randn(n, k, device="cuda"))
+    latent.int8_scores(*latent.quantize_rows(x), p, t, dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = latent.int8_scores(*latent.quantize_rows(x), p, t, dtype=torch.bfloat16)
+    for _ in range(4):
+        x.normal_()
+        graph.replay()
+        assert torch.equal(out, latent.int8_scores(*latent.quantize_rows(x), p, t, dtype=torch.bfloat16))
+
+
 def test_refusals(gpu):
     torch = _torch()
     from blp import latent
