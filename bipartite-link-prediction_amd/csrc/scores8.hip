@@ -102,7 +102,7 @@ __global__ __launch_bounds__(256) void k_pack8(const int8_t* __restrict__ src, i
 }
 
 // ---------------------------------------------------------------- scores
-template <int TO>
+template <int TO, bool STREAM = false>  // past the caches
 struct EpiScores {
   char* out;
   int64_t ld;  // bytes
@@ -125,7 +125,7 @@ struct EpiScores {
 #pragma unroll
     for (int j = 0; j < S::FQ; ++j) far |= fabsf(sq[j]) > 0x1p96f;
     far = __any(far);
-    store_block<TO, S, true>(scratch, out + q0 * ld + p0 * size_of(TO), ld, left, rows, [&](int i, int j) {
+    store_block<TO, S, STREAM>(scratch, out + q0 * ld + p0 * size_of(TO), ld, left, rows, [&](int i, int j) {
       f32x4 v;
       if (far) {  // |sum| < 2^31, times s it may pass the largest float though the score does not: in 64 bits
 #pragma unroll
@@ -187,8 +187,8 @@ template <int FP_>
 struct OuterShape : Shape<1, 8, FP_, 1> {
   static constexpr int SCRATCH = 4096;
 };
-template <int TO>
-__global__ __launch_bounds__(512, 6) void k_outer8(Problem a, EpiScores<TO> epi) {
+template <int TO, bool STREAM>
+__global__ __launch_bounds__(512, 6) void k_outer8(Problem a, EpiScores<TO, STREAM> epi) {
   using S = OuterShape<TO == F32 ? 4 : 8>;
   __shared__ __attribute__((aligned(1024))) char s_all[32768];
   int tp, tq;
@@ -213,8 +213,8 @@ __global__ __launch_bounds__(512, 6) void k_outer8(Problem a, EpiScores<TO> epi)
   epi.template run<S>(acc, p0, q0 + wave * 16, 0, 0, lp + wave * 4096);
 }
 
-// The same where rows of outputs do not begin at whole vectors: k_outer8's stores of 16 bytes would straddle lines and run at
-// half the rate (2.1 TB/s; this one: 3.2 in bf16, 4.8 in float32). A workgroup passes along a strip of columns, W of them a step, with its 128 rows of q in
+// The same where many rows of outputs do not begin at whole vectors: k_outer8's stores of 16 bytes straddle lines, 10,000 x
+// 99,998 take 0.95 ms past the caches, 0.67 through them and 0.62 here (float32: 1.87, 1.01 and 0.83). A workgroup passes along a strip of columns, W of them a step, with its 128 rows of q in
 // registers; the scores go through LDS, where row r begins at its place within its line, so that LINES whole lines of
 // every row leave, aligned, a step; what is left of the last one is carried to the next step. Only a strip's ends are
 // partial lines.
@@ -420,11 +420,15 @@ int launch(const Problem& a, const Split& s, Epi epi, hipStream_t st) {
 template <int TO>
 int scores(const Operand& w, const Operand& x, int k, const float* s, const float* t, void* out, int64_t ldo, char* ws, hipStream_t st) {
   const Problem a = {w, x, k, (int)div_up(k, STAGE), 0, 0, 0, 0};
+  // Outputs that the last-level cache holds (256 MB) are written to it, and so are rows that do not begin at whole vectors,
+  // whose lines meet there; others go past it. 3,000 x 20,001 x 500 bf16, 0.12 GB: 74 us, past it 89; 12,000 x 16,001 x 144,
+  // 0.38 GB: 160 and 290; 10,000 x 100,000 x 64, 2 GB: 659 and 492.
+  const bool vectors = (((uintptr_t)out | (uintptr_t)(ldo * size_of(TO))) & 15) == 0, large = x.rows * ldo * size_of(TO) > 256ll << 20;
   const EpiScores<TO> epi = {(char*)out, ldo * size_of(TO), s, t, w.rows, x.rows};
+  const EpiScores<TO, true> past = {epi.out, epi.ld, s, t, w.rows, x.rows};
   if (k <= STAGE && x.rows > 32) {
-    // rows that do not begin at whole vectors: strips, once the outputs do not stay in the caches (30 MB of bf16: 20 us to
-    // k_outer8's 15; 60 MB: 28 to 30; 2 GB: 0.62 ms to 0.95; 4 GB of float32: 0.83 ms to 1.87)
-    if ((((uintptr_t)out | (uintptr_t)epi.ld) & 15) != 0 && x.rows * epi.ld >= 48ll << 20) {
+    // 0.24 GB of bf16 take 81 us in strips and 62 without, 0.4 GB 134 and 150, 0.48 GB of float32 110 and 134
+    if (!vectors && large) {
       constexpr int W = Strip<TO>::W;
       const int64_t groups = div_up(x.rows, 128), all = div_up(w.rows, W);
       const int64_t want = std::max<int64_t>(std::min<int64_t>(div_up(2560, groups), all / 4), 1);  // 10 workgroups a compute unit
@@ -439,12 +443,16 @@ int scores(const Operand& w, const Operand& x, int k, const float* s, const floa
     o.tiles_p = (int)div_up(w.rows, TO == F32 ? 64 : 128);
     o.tiles_q = (int)div_up(x.rows, 128);
     BLP_CHECK((int64_t)o.tiles_p * o.tiles_q <= 0x7fffffff, BLP_E_ARG, "scores8: too many tiles for one launch");
-    k_outer8<TO><<<(unsigned)(o.tiles_p * o.tiles_q), 512, 0, st>>>(o, epi);
+    const unsigned grid = (unsigned)(o.tiles_p * o.tiles_q);
+    if (large)
+      k_outer8<TO, true><<<grid, 512, 0, st>>>(o, past);
+    else
+      k_outer8<TO, false><<<grid, 512, 0, st>>>(o, epi);
     BLP_HIP(hipGetLastError());
     return 0;
   }
   const Split split = split_of(x.rows, w.rows, k);
-  if (split.n == 1) return launch(a, split, epi, st);
+  if (split.n == 1) return vectors && large ? launch(a, split, past, st) : launch(a, split, epi, st);
   const int64_t ld = up(w.rows, 4);
   const int rc = launch(a, split, EpiSums{(int32_t*)ws, ld, x.rows}, st);
   if (rc) return rc;

@@ -111,9 +111,10 @@ def test_scales_far_apart(gpu, m, n, k, out):
 
 
 @pytest.mark.parametrize("out", ["float32", "bfloat16", "float16"])
-@pytest.mark.parametrize("m,n,k", [(300, 90001, 50), (129, 210002, 128), (37, 700003, 64), (1000, 27004, 100)])
+@pytest.mark.parametrize("m,n,k", [(300, 90001, 50), (129, 210002, 128), (37, 700003, 64), (1000, 27004, 100),
+                                   (1400, 100001, 50), (130, 1100002, 128)])
 def test_many_scores_in_rows_of_odd_lengths(gpu, m, n, k, out):
-    """Past 48 MB of outputs whose rows begin anywhere in a line."""
+    """Rows that begin anywhere in a line, in outputs that the caches hold and past their 256 MB."""
     torch = _torch()
     from blp import latent
 
@@ -130,13 +131,14 @@ def test_many_scores_in_rows_of_odd_lengths(gpu, m, n, k, out):
     check_scores(got, q, s, p, t)
 
 
-def test_rows_of_odd_lengths_leave_their_surroundings(gpu):
+@pytest.mark.parametrize("m", [140, 700])
+def test_rows_of_odd_lengths_leave_their_surroundings(gpu, m):
     """Into rows of a wider buffer: only the scores change."""
     torch = _torch()
     from blp import latent
     from blp._lib import check, lib
 
-    m, n, k, ld = 140, 200001, 64, 200013
+    n, k, ld = 200001, 64, 200013
     q, s = latent.quantize_rows(torch.randn(m, k, device="cuda"))
     p, t = latent.quantize_rows(torch.randn(n, k, device="cuda"))
     for dtype, code in ((torch.float32, 0), (torch.bfloat16, 1)):
@@ -222,7 +224,7 @@ def test_replayed(gpu):
         assert torch.equal(out, latent.int8_scores(*latent.quantize_rows(x), p, t))
 
 
-@pytest.mark.parametrize("m,n,k", [(10, 1266, 6462), (300, 90001, 64), (600, 3000, 300)])
+@pytest.mark.parametrize("m,n,k", [(10, 1266, 6462), (300, 90001, 64), (600, 3000, 300), (1400, 100001, 64)])
 def test_every_path_replayed(gpu, m, n, k):
     torch = _torch()
     from blp import latent
