@@ -126,7 +126,7 @@ def test_large_tiles(gpu, m, n, k, dtype):
 
 @pytest.mark.parametrize("dtype,m,n,k", [("float32", 12000, 24011, 20), ("float32", 9000, 24011, 72), ("bfloat16", 16000, 20011, 136)])
 def test_pieces_of_the_catalogue(gpu, dtype, m, n, k):
-    """More scores than one workspace piece holds (512 MiB: 268M halves, 89M floats of three halves), and as many where
+    """More scores than one workspace piece holds (256 MiB: 134M halves, 45M floats of three halves), and as many where
     nothing is kept."""
     torch = _torch()
     from blp import latent
