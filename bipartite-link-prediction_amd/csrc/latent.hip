@@ -211,12 +211,11 @@ __device__ inline void take_total(const float* loss, const Targets& targets, int
   __shared__ int64_t s_n[THREADS / 64];
   double sum = 0.0;
   int64_t n = 0;
-#pragma unroll 4
-  for (int64_t i = threadIdx.x; i < m; i += THREADS)
-    if (targets(i) >= 0) {
-      sum += loss[i];
-      ++n;
-    }
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < m; i += THREADS) {  // the losses of ignored rows are 0
+    sum += loss[i];
+    n += targets(i) >= 0;
+  }
   for (int o = 32; o; o >>= 1) {
     sum += __shfl_xor(sum, o, 64);
     n += __shfl_xor(n, o, 64);
@@ -321,11 +320,11 @@ __global__ __launch_bounds__(1024) void k_top_grad(const float* __restrict__ g, 
                                                    float* __restrict__ top) {
   __shared__ float s_top[16];
   float t = -1.f;
-  for (int64_t i = threadIdx.x; i < m; i += 1024)
-    if (targets(i) >= 0) {
-      const float v = fabsf(g[i]);
-      if (v <= FLT_MAX) t = fmaxf(t, v);
-    }
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < m; i += 1024) {
+    const float v = fabsf(g[i]);
+    t = targets(i) >= 0 && v <= FLT_MAX ? fmaxf(t, v) : t;
+  }
   for (int o = 32; o; o >>= 1) t = fmaxf(t, __shfl_xor(t, o, 64));
   if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = t;
   __syncthreads();
