@@ -944,21 +944,40 @@ constexpr int64_t PAIR_BYTES = 256ll << 20;   // the forward pass's pairs of the
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int64_t div_up(int64_t v, int64_t by) { return (v + by - 1) / by; }
 
-enum ShapeId { BIG, MID, FLAT };
+enum ShapeId { BIG, MID, FLAT, THIN };
 using Big = Shape<2, 4, 8, 4>;   // 256 x 256, one workgroup a compute unit
 using Mid = Shape<2, 2, 4, 4>;   // 128 x 128, two
 using Flat = Shape<4, 1, 4, 2>;  // 256 x 32, two: few rows
-constexpr int BP_OF[] = {256, 128, 256}, BQ_OF[] = {256, 128, 32}, WP_OF[] = {2, 2, 4}, PER_CU[] = {1, 2, 2};
+using Thin = Shape<4, 1, 1, 2>;  // 64 x 32, four: few tiles
+constexpr int BP_OF[] = {256, 128, 256, 64}, BQ_OF[] = {256, 128, 32, 32}, WP_OF[] = {2, 2, 4, 4}, PER_CU[] = {1, 2, 2, 4};
 
 int64_t tiles_of(int shape, int64_t np, int64_t nq) { return div_up(np, BP_OF[shape]) * div_up(nq, BQ_OF[shape]); }
 
-// The shape whose rounds of tiles over the card cost least. A stage of a tile takes 1.55 us in the large shape and, two
-// workgroups side by side, 1.2 us in the middle one (8,192 x 100,000 x 1,024 halves: 980 and 860 TFLOP/s); a tile's
-// outputs about as long as 2 1/2 stages. Up to 32 rows: 32 of them a tile, bound by reading the other operand.
+// A stage of every tile, in us: 1.55 a round of the large shape and, two workgroups side by side, 1.2 of the middle one
+// (8,192 x 100,000 x 1,024 halves: 980 and 860 TFLOP/s). Where there are few tiles a compute unit's way to memory counts, and
+// small ones on many of them are faster: 80 x 267 x 1,728 halves, 65 us a step in tiles of 128 x 128 and 42 in 64 x 32; 15 x
+// 3,344 x 240 floats, 73 us in 256 x 32 and 54; but 200 x 20,000 x 512 halves 78 and 96.
+double stage_us(int shape, int64_t tiles) {
+  const int64_t slots = 256 * PER_CU[shape], each = std::min<int64_t>(div_up(tiles, 256), PER_CU[shape]);
+  static const double thin[] = {0.4, 0.55, 0.75, 1.0};
+  return (double)div_up(tiles, slots) * (shape == BIG ? 1.55 : shape == THIN ? thin[each - 1] : each > 1 ? 1.2 : 0.8);
+}
+// Up to 32 rows: tiles of 32.
+bool fits(int shape, int64_t nq) { return shape == THIN || (shape == FLAT) == (nq <= 32); }
+
+// The shape whose rounds of tiles over the card cost least.
 int shape_of(int64_t np, int64_t nq) {
-  if (nq <= 32) return FLAT;
-  const double big = (double)div_up(tiles_of(BIG, np, nq), 256) * 1.55, mid = (double)div_up(tiles_of(MID, np, nq), 512) * 1.2;
-  return big <= mid ? BIG : MID;
+  int best = FLAT;
+  double least = -1;
+  for (int shape : {BIG, MID, FLAT, THIN}) {
+    if (!fits(shape, nq)) continue;
+    const double cost = stage_us(shape, std::max<int64_t>(tiles_of(shape, np, nq), 1));
+    if (least < 0 || cost < least) {
+      least = cost;
+      best = shape;
+    }
+  }
+  return best;
 }
 
 struct Layout {
@@ -979,14 +998,14 @@ Slices slices_of(int64_t np, int64_t nq, int64_t k, int planes) {
   const int64_t stages = div_up(k, STAGE / 2) * (planes == 1 ? 1 : SEGMENTS);
   Slices best = {FLAT, 1, (int)stages};
   double least = -1;
-  for (int shape : {BIG, MID, FLAT}) {
-    if ((shape == FLAT) != (nq <= 32)) continue;
+  for (int shape : {BIG, MID, FLAT, THIN}) {
+    if (!fits(shape, nq)) continue;
     const int64_t tiles = std::max<int64_t>(tiles_of(shape, np, nq), 1), slots = 256 * PER_CU[shape];
     int64_t n = std::min<int64_t>(std::max<int64_t>(std::min(slots / tiles, stages / 4), 1), 64);
     const int64_t each = std::max<int64_t>(div_up(stages, n), 1);
     n = std::max<int64_t>(div_up(stages, each), 1);
-    // rounds of tiles, a tile's stages and its outputs
-    const double cost = (double)div_up(tiles * n, slots) * ((double)each + 2.5) * (shape == BIG ? 1.55 : 1.2);
+    // a tile's stages, and its outputs, which take about as long as 2 1/2 of them
+    const double cost = ((double)each + 2.5) * stage_us(shape, tiles * n);
     if (least < 0 || cost < least) {
       least = cost;
       best = {shape, (int)n, (int)each};
@@ -1115,14 +1134,16 @@ int product(int shape, Problem a, int slices, int stages, Epi epi, hipStream_t s
   a.tiles_p = (int)tp;
   a.tiles_q = (int)tq;
   a.slice = stages ? stages : (int)div_up(a.k, KE) * (T == F32 ? SEGMENTS : 1);
-  // one or two workgroups a compute unit, which take tile after tile
+  // as many workgroups as fit the card, which take tile after tile
   const dim3 grid((unsigned)std::min<int64_t>(tp * tq, 256 * PER_CU[shape]), (unsigned)slices);
   if (shape == BIG)
     launch<T, LP, LQ, Big>(a, grid, epi, st);
   else if (shape == MID)
     launch<T, LP, LQ, Mid>(a, grid, epi, st);
-  else
+  else if (shape == FLAT)
     launch<T, LP, LQ, Flat>(a, grid, epi, st);
+  else
+    launch<T, LP, LQ, Thin>(a, grid, epi, st);
   BLP_HIP(hipGetLastError());
   return 0;
 }

@@ -82,7 +82,8 @@ struct Shape {
   static constexpr int WAVES = WP * WQ, THREADS = WAVES * 64;
   static constexpr int BP = WP * FP * 16, BQ = WQ * FQ * 16;
   static constexpr int STAGE_BYTES = (BP + BQ) * 128;
-  static constexpr int SCRATCH = STAGE_BYTES / WAVES / 4096 * 4096;  // LDS for a wave's outputs
+  static constexpr int SHARE = STAGE_BYTES / WAVES, UNIT = SHARE < 4096 ? 1024 : 4096;
+  static constexpr int SCRATCH = SHARE / UNIT * UNIT;  // LDS for a wave's outputs
 };
 
 typedef __attribute__((address_space(3))) char lds_char;
