@@ -461,7 +461,17 @@ int scores(const Operand& w, const Operand& x, int k, const float* s, const floa
   return 0;
 }
 
-bool whole(const void* p, int64_t ld, int k) { return (((uintptr_t)p | (uintptr_t)ld | (uintptr_t)k) & 15) == 0; }
+// Which operands are packed: those whose rows do not begin at whole granules, and, where k ends inside a granule, one of
+// them at least (the shorter): zeros past its k make what the other holds there count for nothing. (A granule that begins
+// inside a row ends on the same page.)
+struct Packed {
+  bool x, w;
+};
+Packed packed(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t cols, int k) {
+  Packed p = {(((uintptr_t)x | (uintptr_t)ldx) & 15) != 0, (((uintptr_t)w | (uintptr_t)ldw) & 15) != 0};
+  if (k % 16 && !p.x && !p.w) (rows <= cols ? p.x : p.w) = true;
+  return p;
+}
 
 int check_args(int64_t rows, int64_t cols, int k) {
   BLP_CHECK(rows >= 0 && rows < (1ll << 31) && cols >= 1 && cols < (1ll << 31), BLP_E_ARG,
@@ -472,7 +482,8 @@ int check_args(int64_t rows, int64_t cols, int k) {
 
 int64_t workspace(const void* q, int64_t ldq, const void* p, int64_t ldp, int64_t rows, int64_t cols, int k) {
   const int64_t kp = up(k, 16);
-  return (whole(q, ldq, k) ? 0 : up(rows * kp, 256)) + (whole(p, ldp, k) ? 0 : up(cols * kp, 256)) + split_of(rows, cols, k).bytes;
+  const Packed pack = packed(q, ldq, p, ldp, rows, cols, k);
+  return (pack.x ? up(rows * kp, 256) : 0) + (pack.w ? up(cols * kp, 256) : 0) + split_of(rows, cols, k).bytes;
 }
 
 int pack(Operand& o, int k, char*& ws, hipStream_t st) {
@@ -542,8 +553,9 @@ extern "C" int blp_scores8(int device, void* stream, const int8_t* q, int64_t ld
   hipStream_t st = (hipStream_t)stream;
   char* at = (char*)ws;
   Operand x = {(const char*)q, ldq, rows}, w = {(const char*)table, ldt, cols};
-  if (!whole(q, ldq, k)) rc = pack(x, k, at, st);
-  if (!rc && !whole(table, ldt, k)) rc = pack(w, k, at, st);
+  const Packed packs = packed(q, ldq, table, ldt, rows, cols, k);
+  if (packs.x) rc = pack(x, k, at, st);
+  if (!rc && packs.w) rc = pack(w, k, at, st);
   if (rc) return rc;
   const int kp = (int)up(k, 16);
   if (out_type == F32) return scores<F32>(w, x, kp, s, ts, out, ldo, at, st);

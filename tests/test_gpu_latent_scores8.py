@@ -169,6 +169,22 @@ def test_long_rows_of_few_tiles(gpu, m, n, k, out):
     check_scores(latent.int8_scores(q, s, p, t, dtype=getattr(torch, out)), q, s, p, t)
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 700, 50), (5, 700, 50), (700, 60, 50), (40, 3000, 201), (300, 301, 1001), (9, 1266, 6462),
+                                   (1400, 100001, 50)])
+def test_rows_end_inside_a_granule_of_anything(gpu, m, n, k):
+    """k not a multiple of 16, rows that begin at whole granules, anything in the bytes behind them."""
+    torch = _torch()
+    from blp import latent
+
+    g = torch.Generator(device="cuda").manual_seed(k)
+    wide = (k + 15) // 16 * 16
+    q = torch.randint(-128, 128, (m, wide), device="cuda", generator=g).to(torch.int8)[:, :k]
+    p = torch.randint(-128, 128, (n, wide + 16), device="cuda", generator=g).to(torch.int8)[:, :k]
+    s = torch.rand(m, device="cuda", generator=g) * 1e-3
+    t = torch.rand(n, device="cuda", generator=g) * 1e-2
+    check_scores(latent.int8_scores(q, s, p, t), q, s, p, t)
+
+
 def test_longest_sums(gpu):
     """The largest k: sums next to 2^31."""
     torch = _torch()
