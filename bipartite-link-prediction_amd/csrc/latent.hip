@@ -840,7 +840,8 @@ __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowAr
     }
   };
 
-  // Three buffers, two stages ahead (floats: two, one ahead). Stages past the range copy zeros and are not computed, so every trip takes all buffers and the counts of outstanding copies stay the same.
+  // Three buffers, two stages ahead (floats: two, one ahead). Stages past the range copy zeros and are not computed, so
+  // every trip takes all buffers and the counts of outstanding copies stay the same.
   load(s_a, s_ra, 0);
   if constexpr (THREE) {
     load(s_b, s_rb, 1);
@@ -1275,9 +1276,11 @@ int forward(const Call& c, float* loss, float* lse, Total total, uint32_t* done)
       const Rows rows = {p.narrow && p.grads ? (float*)(c.ws + p.o_rows) : nullptr};
       const int64_t all = rows.at ? up(m, 64) : m;
       if (m >= 4096)
-        k_join<32><<<(unsigned)div_up(all, 32), 256, 0, c.st>>>(part, pairs, m, hit, targets, loss + r0, lse + r0, rows, extra_of(T), total, done);
+        k_join<32><<<(unsigned)div_up(all, 32), 256, 0, c.st>>>(part, pairs, m, hit, targets, loss + r0, lse + r0, rows,
+                                                                extra_of(T), total, done);
       else
-        k_join<4><<<(unsigned)div_up(all, 4), 256, 0, c.st>>>(part, pairs, m, hit, targets, loss + r0, lse + r0, rows, extra_of(T), total, done);
+        k_join<4><<<(unsigned)div_up(all, 4), 256, 0, c.st>>>(part, pairs, m, hit, targets, loss + r0, lse + r0, rows,
+                                                              extra_of(T), total, done);
       BLP_HIP(hipGetLastError());
     }
   }

@@ -24,8 +24,9 @@ struct __attribute__((packed, aligned(1))) Unaligned4 {
 
 // ---------------------------------------------------------------- quantising
 // x / s rounded to nearest, halves to even -- of the true quotient, not of its 32-bit rounding: the first
-// guess is off by one at most (a division: 1 / s may not be a number of 32 bits), and x - q s is exact in an fma (both are multiples of the smaller last
-// place of x and s, and the difference is at most s), so comparing it with s / 2 settles the guess.
+// guess is off by one at most (a division: 1 / s may not be a number of 32 bits), and x - q s is exact in an fma (both are
+// multiples of the smaller last place of x and s, and the difference is about s / 2 at most), so comparing it with s / 2
+// settles the guess.
 __device__ inline int to8(float x, float s) {
   float q = rintf(x / s);
   const float r = fmaf(-q, s, x), half = 0.5f * s;
@@ -35,11 +36,11 @@ __device__ inline int to8(float x, float s) {
   return (int)fminf(fmaxf(q, -127.f), 127.f);
 }
 
-// `lanes` (a power of two up to 64) lanes a row, one 16-byte vector each a step; two passes over the row, the
-// second out of the cache. Bytes [k, kp) of a row are set to zero. A row with a NaN or an infinity gets the
-// scale NaN and zeros, so its scores are NaN; a row of zeros the scale 0. Bound by reading x: 4,096 and 16,384 rows of 4,096 bf16 together
-// 23 us, 0.25 GB moved, part of it from the caches.
-template <int T>
+// `lanes` (a power of two up to 64) lanes a row, one 16-byte vector each a step. HELD steps (1 or 8) stay in registers between
+// the maximum and the rounding; longer rows (0) are read twice, the second time out of the cache. Bytes [k, kp) of a row are
+// set to zero. A row with a NaN or an infinity gets the scale NaN and zeros, so its scores are NaN; a row of zeros the scale
+// 0. Bound by reading x: 4,096 rows of 4,096 bf16 18 us, half of it arithmetic.
+template <int T, int HELD>
 __global__ __launch_bounds__(256) void k_quantize(const char* __restrict__ x, int64_t ld, int64_t rows, int k, int kp, int lanes,
                                                   int8_t* __restrict__ q, int64_t ldq, float* __restrict__ s) {
   constexpr int ES = size_of(T), NE = Vec<T>::NE;
@@ -48,27 +49,47 @@ __global__ __launch_bounds__(256) void k_quantize(const char* __restrict__ x, in
   if (row >= rows) return;
   const char* src = x + row * ld;
   uint32_t top = 0;
-#pragma unroll 4
-  for (int e0 = l * NE; e0 < k; e0 += lanes * NE) {
-    const Vec<T> v = load_vec<T>(src + (int64_t)e0 * ES, k - e0);
+  auto largest = [&](const Vec<T>& v) {
 #pragma unroll
     for (int e = 0; e < NE; ++e) top = max(top, __float_as_uint(fabsf(v.v[e >> 2][e & 3])));  // a NaN's bits are the largest
+  };
+  auto load = [&](int e0) { return e0 < k ? load_vec<T>(src + (int64_t)e0 * ES, k - e0) : Vec<T>{}; };
+  Vec<T> held[HELD ? HELD : 1];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int u = 0; u < HELD; ++u) held[u] = load((u * lanes + l) * NE);
+#pragma unroll
+    for (int u = 0; u < HELD; ++u) largest(held[u]);
+  } else {
+#pragma unroll 4
+    for (int e0 = l * NE; e0 < k; e0 += lanes * NE) largest(load(e0));
   }
   for (int o = lanes >> 1; o; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
   const bool bad = top >= 0x7f800000u;
   const float scale = bad ? NAN : __builtin_bit_cast(float, top) / 127.f;
   const bool none = bad || scale == 0.f;
   if (l == 0) s[row] = scale;
+  // x / s by a product: a guess that lies within s / 2 of x is right (0 where 1 / s is no number of 32 bits: never)
+  const float inverse = 1.f / scale, border = scale >= 0x1p-126f ? 0.5f * scale : 0.f;
   int8_t* dst = q + row * ldq;
-#pragma unroll 4
-  for (int e0 = l * NE; e0 < kp; e0 += lanes * NE) {
+  auto put = [&](const Vec<T>& v, int e0) {
     uint32_t w[NE / 4];
 #pragma unroll
     for (int i = 0; i < NE / 4; ++i) w[i] = 0;
-    if (!none && e0 < k) {
-      const Vec<T> v = load_vec<T>(src + (int64_t)e0 * ES, k - e0);
+    if (!none) {
+      float off = 0.f;
 #pragma unroll
-      for (int e = 0; e < NE; ++e) w[e >> 2] |= (uint32_t)(uint8_t)(int8_t)to8(v.v[e >> 2][e & 3], scale) << (8 * (e & 3));
+      for (int e = 0; e < NE; ++e) {
+        const float at = v.v[e >> 2][e & 3], guess = rintf(at * inverse);
+        off = fmaxf(off, fabsf(fmaf(-guess, scale, at)));
+        w[e >> 2] |= ((uint32_t)(int)guess & 255u) << (8 * (e & 3));
+      }
+      if (!(off < border)) {  // one of them on or past a border: rare
+#pragma unroll
+        for (int i = 0; i < NE / 4; ++i) w[i] = 0;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) w[e >> 2] |= ((uint32_t)to8(v.v[e >> 2][e & 3], scale) & 255u) << (8 * (e & 3));
+      }
     }
     if (e0 + NE <= kp) {
 #pragma unroll
@@ -78,7 +99,25 @@ __global__ __launch_bounds__(256) void k_quantize(const char* __restrict__ x, in
       for (int e = 0; e < NE; ++e)
         if (e0 + e < kp) dst[e0 + e] = (int8_t)(w[e >> 2] >> (8 * (e & 3)));
     }
+  };
+  if constexpr (HELD) {
+#pragma unroll
+    for (int u = 0; u < HELD; ++u)
+      if ((u * lanes + l) * NE < kp) put(held[u], (u * lanes + l) * NE);
+  } else {
+#pragma unroll 4
+    for (int e0 = l * NE; e0 < kp; e0 += lanes * NE) put(load(e0), e0);
   }
+}
+
+template <int T>
+void quantize(const void* x, int64_t ld, int64_t rows, int k, int kp, int8_t* q, int64_t ldq, float* s, hipStream_t st) {
+  constexpr int NE = Vec<T>::NE;
+  int lanes = 1;
+  while (lanes < 64 && lanes * NE < kp) lanes <<= 1;
+  const unsigned grid = (unsigned)((rows * lanes + 255) / 256);
+  (lanes * NE >= kp ? k_quantize<T, 1> : lanes * NE * 8 >= kp ? k_quantize<T, 8> : k_quantize<T, 0>)<<<grid, 256, 0, st>>>(
+      (const char*)x, ld * size_of(T), rows, k, kp, lanes, q, ldq, s);
 }
 
 // 8-bit rows as the tile engine takes them: whole granules, zeros past k.
@@ -214,8 +253,8 @@ __global__ __launch_bounds__(512, 6) void k_outer8(Problem a, EpiScores<TO, STRE
 }
 
 // The same where many rows of outputs do not begin at whole vectors: k_outer8's stores of 16 bytes straddle lines, 10,000 x
-// 99,998 take 0.95 ms past the caches, 0.67 through them and 0.62 here (float32: 1.87, 1.01 and 0.83). A workgroup passes along a strip of columns, W of them a step, with its 128 rows of q in
-// registers; the scores go through LDS, where row r begins at its place within its line, so that LINES whole lines of
+// 99,998 take 0.95 ms past the caches, 0.67 through them and 0.62 here (float32: 1.87, 1.01 and 0.83). A workgroup passes
+// along a strip of columns, W of them a step, with its 128 rows of q in registers; the scores go through LDS, where row r begins at its place within its line, so that LINES whole lines of
 // every row leave, aligned, a step; what is left of the last one is carried to the next step. Only a strip's ends are
 // partial lines.
 template <int TO>
@@ -509,17 +548,13 @@ extern "C" int blp_quantize_rows(int device, void* stream, int type, const void*
   DeviceGuard guard(device);
   if (guard.rc) return guard.rc;
   hipStream_t st = (hipStream_t)stream;
-  const int ne = 16 / size_of(type);
-  int lanes = 1;
-  while (lanes < 64 && lanes * ne < k) lanes <<= 1;
-  const unsigned grid = (unsigned)div_up(rows * lanes, 256);
-  const int kp = (int)std::min<int64_t>(ldq, up(k, 16));
+  const int kp = (int)std::min<int64_t>(ldq, (k + 15) / 16 * 16);
   if (type == F32)
-    k_quantize<F32><<<grid, 256, 0, st>>>((const char*)x, ldx * 4, rows, k, kp, lanes, q, ldq, s);
+    quantize<F32>(x, ldx, rows, k, kp, q, ldq, s, st);
   else if (type == BF16)
-    k_quantize<BF16><<<grid, 256, 0, st>>>((const char*)x, ldx * 2, rows, k, kp, lanes, q, ldq, s);
+    quantize<BF16>(x, ldx, rows, k, kp, q, ldq, s, st);
   else
-    k_quantize<F16><<<grid, 256, 0, st>>>((const char*)x, ldx * 2, rows, k, kp, lanes, q, ldq, s);
+    quantize<F16>(x, ldx, rows, k, kp, q, ldq, s, st);
   BLP_HIP(hipGetLastError());
   return 0;
 }
