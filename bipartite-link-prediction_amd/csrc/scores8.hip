@@ -254,7 +254,8 @@ __global__ __launch_bounds__(512, 6) void k_outer8(Problem a, EpiScores<TO, STRE
 
 // The same where many rows of outputs do not begin at whole vectors: k_outer8's stores of 16 bytes straddle lines, 10,000 x
 // 99,998 take 0.95 ms past the caches, 0.67 through them and 0.62 here (float32: 1.87, 1.01 and 0.83). A workgroup passes
-// along a strip of columns, W of them a step, with its 128 rows of q in registers; the scores go through LDS, where row r begins at its place within its line, so that LINES whole lines of
+// along a strip of columns, W of them a step, with its 128 rows of q in registers; the scores go through LDS, where row r
+// begins at its place within its line, so that LINES whole lines of
 // every row leave, aligned, a step; what is left of the last one is carried to the next step. Only a strip's ends are
 // partial lines.
 template <int TO>
