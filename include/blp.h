@@ -480,7 +480,8 @@ int blp_lookup_grad(int device, void* stream, int type, const void* grad, int64_
  *     to even). A row of zeros: s = 0; one with a NaN or an infinity: s = NaN, q = 0. Bytes k to
  *     min(ldq, k rounded up to 16) of a row of q are set to 0.
  *   blp_scores8: out[i][j] = s[i] ts[j] sum_k q[i][k] table[j][k], k < 2^17: the sum exact in 32-bit
- *     integers, the rest in float, rounded to out_type once. A workspace of 0 bytes may be NULL. */
+ *     integers, the rest in float, rounded to out_type once. out is aligned to its elements. A workspace
+ *     of 0 bytes may be NULL. Row strides that are multiples of 16 bytes need no copy.       */
 int blp_quantize_rows(int device, void* stream, int type, const void* x, int64_t ldx, int64_t rows, int k, int8_t* q,
                       int64_t ldq, float* s);
 int blp_scores8_workspace(const int8_t* q, int64_t ldq, const int8_t* table, int64_t ldt, int64_t rows, int64_t cols, int k,
