@@ -146,8 +146,9 @@ def softmax_loss(x, table, target, scale=1.0, reduction="mean"):
     missing slots) ignores its row: loss 0, gradient 0, whatever x holds there. reduction "mean" (over
     the rows not ignored; 0 if there is none), "sum" or "none" (one loss a row). Returns float32;
     differentiable in x and table (not inside a graph capture: capture :func:`softmax_loss_grad`).
-    Sums and the softmax's statistics are held in 32 bits. Float32 factors are
-    multiplied as sums of three bfloat16 each, with 32-bit results; they have to be finite."""
+    Sums and the softmax's statistics are held in 32 bits, and gradients are rounded to the type once: the
+    softmax's differences that they sum are held as two halves each, to 2^-16 (bfloat16) or 2^-22 (float16).
+    Float32 factors are multiplied as sums of three bfloat16 each, with 32-bit results; they have to be finite."""
     torch = _t()
     if torch.is_grad_enabled() and (getattr(x, "requires_grad", False) or getattr(table, "requires_grad", False)):
         return _function("loss").apply(x, table, target, scale, reduction)

@@ -6,8 +6,12 @@
 // x_i are the rows scored (users), w_j every row of the catalogue, t_i the row's target. The scores are
 // never kept. Wide factors: the forward pass reduces each tile of them to a (reference, sum) pair a row, and the backward
 // pass recomputes them piece by piece of the catalogue into a workspace of dS, from which the two products of the
-// gradient are taken: four products of 2 M N k operations in all. Narrow factors: k_narrow_lse and k_narrow_grads, five
-// such products, and no dS in memory.
+// gradient are taken. Narrow factors: k_narrow_lse and k_narrow_grads, and no dS in memory.
+//
+// The matrix instructions take halves, and dS is no half: rounded to one it would add 2^-8 (bfloat16) of each term to
+// gradients that are themselves rounded to 2^-8. It is held as a sum of two, d1 = dS rounded and d2 = dS - d1 rounded, which
+// leaves 2^-16 (float16: 2^-22), and both are multiplied: the gradients' products take twice the instructions, six products
+// of 2 M N k operations in all (narrow factors: seven, as the scores are computed once more).
 //
 // Float factors go through the matrix cores as three halves each: x1 = x rounded to bfloat16, x2 = x - x1 rounded,
 // x3 = x - x1 - x2, together all 24 bits; of the nine products of two such sums the six largest are taken (the others lie
@@ -33,6 +37,9 @@ constexpr float LN2 = 0.69314718055994530942f;
 // The matrix instructions' type, and the planes a factor is held in.
 constexpr int mma_type(int t) { return t == F32 ? BF16 : t; }
 constexpr int planes_of(int t) { return t == F32 ? 3 : 1; }
+constexpr int ds_planes_of(int t) { return t == F32 ? 3 : 2; }
+// Products of planes that one of the scores (ROW) or of the gradients (COL) takes.
+constexpr int segments_of(int t, int layout) { return t == F32 ? 6 : layout == COL ? 2 : 1; }
 // float16 holds dS times this: a probability below 2^-24 is not lost.
 constexpr float extra_of(int t) { return t == F16 ? 16384.f : 1.f; }
 
@@ -340,7 +347,7 @@ template <int T>
 struct EpiGrad {
   char* ds;
   int64_t ld;     // elements
-  int64_t plane;  // floats: bytes between the planes of dS
+  int64_t plane;  // bytes between the planes of dS
   const float* lse;
   RowGrad g;
   Targets targets;
@@ -384,23 +391,20 @@ struct EpiGrad {
       }
       return v;
     };
-    if constexpr (T != F32) {
-      store_block<MT, S>(scratch, at, ld * size_of(MT), width, rows, value);
-    } else {
+#pragma unroll
+    for (int i = 0; i < S::FP; ++i)
+#pragma unroll
+      for (int j = 0; j < S::FQ; ++j) acc[i][j] = value(i, j);
+#pragma unroll 1
+    for (int p = 0; p < ds_planes_of(T); ++p) {
+      store_block<MT, S>(scratch, at + p * plane, ld * size_of(MT), width, rows, [&](int i, int j) { return acc[i][j]; });
+      typedef std::conditional_t<MT == BF16, __bf16, _Float16> Half;
 #pragma unroll
       for (int i = 0; i < S::FP; ++i)
 #pragma unroll
-        for (int j = 0; j < S::FQ; ++j) acc[i][j] = value(i, j);
-#pragma unroll 1
-      for (int p = 0; p < 3; ++p) {
-        store_block<MT, S>(scratch, at + p * plane, ld * size_of(MT), width, rows, [&](int i, int j) { return acc[i][j]; });
+        for (int j = 0; j < S::FQ; ++j)
 #pragma unroll
-        for (int i = 0; i < S::FP; ++i)
-#pragma unroll
-          for (int j = 0; j < S::FQ; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][j][e] -= (float)(__bf16)acc[i][j][e];
-      }
+          for (int e = 0; e < 4; ++e) acc[i][j][e] -= (float)(Half)acc[i][j][e];  // what the plane left over
     }
   }
 };
@@ -500,7 +504,7 @@ __global__ __launch_bounds__(256) void k_sum_parts(SumArgs a, SumArgs b, int64_t
 // 32 rows of one side ("own") as fragments for the whole kernel and the other side ("stream") passes through LDS, 64 rows
 // a stage:
 //   LSE  own x, stream w: a running sum of exp2(score - reference) a lane, joined over the lanes at the end
-//   DX   own x, stream w: dS of 32 stream rows at a time, rounded to halves in place, is the second product's
+//   DX   own x, stream w: dS of 32 stream rows at a time, as two halves each (floats: three), is the second product's
 //        operand as it lies (the matrix instruction's k order is free, so its rows of w are read from LDS,
 //        transposed, in the order in which the lanes hold dS); dx accumulates in registers
 //   DW   own w, stream x: the same with the sides changed
@@ -535,14 +539,25 @@ struct NarrowShape {  // the second product's accumulators, for the epilogues
   static constexpr int FP = 2 * KS_, FQ = FO_, SCRATCH = 16384;
 };
 
+// Two values as halves; `rest`: they become what that left over.
 template <int T>
-__device__ inline int pack2(float a, float b) {
+__device__ inline int pack2(float& a, float& b, bool rest) {
   if constexpr (T == BF16) {
     typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(int, b2{(__bf16)a, (__bf16)b});
+    const int both = __builtin_bit_cast(int, b2{(__bf16)a, (__bf16)b});
+    if (rest) {
+      a -= __uint_as_float((uint32_t)both << 16);
+      b -= __uint_as_float((uint32_t)both & 0xffff0000u);
+    }
+    return both;
   } else {
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(int, h2{(_Float16)a, (_Float16)b});
+    const h2 both = {(_Float16)a, (_Float16)b};
+    if (rest) {
+      a -= (float)both[0];
+      b -= (float)both[1];
+    }
+    return __builtin_bit_cast(int, both);
   }
 }
 
@@ -558,7 +573,7 @@ struct NarrowLds {
 template <int T, int KS, int MODE, bool PER_ROW, class Epi>
 __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowArgs& a, const Epi& epi, int block, char* s_a, char* s_b,
                                                                   char* s_c, char* s_ra, char* s_rb, char* s_rc) {
-  constexpr int MT = mma_type(T), PL = planes_of(T);
+  constexpr int MT = mma_type(T), PL = planes_of(T), PD = ds_planes_of(T);
   constexpr int FO = 2;  // own fragments of 16 rows a wave
   constexpr int HALVES = NarrowLds<T, KS>::HALVES, PART = NarrowLds<T, KS>::PART, BUF = NarrowLds<T, KS>::BUF;
   constexpr bool THREE = NarrowLds<T, KS>::THREE;
@@ -802,21 +817,19 @@ __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowAr
 #pragma unroll
             for (int j = 0; j < FO; ++j) acc[i][j] *= g;
         }
-        frag_t q[PL][FO];
+        frag_t q[PD][FO];
 #pragma unroll
-        for (int p = 0; p < PL; ++p)
+        for (int p = 0; p < PD; ++p)
 #pragma unroll
           for (int j = 0; j < FO; ++j)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
               for (int w = 0; w < 2; ++w) {
-                const int both = pack2<MT>(acc[i][j][2 * w], acc[i][j][2 * w + 1]);
-                q[p][j][2 * i + w] = both;
-                if (p + 1 < PL) {  // what the plane left over
-                  acc[i][j][2 * w] -= __uint_as_float((uint32_t)both << 16);
-                  acc[i][j][2 * w + 1] -= __uint_as_float((uint32_t)both & 0xffff0000u);
-                }
+                float a = acc[i][j][2 * w], b = acc[i][j][2 * w + 1];
+                q[p][j][2 * i + w] = pack2<MT>(a, b, p + 1 < PD);
+                acc[i][j][2 * w] = a;
+                acc[i][j][2 * w + 1] = b;
               }
 #pragma unroll
         for (int d = 0; d < 2 * KS; ++d)
@@ -832,7 +845,7 @@ __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowAr
               v[2 * s + 1] = w[1];
             }
 #pragma unroll
-            for (int y = 0; y < PL - x; ++y)
+            for (int y = 0; y < PD - x; ++y)
 #pragma unroll
               for (int j = 0; j < FO; ++j) out[d][j] = mma<MT>(v, q[y][j], out[d][j]);
           }
@@ -924,7 +937,7 @@ struct EpiGradient {
 // Both gradients in one launch: the workgroups of one fill the compute units that the other's leave (10,000 x 100,000
 // x 64: 782 workgroups of dw alone keep three quarters of the card's slots busy).
 template <int T, int KS, bool PER_ROW>
-__global__ __launch_bounds__(256, KS > 3 ? 2 : KS > 2 || T == F32 ? 3 : 4) void k_narrow_grads(NarrowArgs w, EpiGradient<T> ew,
+__global__ __launch_bounds__(256, KS > 2 || T == F32 ? 3 : 4) void k_narrow_grads(NarrowArgs w, EpiGradient<T> ew,
                                                                                               int w_blocks, NarrowArgs x,
                                                                                               EpiGradient<T> ex) {
   using L = NarrowLds<T, KS>;
@@ -995,8 +1008,8 @@ struct Slices {
   int shape, n;
   int stages;  // a slice
 };
-Slices slices_of(int64_t np, int64_t nq, int64_t k, int planes) {
-  const int64_t stages = div_up(k, STAGE / 2) * (planes == 1 ? 1 : SEGMENTS);
+Slices slices_of(int64_t np, int64_t nq, int64_t k, int segments) {
+  const int64_t stages = div_up(k, STAGE / 2) * segments;
   Slices best = {FLAT, 1, (int)stages};
   double least = -1;
   for (int shape : {BIG, MID, FLAT, THIN}) {
@@ -1043,6 +1056,7 @@ Splits splits_of(int64_t own, int64_t stream, int trip, double us, double part_b
 struct Plan {
   int type, es;         // the caller's type and its size
   int planes, kp;       // the engine's: planes of halves, kp of them a row
+  int ds_planes;
   int64_t m, n;
   int k;
   bool grads, pack_w, pack_x;
@@ -1070,6 +1084,7 @@ Plan plan_of(int type, int64_t m, int64_t n, int k, bool forward, bool grads, bo
   p.type = type;
   p.es = size_of(type);
   p.planes = planes_of(type);
+  p.ds_planes = ds_planes_of(type);
   p.kp = (int)up(k, 8);
   p.m = m;
   p.n = n;
@@ -1084,8 +1099,8 @@ Plan plan_of(int type, int64_t m, int64_t n, int k, bool forward, bool grads, bo
   if (p.narrow) {
     p.ks = (p.kp + 31) / 32;
     const int trip = type == F32 ? 2 : 3;  // stages of a trip of k_narrow's loop
-    // measured: halves 0.3 and 0.5 us a stage at k = 64, floats 0.8 and 2 at k = 50
-    const double lse_us = type == F32 ? 0.4 * p.ks : 0.22 + 0.05 * p.ks, grad_us = type == F32 ? 1.0 * p.ks : 0.3 + 0.12 * p.ks;
+    // measured: halves 0.3 and 0.75 us a stage at k = 64, floats 0.8 and 2 at k = 50
+    const double lse_us = type == F32 ? 0.4 * p.ks : 0.22 + 0.05 * p.ks, grad_us = type == F32 ? 1.0 * p.ks : 0.41 + 0.17 * p.ks;
     p.nl = splits_of(m, n, trip, lse_us, 8.0 * m);
     p.nx = splits_of(m, n, trip, grad_us, 4.0 * m * up(k, 4));
     p.nw = splits_of(n, m, trip, grad_us, 4.0 * n * up(k, 4));
@@ -1108,13 +1123,13 @@ Plan plan_of(int type, int64_t m, int64_t n, int k, bool forward, bool grads, bo
   p.o_top = l.take(16);
   if (grads) {
     // whole tiles of columns within the budget, the pieces as equal as that allows
-    const int64_t most = std::max<int64_t>(PIECE_BYTES / (std::max<int64_t>(m, 1) * 2 * p.planes) / 256 * 256, 256);
+    const int64_t most = std::max<int64_t>(PIECE_BYTES / (std::max<int64_t>(m, 1) * 2 * p.ds_planes) / 256 * 256, 256);
     p.pieces = div_up(n, most);
     p.piece = std::min(up(div_up(n, p.pieces), 256), up(n, 64));
     p.pieces = div_up(n, p.piece);
-    p.o_ds = l.take(p.planes * p.ds_plane());
-    p.sx = slices_of(k, m, std::min(p.piece, n), p.planes);
-    p.sw = slices_of(k, p.piece, m, p.planes);
+    p.o_ds = l.take(p.ds_planes * p.ds_plane());
+    p.sx = slices_of(k, m, std::min(p.piece, n), segments_of(type, COL));
+    p.sw = slices_of(k, p.piece, m, segments_of(type, COL));
     p.o_px = l.take(p.sx.n > 1 || p.pieces > 1 ? (int64_t)p.sx.n * m * up(k, 4) * 4 : 0);
     p.o_pw = l.take(p.sw.n > 1 ? (int64_t)p.sw.n * p.piece * up(k, 4) * 4 : 0);
   }
@@ -1124,7 +1139,7 @@ Plan plan_of(int type, int64_t m, int64_t n, int k, bool forward, bool grads, bo
 
 template <int T, int LP, int LQ, class S, class Epi>
 void launch(const Problem& a, dim3 grid, const Epi& epi, hipStream_t st) {
-  k_product<mma_type(T), LP, LQ, T == F32, S, Epi><<<grid, S::THREADS, 0, st>>>(a, epi);
+  k_product<mma_type(T), LP, LQ, segments_of(T, LP), S, Epi><<<grid, S::THREADS, 0, st>>>(a, epi);
 }
 
 // `stages`: of a slice (0: all)
@@ -1134,7 +1149,7 @@ int product(int shape, Problem a, int slices, int stages, Epi epi, hipStream_t s
   BLP_CHECK(tp * tq <= 0x7fffffff, BLP_E_ARG, "softmax loss: too many tiles for one launch");
   a.tiles_p = (int)tp;
   a.tiles_q = (int)tq;
-  a.slice = stages ? stages : (int)div_up(a.k, KE) * (T == F32 ? SEGMENTS : 1);
+  a.slice = stages ? stages : (int)div_up(a.k, KE) * segments_of(T, LP);
   // as many workgroups as fit the card, which take tile after tile
   const dim3 grid((unsigned)std::min<int64_t>(tp * tq, 256 * PER_CU[shape]), (unsigned)slices);
   if (shape == BIG)

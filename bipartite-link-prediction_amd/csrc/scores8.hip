@@ -446,7 +446,7 @@ int launch(Problem a, int slices, int stages, Epi epi, hipStream_t st) {
   a.tiles_q = (int)tq;
   a.slice = stages;
   const dim3 grid((unsigned)std::min<int64_t>(tp * tq, S::BP == 256 && S::BQ == 256 ? 256 : 512), (unsigned)slices);
-  k_product<I8, ROW, ROW, false, S, Epi><<<grid, S::THREADS, 0, st>>>(a, epi);
+  k_product<I8, ROW, ROW, 1, S, Epi><<<grid, S::THREADS, 0, st>>>(a, epi);
   BLP_HIP(hipGetLastError());
   return 0;
 }

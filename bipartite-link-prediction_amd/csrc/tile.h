@@ -220,11 +220,12 @@ struct Problem {
   int64_t k;            // valid k, in elements
   int slice;            // stages of one slice (blockIdx.y) of all segments' stages
   int tiles_p, tiles_q;
-  // Floats as three halves each (x = x1 + x2 + x3, see latent.hip): the six segments x1 w1, x1 w2, x2 w1, x2 w2, x1 w3,
-  // x3 w1 follow one another along k; the planes of an operand lie this many bytes apart.
+  // Values held as sums of halves (x = x1 + x2 + ..., see latent.hip): products of the operands' planes, which lie this many
+  // bytes apart, are segments of one sum over k. Six segments, three planes each: x1 w1, x1 w2, x2 w1, x2 w2, x1 w3, x3 w1,
+  // one after the other. Two, of one plane of P and two of Q: p q1 and p q2 take turns, so that p's stage comes out of the
+  // cache the second time.
   int64_t p_plane, q_plane;
 };
-constexpr int SEGMENTS = 6;
 __host__ __device__ constexpr int p_plane_of(int seg) { return (0x850 >> (2 * seg)) & 3; }
 __host__ __device__ constexpr int q_plane_of(int seg) { return (0x244 >> (2 * seg)) & 3; }
 
@@ -241,7 +242,7 @@ __device__ inline void tile_of(const Problem& a, int b, int* tp, int* tq) {
   *tq = band * BAND + in - *tp * width;
 }
 
-template <int T, int LP, int LQ, bool SEG, class S, class Epi>
+template <int T, int LP, int LQ, int SEGS, class S, class Epi>
 __global__ __launch_bounds__(S::THREADS, 2) void k_product(Problem a, Epi epi) {
   constexpr int KE = STAGE / size_of(T);
   __shared__ __attribute__((aligned(1024))) char s_0[S::STAGE_BYTES], s_1[S::STAGE_BYTES];
@@ -249,15 +250,18 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_product(Problem a, Epi epi) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wp = wave % S::WP, wq = wave / S::WP;
   const uint32_t bp = lane_base<T, LP, S::BP>(), bq = lane_base<T, LQ, S::BQ>();
   const int per_seg = (int)((a.k + KE - 1) / KE), sb = blockIdx.y * a.slice;
-  const int stages = min(a.slice, (SEG ? SEGMENTS : 1) * per_seg - sb), tiles = a.tiles_p * a.tiles_q;
+  const int stages = min(a.slice, SEGS * per_seg - sb), tiles = a.tiles_p * a.tiles_q;
   auto load = [&](lds_char* to, int tp, int tq, int t) {
     int at = sb + t;
     Operand p = a.p, q = a.q;
-    if constexpr (SEG) {
+    if constexpr (SEGS == 6) {
       const int seg = at / per_seg;
       at -= seg * per_seg;
       p.base += p_plane_of(seg) * a.p_plane;
       q.base += q_plane_of(seg) * a.q_plane;
+    } else if constexpr (SEGS == 2) {
+      q.base += (at & 1) * a.q_plane;
+      at >>= 1;
     }
     load_stage<T, LP, S::BP, S::WAVES>(to, p, (int64_t)tp * S::BP, (int64_t)at * KE, a.k);
     load_stage<T, LQ, S::BQ, S::WAVES>(to + S::BP * STAGE, q, (int64_t)tq * S::BQ, (int64_t)at * KE, a.k);

@@ -1,0 +1,94 @@
+"""The softmax loss's gradients keep 32-bit accuracy up to their one rounding (blp.latent.softmax_loss*).
+
+dS is held as a sum of halves (two of them where the factors are halves, three where they are floats), so what its
+rounding leaves is the half step of the type squared, h^2 (bfloat16 2^-16, float16 2^-22), or 2^-24. The bounds are those of
+test_gpu_latent_loss.py with h^2 in the place of h: a gradient is off by
+  scale sum_j (|g_i| (p_ij r_i + 2 u) + h2 |dS_ij|) |w_j| + (n + 8) u scale sum |dS w|, then h of the result,
+  r_i = 2 dz_i + (depth + 16) u + 4 u (S_i + |lse_i|)
+u = 2^-23. Catalogues are small, so that (n + 8) u stays far below h.
+float16 holds dS times 2^14: its lowest step leaves 2^-25 2^-14 = 2^-39 of the largest row gradient.
+"""
+import pytest
+
+from test_gpu_latent_loss import U, _half_step, _torch, make, near
+
+pytestmark = pytest.mark.gpu
+
+
+def gradients(x, w, t, scale, gi, floor_dx):
+    """-> ((dx, bound), (dw, bound)) of row gradients gi (64 bits); floor_dx: what float16's lowest step leaves in a row's dS."""
+    import torch
+
+    X, W = x.double(), w.double()
+    n, k = W.shape
+    ok = (t >= 0) & (t < n)
+    X = torch.where(ok[:, None], X, 0.0)
+    at = t.clamp(0, n - 1).long()[:, None]
+    z = scale * (X @ W.t().contiguous())
+    S = abs(scale) * (X.abs() @ W.abs().t().contiguous()).amax(1)
+    lse = torch.logsumexp(z, 1)
+    gi = torch.where(ok, gi, 0.0)
+    p = torch.exp(z - lse[:, None])
+    d = gi[:, None] * (p - torch.zeros_like(p).scatter_(1, at, 1.0))
+    h = _half_step(x.dtype)
+    h2 = 2.0 ** -24 if x.dtype == torch.float32 else h * h
+    r = 2 * (k + 4) * U * S + (64 + n / 64 + 16) * U + 4 * U * (S + lse.abs())
+    e = gi.abs()[:, None] * (p * r[:, None] + 2 * U) + h2 * d.abs()
+    half = x.dtype == torch.float16
+    tiny = 2.0 ** -25 if half else 0.0
+
+    def mm(a, b):
+        return a @ b.contiguous()
+
+    out = []
+    for a, b, floor in ((lambda v: v, W, floor_dx), (lambda v: v.t(), X, gi.abs().max())):
+        want = scale * mm(a(d), b)
+        bound = abs(scale) * (mm(a(e + (floor * 2.0 ** -39 if half else 0.0)), b.abs()) + (max(x.shape[0], n) + 8) * U * mm(a(d).abs(), b.abs()))
+        out.append((want, bound * (1 + 2 * h) + h * want.abs() + tiny))
+    return out
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("m,n,k", [(200, 260, 24), (300, 150, 64), (130, 333, 100), (129, 257, 128), (150, 300, 136), (300, 200, 328),
+                                   (40, 90, 700), (600, 700, 200)])
+def test_gradients_are_rounded_once(gpu, m, n, k, dtype):
+    torch = _torch()
+    from blp import latent
+
+    x, w, t = make(m, n, k, getattr(torch, dtype), seed=m + k, ignored=0.1, scale=1.25)
+    _, dx, dw = latent.softmax_loss_grad(x, w, t, scale=1.25, reduction="sum")
+    one = torch.ones(m, dtype=torch.float64, device="cuda")
+    for got, (want, bound) in zip((dx, dw), gradients(x, w, t, 1.25, one, one[:, None])):
+        near(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("k", [64, 200])
+def test_backward_of_row_gradients_is_rounded_once(gpu, k, dtype):
+    """The same through autograd, with gradients of their own for the rows."""
+    torch = _torch()
+    from blp import latent
+
+    x, w, t = make(140, 300, k, getattr(torch, dtype), seed=k, ignored=0.1)
+    g = torch.linspace(-2, 3, 140, device="cuda")
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    dx, dw = torch.autograd.grad(latent.softmax_loss(x, w, t, reduction="none"), (x, w), g)
+    for got, (want, bound) in zip((dx, dw), gradients(x.detach(), w.detach(), t, 1.0, g.double(), g.double().abs().max())):
+        near(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_pieces_of_the_catalogue_add_up(gpu, dtype):
+    """dx of a catalogue of several pieces: 131,072 rows leave room for 512 columns of two halves each, 1,100 columns are three pieces."""
+    torch = _torch()
+    from blp import latent
+
+    m, n, k = 131072, 1100, 136
+    x, w, t = make(m, n, k, getattr(torch, dtype), seed=2, ignored=0.05)
+    _, dx, dw = latent.softmax_loss_grad(x, w, t, reduction="sum")
+    at = torch.cat([torch.arange(0, 200), torch.arange(m - 100, m)]).cuda()
+    one = torch.ones(len(at), dtype=torch.float64, device="cuda")
+    (want, bound), _ = gradients(x[at], w, t[at], 1.0, one, one[:, None])
+    near(dx[at], want, bound)
+    assert dw.isfinite().all()
