@@ -1346,8 +1346,10 @@ int backward(const Call& c, bool fwd, const float* lse, RowGrad g, void* dx, int
     const Operand dsr = {ds, p.piece * 2, p.m};
     if (dx) {
       const Problem ax = {{wj.base, wj.ld, p.k}, dsr, nj, 0, 0, 0, p.w_plane(), p.ds_plane()};
+      // the last piece is narrower: its slices are those that have stages (the first piece, which is whole, has set them all)
+      const int slices = (int)std::min<int64_t>(p.sx.n, div_up(div_up(nj, KE) * segments_of(T, COL), p.sx.stages));
       if (parts_x)
-        rc = product<T, COL, ROW>(p.sx.shape, ax, p.sx.n, p.sx.stages, EpiPart{px, ldp, p.k, p.m, j0 > 0}, c.st);
+        rc = product<T, COL, ROW>(p.sx.shape, ax, slices, p.sx.stages, EpiPart{px, ldp, p.k, p.m, j0 > 0}, c.st);
       else
         rc = product<T, COL, ROW>(p.sx.shape, ax, 1, 0, EpiOut<T>{(char*)dx, lddx * p.es, p.k, p.m, g, c.scale}, c.st);
       if (rc) break;

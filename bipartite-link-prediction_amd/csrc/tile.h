@@ -218,7 +218,7 @@ __device__ inline void ring_barrier() {
 struct Problem {
   Operand p, q;
   int64_t k;            // valid k, in elements
-  int slice;            // stages of one slice (blockIdx.y) of all segments' stages
+  int slice;            // stages of one slice (blockIdx.y) of all segments' stages; every slice launched has at least one
   int tiles_p, tiles_q;
   // Values held as sums of halves (x = x1 + x2 + ..., see latent.hip): products of the operands' planes, which lie this many
   // bytes apart, are segments of one sum over k. Six segments, three planes each: x1 w1, x1 w2, x2 w1, x2 w2, x1 w3, x3 w1,

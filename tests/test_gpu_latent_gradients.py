@@ -92,3 +92,17 @@ def test_pieces_of_the_catalogue_add_up(gpu, dtype):
     (want, bound), _ = gradients(x[at], w, t[at], 1.0, one, one[:, None])
     near(dx[at], want, bound)
     assert dw.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype,m,n,k", [("bfloat16", 16384, 87300, 200), ("float32", 14875, 70587, 104)])
+def test_a_last_piece_of_fewer_slices(gpu, dtype, m, n, k):
+    """A catalogue whose last piece has fewer stages than the slices of the others take: the row gradient's parts add up."""
+    torch = _torch()
+    from blp import latent
+
+    x, w, t = make(m, n, k, getattr(torch, dtype), seed=4)
+    _, dx, _ = latent.softmax_loss_grad(x, w, t, reduction="sum")
+    at = torch.cat([torch.arange(0, 100), torch.arange(m - 60, m)]).cuda()
+    one = torch.ones(len(at), dtype=torch.float64, device="cuda")
+    (want, bound), _ = gradients(x[at], w, t[at], 1.0, one, one[:, None])
+    near(dx[at], want, bound)
