@@ -1367,10 +1367,8 @@ int backward(const Call& c, bool fwd, const float* lse, RowGrad g, void* dx, int
     }
   }
   if (rc) return rc;
-  if (dx && parts_x && p.m > 0) {
-    rc = sum_parts<T>(SumArgs{px, p.sx.n, p.m, (char*)dx, lddx * p.es, 0}, SumArgs{}, p.k, g, c.scale, c.st);
-  }
-  return 0;
+  if (dx && parts_x) rc = sum_parts<T>(SumArgs{px, p.sx.n, p.m, (char*)dx, lddx * p.es, 0}, SumArgs{}, p.k, g, c.scale, c.st);
+  return rc;
 }
 
 constexpr int64_t MOST_ROWS = (1ll << 31) - (1 << 16);  // the row numbers of stages past the end fit 31 bits

@@ -29,3 +29,37 @@ def test_every_slice_of_a_product_has_stages(type, m, n, k):
         assert len(products) >= 3
         for grid, p in products:
             assert grid[1] == math.ceil(p["segments"] * math.ceil(p["k"] / STAGE[p["type"]]) / p["slice"]), (grid, p)
+
+
+def lookup_grad(type, n, rows, k):
+    return ("blp_lookup_grad", [0, None, type, ONE, k, ONE, 1, n, rows, k, 1.0, ONE, k, 0, ONE, 1 << 50], None)
+
+
+def scores8(m, n, k, type, out=ONE, ldo=None):
+    return ("blp_scores8", [0, None, ONE, k, ONE, ONE, k, ONE, m, n, k, type, out, ldo or n, ONE, 1 << 50], None)
+
+
+CALLS = {
+    "loss_narrow": loss(1, 500, 3000, 64), "loss_narrow_f32": loss(0, 2000, 30011, 50), "loss_wide": loss(1, 600, 3000, 200),
+    "loss_pieces": loss(1, 16384, 87300, 200), "loss_pieces_f32": loss(0, 9000, 24011, 72), "loss_forward": loss(2, 3000, 9000, 72, grads=0),
+    "loss_no_rows": loss(1, 0, 3000, 64), "backward_narrow": backward(2, 500, 3000, 64), "backward_wide": backward(0, 600, 3000, 200),
+    "lookup": ("blp_lookup", [0, None, 1, ONE, 64, 5000, 64, ONE, 1, 3000, 2.0, ONE, 64], None),
+    "lookup_grad_short": lookup_grad(0, 3000, 500, 64), "lookup_grad_long": lookup_grad(1, 300000, 50000, 64),
+    "quantize": ("blp_quantize_rows", [0, None, 0, ONE, 64, 500, 64, ONE, 64, ONE], None),
+    "scores8_narrow": scores8(500, 3000, 64, 0), "scores8_strips": scores8(10000, 99998, 64, 1), "scores8_slices": scores8(10, 1266, 6462, 1),
+    "scores8_wide": scores8(4096, 16384, 4096, 1),
+}
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_the_status_of_every_launch_is_returned(name):
+    """Each launch of the call in turn fails as the runtime says: the call does, and launches nothing more."""
+    fn, args, _ = CALLS[name]
+    (whole,) = run([(fn, args, None)])
+    assert whole["rc"] == 0, whole["error"]
+    n = len(whole["launches"])
+    assert n > 0
+    at = sorted(set(range(min(n, 24))) | set(range(max(n - 24, 0), n)))
+    for i, got in zip(at, run([(fn, args, (i, 2)) for i in at])):
+        assert got["rc"] != 0 and got["error"], "launch %d of %d (%s) failed unseen" % (i, n, whole["launches"][i]["name"])
+        assert len(got["launches"]) == i + 1
