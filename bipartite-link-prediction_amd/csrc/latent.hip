@@ -18,6 +18,10 @@
 // below 2^-25 of the product), each exact in the 32-bit accumulators. That is 6 matrix instructions of 16 cycles for
 // 16 x 16 x 32 products where the float instructions take 256 cycles.
 //
+// float16 factors whose rows have gradients of their own are taken as floats ("T" the type they are multiplied as, "ST" the
+// one they are stored as): a row's dS may be any times smaller than the largest row's, and float16 ends at 2^-24 where
+// bfloat16 planes go on. Gradients 10^7 times below the largest would keep two digits, and lose all at 10^9.
+//
 // A row whose target lies outside [0, n_cols) is ignored: loss 0, gradient 0, and its x is never multiplied
 // (it may hold anything, NaN too).
 #include <algorithm>
@@ -40,7 +44,7 @@ constexpr int planes_of(int t) { return t == F32 ? 3 : 1; }
 constexpr int ds_planes_of(int t) { return t == F32 ? 3 : 2; }
 // Products of planes that one of the scores (ROW) or of the gradients (COL) takes.
 constexpr int segments_of(int t, int layout) { return t == F32 ? 6 : layout == COL ? 2 : 1; }
-// float16 holds dS times this: a probability below 2^-24 is not lost.
+// float16 holds dS times this: its lowest step is then 2^-38, far below the 2^-24 of a 32-bit difference from 1.
 constexpr float extra_of(int t) { return t == F16 ? 16384.f : 1.f; }
 
 using blp::DeviceGuard;
@@ -61,7 +65,7 @@ struct PackArgs {
   unsigned blocks;
 };
 
-template <int T>
+template <int T, int ST>
 __device__ inline void pack_rows(const PackArgs& a, int k, FastDiv per, unsigned block) {
   const int64_t n = a.rows * per.d, step = (int64_t)a.blocks * 256;
   for (int64_t i = block * 256ll + threadIdx.x; i < n; i += step) {
@@ -70,10 +74,10 @@ __device__ inline void pack_rows(const PackArgs& a, int k, FastDiv per, unsigned
     const bool keep = !a.targets.at || a.targets(r) >= 0;
     if constexpr (T == F32) {
       bf16x8 v[3];
-      const float* s = reinterpret_cast<const float*>(a.src + r * a.ld) + e0;
+      const char* s = a.src + r * a.ld + (int64_t)e0 * size_of(ST);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float x = keep && e0 + e < k ? s[e] : 0.f;
+        const float x = keep && e0 + e < k ? load1<ST>(s + e * size_of(ST)) : 0.f;
         const bool finite = fabsf(x) <= 3.4028235e38f;
         __bf16 first = (__bf16)x;
         if (finite && !(fabsf((float)first) <= 3.4e38f)) first = __builtin_bit_cast(__bf16, (uint16_t)(__float_as_uint(x) >> 16));
@@ -102,13 +106,13 @@ __device__ inline void pack_rows(const PackArgs& a, int k, FastDiv per, unsigned
   }
 }
 
-template <int T>
+template <int T, int ST>
 __global__ __launch_bounds__(256) void k_pack(PackArgs x, PackArgs w, int k, FastDiv per, uint32_t* flag) {
   if (flag && blockIdx.x == 0 && threadIdx.x == 0) *flag = 0;
   if (blockIdx.x < x.blocks)
-    pack_rows<T>(x, k, per, blockIdx.x);
+    pack_rows<T, ST>(x, k, per, blockIdx.x);
   else
-    pack_rows<T>(w, k, per, blockIdx.x - x.blocks);
+    pack_rows<T, ST>(w, k, per, blockIdx.x - x.blocks);
 }
 
 // What the narrow gradients read of a row of x, in blocks of 64 rows: log2(e) lse - log2(extra) (infinite: ignored),
@@ -570,7 +574,7 @@ struct NarrowLds {
   static constexpr bool THREE = T != F32;
 };
 
-template <int T, int KS, int MODE, bool PER_ROW, class Epi>
+template <int T, int ST, int KS, int MODE, bool PER_ROW, class Epi>
 __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowArgs& a, const Epi& epi, int block, char* s_a, char* s_b,
                                                                   char* s_c, char* s_ra, char* s_rb, char* s_rc) {
   constexpr int MT = mma_type(T), PL = planes_of(T), PD = ds_planes_of(T);
@@ -901,7 +905,7 @@ __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowAr
     lds_char* scratch;
     {  // a wave's 32 rows of up to 128 halves: the ring's buffers in parts
       __syncthreads();
-      constexpr int WAVE = 16 * FO * pow2_up(32 * KS * size_of(T));
+      constexpr int WAVE = 16 * FO * pow2_up(32 * KS * size_of(ST));
       if constexpr (WAVE * 4 <= BUF)
         scratch = (lds_char*)s_a + wave * WAVE;
       else
@@ -916,7 +920,7 @@ template <int T, int KS>
 __global__ __launch_bounds__(256, KS > 2 || T == F32 ? 3 : 4) void k_narrow_lse(NarrowArgs a) {
   using L = NarrowLds<T, KS>;
   __shared__ __attribute__((aligned(1024))) char s_a[L::BUF], s_b[L::BUF], s_c[L::THREE ? L::BUF : 16];
-  narrow_body<T, KS, LSE, false>(a, 0, blockIdx.x, s_a, s_b, s_c, nullptr, nullptr, nullptr);
+  narrow_body<T, T, KS, LSE, false>(a, 0, blockIdx.x, s_a, s_b, s_c, nullptr, nullptr, nullptr);
 }
 
 // A gradient's outputs: splits' partial sums, or rounded in place.
@@ -936,17 +940,16 @@ struct EpiGradient {
 
 // Both gradients in one launch: the workgroups of one fill the compute units that the other's leave (10,000 x 100,000
 // x 64: 782 workgroups of dw alone keep three quarters of the card's slots busy).
-template <int T, int KS, bool PER_ROW>
-__global__ __launch_bounds__(256, KS > 2 || T == F32 ? 3 : 4) void k_narrow_grads(NarrowArgs w, EpiGradient<T> ew,
-                                                                                              int w_blocks, NarrowArgs x,
-                                                                                              EpiGradient<T> ex) {
+template <int T, int ST, int KS, bool PER_ROW>
+__global__ __launch_bounds__(256, KS > 2 || T == F32 ? 3 : 4) void k_narrow_grads(NarrowArgs w, EpiGradient<ST> ew, int w_blocks,
+                                                                                  NarrowArgs x, EpiGradient<ST> ex) {
   using L = NarrowLds<T, KS>;
   __shared__ __attribute__((aligned(1024))) char s_a[L::BUF], s_b[L::BUF], s_c[L::THREE ? L::BUF : 16];
   __shared__ __attribute__((aligned(1024))) char s_ra[1024], s_rb[1024], s_rc[L::THREE ? 1024 : 16];
   if ((int)blockIdx.x < w_blocks)
-    narrow_body<T, KS, DW, PER_ROW>(w, ew, blockIdx.x, s_a, s_b, s_c, s_ra, s_rb, s_rc);
+    narrow_body<T, ST, KS, DW, PER_ROW>(w, ew, blockIdx.x, s_a, s_b, s_c, s_ra, s_rb, s_rc);
   else
-    narrow_body<T, KS, DX, PER_ROW>(x, ex, blockIdx.x - w_blocks, s_a, s_b, s_c, s_ra, s_rb, s_rc);
+    narrow_body<T, ST, KS, DX, PER_ROW>(x, ex, blockIdx.x - w_blocks, s_a, s_b, s_c, s_ra, s_rb, s_rc);
 }
 
 // ---------------------------------------------------------------- host side
@@ -1054,7 +1057,7 @@ Splits splits_of(int64_t own, int64_t stream, int trip, double us, double part_b
 }
 
 struct Plan {
-  int type, es;         // the caller's type and its size
+  int type, es;         // the type that the factors are multiplied as, and the size of the one they are stored as
   int planes, kp;       // the engine's: planes of halves, kp of them a row
   int ds_planes;
   int64_t m, n;
@@ -1079,10 +1082,10 @@ bool aligned(const void* p, int64_t ld_bytes, int64_t row_bytes) {
 }
 
 // `pack_x`, `pack_w`: whether the rows have to be packed (they are not whole aligned granules)
-Plan plan_of(int type, int64_t m, int64_t n, int k, bool forward, bool grads, bool pack_x, bool pack_w) {
+Plan plan_of(int type, int es, int64_t m, int64_t n, int k, bool forward, bool grads, bool pack_x, bool pack_w) {
   Plan p;
   p.type = type;
-  p.es = size_of(type);
+  p.es = es;
   p.planes = planes_of(type);
   p.ds_planes = ds_planes_of(type);
   p.kp = (int)up(k, 8);
@@ -1191,7 +1194,7 @@ struct Call {
   char* ws;
 };
 
-template <int T>
+template <int T, int ST>
 int bind(Call& c, const void* x, int64_t ldx, const void* w, int64_t ldw, uint32_t* flag) {
   const Plan& p = c.p;
   c.x = {(const char*)x, ldx * p.es, p.m};
@@ -1209,7 +1212,7 @@ int bind(Call& c, const void* x, int64_t ldx, const void* w, int64_t ldw, uint32
     c.w = {aw.dst, (int64_t)p.kp * 2, p.n};
   }
   if (ax.blocks + aw.blocks == 0) return 0;
-  k_pack<T><<<ax.blocks + aw.blocks, 256, 0, c.st>>>(ax, aw, p.k, FastDiv((uint32_t)per), flag);
+  k_pack<T, ST><<<ax.blocks + aw.blocks, 256, 0, c.st>>>(ax, aw, p.k, FastDiv((uint32_t)per), flag);
   BLP_HIP(hipGetLastError());
   return 0;
 }
@@ -1240,7 +1243,7 @@ int narrow_lse(const Call& c, float2* part, float* hit) {
   return 0;
 }
 
-template <int T>
+template <int T, int ST>
 int narrow_grads(const Call& c, RowGrad g, void* dx, int64_t lddx, void* dw, int64_t lddw) {
   const Plan& p = c.p;
   const int64_t ldp = up(p.k, 4);
@@ -1250,23 +1253,25 @@ int narrow_grads(const Call& c, RowGrad g, void* dx, int64_t lddx, void* dw, int
                         c.targets, nullptr, nullptr, rows};
   const NarrowArgs w = {c.w, c.x, p.w_plane(), p.x_plane(), p.kp, p.nw.range, dw ? p.nw.own_tiles : 0, p.nw.n, c.scale, g.extra,
                         c.targets, nullptr, nullptr, rows};
-  const EpiGradient<T> ex = {p.nx.n > 1, {px, ldp, p.k, p.m, 0}, {(char*)dx, lddx * p.es, p.k, p.m, g, c.scale}};
-  const EpiGradient<T> ew = {p.nw.n > 1, {pw, ldp, p.k, p.n, 0}, {(char*)dw, lddw * p.es, p.k, p.n, g, c.scale}};
+  const EpiGradient<ST> ex = {p.nx.n > 1, {px, ldp, p.k, p.m, 0}, {(char*)dx, lddx * p.es, p.k, p.m, g, c.scale}};
+  const EpiGradient<ST> ew = {p.nw.n > 1, {pw, ldp, p.k, p.n, 0}, {(char*)dw, lddw * p.es, p.k, p.n, g, c.scale}};
   const int64_t bw = up((int64_t)w.own_tiles * w.splits, 8), bx = (int64_t)x.own_tiles * x.splits;  // eights: x keeps its dies
   BLP_CHECK(bw + bx <= 0x7fffffff, BLP_E_ARG, "softmax loss: too many tiles for one launch");
   if (bw + bx == 0) return 0;
   const bool per_row = g.g && g.stride;
   with_steps<T>(p.ks, [&](auto ks) {
     constexpr int KS = decltype(ks)::value;
-    if (per_row)
-      k_narrow_grads<T, KS, true><<<(unsigned)(bw + bx), 256, 0, c.st>>>(w, ew, (int)bw, x, ex);
-    else
-      k_narrow_grads<T, KS, false><<<(unsigned)(bw + bx), 256, 0, c.st>>>(w, ew, (int)bw, x, ex);
+    if constexpr (T != F16) {  // row gradients of float16 are taken as floats
+      if (per_row) k_narrow_grads<T, ST, KS, true><<<(unsigned)(bw + bx), 256, 0, c.st>>>(w, ew, (int)bw, x, ex);
+    }
+    if constexpr (T == ST) {
+      if (!per_row) k_narrow_grads<T, ST, KS, false><<<(unsigned)(bw + bx), 256, 0, c.st>>>(w, ew, (int)bw, x, ex);
+    }
   });
   BLP_HIP(hipGetLastError());
   const SumArgs sx = {px, p.nx.n, dx && p.nx.n > 1 ? p.m : 0, (char*)dx, lddx * p.es, 0};
   const SumArgs sw = {pw, p.nw.n, dw && p.nw.n > 1 ? p.n : 0, (char*)dw, lddw * p.es, 0};
-  return sum_parts<T>(sx, sw, p.k, g, c.scale, c.st);
+  return sum_parts<ST>(sx, sw, p.k, g, c.scale, c.st);
 }
 
 template <int T>
@@ -1306,12 +1311,12 @@ int forward(const Call& c, float* loss, float* lse, Total total, uint32_t* done)
   return 0;
 }
 
-template <int T>
+template <int T, int ST>
 int backward(const Call& c, bool fwd, const float* lse, RowGrad g, void* dx, int64_t lddx, void* dw, int64_t lddw) {
   const Plan& p = c.p;
   if (p.m == 0) {  // no rows: the catalogue's gradient is zero
     if (dw) {
-      return sum_parts<T>(SumArgs{nullptr, 0, p.n, (char*)dw, lddw * p.es, 0}, SumArgs{}, p.k, RowGrad{nullptr, 0, nullptr, nullptr, 1.f},
+      return sum_parts<ST>(SumArgs{nullptr, 0, p.n, (char*)dw, lddw * p.es, 0}, SumArgs{}, p.k, RowGrad{nullptr, 0, nullptr, nullptr, 1.f},
                           1.f, c.st);
     }
     return 0;
@@ -1328,7 +1333,7 @@ int backward(const Call& c, bool fwd, const float* lse, RowGrad g, void* dx, int
       k_rows<<<(unsigned)div_up(p.m, 64), 64, 0, c.st>>>(lse, g, c.targets, p.m, Rows{(float*)(c.ws + p.o_rows)});
       BLP_HIP(hipGetLastError());
     }
-    return narrow_grads<T>(c, g, dx, lddx, dw, lddw);
+    return narrow_grads<T, ST>(c, g, dx, lddx, dw, lddw);
   }
   char* ds = c.ws + p.o_ds;
   float *px = (float*)(c.ws + p.o_px), *pw = (float*)(c.ws + p.o_pw);
@@ -1351,7 +1356,7 @@ int backward(const Call& c, bool fwd, const float* lse, RowGrad g, void* dx, int
       if (parts_x)
         rc = product<T, COL, ROW>(p.sx.shape, ax, slices, p.sx.stages, EpiPart{px, ldp, p.k, p.m, j0 > 0}, c.st);
       else
-        rc = product<T, COL, ROW>(p.sx.shape, ax, 1, 0, EpiOut<T>{(char*)dx, lddx * p.es, p.k, p.m, g, c.scale}, c.st);
+        rc = product<T, COL, ROW>(p.sx.shape, ax, 1, 0, EpiOut<ST>{(char*)dx, lddx * p.es, p.k, p.m, g, c.scale}, c.st);
       if (rc) break;
     }
     if (dw) {
@@ -1360,14 +1365,14 @@ int backward(const Call& c, bool fwd, const float* lse, RowGrad g, void* dx, int
       if (p.sw.n > 1) {
         rc = product<T, COL, COL>(p.sw.shape, aw, p.sw.n, p.sw.stages, EpiPart{pw, ldp, p.k, nj, 0}, c.st);
         if (rc) break;
-        rc = sum_parts<T>(SumArgs{pw, p.sw.n, nj, out, lddw * p.es, 0}, SumArgs{}, p.k, g, c.scale, c.st);
+        rc = sum_parts<ST>(SumArgs{pw, p.sw.n, nj, out, lddw * p.es, 0}, SumArgs{}, p.k, g, c.scale, c.st);
       } else {
-        rc = product<T, COL, COL>(p.sw.shape, aw, 1, 0, EpiOut<T>{out, lddw * p.es, p.k, nj, g, c.scale}, c.st);
+        rc = product<T, COL, COL>(p.sw.shape, aw, 1, 0, EpiOut<ST>{out, lddw * p.es, p.k, nj, g, c.scale}, c.st);
       }
     }
   }
   if (rc) return rc;
-  if (dx && parts_x) rc = sum_parts<T>(SumArgs{px, p.sx.n, p.m, (char*)dx, lddx * p.es, 0}, SumArgs{}, p.k, g, c.scale, c.st);
+  if (dx && parts_x) rc = sum_parts<ST>(SumArgs{px, p.sx.n, p.m, (char*)dx, lddx * p.es, 0}, SumArgs{}, p.k, g, c.scale, c.st);
   return rc;
 }
 
@@ -1381,15 +1386,17 @@ int check_args(int type, int64_t rows, int64_t cols, int k) {
   return 0;
 }
 
-template <int T>
+template <int T, int ST>
 int run(Call& c, const void* x, int64_t ldx, const void* w, int64_t ldw, float* loss, float* lse, float* total, int mean,
         bool fwd, RowGrad g, void* dx, int64_t lddx, void* dw, int64_t lddw) {
   // With gradients the packing comes first and clears the mark by which the last block to end takes the total. Every
   // block's fence writes its die's cache back, so that pays for few of them (106 rows: 40 -> 33 us a step; 1,590: 70 -> 93).
   uint32_t* done = fwd && total && c.p.grads && c.p.m > 0 && c.p.m <= 512 ? (uint32_t*)(c.ws + c.p.o_top) + 1 : nullptr;
-  int rc = bind<T>(c, x, ldx, w, ldw, done);
-  if (!rc && fwd) rc = forward<T>(c, loss, lse, Total{total, mean}, done);
-  if (!rc && c.p.grads) rc = backward<T>(c, fwd, lse, g, dx, lddx, dw, lddw);
+  int rc = bind<T, ST>(c, x, ldx, w, ldw, done);
+  if constexpr (T == ST) {
+    if (!rc && fwd) rc = forward<T>(c, loss, lse, Total{total, mean}, done);
+  }
+  if (!rc && c.p.grads) rc = backward<T, ST>(c, fwd, lse, g, dx, lddx, dw, lddw);
   return rc;
 }
 
@@ -1405,7 +1412,8 @@ int dispatch(int device, void* stream, int type, const void* x, int64_t ldx, con
             "softmax loss: a row stride is smaller than k");
   BLP_CHECK(std::max(ldx, ldw) <= (1 << 20), BLP_E_ARG, "softmax loss: row strides must be at most 2^20 elements");
   Call c;
-  c.p = plan_of(type, m, n, k, fwd, grads, !aligned(x, ldx * es, (int64_t)k * es), !aligned(w, ldw * es, (int64_t)k * es));
+  const bool as_floats = type == F16 && g.g && g.stride;
+  c.p = plan_of(as_floats ? F32 : type, es, m, n, k, fwd, grads, !aligned(x, ldx * es, (int64_t)k * es), !aligned(w, ldw * es, (int64_t)k * es));
   BLP_CHECK(ws_bytes >= c.p.bytes, BLP_E_ARG, "softmax loss: the workspace is too small (blp_softmax_loss_workspace)");
   BLP_CHECK(((uintptr_t)ws & 255) == 0, BLP_E_ARG, "softmax loss: the workspace must be 256-byte aligned");
   DeviceGuard guard(device);
@@ -1414,9 +1422,10 @@ int dispatch(int device, void* stream, int type, const void* x, int64_t ldx, con
   c.targets = {target, target64, n};
   c.scale = scale;
   c.ws = (char*)ws;
-  if (type == F32) return run<F32>(c, x, ldx, w, ldw, loss, lse, total, mean, fwd, g, dx, lddx, dw, lddw);
-  if (type == BF16) return run<BF16>(c, x, ldx, w, ldw, loss, lse, total, mean, fwd, g, dx, lddx, dw, lddw);
-  return run<F16>(c, x, ldx, w, ldw, loss, lse, total, mean, fwd, g, dx, lddx, dw, lddw);
+  if (as_floats) return run<F32, F16>(c, x, ldx, w, ldw, loss, lse, total, mean, fwd, g, dx, lddx, dw, lddw);
+  if (type == F32) return run<F32, F32>(c, x, ldx, w, ldw, loss, lse, total, mean, fwd, g, dx, lddx, dw, lddw);
+  if (type == BF16) return run<BF16, BF16>(c, x, ldx, w, ldw, loss, lse, total, mean, fwd, g, dx, lddx, dw, lddw);
+  return run<F16, F16>(c, x, ldx, w, ldw, loss, lse, total, mean, fwd, g, dx, lddx, dw, lddw);
 }
 
 }  // namespace
@@ -1427,9 +1436,13 @@ extern "C" int blp_softmax_loss_workspace(int type, const void* x, int64_t ldx, 
   if (rc) return rc;
   BLP_CHECK(bytes, BLP_E_ARG, "softmax loss: null pointer");
   const int es = size_of(type);
-  *bytes = plan_of(type, rows, cols, k, forward != 0, grads != 0, !aligned(x, ldx * es, (int64_t)k * es),
+  auto need = [&](int as) {
+    return plan_of(as, es, rows, cols, k, forward != 0, grads != 0, !aligned(x, ldx * es, (int64_t)k * es),
                    !aligned(table, ldt * es, (int64_t)k * es))
-               .bytes;
+        .bytes;
+  };
+  *bytes = need(type);
+  if (type == F16 && !forward && grads) *bytes = std::max(*bytes, need(F32));  // row gradients, if it gets them
   return 0;
 }
 

@@ -15,8 +15,9 @@ from test_gpu_latent_loss import U, _half_step, _torch, make, near
 pytestmark = pytest.mark.gpu
 
 
-def gradients(x, w, t, scale, gi, floor_dx):
-    """-> ((dx, bound), (dw, bound)) of row gradients gi (64 bits); floor_dx: what float16's lowest step leaves in a row's dS."""
+def gradients(x, w, t, scale, gi, floor_dx, floor_dw=None):
+    """-> ((dx, bound), (dw, bound)) of row gradients gi (64 bits); floor_dx, floor_dw: what float16's lowest step leaves of dS, in
+    units of 2^-39 (dw: of the largest gi)."""
     import torch
 
     X, W = x.double(), w.double()
@@ -41,9 +42,9 @@ def gradients(x, w, t, scale, gi, floor_dx):
         return a @ b.contiguous()
 
     out = []
-    for a, b, floor in ((lambda v: v, W, floor_dx), (lambda v: v.t(), X, gi.abs().max())):
+    for a, b, floor in ((lambda v: v, W, floor_dx), (lambda v: v.t(), X, gi.abs().max() if floor_dw is None else floor_dw)):
         want = scale * mm(a(d), b)
-        bound = abs(scale) * (mm(a(e + (floor * 2.0 ** -39 if half else 0.0)), b.abs()) + (max(x.shape[0], n) + 8) * U * mm(a(d).abs(), b.abs()))
+        bound = abs(scale) * (mm(a(e + floor * (2.0 ** -39 if half else 0.0)), b.abs()) + (max(x.shape[0], n) + 8) * U * mm(a(d).abs(), b.abs()))
         out.append((want, bound * (1 + 2 * h) + h * want.abs() + tiny))
     return out
 
@@ -106,3 +107,50 @@ def test_a_last_piece_of_fewer_slices(gpu, dtype, m, n, k):
     one = torch.ones(len(at), dtype=torch.float64, device="cuda")
     (want, bound), _ = gradients(x[at], w, t[at], 1.0, one, one[:, None])
     near(dx[at], want, bound)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("k", [40, 64, 100, 160, 328])
+def test_row_gradients_of_very_different_sizes(gpu, k, dtype):
+    """Three decades of row gradients beside some 10^9 times larger, of rows whose target has all of the softmax: these have no part
+    in dx or (but for component 0) in dtable, and the other rows' are as accurate as if they were alone."""
+    torch = _torch()
+    from blp import latent
+
+    m, n = 150, 400
+    x, w, t = make(m, n, k, getattr(torch, dtype), seed=k)
+    t %= n - 1
+    sure = torch.arange(m, device="cuda") % 10 == 3
+    x[:, 0], w[:, 0] = 0, 0
+    w[n - 1] = 0
+    w[n - 1, 0] = 30  # the row that the sure ones are sure of: a score of 240 there, 0 everywhere else
+    x[sure] = 0
+    x[sure, 0] = 8
+    t[sure] = n - 1
+    g = torch.logspace(-3, 0, m, device="cuda") * torch.where(torch.arange(m, device="cuda") % 2 == 0, 1.0, -1.0)
+    g[sure] *= 1e9
+    lse = torch.logsumexp(x.double() @ w.double().t().contiguous(), 1).float()
+    got = latent.softmax_loss_backward(g, lse, None, x, w, t)
+    zero = torch.zeros((), dtype=torch.float64, device="cuda")
+    (want_x, bound_x), (want_w, bound_w) = gradients(x, w, t, 1.0, g.double(), zero, zero)
+    near(got[0][~sure], want_x[~sure], bound_x[~sure])
+    near(got[1][:, 1:], want_w[:, 1:], bound_w[:, 1:])
+    # without the sure rows: the same row gradients of x
+    alone = latent.softmax_loss_backward(torch.where(sure, 0.0, g), lse, None, x, w, t)
+    near(alone[0][~sure], want_x[~sure], bound_x[~sure])
+
+
+@pytest.mark.parametrize("k", [8, 64, 72, 200])
+def test_workspace_of_row_gradients(gpu, k):
+    """float16 with one gradient and with one a row, of the same sizes, on strided rows."""
+    torch = _torch()
+    from blp import latent
+
+    m, n = 90, 700
+    x, w, t = make(m, n, k + 5, torch.float16, seed=k)
+    x, w = x[:, 3:3 + k], w[:, 2:2 + k]
+    lse = torch.logsumexp(x.double() @ w.double().t().contiguous(), 1).float()
+    for g in (torch.full((), 0.5, device="cuda"), torch.full((m,), 0.5, device="cuda")):
+        half = torch.full((m,), 0.5, dtype=torch.float64, device="cuda")
+        for got, (want, bound) in zip(latent.softmax_loss_backward(g, lse, None, x, w, t), gradients(x, w, t, 1.0, half, half[:, None])):
+            near(got, want, bound)
