@@ -446,9 +446,10 @@ int blp_walk_stats(blp_walk* w, double* total_ms, int64_t* launches);
  *     With grads also dx (rows x k) and dtable (cols x k), either may be NULL: the gradients of the sum
  *     of the losses (of the mean when total and mean are given), each rounded to `type` once: the
  *     softmax differences that they sum are held as two halves (2^-16 of each for bfloat16, 2^-22 for
- *     float16, down to 2^-39 of the largest row gradient there) or, for float32, as three (2^-24).
+ *     float16, where they end at 2^-39) or, for float32, as three (2^-24).
  *   blp_softmax_loss_backward: the gradients from lse: row i's gradient is grad[i * grad_stride] (NULL:
- *     1; grad_stride 0 or 1) divided by *count (NULL: 1).                                     */
+ *     1; grad_stride 0 or 1) divided by *count (NULL: 1). float16 rows with gradients of their own are
+ *     multiplied as float32 ones are, so that small gradients beside large ones keep their digits. */
 #define BLP_F32 0
 #define BLP_BF16 1
 #define BLP_F16 2
