@@ -28,6 +28,7 @@ _lib.register("blp_scores8_workspace", [_P, _I64, _P, _I64, _I64, _I64, _I32, _P
 _lib.register("blp_scores8", [_I32, _P, _P, _I64, _P, _P, _I64, _P, _I64, _I64, _I32, _I32, _P, _I64, _P, _I64])
 
 _torch = None
+_forward_ad = None
 _TYPES = {}   # torch dtype -> BLP_F32 / BLP_BF16 / BLP_F16
 _INT8 = {}
 _stream = None
@@ -35,9 +36,10 @@ _stream = None
 
 def _t():
     """torch, imported on the first call: the graph engine works without it."""
-    global _torch, _stream
+    global _torch, _forward_ad, _stream
     if _torch is None:
         import torch
+        from torch.autograd import forward_ad as _forward_ad
 
         _TYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
         _INT8[torch.int8] = 3
@@ -52,9 +54,18 @@ def _say(t):
     return "%s %s on %s" % (tuple(t.shape), t.dtype, t.device) if isinstance(t, _torch.Tensor) else str(type(t))
 
 
+def _no_tangent(t, what):
+    """Refuse a dual tensor of forward-mode differentiation: the kernels see its values alone, and a result without a tangent
+    would be a derivative of zero. (Outside of a level there are none: that is all the common path looks at.)"""
+    if getattr(_forward_ad, "_current_level", 0) >= 0 and isinstance(t, _torch.Tensor) \
+            and _forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError("%s: forward-mode derivatives are not implemented" % what)
+
+
 def _rows(t, what, dtypes):
     """The row stride of `t`, checked to be (n, k) rows: a 2-d tensor on a GPU whose rows are contiguous and do not
     overlap."""
+    _no_tangent(t, what)
     if not (isinstance(t, _torch.Tensor) and t.dtype in dtypes and t.is_cuda and t.dim() == 2):
         raise ValueError("%s must be a 2-d GPU tensor of %s (got %s)" % (
             what, " / ".join(str(d)[6:] for d in dtypes), _say(t)))
@@ -76,6 +87,7 @@ def _ids(t, what, device, n=None):
 
 
 def _floats(t, what, device, shapes):
+    _no_tangent(t, what)
     if not (isinstance(t, _torch.Tensor) and t.dtype == _torch.float32 and t.device == device and t.is_contiguous()
             and t.shape in shapes):
         raise ValueError("%s must be a contiguous float32 tensor of shape %s on %s (got %s)" % (

@@ -1,0 +1,72 @@
+"""What blp.latent's calls refuse before they look at a device: transformations that would see only the allocation of their outputs,
+and tensors whose memory is not their value."""
+import pytest
+
+from blp import latent
+
+torch = pytest.importorskip("torch")
+
+
+def calls(x, ids):
+    """-> every entry point, as a call of the float tensor x (n, k)"""
+    one = torch.ones(len(x))
+    return {
+        "softmax_loss": lambda: latent.softmax_loss(x, torch.ones_like(x.detach()), ids),
+        "softmax_loss_grad": lambda: latent.softmax_loss_grad(x, x, ids),
+        "softmax_loss_backward": lambda: latent.softmax_loss_backward(one, one, None, x, x, ids),
+        "lookup": lambda: latent.lookup(x, ids),
+        "lookup_grad": lambda: latent.lookup_grad(x, ids, 5),
+        "quantize_rows": lambda: latent.quantize_rows(x),
+    }
+
+
+NAMES = sorted(calls(torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64)))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_is_refused(name):
+    """A dual tensor does not require a gradient: a result without its tangent would be a derivative of zero."""
+    from torch.autograd import forward_ad
+
+    x, ids = torch.randn(4, 8), torch.zeros(4, dtype=torch.int64)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            calls(dual, ids)[name]()
+    with pytest.raises(ValueError, match="GPU"):  # outside of it: a tensor on the host
+        calls(x, ids)[name]()
+
+
+def test_forward_mode_of_scales_is_refused():
+    from torch.autograd import forward_ad
+
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(torch.ones(4), torch.ones(4))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            latent._t()
+            latent._floats(dual, "s", dual.device, ((4,),))
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused_for_every_argument(gpu):
+    from torch.autograd import forward_ad
+
+    x, ids, q = torch.randn(4, 8, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda"), torch.ones(
+        4, 8, dtype=torch.int8, device="cuda")
+    one = torch.ones(4, device="cuda")
+    with forward_ad.dual_level():
+        d, done = forward_ad.make_dual(x, x), forward_ad.make_dual(one, one)
+        for call in (lambda: latent.softmax_loss(x, d, ids), lambda: latent.softmax_loss(d.clone().requires_grad_(), x, ids),
+                     lambda: latent.softmax_loss_grad(x, d, ids), lambda: latent.softmax_loss_backward(done, one, None, x, x, ids),
+                     lambda: latent.softmax_loss_backward(one, done, None, x, x, ids), lambda: latent.lookup(d, ids),
+                     lambda: latent.lookup_grad(x, ids, 4, into=d), lambda: latent.int8_scores(q, done, q, one),
+                     lambda: latent.int8_scores(q, one, q, done)):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()
+        assert latent.lookup(x, ids).shape == (4, 8)  # others go through
+    # the transformations that wrap their tensors refuse by themselves
+    for call in (lambda: torch.func.jvp(lambda a: latent.lookup(a, ids), (x,), (x,)),
+                 lambda: torch.func.vmap(lambda a: latent.softmax_loss(a, x, ids))(x[None]),
+                 lambda: torch.func.grad(lambda a: latent.softmax_loss(a, x, ids))(x)):
+        with pytest.raises(RuntimeError):
+            call()
