@@ -54,9 +54,13 @@ def _say(t):
     return "%s %s on %s" % (tuple(t.shape), t.dtype, t.device) if isinstance(t, _torch.Tensor) else str(type(t))
 
 
-def _no_tangent(t, what):
-    """Refuse a dual tensor of forward-mode differentiation: the kernels see its values alone, and a result without a tangent
-    would be a derivative of zero. (Outside of a level there are none: that is all the common path looks at.)"""
+def _plain(t, what):
+    """Refuse what the kernels, which see a tensor's memory alone, would answer wrongly without an error. A dual tensor of forward-mode
+    differentiation: a result without a tangent would be a derivative of zero (outside of a level there are none: that is
+    all the common path looks at). A traced one: the trace would hold the allocation of the outputs and nothing that fills
+    them (sizes are numbers, but tensors while torch.jit traces)."""
+    if isinstance(t, _torch.Tensor) and t.dim() and type(t.shape[0]) is not int:
+        raise RuntimeError("%s: this call cannot be traced" % what)
     if getattr(_forward_ad, "_current_level", 0) >= 0 and isinstance(t, _torch.Tensor) \
             and _forward_ad.unpack_dual(t).tangent is not None:
         raise RuntimeError("%s: forward-mode derivatives are not implemented" % what)
@@ -65,7 +69,7 @@ def _no_tangent(t, what):
 def _rows(t, what, dtypes):
     """The row stride of `t`, checked to be (n, k) rows: a 2-d tensor on a GPU whose rows are contiguous and do not
     overlap."""
-    _no_tangent(t, what)
+    _plain(t, what)
     if not (isinstance(t, _torch.Tensor) and t.dtype in dtypes and t.is_cuda and t.dim() == 2):
         raise ValueError("%s must be a 2-d GPU tensor of %s (got %s)" % (
             what, " / ".join(str(d)[6:] for d in dtypes), _say(t)))
@@ -87,7 +91,7 @@ def _ids(t, what, device, n=None):
 
 
 def _floats(t, what, device, shapes):
-    _no_tangent(t, what)
+    _plain(t, what)
     if not (isinstance(t, _torch.Tensor) and t.dtype == _torch.float32 and t.device == device and t.is_contiguous()
             and t.shape in shapes):
         raise ValueError("%s must be a contiguous float32 tensor of shape %s on %s (got %s)" % (

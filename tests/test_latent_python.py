@@ -70,3 +70,29 @@ def test_forward_mode_is_refused_for_every_argument(gpu):
                  lambda: torch.func.grad(lambda a: latent.softmax_loss(a, x, ids))(x)):
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tracing_is_refused(name):
+    """A trace would record the allocation of the outputs, and nothing that fills them."""
+    ids = torch.zeros(4, dtype=torch.int64)
+
+    def traced(x):
+        with pytest.raises(RuntimeError, match="traced"):
+            calls(x, ids)[name]()
+        return x
+
+    torch.jit.trace(traced, torch.randn(4, 8), check_trace=False)
+
+
+@pytest.mark.gpu
+def test_tracing_is_refused_on_the_device(gpu):
+    x, ids, q = torch.randn(4, 8, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda"), torch.ones(
+        4, 8, dtype=torch.int8, device="cuda")
+    for call in (lambda a: latent.lookup(a, ids), lambda a: latent.softmax_loss(a, x, ids), lambda a: latent.softmax_loss(x, a, ids),
+                 lambda a: latent.int8_scores(q, a[:, 0].contiguous(), q, a[:, 0].contiguous())):
+        for arg in (x, x.clone().requires_grad_()):
+            with pytest.raises(RuntimeError, match="traced"):
+                torch.jit.trace(call, arg, check_trace=False)
+    fn = torch.compile(lambda a: latent.softmax_loss(a, x, ids) * 2, backend="eager")  # falls back to running the call
+    assert torch.equal(fn(x), latent.softmax_loss(x, x, ids) * 2)
