@@ -236,7 +236,8 @@ def lookup_grad(grad, ids, n_rows, scale=1.0, into=None):
     """The gradient of :func:`lookup` in its table: (n_rows, k) with row r = scale * the sum of grad[i] over
     ids[i] == r, in 32 bits and ascending i (the same every time), rounded to grad's type once; rows
     without ids are zero. grad: ids.shape + (k,). With `into` (n_rows, k) the sums are added to what it
-    holds -- e.g. the softmax loss's gradient of the same table -- and it is returned."""
+    holds -- e.g. the softmax loss's gradient of the same table -- and it is returned; to autograd that is a change
+    in place, and `into` must not require a gradient (but under torch.no_grad)."""
     torch = _t()
     if not isinstance(grad, torch.Tensor) or not isinstance(ids, torch.Tensor) or grad.dim() < 1 \
             or tuple(grad.shape[:-1]) != tuple(ids.shape):
@@ -255,6 +256,8 @@ def lookup_grad(grad, ids, n_rows, scale=1.0, into=None):
         out, ldo = grad.new_empty(n_rows, k), k
     else:
         out, ldo = into, _rows(into, "into", (grad.dtype,))
+        if into.requires_grad and torch.is_grad_enabled():
+            raise ValueError("into must not require a gradient: the sums are added without a record of it")
         if tuple(into.shape) != (n_rows, k) or into.device != grad.device:
             raise ValueError("into must be of shape %s on %s" % ((n_rows, k), grad.device))
         if n and into.data_ptr() < grad.data_ptr() + ((n - 1) * ld + k) * grad.element_size() \
@@ -266,6 +269,8 @@ def lookup_grad(grad, ids, n_rows, scale=1.0, into=None):
     check(lib().blp_lookup_grad(grad.device.index, _stream(grad.device.index), _TYPES[grad.dtype], grad.data_ptr(), ld,
                                 ids.data_ptr(), wide, n, n_rows, k, _scale(scale), out.data_ptr(), ldo,
                                 0 if into is None else 1, ws.data_ptr(), ws.numel()))
+    if into is not None:
+        torch.autograd.graph.increment_version(into)  # autograd sees that what it may have kept of `into` has changed
     return out
 
 

@@ -217,3 +217,27 @@ def test_refusals(gpu):
                 lambda: latent.lookup_grad(grad, ids, 10, into=torch.zeros(10, 8, device="cuda", dtype=torch.float16))):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("n", [100, 9000])
+def test_into_counts_as_changed(gpu, n):
+    torch = _torch()
+    from blp import latent
+
+    grad, ids = torch.randn(n, 8, device="cuda"), torch.randint(0, 20, (n,), device="cuda")
+    into, p = torch.zeros(20, 8, device="cuda"), torch.randn(20, 8, device="cuda", requires_grad=True)
+    loss = (into * p).sum()  # autograd keeps `into`
+    before = into._version
+    latent.lookup_grad(grad, ids, 20, into=into)
+    assert into._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+    wide = torch.zeros(20, 12, device="cuda")
+    loss = (wide * torch.randn(20, 12, device="cuda", requires_grad=True)).sum()
+    latent.lookup_grad(grad, ids, 20, into=wide[:, 2:10])  # a view: what it is a view of has changed
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+    with pytest.raises(ValueError, match="require"):
+        latent.lookup_grad(grad, ids, 20, into=p)
+    with torch.no_grad():
+        latent.lookup_grad(grad, ids, 20, into=p)
