@@ -58,12 +58,16 @@ def _plain(t, what):
     """Refuse what the kernels, which see a tensor's memory alone, would answer wrongly without an error. A dual tensor of forward-mode
     differentiation: a result without a tangent would be a derivative of zero (outside of a level there are none: that is
     all the common path looks at). A traced one: the trace would hold the allocation of the outputs and nothing that fills
-    them (sizes are numbers, but tensors while torch.jit traces)."""
-    if isinstance(t, _torch.Tensor) and t.dim() and type(t.shape[0]) is not int:
+    them (sizes are numbers, but tensors while torch.jit traces). A negated view (z.conj().imag): its memory holds the
+    values before the sign."""
+    if not isinstance(t, _torch.Tensor):
+        return
+    if t.dim() and type(t.shape[0]) is not int:
         raise RuntimeError("%s: this call cannot be traced" % what)
-    if getattr(_forward_ad, "_current_level", 0) >= 0 and isinstance(t, _torch.Tensor) \
-            and _forward_ad.unpack_dual(t).tangent is not None:
+    if getattr(_forward_ad, "_current_level", 0) >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
         raise RuntimeError("%s: forward-mode derivatives are not implemented" % what)
+    if t.is_neg():
+        raise ValueError("%s must not be a negated view (resolve_neg() makes a tensor of it)" % what)
 
 
 def _rows(t, what, dtypes):

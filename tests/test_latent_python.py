@@ -96,3 +96,16 @@ def test_tracing_is_refused_on_the_device(gpu):
                 torch.jit.trace(call, arg, check_trace=False)
     fn = torch.compile(lambda a: latent.softmax_loss(a, x, ids) * 2, backend="eager")  # falls back to running the call
     assert torch.equal(fn(x), latent.softmax_loss(x, x, ids) * 2)
+
+
+@pytest.mark.gpu
+def test_negated_views_are_refused(gpu):
+    ids = torch.zeros(4, dtype=torch.int64, device="cuda")
+    neg = torch.complex(torch.zeros(4, 1, device="cuda"), torch.ones(4, 1, device="cuda")).conj().imag
+    assert neg.is_neg() and neg[0] == -1
+    one, q = torch.ones(1, device="cuda"), torch.ones(1, 8, dtype=torch.int8, device="cuda")
+    for call in (lambda: latent.lookup(neg, ids), lambda: latent.lookup_grad(neg, ids, 4), lambda: latent.quantize_rows(neg),
+                 lambda: latent.softmax_loss(neg, neg, ids), lambda: latent.int8_scores(q, neg[0], q, one)):
+        with pytest.raises(ValueError, match="negat"):
+            call()
+    assert torch.equal(latent.lookup(neg.resolve_neg(), ids), -torch.ones(4, 1, device="cuda"))
