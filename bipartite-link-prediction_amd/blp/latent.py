@@ -6,12 +6,13 @@ They stand beside :class:`blp.factor.DeviceSVD`, whose factors they read, train 
 user table and of a business table, ``k`` components a row. Every argument that holds data is a torch
 tensor on one GPU, its rows contiguous (a row stride larger than the row is fine); the work is queued
 on torch's current stream of that device, workspaces come from torch's allocator, and nothing waits
-for the device. Wrong arguments raise ValueError before anything is queued.
+for the device. Wrong arguments raise ValueError before anything is queued: row strides of the loss's operands past 2^20
+elements and of 8-bit ones past 2^22 are among them.
 """
 import ctypes
 
 from . import _lib
-from ._lib import check, lib
+from ._lib import BLPError, lib
 
 _P, _I64, _I32, _F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
 _PI64 = ctypes.POINTER(ctypes.c_int64)
@@ -26,6 +27,16 @@ _lib.register("blp_lookup_grad", [_I32, _P, _I32, _P, _I64, _P, _I32, _I64, _I64
 _lib.register("blp_quantize_rows", [_I32, _P, _I32, _P, _I64, _I64, _I32, _P, _I64, _P])
 _lib.register("blp_scores8_workspace", [_P, _I64, _P, _I64, _I64, _I64, _I32, _PI64])
 _lib.register("blp_scores8", [_I32, _P, _P, _I64, _P, _P, _I64, _P, _I64, _I64, _I32, _I32, _P, _I64, _P, _I64])
+
+class ArgumentError(BLPError, ValueError):
+    """Arguments that the library refuses (BLP_E_ARG): sizes and strides past its limits."""
+
+
+def check(rc):
+    if rc == -1:
+        raise ArgumentError(rc, lib().blp_last_error().decode(errors="replace"))
+    return _lib.check(rc)
+
 
 _torch = None
 _forward_ad = None

@@ -438,7 +438,7 @@ int blp_walk_stats(blp_walk* w, double* total_ms, int64_t* launches);
  *   z_ij = scale x_i . table_j     lse_i = log sum_j exp z_ij     loss_i = lse_i - z_{i, target_i}
  * target: int32, or int64 with target64; outside [0, cols) the row is ignored (loss 0, gradient 0,
  * whatever x holds). The scores are not kept: the workspace holds one piece of the catalogue's.
- * rows and cols up to 2^31 - 2^16, k up to 2^20.
+ * rows and cols up to 2^31 - 2^16, k up to 2^20, row strides of x and table up to 2^20 elements.
  *   blp_softmax_loss_workspace: bytes of workspace (256-byte aligned) for the same arguments;
  *     `forward` / `grads`: whether the call runs the forward / the backward pass.
  *   blp_softmax_loss: loss[rows], lse[rows] (float); total (or NULL): total[0] = the sum of the losses
@@ -484,7 +484,8 @@ int blp_lookup_grad(int device, void* stream, int type, const void* grad, int64_
  *     min(ldq, k rounded up to 16) of a row of q are set to 0.
  *   blp_scores8: out[i][j] = s[i] ts[j] sum_k q[i][k] table[j][k], k < 2^17: the sum exact in 32-bit
  *     integers, the rest in float, rounded to out_type once. out is aligned to its elements. A workspace
- *     of 0 bytes may be NULL. Row strides that are multiples of 16 bytes need no copy.       */
+ *     of 0 bytes may be NULL. Row strides of q and table are at most 2^22; multiples of 16 bytes need
+ *     no copy.                                                                                    */
 int blp_quantize_rows(int device, void* stream, int type, const void* x, int64_t ldx, int64_t rows, int k, int8_t* q,
                       int64_t ldq, float* s);
 int blp_scores8_workspace(const int8_t* q, int64_t ldq, const int8_t* table, int64_t ldt, int64_t rows, int64_t cols, int k,

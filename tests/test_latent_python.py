@@ -109,3 +109,27 @@ def test_negated_views_are_refused(gpu):
         with pytest.raises(ValueError, match="negat"):
             call()
     assert torch.equal(latent.lookup(neg.resolve_neg(), ids), -torch.ones(4, 1, device="cuda"))
+
+
+def test_arguments_that_the_library_refuses_are_value_errors():
+    from blp import _lib
+
+    latent._t()
+    for args in ((0, None, 0, 256, 8, 5, 8, 256, 0, 3, float("inf"), 256, 8), (0, None, 0, 256, 8, 1 << 31, 8, 256, 0, 3, 1.0, 256, 8)):
+        with pytest.raises(ValueError) as e:
+            latent.check(_lib.lib().blp_lookup(*args))
+        assert isinstance(e.value, _lib.BLPError) and e.value.code == -1
+
+
+@pytest.mark.gpu
+def test_far_strides_are_value_errors(gpu):
+    far = torch.zeros(2, (1 << 20) + 8, dtype=torch.float16, device="cuda")[:, :8]
+    t = torch.zeros(2, dtype=torch.int64, device="cuda")
+    w = torch.zeros(5, 8, dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError, match="stride"):
+        latent.softmax_loss(far, w, t)
+    q = torch.zeros(2, (1 << 22) + 16, dtype=torch.int8, device="cuda")[:, :16]
+    with pytest.raises(ValueError, match="stride"):
+        latent.int8_scores(q, torch.ones(2, device="cuda"), q, torch.ones(2, device="cuda"))
+    with pytest.raises(ValueError, match="scale"):
+        latent.lookup(w, t, 1e39)
