@@ -320,8 +320,8 @@ struct RowGrad {
     if (!(fabsf(v) <= FLT_MAX)) return v;  // an infinite or NaN gradient: its row's, and the catalogue's
     return t > 0.f ? v / t * extra : 0.f;
   }
-  __device__ float all() const {
-    const float f = (g ? (stride ? *top : *g) : 1.f) / extra;
+  __device__ double all() const {  // in 64 bits: times a scale it may leave the floats' range where the gradient does not
+    const double f = (g ? (stride ? *top : *g) : 1.f) / (double)extra;
     return count ? f / *count : f;
   }
 };
@@ -424,9 +424,14 @@ struct EpiOut {
   template <class S>
   __device__ void run(f32x4 (&acc)[S::FP][S::FQ], int64_t p0, int64_t q0, int, int, lds_char* scratch) const {
     if (p0 >= np || q0 >= nq) return;
-    const float alpha = scale * g.all();
+    const double alpha = scale * g.all();
     const int left = (int)min(np - p0, (int64_t)(S::FP * 16)), rows = (int)min(nq - q0, (int64_t)(S::FQ * 16));
-    store_block<T, S>(scratch, out + q0 * ld + p0 * size_of(T), ld, left, rows, [&](int i, int j) { return acc[i][j] * alpha; });
+    store_block<T, S>(scratch, out + q0 * ld + p0 * size_of(T), ld, left, rows, [&](int i, int j) {
+      f32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (float)(acc[i][j][e] * alpha);
+      return v;
+    });
   }
 };
 
@@ -466,7 +471,7 @@ struct SumArgs {
 };
 
 template <int T, int G>
-__device__ inline void sum_rows(const SumArgs& a, int64_t np, FastDiv per, float alpha, unsigned block, f32x4* s_sum) {
+__device__ inline void sum_rows(const SumArgs& a, int64_t np, FastDiv per, double alpha, unsigned block, f32x4* s_sum) {
   constexpr int V = 256 / G;
   const int64_t n = a.nq * per.d;
   const int v = threadIdx.x & (V - 1), gr = threadIdx.x / V;
@@ -488,7 +493,7 @@ __device__ inline void sum_rows(const SumArgs& a, int64_t np, FastDiv per, float
     if (i < n) {
       const int64_t q = n < (1ll << 31) ? (int64_t)per((uint32_t)i) : i / per.d, p = (i - q * per.d) * 4;
       for (int e = 0; e < 4; ++e)
-        if (p + e < np) store1<T>(a.out + q * a.ldo + (p + e) * size_of(T), sum[e] * alpha);
+        if (p + e < np) store1<T>(a.out + q * a.ldo + (p + e) * size_of(T), (float)(sum[e] * alpha));
     }
   }
 }
@@ -496,7 +501,7 @@ __device__ inline void sum_rows(const SumArgs& a, int64_t np, FastDiv per, float
 template <int T, int G>
 __global__ __launch_bounds__(256) void k_sum_parts(SumArgs a, SumArgs b, int64_t np, FastDiv per, RowGrad g, float scale) {
   __shared__ f32x4 s_sum[G > 1 ? 256 : 1];
-  const float alpha = scale * g.all();
+  const double alpha = scale * g.all();
   if (blockIdx.x < a.blocks)
     sum_rows<T, G>(a, np, per, alpha, blockIdx.x, s_sum);
   else

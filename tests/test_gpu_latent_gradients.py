@@ -36,7 +36,7 @@ def gradients(x, w, t, scale, gi, floor_dx, floor_dw=None):
     r = 2 * (k + 4) * U * S + (64 + n / 64 + 16) * U + 4 * U * (S + lse.abs())
     e = gi.abs()[:, None] * (p * r[:, None] + 2 * U) + h2 * d.abs()
     half = x.dtype == torch.float16
-    tiny = 2.0 ** -25 if half else 0.0
+    tiny = torch.finfo(x.dtype).tiny * torch.finfo(x.dtype).eps / 2  # half the lowest step: results below the normal numbers
 
     def mm(a, b):
         return a @ b.contiguous()
@@ -154,3 +154,23 @@ def test_workspace_of_row_gradients(gpu, k):
         half = torch.full((m,), 0.5, dtype=torch.float64, device="cuda")
         for got, (want, bound) in zip(latent.softmax_loss_backward(g, lse, None, x, w, t), gradients(x, w, t, 1.0, half, half[:, None])):
             near(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("k", [8, 64, 128, 200])
+def test_gradients_where_scale_and_gradient_pass_the_floats(gpu, k, dtype):
+    """scale / count is no normal number, or scale times the loss's gradient is infinite; the gradients themselves are floats."""
+    torch = _torch()
+    from blp import latent
+
+    m, n = 12, 20
+    x, w, t = make(m, n, k, getattr(torch, dtype), seed=k)
+    one = torch.ones(m, dtype=torch.float64, device="cuda")
+    X, W = x * 2.0 ** 50, w * 2.0 ** 50
+    for scale in (2.0 ** -130, 2.0 ** -127, -(2.0 ** -128)):
+        for p, (want, bound) in zip(latent.softmax_loss_grad(X, W, t, scale=scale)[1:], gradients(X, W, t, scale, one / m, one[:, None])):
+            near(p, want, bound)
+    X, W, top = x * 2.0 ** -20, w * 2.0 ** -100, torch.full((), 2.0 ** 100, device="cuda")
+    lse = torch.logsumexp(2.0 ** 100 * (X.double() @ W.double().t().contiguous()), 1).float()
+    dx, _ = latent.softmax_loss_backward(top, lse, None, X, W, t, scale=2.0 ** 100, need_table=False)
+    near(dx, *gradients(X, W, t, 2.0 ** 100, one * 2.0 ** 100, one[:, None])[0])
