@@ -597,7 +597,7 @@ __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowAr
   const int64_t own0 = (int64_t)own_tile * (64 * FO) + wave * (16 * FO);
   const int64_t s0 = split * a.range, s1 = min(a.stream.rows, s0 + a.range);
   const int stages = (int)((s1 - s0 + 63) >> 6);
-  const float c = fmaxf(fabsf(a.scale) * LOG2E, 1.2e-38f);  // positive: -inf c is -inf for a scale of 0, too
+  const float c = fabsf(a.scale) * LOG2E;
   const Operand stream = {a.stream.base, a.stream.ld, s1};
 
   frag_t own[PL][FO][KS];
@@ -754,8 +754,7 @@ __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowAr
             for (int e = 0; e < 4; ++e) {
               const int r = first + i * 16 + e;
               if (r == target[j] && r < (int)s1) a.hit[own0 + j * 16 + l] = acc[i][j][e] * fabsf(a.scale);
-              if (r >= (int)s1) acc[i][j][e] = -INFINITY;  // past the range's end: zeros in LDS
-              high = fmaxf(high, acc[i][j][e]);
+              if (r < (int)s1) high = fmaxf(high, acc[i][j][e]);  // past the range's end: zeros in LDS
             }
           if (high > top[j]) {
             if (top[j] != -INFINITY) sum[j] *= __builtin_amdgcn_exp2f((top[j] - high) * c);
@@ -765,7 +764,8 @@ __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowAr
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum[j] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, shift[j]));
+            for (int e = 0; e < 4; ++e)
+              if (first + i * 16 + e < (int)s1) sum[j] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], c, shift[j]));
         }
       }
     } else {
@@ -1413,6 +1413,7 @@ int dispatch(int device, void* stream, int type, const void* x, int64_t ldx, con
   const int es = size_of(type);
   BLP_CHECK(w && (m == 0 || (x && target && loss && lse)) && ws, BLP_E_ARG, "softmax loss: null pointer");
   BLP_CHECK(fabsf(scale) <= 3.4028235e38f, BLP_E_ARG, "softmax loss: scale must be finite");
+  BLP_CHECK(fabsf(scale) <= 0x1p127f, BLP_E_ARG, "softmax loss: scale must be at most 2^127 (times log2 e it has to be a float)");
   BLP_CHECK(ldx >= k && ldw >= k && (!dx || lddx >= k) && (!dw || lddw >= k), BLP_E_ARG,
             "softmax loss: a row stride is smaller than k");
   BLP_CHECK(std::max(ldx, ldw) <= (1 << 20), BLP_E_ARG, "softmax loss: row strides must be at most 2^20 elements");

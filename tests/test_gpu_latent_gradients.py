@@ -10,7 +10,7 @@ float16 holds dS times 2^14: its lowest step leaves 2^-25 2^-14 = 2^-39 of the l
 """
 import pytest
 
-from test_gpu_latent_loss import U, _half_step, _torch, make, near
+from test_gpu_latent_loss import U, _half_step, _torch, make, near, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -174,3 +174,20 @@ def test_gradients_where_scale_and_gradient_pass_the_floats(gpu, k, dtype):
     lse = torch.logsumexp(2.0 ** 100 * (X.double() @ W.double().t().contiguous()), 1).float()
     dx, _ = latent.softmax_loss_backward(top, lse, None, X, W, t, scale=2.0 ** 100, need_table=False)
     near(dx, *gradients(X, W, t, 2.0 ** 100, one * 2.0 ** 100, one[:, None])[0])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("k", [8, 64, 128, 200])
+def test_scales_next_to_zero(gpu, k, dtype):
+    """Products next to the largest float times scales next to its smallest: 0 is 0, and 2^-130 is itself."""
+    torch = _torch()
+    from blp import latent
+    m, n = 40, 333
+    x, w, t = make(m, n, k, getattr(torch, dtype), seed=k)
+    x, w = x * 2.0 ** 62, w * (2.0 ** 62 * k ** 0.5 / k)
+    for scale in (0.0, 2.0 ** -130, 2.0 ** -126, -(2.0 ** -128)):
+        ref = reference(x, w, t, scale)
+        near(latent.softmax_loss(x, w, t, scale=scale, reduction="none"), ref["loss"], ref["b_loss"])
+        total, dx, dw = latent.softmax_loss_grad(x, w, t, scale=scale)
+        near(dx, ref["dx"], ref["b_dx"] + 2.0 ** -133)
+        near(dw, ref["dw"], ref["b_dw"] + 2.0 ** -133)

@@ -63,3 +63,13 @@ def test_the_status_of_every_launch_is_returned(name):
     for i, got in zip(at, run([(fn, args, (i, 2)) for i in at])):
         assert got["rc"] != 0 and got["error"], "launch %d of %d (%s) failed unseen" % (i, n, whole["launches"][i]["name"])
         assert len(got["launches"]) == i + 1
+
+
+@pytest.mark.parametrize("scale", [2e38, 3.4e38, -3e38])
+def test_scales_whose_product_with_log2_e_is_no_float_are_refused(scale):
+    fn, args, _ = loss(1, 100, 300, 64)
+    args[12] = scale
+    (got,) = run([(fn, args, None)])
+    assert got["rc"] == -1 and "scale" in got["error"] and not got["launches"]
+    args[12] = 2.0 ** 127
+    assert run([(fn, args, None)])[0]["rc"] == 0
