@@ -111,13 +111,19 @@ __global__ __launch_bounds__(256) void k_quantize(const char* __restrict__ x, in
 }
 
 template <int T>
-void quantize(const void* x, int64_t ld, int64_t rows, int k, int kp, int8_t* q, int64_t ldq, float* s, hipStream_t st) {
+int quantize(const void* x, int64_t ld, int64_t rows, int k, int kp, int8_t* q, int64_t ldq, float* s, hipStream_t st) {
   constexpr int NE = Vec<T>::NE;
   int lanes = 1;
   while (lanes < 64 && lanes * NE < kp) lanes <<= 1;
-  const unsigned grid = (unsigned)((rows * lanes + 255) / 256);
-  (lanes * NE >= kp ? k_quantize<T, 1> : lanes * NE * 8 >= kp ? k_quantize<T, 8> : k_quantize<T, 0>)<<<grid, 256, 0, st>>>(
-      (const char*)x, ld * size_of(T), rows, k, kp, lanes, q, ldq, s);
+  const int64_t most = (1ll << 31) / lanes;  // rows of a launch, which takes less than 2^32 threads
+  for (int64_t r0 = 0; r0 < rows; r0 += most) {
+    const int64_t n = std::min(most, rows - r0);
+    const unsigned grid = (unsigned)((n * lanes + 255) / 256);
+    (lanes * NE >= kp ? k_quantize<T, 1> : lanes * NE * 8 >= kp ? k_quantize<T, 8> : k_quantize<T, 0>)<<<grid, 256, 0, st>>>(
+        (const char*)x + r0 * ld * size_of(T), ld * size_of(T), n, k, kp, lanes, q + r0 * ldq, ldq, s + r0);
+    BLP_HIP(hipGetLastError());
+  }
+  return 0;
 }
 
 // 8-bit rows as the tile engine takes them: whole granules, zeros past k.
@@ -550,14 +556,9 @@ extern "C" int blp_quantize_rows(int device, void* stream, int type, const void*
   if (guard.rc) return guard.rc;
   hipStream_t st = (hipStream_t)stream;
   const int kp = (int)std::min<int64_t>(ldq, (k + 15) / 16 * 16);
-  if (type == F32)
-    quantize<F32>(x, ldx, rows, k, kp, q, ldq, s, st);
-  else if (type == BF16)
-    quantize<BF16>(x, ldx, rows, k, kp, q, ldq, s, st);
-  else
-    quantize<F16>(x, ldx, rows, k, kp, q, ldq, s, st);
-  BLP_HIP(hipGetLastError());
-  return 0;
+  if (type == F32) return quantize<F32>(x, ldx, rows, k, kp, q, ldq, s, st);
+  if (type == BF16) return quantize<BF16>(x, ldx, rows, k, kp, q, ldq, s, st);
+  return quantize<F16>(x, ldx, rows, k, kp, q, ldq, s, st);
 }
 
 extern "C" int blp_scores8_workspace(const int8_t* q, int64_t ldq, const int8_t* table, int64_t ldt, int64_t rows, int64_t cols,

@@ -308,3 +308,18 @@ def test_training_step_then_scores(gpu):
         x, w = users[ids.clamp(min=0)].double().abs().sum(1), businesses.double().abs().sum(1)
         bound = 0.5 * x[:, None] * t.double() + 0.5 * s.double()[:, None] * w + 16.0 * s.double()[:, None] * t.double()
         assert bool(((got.double() - full).abs() <= bound * 1.0001).all())
+
+
+def test_more_rows_than_a_launch_takes(gpu):
+    """64 lanes a row: 2^25 rows are 2^31 threads, the most of a launch."""
+    torch = _torch()
+    from blp import latent
+
+    n, k, edge = (1 << 25) + 70, 513, 1 << 25
+    x = torch.empty(n, k, dtype=torch.bfloat16, device="cuda")
+    for at in range(0, n, 1 << 22):
+        x[at:at + (1 << 22)].normal_()
+    q, s = latent.quantize_rows(x)
+    for lo, hi in ((0, 100), (edge - 100, edge + 70), (n - 100, n)):
+        want_q, want_s = latent.quantize_rows(x[lo:hi])
+        assert torch.equal(q[lo:hi], want_q) and torch.equal(s[lo:hi], want_s)

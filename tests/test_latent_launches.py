@@ -73,3 +73,24 @@ def test_scales_whose_product_with_log2_e_is_no_float_are_refused(scale):
     assert got["rc"] == -1 and "scale" in got["error"] and not got["launches"]
     args[12] = 2.0 ** 127
     assert run([(fn, args, None)])[0]["rc"] == 0
+
+
+def quantize(type, rows, k):
+    return ("blp_quantize_rows", [0, None, type, ONE, k, rows, k, ONE, k, ONE], None)
+
+
+HUGE = {
+    # 2^26 rows of 64 lanes each: 2^32 threads
+    "quantize": [quantize(1, 1 << 26, 513), quantize(0, (1 << 27) + 5, 300), quantize(2, (1 << 31) - 1, 8), quantize(0, (1 << 31) - 1, 1 << 12)],
+    "lookup": [("blp_lookup", [0, None, 0, ONE, 1 << 20, 5000, 1 << 20, ONE, 1, 1 << 20, 2.0, ONE, 1 << 20], None),
+               lookup_grad(1, (1 << 31) - 1, 100, 8), lookup_grad(0, 5, (1 << 31) - 1, 8), lookup_grad(1, 1 << 24, 1000, 1 << 12)],
+}
+
+
+@pytest.mark.parametrize("name", HUGE)
+def test_sizes_that_are_accepted_are_launched(name):
+    """No launch has 2^32 threads or more, and none is refused by the runtime, at the largest sizes that memory could hold."""
+    for got in run(HUGE[name]):
+        assert got["rc"] == 0, got["error"]
+        for l in got["launches"]:
+            assert l["grid"][0] * l["block"][0] < 1 << 32, l
