@@ -447,7 +447,6 @@ Split split_of(int64_t rows, int64_t cols, int k) {
 template <class S, class Epi>
 int launch(Problem a, int slices, int stages, Epi epi, hipStream_t st) {
   const int64_t tp = div_up(a.p.rows, S::BP), tq = div_up(a.q.rows, S::BQ);
-  BLP_CHECK(tp * tq <= 0x7fffffff, BLP_E_ARG, "scores8: too many tiles for one launch");
   a.tiles_p = (int)tp;
   a.tiles_q = (int)tq;
   a.slice = stages;
@@ -462,6 +461,8 @@ int launch(const Problem& a, const Split& s, Epi epi, hipStream_t st) {
   if (s.tiles == BIG) return launch<Big>(a, s.n, s.stages, epi, st);
   return launch<Mid>(a, s.n, s.stages, epi, st);
 }
+
+constexpr int64_t MOST_BLOCKS = (1 << 23) - 1;  // of 512 threads: a launch takes less than 2^32 threads
 
 template <int TO>
 int scores(const Operand& w, const Operand& x, int k, const float* s, const float* t, void* out, int64_t ldo, char* ws, hipStream_t st) {
@@ -480,23 +481,26 @@ int scores(const Operand& w, const Operand& x, int k, const float* s, const floa
       const int64_t want = std::max<int64_t>(std::min<int64_t>(div_up(2560, groups), all / 4), 1);  // 10 workgroups a compute unit
       const int64_t steps = std::min<int64_t>(div_up(all, want), (1 << 29) / W);  // a strip's columns are counted in 31 bits
       const int64_t strips = div_up(all, steps);
-      BLP_CHECK(groups * strips <= 0x7fffffff, BLP_E_ARG, "scores8: too many tiles for one launch");
-      (k <= 64 ? k_strip8<TO, 1> : k_strip8<TO, 2>)<<<(unsigned)(groups * strips), 512, 0, st>>>(w, x, k, epi, (int)strips, (int)steps);
-      BLP_HIP(hipGetLastError());
-      return 0;
+      if (groups * strips <= MOST_BLOCKS) {
+        (k <= 64 ? k_strip8<TO, 1> : k_strip8<TO, 2>)<<<(unsigned)(groups * strips), 512, 0, st>>>(w, x, k, epi, (int)strips, (int)steps);
+        BLP_HIP(hipGetLastError());
+        return 0;
+      }
     }
     Problem o = a;
     o.tiles_p = (int)div_up(w.rows, TO == F32 ? 64 : 128);
     o.tiles_q = (int)div_up(x.rows, 128);
-    BLP_CHECK((int64_t)o.tiles_p * o.tiles_q <= 0x7fffffff, BLP_E_ARG, "scores8: too many tiles for one launch");
-    const unsigned grid = (unsigned)(o.tiles_p * o.tiles_q);
-    if (large)
-      k_outer8<TO, true><<<grid, 512, 0, st>>>(o, past);
-    else
-      k_outer8<TO, false><<<grid, 512, 0, st>>>(o, epi);
-    BLP_HIP(hipGetLastError());
-    return 0;
+    if ((int64_t)o.tiles_p * o.tiles_q <= MOST_BLOCKS) {
+      const unsigned grid = (unsigned)(o.tiles_p * o.tiles_q);
+      if (large)
+        k_outer8<TO, true><<<grid, 512, 0, st>>>(o, past);
+      else
+        k_outer8<TO, false><<<grid, 512, 0, st>>>(o, epi);
+      BLP_HIP(hipGetLastError());
+      return 0;
+    }
   }
+  // longer rows, and outputs of more than 2^37 scores: workgroups that take tile after tile
   const Split split = split_of(x.rows, w.rows, k);
   if (split.n == 1) return vectors && large ? launch(a, split, past, st) : launch(a, split, epi, st);
   const int64_t ld = up(w.rows, 4);
@@ -523,6 +527,7 @@ int check_args(int64_t rows, int64_t cols, int k) {
   BLP_CHECK(rows >= 0 && rows < (1ll << 31) && cols >= 1 && cols < (1ll << 31), BLP_E_ARG,
             "scores8: rows must be in [0, 2^31), columns in [1, 2^31)");
   BLP_CHECK(k >= 1 && k < (1 << 17), BLP_E_ARG, "scores8: k must be in [1, 2^17)");
+  BLP_CHECK(div_up(rows, 128) * div_up(cols, 128) < (1ll << 31), BLP_E_ARG, "scores8: rows x columns must be below 2^45");
   return 0;
 }
 

@@ -323,3 +323,25 @@ def test_more_rows_than_a_launch_takes(gpu):
     for lo, hi in ((0, 100), (edge - 100, edge + 70), (n - 100, n)):
         want_q, want_s = latent.quantize_rows(x[lo:hi])
         assert torch.equal(q[lo:hi], want_q) and torch.equal(s[lo:hi], want_s)
+
+
+def test_more_tiles_than_a_launch_takes(gpu):
+    """2^23 tiles of 512 threads are 2^32: workgroups that take tile after tile. 139 GB of scores."""
+    torch = _torch()
+    from blp import latent
+
+    m, n, k = 129, 1 << 29, 16
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 180e9:
+        pytest.skip("needs 180 GB of device memory")
+    q = torch.randint(-127, 128, (m, k), dtype=torch.int8, device="cuda")
+    p = torch.empty(n, k, dtype=torch.int8, device="cuda")
+    for at in range(0, n, 1 << 26):
+        p[at:at + (1 << 26)].random_(-127, 128)
+    s, t = torch.rand(m, device="cuda"), torch.rand(n, device="cuda")
+    got = latent.int8_scores(q, s, p, t, dtype=torch.bfloat16)
+    for lo in (0, 128 * 12345 - 50, (1 << 28) - 50, n - 1000):
+        want = latent.int8_scores(q, s, p[lo:lo + 1000], t[lo:lo + 1000], dtype=torch.bfloat16)
+        assert torch.equal(got[:, lo:lo + 1000], want)
+    del got
+    torch.cuda.empty_cache()

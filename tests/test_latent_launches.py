@@ -82,6 +82,8 @@ def quantize(type, rows, k):
 HUGE = {
     # 2^26 rows of 64 lanes each: 2^32 threads
     "quantize": [quantize(1, 1 << 26, 513), quantize(0, (1 << 27) + 5, 300), quantize(2, (1 << 31) - 1, 8), quantize(0, (1 << 31) - 1, 1 << 12)],
+    "scores8_outer": [scores8(129, 1 << 29, 64, 1), scores8(129, 1 << 28, 64, 0)],
+    "scores8_strips": [scores8(1 << 30, 33, 64, 1), scores8((1 << 31) - 1, 35, 128, 2)],
     "lookup": [("blp_lookup", [0, None, 0, ONE, 1 << 20, 5000, 1 << 20, ONE, 1, 1 << 20, 2.0, ONE, 1 << 20], None),
                lookup_grad(1, (1 << 31) - 1, 100, 8), lookup_grad(0, 5, (1 << 31) - 1, 8), lookup_grad(1, 1 << 24, 1000, 1 << 12)],
 }
@@ -94,3 +96,10 @@ def test_sizes_that_are_accepted_are_launched(name):
         assert got["rc"] == 0, got["error"]
         for l in got["launches"]:
             assert l["grid"][0] * l["block"][0] < 1 << 32, l
+
+
+def test_more_scores_than_tiles_can_be_counted_are_refused():
+    """Before anything is packed."""
+    for k in (64, 300, 15):
+        (got,) = run([scores8((1 << 31) - 1, (1 << 31) - 1, k, 1)])
+        assert got["rc"] == -1 and "2^45" in got["error"] and not got["launches"]
