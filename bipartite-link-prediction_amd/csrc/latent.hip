@@ -252,16 +252,16 @@ __global__ __launch_bounds__(1024) void k_total(const float* __restrict__ loss, 
 
 // R rows a block, 256 / R threads a row over the tiles' pairs: 32 rows read whole lines of pairs, 4 rows have 64 threads
 // each where there are too few rows to fill the card. Leaves the rows' parameters of the narrow gradients (`rows`), and
-// with `done` (0 before) the block that ends last takes the total.
+// with `done` (0 before) the block that ends last takes the total. The rows from `row0` on.
 template <int R>
-__global__ __launch_bounds__(256) void k_join(const float2* __restrict__ part, int64_t tiles, int64_t m,
+__global__ __launch_bounds__(256) void k_join(const float2* __restrict__ part, int64_t tiles, int64_t m, int64_t row0,
                                               const float* __restrict__ hit, Targets targets, float* __restrict__ loss,
                                               float* __restrict__ lse, Rows rows, float extra, Total total, uint32_t* done) {
   constexpr int G = 256 / R;
   __shared__ float2 s_part[G][R];
   __shared__ int s_last;
   const int r = threadIdx.x & (R - 1), g = threadIdx.x / R;
-  const int64_t row = blockIdx.x * (int64_t)R + r;
+  const int64_t row = row0 + blockIdx.x * (int64_t)R + r;
   float top = -INFINITY, sum = 0.f;
   if (row < m) {
     int64_t t = g;
@@ -961,6 +961,7 @@ __global__ __launch_bounds__(256, KS > 2 || T == F32 ? 3 : 4) void k_narrow_grad
 // dS of one piece of the catalogue: what the last-level cache holds (8,192 x 100,000 x 1,024 halves: 6.6 ms a step; 128 MiB
 // 7.0, 512 MiB 6.8, 1 GiB 6.9).
 constexpr int64_t PIECE_BYTES = 256ll << 20;
+constexpr int64_t JOINED = 1ll << 28;         // rows of a launch of k_join, 8 threads each: less than 2^32 threads
 constexpr int64_t PAIR_BYTES = 256ll << 20;   // the forward pass's pairs of the rows taken at a time
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
@@ -1261,19 +1262,30 @@ int narrow_grads(const Call& c, RowGrad g, void* dx, int64_t lddx, void* dw, int
   const EpiGradient<ST> ex = {p.nx.n > 1, {px, ldp, p.k, p.m, 0}, {(char*)dx, lddx * p.es, p.k, p.m, g, c.scale}};
   const EpiGradient<ST> ew = {p.nw.n > 1, {pw, ldp, p.k, p.n, 0}, {(char*)dw, lddw * p.es, p.k, p.n, g, c.scale}};
   const int64_t bw = up((int64_t)w.own_tiles * w.splits, 8), bx = (int64_t)x.own_tiles * x.splits;  // eights: x keeps its dies
-  BLP_CHECK(bw + bx <= 0x7fffffff, BLP_E_ARG, "softmax loss: too many tiles for one launch");
-  if (bw + bx == 0) return 0;
   const bool per_row = g.g && g.stride;
-  with_steps<T>(p.ks, [&](auto ks) {
-    constexpr int KS = decltype(ks)::value;
-    if constexpr (T != F16) {  // row gradients of float16 are taken as floats
-      if (per_row) k_narrow_grads<T, ST, KS, true><<<(unsigned)(bw + bx), 256, 0, c.st>>>(w, ew, (int)bw, x, ex);
-    }
-    if constexpr (T == ST) {
-      if (!per_row) k_narrow_grads<T, ST, KS, false><<<(unsigned)(bw + bx), 256, 0, c.st>>>(w, ew, (int)bw, x, ex);
-    }
-  });
-  BLP_HIP(hipGetLastError());
+  auto launch = [&](int64_t bw, int64_t bx) -> int {
+    if (bw + bx == 0) return 0;
+    with_steps<T>(p.ks, [&](auto ks) {
+      constexpr int KS = decltype(ks)::value;
+      if constexpr (T != F16) {  // row gradients of float16 are taken as floats
+        if (per_row) k_narrow_grads<T, ST, KS, true><<<(unsigned)(bw + bx), 256, 0, c.st>>>(w, ew, (int)bw, x, ex);
+      }
+      if constexpr (T == ST) {
+        if (!per_row) k_narrow_grads<T, ST, KS, false><<<(unsigned)(bw + bx), 256, 0, c.st>>>(w, ew, (int)bw, x, ex);
+      }
+    });
+    BLP_HIP(hipGetLastError());
+    return 0;
+  };
+  // a launch takes less than 2^32 threads: each gradient's workgroups do (a 128th of up to 2^31 - 2^16 rows), both's may not
+  int rc = 0;
+  if (bw + bx < 1 << 24) {
+    rc = launch(bw, bx);
+  } else {
+    rc = launch(bw, 0);
+    if (!rc) rc = launch(0, bx);
+  }
+  if (rc) return rc;
   const SumArgs sx = {px, p.nx.n, dx && p.nx.n > 1 ? p.m : 0, (char*)dx, lddx * p.es, 0};
   const SumArgs sw = {pw, p.nw.n, dw && p.nw.n > 1 ? p.n : 0, (char*)dw, lddw * p.es, 0};
   return sum_parts<ST>(sx, sw, p.k, g, c.scale, c.st);
@@ -1300,13 +1312,16 @@ int forward(const Call& c, float* loss, float* lse, Total total, uint32_t* done)
       const int64_t pairs = p.narrow ? p.nl.n : p.fwd_tiles;
       const Rows rows = {p.narrow && p.grads ? (float*)(c.ws + p.o_rows) : nullptr};
       const int64_t all = rows.at ? up(m, 64) : m;
-      if (m >= 4096)
-        k_join<32><<<(unsigned)div_up(all, 32), 256, 0, c.st>>>(part, pairs, m, hit, targets, loss + r0, lse + r0, rows,
+      for (int64_t j0 = 0; j0 < all; j0 += JOINED) {
+        const int64_t n = std::min(JOINED, all - j0);
+        if (m >= 4096)
+          k_join<32><<<(unsigned)div_up(n, 32), 256, 0, c.st>>>(part, pairs, m, j0, hit, targets, loss + r0, lse + r0, rows,
                                                                 extra_of(T), total, done);
-      else
-        k_join<4><<<(unsigned)div_up(all, 4), 256, 0, c.st>>>(part, pairs, m, hit, targets, loss + r0, lse + r0, rows,
+        else
+          k_join<4><<<(unsigned)div_up(n, 4), 256, 0, c.st>>>(part, pairs, m, j0, hit, targets, loss + r0, lse + r0, rows,
                                                               extra_of(T), total, done);
-      BLP_HIP(hipGetLastError());
+        BLP_HIP(hipGetLastError());
+      }
     }
   }
   if (total.at && !(done && p.m > 0)) {

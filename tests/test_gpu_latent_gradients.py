@@ -191,3 +191,27 @@ def test_scales_next_to_zero(gpu, k, dtype):
         total, dx, dw = latent.softmax_loss_grad(x, w, t, scale=scale)
         near(dx, ref["dx"], ref["b_dx"] + 2.0 ** -133)
         near(dw, ref["dw"], ref["b_dw"] + 2.0 ** -133)
+
+
+def test_more_rows_than_a_launch_joins(gpu):
+    """2^28 rows and some more, whose pairs are joined in two launches; forward alone and with gradients."""
+    torch = _torch()
+    from blp import latent
+
+    m, n, k, edge = (1 << 28) + 300, 50, 8, 1 << 28
+    torch.cuda.empty_cache()
+    x = torch.empty(m, k, dtype=torch.bfloat16, device="cuda")
+    for at in range(0, m, 1 << 25):
+        x[at:at + (1 << 25)].normal_()
+    w = torch.randn(n, k, device="cuda").to(torch.bfloat16)
+    t = torch.randint(-1, n, (m,), device="cuda", dtype=torch.int32)
+    loss = latent.softmax_loss(x, w, t, reduction="none")
+    total, dx, dw = latent.softmax_loss_grad(x, w, t, reduction="sum")
+    for lo, hi in ((0, 200), (edge - 200, edge + 300)):
+        ref = reference(x[lo:hi], w, t[lo:hi], 1.0)
+        near(loss[lo:hi], ref["loss"], ref["b_loss"])
+        one = torch.ones(hi - lo, dtype=torch.float64, device="cuda")
+        near(dx[lo:hi], *gradients(x[lo:hi], w, t[lo:hi], 1.0, one, one[:, None])[0])
+    assert abs(float(total) - float(loss.double().sum())) <= U * float(total) and dw.isfinite().all()
+    del x, loss, dx
+    torch.cuda.empty_cache()

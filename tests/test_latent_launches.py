@@ -84,6 +84,9 @@ HUGE = {
     "quantize": [quantize(1, 1 << 26, 513), quantize(0, (1 << 27) + 5, 300), quantize(2, (1 << 31) - 1, 8), quantize(0, (1 << 31) - 1, 1 << 12)],
     "scores8_outer": [scores8(129, 1 << 29, 64, 1), scores8(129, 1 << 28, 64, 0)],
     "scores8_strips": [scores8(1 << 30, 33, 64, 1), scores8((1 << 31) - 1, 35, 128, 2)],
+    "loss_forward": [loss(1, 1 << 29, 1000, 8, grads=0), loss(0, (1 << 31) - (1 << 16), 77, 3, grads=0), loss(2, 1 << 30, 5, 200, grads=0)],
+    "loss_step": [loss(1, 1 << 29, 1000, 8), loss(0, 1 << 29, 1000, 130), loss(1, 1000, 1 << 30, 64), backward(1, 1 << 30, 300, 8),
+                  backward(0, (1 << 31) - (1 << 16), 100000, 1), backward(1, 100000, (1 << 31) - (1 << 16), 8)],
     "lookup": [("blp_lookup", [0, None, 0, ONE, 1 << 20, 5000, 1 << 20, ONE, 1, 1 << 20, 2.0, ONE, 1 << 20], None),
                lookup_grad(1, (1 << 31) - 1, 100, 8), lookup_grad(0, 5, (1 << 31) - 1, 8), lookup_grad(1, 1 << 24, 1000, 1 << 12)],
 }
