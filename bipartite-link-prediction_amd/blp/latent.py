@@ -122,6 +122,7 @@ _REDUCTIONS = ("mean", "sum", "none")
 
 def _loss_args(x, table, target, scale, reduction):
     _t()
+    scale = _scale(scale)
     ldx = _rows(x, "x", _TYPES)
     if not isinstance(table, _torch.Tensor) or table.dtype != x.dtype:
         raise ValueError("x and table must be tensors of the same type (got %s and %s)" % (_say(x), _say(table)))
@@ -134,7 +135,7 @@ def _loss_args(x, table, target, scale, reduction):
     wide = _ids(target, "target", x.device, x.shape[0])
     if reduction not in _REDUCTIONS:
         raise ValueError("reduction must be one of %s (got %r)" % (", ".join(_REDUCTIONS), reduction))
-    return ldx, ldt, wide, _scale(scale)
+    return ldx, ldt, wide, scale
 
 
 def _loss_workspace(x, ldx, table, ldt, forward, grads):
@@ -182,7 +183,7 @@ def softmax_loss(x, table, target, scale=1.0, reduction="mean"):
     Float32 factors are multiplied as sums of three bfloat16 each, with 32-bit results; they have to be finite."""
     torch = _t()
     if torch.is_grad_enabled() and (getattr(x, "requires_grad", False) or getattr(table, "requires_grad", False)):
-        return _function("loss").apply(x, table, target, scale, reduction)
+        return _function("loss").apply(x, table, target, _scale(scale), reduction)
     return _loss_forward(x, table, target, scale, reduction, 0)[0]
 
 
@@ -217,6 +218,13 @@ def softmax_loss_backward(grad, lse, count, x, table, target, scale=1.0, need_x=
 
 
 def _scale(scale):
+    """The number; a tensor of one element is one if nothing would be lost: neither its derivative nor its place in a trace."""
+    if isinstance(scale, _torch.Tensor):
+        _plain(scale, "scale")
+        if scale.requires_grad and _torch.is_grad_enabled():
+            raise ValueError("scale must not require a gradient: its derivative is not taken")
+        if _torch.jit.is_tracing():
+            raise RuntimeError("scale: this call cannot be traced")
     scale = float(scale)
     if not abs(scale) < float("inf"):
         raise ValueError("scale must be finite (got %r)" % scale)
@@ -229,12 +237,13 @@ def lookup(table, ids, scale=1.0):
     Differentiable in table (not inside a graph capture: capture :func:`lookup_grad`)."""
     torch = _t()
     if torch.is_grad_enabled() and getattr(table, "requires_grad", False):
-        return _function("lookup").apply(table, ids, scale)
+        return _function("lookup").apply(table, ids, _scale(scale))
     return _lookup(table, ids, scale)
 
 
 def _lookup(table, ids, scale):
     _t()
+    scale = _scale(scale)
     ld = _rows(table, "table", _TYPES)
     rows, k = table.shape
     if rows < 1:
@@ -243,7 +252,7 @@ def _lookup(table, ids, scale):
     wide = _ids(ids, "ids", device)
     out = table.new_empty(*ids.shape, k)
     check(lib().blp_lookup(device.index, _stream(device.index), _TYPES[table.dtype], table.data_ptr(), ld, rows, k,
-                           ids.data_ptr(), wide, ids.numel(), _scale(scale), out.data_ptr(), k))
+                           ids.data_ptr(), wide, ids.numel(), scale, out.data_ptr(), k))
     return out
 
 
@@ -254,6 +263,7 @@ def lookup_grad(grad, ids, n_rows, scale=1.0, into=None):
     holds -- e.g. the softmax loss's gradient of the same table -- and it is returned; to autograd that is a change
     in place, and `into` must not require a gradient (but under torch.no_grad)."""
     torch = _t()
+    scale = _scale(scale)
     if not isinstance(grad, torch.Tensor) or not isinstance(ids, torch.Tensor) or grad.dim() < 1 \
             or tuple(grad.shape[:-1]) != tuple(ids.shape):
         raise ValueError("grad must have the shape of ids and one more dimension")
@@ -282,7 +292,7 @@ def lookup_grad(grad, ids, n_rows, scale=1.0, into=None):
     check(lib().blp_lookup_grad_workspace(_TYPES[grad.dtype], n, n_rows, k, ctypes.byref(b)))
     ws = _bytes(grad, b.value)
     check(lib().blp_lookup_grad(grad.device.index, _stream(grad.device.index), _TYPES[grad.dtype], grad.data_ptr(), ld,
-                                ids.data_ptr(), wide, n, n_rows, k, _scale(scale), out.data_ptr(), ldo,
+                                ids.data_ptr(), wide, n, n_rows, k, scale, out.data_ptr(), ldo,
                                 0 if into is None else 1, ws.data_ptr(), ws.numel()))
     if into is not None:
         torch.autograd.graph.increment_version(into)  # autograd sees that what it may have kept of `into` has changed
@@ -309,7 +319,7 @@ def int8_scores(q, s, table_q, table_s, dtype=None):
     """``s[:, None] * table_s * (q @ table_q.T)``: every score of the catalogue from 8-bit factors and their row
     scales (:func:`quantize_rows`). q (m, k), table_q (n, k) int8, k < 131072; s (m,), table_s (n,) float32.
     The products are summed exactly in 32-bit integers; scaled in float32 and rounded once to `dtype`
-    (float32, the default, bfloat16 or float16)."""
+    (float32, the default, bfloat16 or float16). Not differentiable."""
     torch = _t()
     dtype = torch.float32 if dtype is None else dtype
     if dtype not in _TYPES:

@@ -133,3 +133,33 @@ def test_far_strides_are_value_errors(gpu):
         latent.int8_scores(q, torch.ones(2, device="cuda"), q, torch.ones(2, device="cuda"))
     with pytest.raises(ValueError, match="scale"):
         latent.lookup(w, t, 1e39)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tracing_by_the_ids_is_refused(name):
+    x = torch.randn(4, 8)
+
+    def traced(ids):
+        with pytest.raises(RuntimeError, match="traced"):
+            calls(x, ids)[name]()
+        return ids
+
+    torch.jit.trace(traced, torch.zeros(4, dtype=torch.int64), check_trace=False)
+
+
+def test_scales_whose_derivative_would_be_dropped_are_refused():
+    """A scale is a number. One that requires a gradient, or is traced or dual, would lose it without an error."""
+    from torch.autograd import forward_ad
+
+    x, ids = torch.randn(4, 8), torch.zeros(4, dtype=torch.int64)
+    uses = (lambda s: latent.softmax_loss(x, x, ids, scale=s), lambda s: latent.softmax_loss(x.requires_grad_(), x, ids, scale=s),
+            lambda s: latent.softmax_loss_grad(x, x, ids, scale=s), lambda s: latent.lookup(x, ids, s),
+            lambda s: latent.lookup_grad(x, ids, 4, scale=s))
+    for use in uses:
+        with pytest.raises(ValueError, match="scale must not require"):
+            use(torch.tensor(2.0, requires_grad=True))
+        with forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match="scale: forward-mode"):
+                use(forward_ad.make_dual(torch.tensor(2.0), torch.tensor(1.0)))
+        with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+            use(torch.tensor(2.0, requires_grad=True))
