@@ -196,9 +196,17 @@ def softmax_loss_grad(x, table, target, scale=1.0, reduction="mean"):
     return loss, dx, dt
 
 
+def softmax_loss_forward(x, table, target, scale=1.0, reduction="mean"):
+    """-> (loss, lse, count): :func:`softmax_loss` and what :func:`softmax_loss_backward` takes of it, for loops that do not go
+    through autograd: lse (m,) float32, each row's log-sum-exp (of a row that is ignored: anything); count the number of rows not ignored (at least 1; float32)
+    for "mean", else None."""
+    loss, lse, total, _, _ = _loss_forward(x, table, target, scale, reduction, 0, keep=True)
+    return loss, lse, total[1] if reduction == "mean" else None
+
+
 def softmax_loss_backward(grad, lse, count, x, table, target, scale=1.0, need_x=True, need_table=True):
-    """-> (dx, dtable) of :func:`softmax_loss`: `grad` float32, one value or one a row; `lse` (m,) the
-    forward pass's; `count` a float32 value that divides the gradient (mean) or None."""
+    """-> (dx, dtable) of :func:`softmax_loss`: `grad` float32, one value or one a row; `lse` (m,) and `count`,
+    which divides the gradient (mean) or is None, from :func:`softmax_loss_forward`."""
     ldx, ldt, wide, scale = _loss_args(x, table, target, scale, "none")
     m, k = x.shape
     device = x.device

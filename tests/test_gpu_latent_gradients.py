@@ -215,3 +215,43 @@ def test_more_rows_than_a_launch_joins(gpu):
     assert abs(float(total) - float(loss.double().sum())) <= U * float(total) and dw.isfinite().all()
     del x, loss, dx
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("k", [40, 200])
+def test_forward_leaves_what_backward_takes(gpu, k, reduction):
+    """softmax_loss_forward, then softmax_loss_backward: the loss and the gradients of softmax_loss, also captured and replayed."""
+    torch = _torch()
+    from blp import latent
+
+    m, n = 70, 300
+    x, w, t = make(m, n, k, torch.bfloat16, seed=k, ignored=0.2)
+    g = torch.randn(m, device="cuda") if reduction == "none" else torch.full((), 1.5, device="cuda")
+
+    def step():
+        loss, lse, count = latent.softmax_loss_forward(x, w, t, 0.5, reduction)
+        return (loss, lse, *latent.softmax_loss_backward(g, lse, count, x, w, t, 0.5))
+
+    def check(got):
+        ref = reference(x, w, t, 0.5)
+        scale = {"mean": 1.5 / ref["count"], "sum": 1.5, "none": 1.0}[reduction]
+        per_row = g.double() if reduction == "none" else torch.full((m,), scale, dtype=torch.float64, device="cuda")
+        near(got[1][ref["ok"]], ref["lse"][ref["ok"]], ref["b_loss"][ref["ok"]])
+        xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+        loss = latent.softmax_loss(xr, wr, t, 0.5, reduction)
+        assert torch.equal(got[0], loss) and not got[0].requires_grad
+        for p, (want, bound) in zip(got[2:], gradients(x, w, t, 0.5, per_row, per_row.abs().max())):
+            near(p, want, bound)
+        for p, q in zip(got[2:], torch.autograd.grad(loss, (xr, wr), g)):
+            assert torch.equal(p, q)
+
+    check(step())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(3):
+        for dst, src in zip((x, w, t), make(m, n, k, torch.bfloat16, seed=50 + i, ignored=0.2)):
+            dst.copy_(src)
+        graph.replay()
+        check(out)

@@ -12,6 +12,7 @@ def calls(x, ids):
     one = torch.ones(len(x))
     return {
         "softmax_loss": lambda: latent.softmax_loss(x, torch.ones_like(x.detach()), ids),
+        "softmax_loss_forward": lambda: latent.softmax_loss_forward(x, x, ids),
         "softmax_loss_grad": lambda: latent.softmax_loss_grad(x, x, ids),
         "softmax_loss_backward": lambda: latent.softmax_loss_backward(one, one, None, x, x, ids),
         "lookup": lambda: latent.lookup(x, ids),
