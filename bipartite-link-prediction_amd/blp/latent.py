@@ -14,6 +14,7 @@ import ctypes
 from . import _lib
 from ._lib import BLPError, lib
 
+_INF = float("inf")
 _P, _I64, _I32, _F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
 _PI64 = ctypes.POINTER(ctypes.c_int64)
 _lib.register("blp_softmax_loss_workspace", [_I32, _P, _I64, _P, _I64, _I64, _I64, _I32, _I32, _I32, _PI64])
@@ -69,14 +70,15 @@ def _plain(t, what):
     """Refuse what the kernels, which see a tensor's memory alone, would answer wrongly without an error. A dual tensor of forward-mode
     differentiation: a result without a tangent would be a derivative of zero (outside of a level there are none: that is
     all the common path looks at). A traced one: the trace would hold the allocation of the outputs and nothing that fills
-    them (sizes are numbers, but tensors while torch.jit traces). A negated view (z.conj().imag): its memory holds the
-    values before the sign."""
-    if not isinstance(t, _torch.Tensor):
-        return
-    if t.dim() and type(t.shape[0]) is not int:
-        raise RuntimeError("%s: this call cannot be traced" % what)
-    if getattr(_forward_ad, "_current_level", 0) >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
+    them (any tensor's sizes are numbers, but tensors while torch.jit traces; _rows looks)."""
+    if getattr(_forward_ad, "_current_level", 0) >= 0 and isinstance(t, _torch.Tensor) \
+            and _forward_ad.unpack_dual(t).tangent is not None:
         raise RuntimeError("%s: forward-mode derivatives are not implemented" % what)
+
+
+def _positive(t, what):
+    """Refuse a negated view (z.conj().imag), whose memory holds the values before the sign. Its elements are two apart: only
+    one of single elements passes for contiguous."""
     if t.is_neg():
         raise ValueError("%s must not be a negated view (resolve_neg() makes a tensor of it)" % what)
 
@@ -85,15 +87,19 @@ def _rows(t, what, dtypes):
     """The row stride of `t`, checked to be (n, k) rows: a 2-d tensor on a GPU whose rows are contiguous and do not
     overlap."""
     _plain(t, what)
-    if not (isinstance(t, _torch.Tensor) and t.dtype in dtypes and t.is_cuda and t.dim() == 2):
-        raise ValueError("%s must be a 2-d GPU tensor of %s (got %s)" % (
-            what, " / ".join(str(d)[6:] for d in dtypes), _say(t)))
-    n, k = t.shape
-    ld, step = t.stride()
-    if k < 1 or (k > 1 and step != 1) or (n > 1 and ld < k):
-        raise ValueError("%s must have contiguous, non-overlapping rows of at least one element (shape %s, strides %s)" % (
-            what, (n, k), (ld, step)))
-    return ld if n > 1 else k
+    if isinstance(t, _torch.Tensor) and t.dim() == 2:
+        n, k = t.shape
+        if type(n) is not int:
+            raise RuntimeError("%s: this call cannot be traced" % what)
+        if t.dtype in dtypes and t.is_cuda:
+            ld, step = t.stride()
+            if k < 1 or (k > 1 and step != 1) or (n > 1 and ld < k):
+                raise ValueError("%s must have contiguous, non-overlapping rows of at least one element (shape %s, strides %s)" % (
+                    what, (n, k), (ld, step)))
+            if k == 1:
+                _positive(t, what)
+            return ld if n > 1 else k
+    raise ValueError("%s must be a 2-d GPU tensor of %s (got %s)" % (what, " / ".join(str(d)[6:] for d in dtypes), _say(t)))
 
 
 def _ids(t, what, device, n=None):
@@ -111,6 +117,8 @@ def _floats(t, what, device, shapes):
             and t.shape in shapes):
         raise ValueError("%s must be a contiguous float32 tensor of shape %s on %s (got %s)" % (
             what, " or ".join(str(tuple(x)) for x in shapes), device, _say(t)))
+    if t.numel() == 1:
+        _positive(t, what)
 
 
 def _bytes(like, n):
@@ -198,8 +206,8 @@ def softmax_loss_grad(x, table, target, scale=1.0, reduction="mean"):
 
 def softmax_loss_forward(x, table, target, scale=1.0, reduction="mean"):
     """-> (loss, lse, count): :func:`softmax_loss` and what :func:`softmax_loss_backward` takes of it, for loops that do not go
-    through autograd: lse (m,) float32, each row's log-sum-exp (of a row that is ignored: anything); count the number of rows not ignored (at least 1; float32)
-    for "mean", else None."""
+    through autograd: lse (m,) float32, each row's log-sum-exp (of a row that is ignored: anything); count
+    the number of rows not ignored (at least 1; float32) for "mean", else None."""
     loss, lse, total, _, _ = _loss_forward(x, table, target, scale, reduction, 0, keep=True)
     return loss, lse, total[1] if reduction == "mean" else None
 
@@ -227,14 +235,14 @@ def softmax_loss_backward(grad, lse, count, x, table, target, scale=1.0, need_x=
 
 def _scale(scale):
     """The number; a tensor of one element is one if nothing would be lost: neither its derivative nor its place in a trace."""
-    if isinstance(scale, _torch.Tensor):
+    if type(scale) is not float and isinstance(scale, _torch.Tensor):
         _plain(scale, "scale")
         if scale.requires_grad and _torch.is_grad_enabled():
             raise ValueError("scale must not require a gradient: its derivative is not taken")
         if _torch.jit.is_tracing():
             raise RuntimeError("scale: this call cannot be traced")
     scale = float(scale)
-    if not abs(scale) < float("inf"):
+    if not abs(scale) < _INF:
         raise ValueError("scale must be finite (got %r)" % scale)
     return scale
 
