@@ -2,8 +2,9 @@
 softmax loss over the whole catalogue with its gradients (blp_softmax_loss*), and scores of the catalogue
 from 8-bit factors (blp_quantize_rows, blp_scores8) -- all in blp.h.
 
-They stand beside :class:`blp.factor.DeviceSVD`, whose factors they read, train and score: rows of a
-user table and of a business table, ``k`` components a row. Every argument that holds data is a torch
+They stand beside :class:`blp.factor.DeviceSVD`, whose factors, copied to float32 (or halves) tensors, they read, train
+and score: rows of a user table and of a business table, ``k`` components a row --
+``users = torch.from_numpy(svd.us).float().cuda()``, and back ``DeviceSVD(users.double().cpu().numpy(), ...)``. Every argument that holds data is a torch
 tensor on one GPU, its rows contiguous (a row stride larger than the row is fine); the work is queued
 on torch's current stream of that device, workspaces come from torch's allocator, and nothing waits
 for the device. Wrong arguments raise ValueError before anything is queued: row strides of the loss's operands past 2^20
@@ -274,8 +275,8 @@ def _lookup(table, ids, scale):
 
 def lookup_grad(grad, ids, n_rows, scale=1.0, into=None):
     """The gradient of :func:`lookup` in its table: (n_rows, k) with row r = scale * the sum of grad[i] over
-    ids[i] == r, in 32 bits and ascending i (the same every time), rounded to grad's type once; rows
-    without ids are zero. grad: ids.shape + (k,). With `into` (n_rows, k) the sums are added to what it
+    ids[i] == r, rounded to grad's type once: up to 64 entries at a time in 32 bits and ascending i, these sums
+    in 64 bits and a fixed order (the same every time); rows without ids are zero. grad: ids.shape + (k,). With `into` (n_rows, k) the sums are added to what it
     holds -- e.g. the softmax loss's gradient of the same table -- and it is returned; to autograd that is a change
     in place, and `into` must not require a gradient (but under torch.no_grad)."""
     torch = _t()

@@ -6,6 +6,9 @@
 
 namespace blp {
 
+inline int64_t div_up(int64_t v, int64_t by) { return (v + by - 1) / by; }
+inline int64_t up(int64_t v, int64_t to) { return div_up(v, to) * to; }
+
 // `device` current while it lives, then the one before.
 struct DeviceGuard {
   int before = -1, rc = 0;

@@ -48,7 +48,9 @@ constexpr int segments_of(int t, int layout) { return t == F32 ? 6 : layout == C
 constexpr float extra_of(int t) { return t == F16 ? 16384.f : 1.f; }
 
 using blp::DeviceGuard;
+using blp::div_up;
 using blp::FastDiv;
+using blp::up;
 using Targets = blp::Ids;  // the target of row i, or -1 (ignored)
 
 // ---------------------------------------------------------------- packing
@@ -964,12 +966,7 @@ constexpr int64_t PIECE_BYTES = 256ll << 20;
 constexpr int64_t JOINED = 1ll << 28;         // rows of a launch of k_join, 8 threads each: less than 2^32 threads
 constexpr int64_t PAIR_BYTES = 256ll << 20;   // the forward pass's pairs of the rows taken at a time
 
-int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
-int64_t div_up(int64_t v, int64_t by) { return (v + by - 1) / by; }
-
 enum ShapeId { BIG, MID, FLAT, THIN };
-using Big = Shape<2, 4, 8, 4>;   // 256 x 256, one workgroup a compute unit
-using Mid = Shape<2, 2, 4, 4>;   // 128 x 128, two
 using Flat = Shape<4, 1, 4, 2>;  // 256 x 32, two: few rows
 using Thin = Shape<4, 1, 1, 2>;  // 64 x 32, four: few tiles
 constexpr int BP_OF[] = {256, 128, 256, 64}, BQ_OF[] = {256, 128, 32, 32}, WP_OF[] = {2, 2, 4, 4}, PER_CU[] = {1, 2, 2, 4};
@@ -1363,7 +1360,7 @@ int backward(const Call& c, bool fwd, const float* lse, RowGrad g, void* dx, int
   for (int64_t j0 = 0; j0 < p.n && !rc; j0 += p.piece) {
     const int64_t nj = std::min(p.piece, p.n - j0);
     const Operand wj = {c.w.base + j0 * c.w.ld, c.w.ld, nj};
-    // the scores of the piece again, as dS. All of its width is written: zeros past the end
+    // the scores of the piece again, as dS. Its width is written up to the end of the last tile: zeros past the catalogue's
     const Problem as = {wj, c.x, p.kp, 0, 0, 0, p.w_plane(), p.x_plane()};
     const EpiGrad<T> eg = {ds, p.piece, p.ds_plane(), lse, g, c.targets, j0, nj, p.m, c.scale};
     rc = product<T, ROW, ROW>(shape_of(nj, p.m), as, 1, 0, eg, c.st);

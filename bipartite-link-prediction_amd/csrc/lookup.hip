@@ -2,11 +2,11 @@
 //
 //   y_i = scale table[id_i] (an id outside the table: zeros)      dT_r = scale sum_{i : id_i = r} dy_i
 //
-// The gradient is a sum over each row's positions in ascending order, with no float atomics: the ids are
-// sorted (stable, with their positions), chunks of sorted entries are summed by one group of lanes each, a
-// row's sum that lies inside a chunk is written at once and one that crosses chunks is left as partial
-// sums, which a second kernel adds up in the chunks' order. Every row of dy is read once, every row of dT
-// written once, and the result does not depend on timing.
+// The gradient is a sum over each row's positions, in an order that is the same every time, with no float atomics: the ids
+// are sorted (stable, with their positions), chunks of up to 64 sorted entries are summed in ascending order and 32 bits by one
+// group of lanes each, a row's sum that lies inside a chunk is written at once and one that crosses chunks is left as
+// partial sums, which a second kernel adds up in 64 bits: in the chunks' order, or, for rows of more than 8 chunks, those of
+// each group of lanes in turn, then the groups'. Every row of dy is read once, every row of dT written once.
 #include <algorithm>
 #include <type_traits>
 
@@ -17,6 +17,8 @@ namespace {
 
 using namespace blp::tile;
 using blp::DeviceGuard;
+using blp::div_up;
+using blp::up;
 using namespace blp::rows;
 using blp::FastDiv;
 using blp::Ids;
@@ -496,9 +498,6 @@ __global__ __launch_bounds__(256) void k_join_chunks(Sums a, unsigned heavy_bloc
 }
 
 // ---------------------------------------------------------------- host side
-int64_t div_up(int64_t v, int64_t by) { return (v + by - 1) / by; }
-int64_t up(int64_t v, int64_t to) { return div_up(v, to) * to; }
-
 struct Plan {
   int passes, bits, rounds, lanes, tiles;
   int64_t blocks, chunk, chunks, kv;

@@ -5,8 +5,8 @@
 // integers). A stage of each operand is copied from memory straight into LDS (16 bytes a lane, no register
 // in between). A fragment is 16 bytes of a row: 8 halves or 16 8-bit integers, one 16-row matrix instruction.
 // The next stage is in flight while this one is multiplied, in the other of two buffers, so a stage costs one
-// barrier. A workgroup takes tile after tile, and the next one's first stage is on its way while this one's
-// outputs leave. A stage of 256 x 256 x 64 halves is 64 KiB of copies and 2,048 cycles of the matrix unit; 8,192 x
+// barrier. A workgroup takes tile after tile, and the next one's first stage is on its way while this one is finished: with
+// an odd number of stages while its outputs leave, with an even one it has landed before they do. A stage of 256 x 256 x 64 halves is 64 KiB of copies and 2,048 cycles of the matrix unit; 8,192 x
 // 32,768 x 4,096 random halves run at 1,061 TFLOP/s, at 1,346 without the copies, and the copies alone take as long as
 // 1,717 would (constant halves, which draw less power: 1,319): bound by power and the second-level cache together.
 //
@@ -85,6 +85,9 @@ struct Shape {
   static constexpr int SHARE = STAGE_BYTES / WAVES, UNIT = SHARE < 4096 ? 1024 : 4096;
   static constexpr int SCRATCH = SHARE / UNIT * UNIT;  // LDS for a wave's outputs
 };
+
+using Big = Shape<2, 4, 8, 4>;  // 256 x 256, one workgroup a compute unit
+using Mid = Shape<2, 2, 4, 4>;  // 128 x 128, two
 
 typedef __attribute__((address_space(3))) char lds_char;
 
@@ -307,7 +310,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_product(Problem a, Epi epi) {
       landed();
       multiply(l0);
     }
-    __syncthreads();  // every wave's last reads are done: the second buffer is free for the outputs
+    __syncthreads();  // every wave's last reads are done, and its copies: the second buffer is free for the outputs
     if (t < stages && more) load(l0, np, nq, 0);
     epi.template run<S>(acc, (int64_t)tp * S::BP + wp * S::FP * 16, (int64_t)tq * S::BQ + wq * S::FQ * 16, tp * S::WP + wp, blockIdx.y,
                         l1 + wave * S::SCRATCH);
@@ -316,17 +319,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_product(Problem a, Epi epi) {
   }
 }
 
-// round to the type once; four consecutive values
-template <int T>
-__device__ inline void store4(char* at, f32x4 v) {
-  if constexpr (T == F32) {
-    *reinterpret_cast<f32x4*>(at) = v;
-  } else if constexpr (T == BF16) {
-    *reinterpret_cast<bf16x4*>(at) = __builtin_convertvector(v, bf16x4);
-  } else {
-    *reinterpret_cast<f16x4*>(at) = __builtin_convertvector(v, f16x4);
-  }
-}
+// round to the type once
 template <int T>
 __device__ inline void store1(char* at, float v) {
   if constexpr (T == F32) {

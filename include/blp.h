@@ -469,8 +469,9 @@ int blp_softmax_loss_backward(int device, void* stream, int type, const void* x,
  * (conventions as for the softmax loss; ids int32, or int64 with ids64)
  *   blp_lookup: out[i] = scale table[ids[i]] (k elements a row, rounded once); ids outside [0, rows)
  *     give zeros.
- *   blp_lookup_grad: out[r] (rows x k) = scale * the sum of grad[i] over ids[i] == r, ascending i, in 32
- *     bits; rows without ids are zero. With add, the sums are added to what out holds (rows without
+ *   blp_lookup_grad: out[r] (rows x k) = scale * the sum of grad[i] over ids[i] == r: up to 64 entries at a
+ *     time in ascending i and 32 bits, these sums in 64 bits and a fixed order, the same every time; rows
+ *     without ids are zero. With add, the sums are added to what out holds (rows without
  *     ids are left alone).                                                                  */
 int blp_lookup(int device, void* stream, int type, const void* table, int64_t ldt, int64_t rows, int k, const void* ids,
                int ids64, int64_t n, float scale, void* out, int64_t ldo);
