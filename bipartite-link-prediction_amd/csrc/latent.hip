@@ -960,9 +960,9 @@ __global__ __launch_bounds__(256, KS > 2 || T == F32 ? 3 : 4) void k_narrow_grad
 }
 
 // ---------------------------------------------------------------- host side
-// dS of one piece of the catalogue: what the last-level cache holds (8,192 x 100,000 x 1,024 halves: 6.6 ms a step; 128 MiB
-// 7.0, 512 MiB 6.8, 1 GiB 6.9).
-constexpr int64_t PIECE_BYTES = 256ll << 20;
+// dS of one piece of the catalogue, all planes: 8,192 x 100,000 x 1,024 halves take 10.1 ms a step; 128 MiB 10.7, 256 MiB
+// 10.3, 1 GiB 10.4 (smaller pieces pay for dx's sums, which each adds to, larger ones for dS leaving the last-level cache).
+constexpr int64_t PIECE_BYTES = 512ll << 20;
 constexpr int64_t JOINED = 1ll << 28;         // rows of a launch of k_join, 8 threads each: less than 2^32 threads
 constexpr int64_t PAIR_BYTES = 256ll << 20;   // the forward pass's pairs of the rows taken at a time
 
@@ -975,8 +975,8 @@ int64_t tiles_of(int shape, int64_t np, int64_t nq) { return div_up(np, BP_OF[sh
 
 // A stage of every tile, in us: 1.55 a round of the large shape and, two workgroups side by side, 1.2 of the middle one
 // (8,192 x 100,000 x 1,024 halves: 980 and 860 TFLOP/s). Where there are few tiles a compute unit's way to memory counts, and
-// small ones on many of them are faster: 80 x 267 x 1,728 halves, 65 us a step in tiles of 128 x 128 and 42 in 64 x 32; 15 x
-// 3,344 x 240 floats, 73 us in 256 x 32 and 54; but 200 x 20,000 x 512 halves 78 and 96.
+// small ones on many of them are faster: 80 x 267 x 1,728 halves, 75 us a step in tiles of 128 x 128 and 47 in 64 x 32; 15 x
+// 3,344 x 240 floats, 75 us in 256 x 32 and 55; but 200 x 20,000 x 512 halves 92 and 121.
 double stage_us(int shape, int64_t tiles) {
   const int64_t slots = 256 * PER_CU[shape], each = std::min<int64_t>(div_up(tiles, 256), PER_CU[shape]);
   static const double thin[] = {0.4, 0.55, 0.75, 1.0};
@@ -1407,7 +1407,8 @@ template <int T, int ST>
 int run(Call& c, const void* x, int64_t ldx, const void* w, int64_t ldw, float* loss, float* lse, float* total, int mean,
         bool fwd, RowGrad g, void* dx, int64_t lddx, void* dw, int64_t lddw) {
   // With gradients the packing comes first and clears the mark by which the last block to end takes the total. Every
-  // block's fence writes its die's cache back, so that pays for few of them (106 rows: 40 -> 33 us a step; 1,590: 70 -> 93).
+  // block's fence writes its die's cache back, so that pays for few of them (106 x 7,073 x 31 floats:
+  // 31.4 -> 28.2 us a step; 1,590 x 7,073 x 31: 50 -> 75).
   uint32_t* done = fwd && total && c.p.grads && c.p.m > 0 && c.p.m <= 512 ? (uint32_t*)(c.ws + c.p.o_top) + 1 : nullptr;
   int rc = bind<T, ST>(c, x, ldx, w, ldw, done);
   if constexpr (T == ST) {

@@ -81,7 +81,7 @@ def test_backward_of_row_gradients_is_rounded_once(gpu, k, dtype):
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 def test_pieces_of_the_catalogue_add_up(gpu, dtype):
-    """dx of a catalogue of several pieces: 131,072 rows leave room for 512 columns of two halves each, 1,100 columns are three pieces."""
+    """dx of a catalogue of several pieces: 131,072 rows leave room for 1,024 columns of two halves each, 1,100 columns are two pieces."""
     torch = _torch()
     from blp import latent
 
@@ -95,7 +95,7 @@ def test_pieces_of_the_catalogue_add_up(gpu, dtype):
     assert dw.isfinite().all()
 
 
-@pytest.mark.parametrize("dtype,m,n,k", [("bfloat16", 16384, 87300, 200), ("float32", 14875, 70587, 104)])
+@pytest.mark.parametrize("dtype,m,n,k", [("bfloat16", 16384, 87300, 200), ("float32", 15162, 62966, 104)])
 def test_a_last_piece_of_fewer_slices(gpu, dtype, m, n, k):
     """A catalogue whose last piece has fewer stages than the slices of the others take: the row gradient's parts add up."""
     torch = _torch()
