@@ -347,8 +347,8 @@ __global__ __launch_bounds__(1024) void k_top_grad(const float* __restrict__ g, 
   }
 }
 
-// dS of one piece: ds[row * ld + p], zeros past the catalogue's end. A piece of 8,192 x 14,336 x 1,024 bf16 0.27 ms, 900
-// TFLOP/s with 0.23 GB written; dX and dW of it, which read that, 0.24 and 0.25 ms.
+// dS of one piece: ds[row * ld + p], zeros past the catalogue's end. A piece of 8,192 x 14,336 x 1,024 bf16 0.31 ms, 770
+// TFLOP/s with 0.47 GB written; dX and dW of it, which read that, 0.45 and 0.49 ms (1,070 and 990).
 template <int T>
 struct EpiGrad {
   char* ds;
@@ -519,10 +519,11 @@ __global__ __launch_bounds__(256) void k_sum_parts(SumArgs a, SumArgs b, int64_t
 //        operand as it lies (the matrix instruction's k order is free, so its rows of w are read from LDS,
 //        transposed, in the order in which the lanes hold dS); dx accumulates in registers
 //   DW   own w, stream x: the same with the sides changed
-// 64 scores at k = 64 need 8 (LSE) or 16 (DX, DW) cycles of a SIMD's matrix unit and about 17 of its vector unit, 8 of them
-// exp2; two waves' shares of the two units overlap by half at most on this chip. 10,000 x 100,000 x 64: LSE 225 us (29 cycles
-// a 64 scores; the vector unit is busy 78% of them), both gradients 510 to 580 us (31 cycles; vector unit 65%, matrix unit
-// 51%). Computing the exponentials again in DX and DW costs less than writing dS once and reading it twice (2.36 ms in all).
+// 64 scores at k = 64 need 8 (LSE) or 24 (DX, DW) cycles of a SIMD's matrix unit and about 17 (LSE) or 27 of its vector unit, 8
+// of them exp2; two waves' shares of the two units overlap by half at most on this chip. 10,000 x 100,000 x 64: LSE 184 to
+// 220 us (of the cycles that a compute unit is busy its vector unit is in 87%, the matrix unit in 32%, LDS in 16%), both
+// gradients 730 to 840 us (77%, 53%, 20%). Computing the exponentials again in DX and DW costs less than writing dS once and
+// reading it twice: that took 2.36 ms in all with one plane of it.
 // Larger waves (64 rows: 275 us for LSE) hide less of each other's waits, one more stage ahead does not matter.
 __global__ __launch_bounds__(64) void k_rows(const float* __restrict__ lse, RowGrad g, Targets targets, int64_t m, Rows rows) {
   const int64_t i = blockIdx.x * 64ll + threadIdx.x;

@@ -41,7 +41,7 @@ __device__ inline int to8(float x, float s) {
 // `lanes` (a power of two up to 64) lanes a row, one 16-byte vector each a step. HELD steps (1 or 8) stay in registers between
 // the maximum and the rounding; longer rows (0) are read twice, the second time out of the cache. Bytes [k, kp) of a row are
 // set to zero. A row with a NaN or an infinity gets the scale NaN and zeros, so its scores are NaN; a row of zeros the scale
-// 0. 4,096 rows of 4,096 bf16 take 18 us: reading x would take 11 (4.68 TB/s), the arithmetic after it is not hidden.
+// 0. 4,096 rows of 4,096 bf16 take 18 us: moving x and q would take 11 (4.68 TB/s), the arithmetic after the loads is not hidden.
 template <int T, int HELD>
 __global__ __launch_bounds__(256) void k_quantize(const char* __restrict__ x, int64_t ld, int64_t rows, int k, int kp, int lanes,
                                                   int8_t* __restrict__ q, int64_t ldq, float* __restrict__ s) {
