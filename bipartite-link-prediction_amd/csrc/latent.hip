@@ -742,7 +742,8 @@ __device__ __attribute__((always_inline)) inline void narrow_body(const NarrowAr
           }
         }
       }
-      // The range's last stage, and rows that rise far: rare.
+      // The range's last stage, and rows that rise far or hold a NaN: rare. A NaN keeps its wave's 32 rows here: 10,000 x 100,000
+      // x 64 bf16 200 us without one, 250 with one, 510 with one in every 32 rows.
 #pragma unroll 1
       for (int half = 0; half < 2; ++half) {
         f32x4 acc[2][FO];
