@@ -4,10 +4,11 @@ from 8-bit factors (blp_quantize_rows, blp_scores8) -- all in blp.h.
 
 They stand beside :class:`blp.factor.DeviceSVD`, whose factors, copied to float32 (or halves) tensors, they read, train
 and score: rows of a user table and of a business table, ``k`` components a row --
-``users = torch.from_numpy(svd.us).float().cuda()``, and back ``DeviceSVD(users.double().cpu().numpy(), ...)``. Every argument that holds data is a torch
-tensor on one GPU, its rows contiguous (a row stride larger than the row is fine); the work is queued
-on torch's current stream of that device, workspaces come from torch's allocator, and nothing waits
-for the device. Wrong arguments raise ValueError before anything is queued: row strides of the loss's operands past 2^20
+``users = torch.from_numpy(svd.us).float().cuda()``, and back ``DeviceSVD(users.double().cpu().numpy(), ...)``.
+
+Every argument that holds data is a torch tensor on one GPU, its rows contiguous (a row stride larger than the
+row is fine); the work is queued on torch's current stream of that device, workspaces come from torch's
+allocator, and nothing waits for the device. Wrong arguments raise ValueError before anything is queued: row strides of the loss's operands past 2^20
 elements and of 8-bit ones past 2^22 are among them.
 """
 import ctypes
@@ -68,9 +69,9 @@ def _say(t):
 
 
 def _plain(t, what):
-    """Refuse what the kernels, which see a tensor's memory alone, would answer wrongly without an error. A dual tensor of forward-mode
-    differentiation: a result without a tangent would be a derivative of zero (outside of a level there are none: that is
-    all the common path looks at). A traced one: the trace would hold the allocation of the outputs and nothing that fills
+    """Refuse what the kernels, which see a tensor's memory alone, would answer wrongly without an error. A dual tensor
+    of forward-mode differentiation: a result without a tangent would be a derivative of zero (outside of a level there
+    are none: that is all the common path looks at). A traced one: the trace would hold the allocation of the outputs and nothing that fills
     them (any tensor's sizes are numbers, but tensors while torch.jit traces; _rows looks)."""
     if getattr(_forward_ad, "_current_level", 0) >= 0 and isinstance(t, _torch.Tensor) \
             and _forward_ad.unpack_dual(t).tangent is not None:
@@ -276,8 +277,8 @@ def _lookup(table, ids, scale):
 def lookup_grad(grad, ids, n_rows, scale=1.0, into=None):
     """The gradient of :func:`lookup` in its table: (n_rows, k) with row r = scale * the sum of grad[i] over
     ids[i] == r, rounded to grad's type once: up to 64 entries at a time in 32 bits and ascending i, these sums
-    in 64 bits and a fixed order (the same every time); rows without ids are zero. grad: ids.shape + (k,). With `into` (n_rows, k) the sums are added to what it
-    holds -- e.g. the softmax loss's gradient of the same table -- and it is returned; to autograd that is a change
+    in 64 bits and a fixed order (the same every time); rows without ids are zero. grad: ids.shape + (k,). With
+    `into` (n_rows, k) the sums are added to what it holds -- e.g. the softmax loss's gradient of the same table -- and it is returned; to autograd that is a change
     in place, and `into` must not require a gradient (but under torch.no_grad)."""
     torch = _t()
     scale = _scale(scale)

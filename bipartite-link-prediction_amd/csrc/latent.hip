@@ -1154,7 +1154,6 @@ void launch(const Problem& a, dim3 grid, const Epi& epi, hipStream_t st) {
 template <int T, int LP, int LQ, class Epi>
 int product(int shape, Problem a, int slices, int stages, Epi epi, hipStream_t st) {
   const int64_t tp = div_up(a.p.rows, BP_OF[shape]), tq = div_up(a.q.rows, BQ_OF[shape]);
-  BLP_CHECK(tp * tq <= 0x7fffffff, BLP_E_ARG, "softmax loss: too many tiles for one launch");
   a.tiles_p = (int)tp;
   a.tiles_q = (int)tq;
   a.slice = stages ? stages : (int)div_up(a.k, KE) * segments_of(T, LP);
@@ -1242,7 +1241,6 @@ int narrow_lse(const Call& c, float2* part, float* hit) {
   const NarrowArgs a = {c.x, c.w, p.x_plane(), p.w_plane(), p.kp, p.nl.range, p.nl.own_tiles, p.nl.n, c.scale, 1.f, c.targets,
                         part, hit, Rows{nullptr}};
   const int64_t blocks = (int64_t)p.nl.own_tiles * p.nl.n;
-  BLP_CHECK(blocks <= 0x7fffffff, BLP_E_ARG, "softmax loss: too many tiles for one launch");
   with_steps<T>(p.ks, [&](auto ks) { k_narrow_lse<T, decltype(ks)::value><<<(unsigned)blocks, 256, 0, c.st>>>(a); });
   BLP_HIP(hipGetLastError());
   return 0;
@@ -1402,6 +1400,8 @@ int check_args(int type, int64_t rows, int64_t cols, int k) {
   BLP_CHECK(rows >= 0 && rows <= MOST_ROWS, BLP_E_ARG, "softmax loss: rows must be in [0, 2^31 - 2^16]");
   BLP_CHECK(cols >= 1 && cols <= MOST_ROWS, BLP_E_ARG, "softmax loss: the catalogue must have 1 to 2^31 - 2^16 rows");
   BLP_CHECK(k >= 1 && k <= (1 << 20), BLP_E_ARG, "softmax loss: k must be in [1, 2^20]");
+  // the gradients' tiles, 64 x 32 or larger, are counted in 31 bits; the scores' are fewer (pieces and pairs bound them)
+  BLP_CHECK(std::max(rows, cols) <= (1ll << 41) / k, BLP_E_ARG, "softmax loss: rows x k and columns x k must be at most 2^41");
   return 0;
 }
 

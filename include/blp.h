@@ -438,7 +438,7 @@ int blp_walk_stats(blp_walk* w, double* total_ms, int64_t* launches);
  *   z_ij = scale x_i . table_j     lse_i = log sum_j exp z_ij     loss_i = lse_i - z_{i, target_i}
  * target: int32, or int64 with target64; outside [0, cols) the row is ignored (loss 0, gradient 0,
  * whatever x holds). The scores are not kept: the workspace holds one piece of the catalogue's.
- * rows and cols up to 2^31 - 2^16, k up to 2^20, row strides of x and table up to 2^20 elements, scale
+ * rows and cols up to 2^31 - 2^16, k up to 2^20, rows k and cols k up to 2^41, row strides of x and table up to 2^20 elements, scale
  * from -2^127 to 2^127.
  *   blp_softmax_loss_workspace: bytes of workspace (256-byte aligned) for the same arguments;
  *     `forward` / `grads`: whether the call runs the forward / the backward pass.

@@ -20,7 +20,7 @@ static int n_kernels;
 static struct launch {
   const char* name;
   dim3_t grid, block;
-  unsigned char first[96]; /* of the kernel's first argument, where its name says that it is a Problem */
+  unsigned char first[88]; /* of the kernel's first argument, where its name says that it is a Problem */
 } launches[MOST];
 static int n_launches, fail_at = -1, fail_with, last_error;
 

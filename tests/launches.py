@@ -56,7 +56,7 @@ def _child(stub):
             S.stub_shape(i, shape)
             name = S.stub_name(i).decode()
             launches.append({"name": name, "grid": list(shape[:3]), "block": list(shape[3:]),
-                             "product": _product(name, bytes(S.stub_first(i)[:96]))})
+                             "product": _product(name, bytes(S.stub_first(i)[:88]))})
         out.append({"rc": rc, "error": L.blp_last_error().decode() if rc else "", "launches": launches})
     json.dump(out, sys.stdout)
 

@@ -106,3 +106,20 @@ def test_more_scores_than_tiles_can_be_counted_are_refused():
     for k in (64, 300, 15):
         (got,) = run([scores8((1 << 31) - 1, (1 << 31) - 1, k, 1)])
         assert got["rc"] == -1 and "2^45" in got["error"] and not got["launches"]
+
+
+@pytest.mark.parametrize("m,n,k", [((1 << 31) - (1 << 16), 1000, 1 << 20), (1000, (1 << 31) - (1 << 16), 1 << 11)])
+def test_more_elements_than_tiles_can_be_counted_are_refused(m, n, k):
+    """Before anything is packed."""
+    for got in run([loss(1, m, n, k), backward(0, m, n, k)]):
+        assert got["rc"] == -1 and "2^41" in got["error"] and not got["launches"]
+
+
+def test_grids_fit_31_bits():
+    for m, n, k in (((1 << 31) - (1 << 16), 1 << 10, 1 << 10), (1 << 10, (1 << 31) - (1 << 16), 1 << 10), (1 << 21, 1 << 21, 1 << 20)):
+        for got in run([loss(t, m, n, k) for t in (0, 1)] if m * n < 1 << 42 else [loss(1, m, n, k, grads=0)]):
+            assert got["rc"] == 0, got["error"]
+            for l in got["launches"]:
+                assert l["grid"][0] * l["block"][0] < 1 << 32
+                if l["product"]:
+                    assert 0 < l["product"]["tiles_p"] * l["product"]["tiles_q"] < 1 << 31
